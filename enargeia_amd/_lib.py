@@ -71,6 +71,12 @@ SIGNATURES: dict[str, tuple] = {
     "eg_decoder_create_cache": (_i, [_vp, _vp, _i, ctypes.POINTER(_vp)]),
     "eg_attention_prefill": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "eg_attention_prefill_f32": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "eg_kv4_page_bytes": (_i, [_vp, ctypes.POINTER(ctypes.c_uint64)]),
+    "eg_kv4_append": (_i, [_vp] * 14),
+    "eg_kv4_read": (_i, [_vp] * 7 + [ctypes.c_uint32, _i, _vp]),
+    "eg_kv4_copy_pages": (_i, [_vp, _vp, _vp, ctypes.c_uint32, _vp]),
+    "eg_attention_decode_kv4": (_i, [_vp] * 8),
+    "eg_attention_packed": (_i, [_vp] * 8),
     "eg_container_open": (_i, [_vp, ctypes.c_char_p, ctypes.POINTER(_vp)]),
     "eg_container_close": (_i, [_vp]),
     "eg_container_header_get": (_i, [_vp, _vp]),

@@ -42,9 +42,10 @@ HIP_FLAGS = [
 ]
 
 
-# Per-file additions: the chunk attention keeps its MFMA results in ordinary VGPRs (its softmax
+# Per-file additions: the attentions keep their MFMA results in ordinary VGPRs (a softmax
 # reads and rescales them every key tile; held in AGPRs, each of those accesses is a copy).
-FILE_FLAGS = {"eg_prefill_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+FILE_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form"]
+              for name in ("eg_prefill_attention.hip", "eg_packed_attention.hip", "eg_kv4_attention.hip")}
 
 
 def sources() -> list[str]:

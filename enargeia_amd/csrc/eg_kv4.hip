@@ -1,0 +1,384 @@
+// The paged 4-bit cache (enargeia_hip.h): rows appended, rows read back, pages copied. All three move
+// bytes: their floor is what they read and write once at the memory's rate.
+//
+// Append and read go by blocks of 8 positions of a page: a V code word holds 8 positions of one dim,
+// so a block's V words are written by one wave from its 8 rows, whole - or, where the batch has only
+// some of the 8, merged into what is there (one wave per block and kv head: no race). Packed rows
+// and blocks do not align, so a wave that owns `span` packed rows takes the blocks whose first row
+// of this call lies among them, up to 7 rows past its span.
+#include <algorithm>
+
+#include "eg_kv4.hpp"
+
+namespace {
+
+using namespace eg_kv4;
+
+constexpr uint32_t kThreads = 256;
+
+// The runs of rows that lie in one 8-position block, for the packed rows [r0, r0 + span):
+// f(sequence, first row, its position, rows).
+template <class F>
+__device__ __forceinline__ void for_blocks(const uint32_t* offsets, const uint32_t* starts, uint32_t sequences,
+                                           uint32_t rows, uint32_t r0, uint32_t span, F&& f) {
+  uint32_t r = r0, seq = 0, first = 0, end = 0, start = 0;
+  bool have = false;
+  const uint32_t stop = min(r0 + span, rows);
+  while (r < stop) {
+    if (!have || r >= end) {
+      // rows before the first sequence are in none: go on with the next row of the span
+      if (!find_sequence(offsets, sequences, r, seq, first, end)) {
+        if (r >= offsets[sequences]) return;
+        r++;
+        continue;
+      }
+      have = true;
+      start = starts[seq];
+    }
+    const uint32_t position = start + (r - first), in_block = position & 7u;
+    const uint32_t n = min(min(8u - in_block, end - r), rows - r);
+    if (in_block == 0 || r == first) f(seq, r, position, n);
+    r += n;
+  }
+}
+
+// Max over aligned groups of 32 lanes, in every lane.
+__device__ __forceinline__ uint32_t max_of_32(uint32_t v) {
+  const auto step = [&](int o) { v = max(v, (uint32_t)o); };
+  step(__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true));
+  step(__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true));
+  step(__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, true));
+  step(__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, true));
+  step(__builtin_amdgcn_ds_swizzle((int)v, 0x401F));
+  return v;
+}
+
+// OR over aligned groups of 8 lanes, in every lane.
+__device__ __forceinline__ uint32_t or_of_8(uint32_t v) {
+  v |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true);
+  v |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true);
+  v |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, true);
+  return v;
+}
+
+// The code (0..15) of this lane's value and the f16 bits of its group's scale; a group is 32 lanes.
+// The absmax is taken over the values' bits, which order magnitudes and put infinities and NaN on top.
+__device__ __forceinline__ uint32_t quantize(float x, uint32_t& scale) {
+#pragma clang fp contract(off)
+  const uint32_t top = max_of_32(__float_as_uint(x) & 0x7FFFFFFFu);
+  if (top >= 0x7F800000u) {
+    scale = 0x7E00u;
+    return 8u;
+  }
+  const float t = fminf(__uint_as_float(top) * (1.0f / 7.0f), 9344.0f);
+  scale = (egd::float_to_half(t) + 4u) & 0xFFF8u;
+  const float s = egd::half_to_float((uint16_t)scale);
+  const float r = s > 0.f ? 1.0f / s : 0.f;
+  return (uint32_t)((int)fminf(fmaxf(rintf(x * r), -7.f), 7.f) + 8);
+}
+
+struct AppendArgs {
+  const void *q, *k, *v;
+  const float2* rope;
+  const uint32_t *offsets, *starts;
+  void *q_out, *k_out, *v_out;
+  uint32_t rows, heads, q_stride, k_stride, v_stride, rope_positions, span;
+};
+
+// A wave per (span of packed rows, kv head's K, kv head's V or query head). A lane holds dim `lane`
+// of up to 8 rows (and dim lane + 64 at head_dim 128), all read at once. Bound by latency where the
+// rows are few, by memory where they are many.
+template <int D, class TI, class TO>
+__global__ __launch_bounds__(256) void append_kernel(AppendArgs a, Pool pool) {
+  constexpr int kPer = D / 64;  // dims per lane
+  const uint32_t lane = threadIdx.x & 63u;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t task = blockIdx.y * 4 + wave, kvh = pool.kv_heads;
+  if (task >= 2 * kvh + a.heads) return;
+  const bool is_k = task < kvh, is_v = !is_k && task < 2 * kvh;
+  const uint32_t head = is_k ? task : is_v ? task - kvh : task - 2 * kvh;
+  const TI* src = static_cast<const TI*>(is_k ? a.k : is_v ? a.v : a.q);
+  TO* dst = static_cast<TO*>(is_k ? a.k_out : is_v ? a.v_out : a.q_out);
+  const uint32_t stride = is_k ? a.k_stride : is_v ? a.v_stride : a.q_stride;
+  const uint32_t out_stride = (is_k || is_v ? kvh : a.heads) * D;
+  const Layout at = layout<D>(1u << pool.page_shift);
+
+  for_blocks(a.offsets, a.starts, pool.sequences, a.rows, blockIdx.x * a.span, a.span,
+             [&](uint32_t seq, uint32_t row, uint32_t position, uint32_t n) {
+    const uint32_t page = pool.page_of(seq, position);
+    if ((position >> pool.page_shift) >= pool.max_pages) return;
+    if (a.rope) {  // rows that the rope does not reach are skipped
+      if (position >= a.rope_positions) return;
+      n = min(n, a.rope_positions - position);
+    }
+    float x[8][kPer];
+    float2 cs[8];
+#pragma unroll
+    for (uint32_t i = 0; i < 8; i++) {
+      const uint32_t r = row + min(i, n - 1);  // (rows past n are read as the last one: never used)
+#pragma unroll
+      for (int j = 0; j < kPer; j++) x[i][j] = to_f32(src[(size_t)r * stride + head * D + 64 * j + lane]);
+      cs[i] = make_float2(1.f, 0.f);
+      if (a.rope && !is_v)
+        cs[i] = a.rope[(size_t)(position + min(i, n - 1)) * (D / 2) + (D == 64 ? lane & 31u : lane)];
+    }
+    if (a.rope && !is_v) {
+#pragma clang fp contract(off)
+#pragma unroll
+      for (uint32_t i = 0; i < 8; i++) {
+        if constexpr (D == 64) {  // the pair's other half is 32 lanes away
+          const float y = __shfl_xor(x[i][0], 32, 64);
+          const float p = x[i][0] * cs[i].x, t = y * cs[i].y;
+          x[i][0] = lane < 32 ? p - t : p + t;
+        } else {
+          const float u = x[i][0], w = x[i][1];
+          x[i][0] = u * cs[i].x - w * cs[i].y;
+          x[i][1] = w * cs[i].x + u * cs[i].y;
+        }
+      }
+    }
+    if (dst) {
+#pragma unroll
+      for (uint32_t i = 0; i < 8; i++)
+        if (i < n) {
+#pragma unroll
+          for (int j = 0; j < kPer; j++)
+            dst[(size_t)(row + i) * out_stride + head * D + 64 * j + lane] = from_f32<TO>(x[i][j]);
+        }
+    }
+    if ((!is_k && !is_v) || page >= pool.pages) return;
+    uint8_t* block = pool.block(page, head, at.head_bytes);
+    const uint32_t slot = position & ((1u << pool.page_shift) - 1u), mine = lane & 7u;
+#pragma unroll
+    for (int j = 0; j < kPer; j++) {
+      uint32_t kword = 0, vword = 0, my_scale = 0;
+#pragma unroll
+      for (uint32_t i = 0; i < 8; i++) {
+        uint32_t s;
+        const uint32_t u = quantize(x[i][j], s);
+        if ((lane & 31u) == i) my_scale = s;  // lane i of a group keeps row i's scale
+        if (is_k) {
+          const uint32_t w = or_of_8(u << (4 * mine));
+          if (mine == i) kword = w;  // lane i of eight keeps row i's word
+        } else if (i < n) {
+          vword |= u << (4 * ((slot + i) & 7u));
+        }
+      }
+      const uint32_t group = 2 * j + (lane >> 5);
+      if (is_k) {
+        if (mine < n)
+          reinterpret_cast<uint32_t*>(block)[(slot + mine) * (D / 8) + ((lane >> 3) & 3u) * (D / 32) + group] = kword;
+      } else {
+        uint32_t* word = reinterpret_cast<uint32_t*>(block + at.v_codes) + (slot >> 3) * D + 64 * j + lane;
+        if (n < 8) {
+          const uint32_t mask = ((1u << (4 * n)) - 1u) << (4 * (slot & 7u));
+          vword |= *word & ~mask;
+        }
+        *word = vword;
+      }
+      if ((lane & 31u) < n)
+        reinterpret_cast<uint16_t*>(block + (is_k ? at.k_scales : at.v_scales))
+            [(group << pool.page_shift) + slot + (lane & 31u)] = (uint16_t)my_scale;
+    }
+  });
+}
+
+struct ReadArgs {
+  const uint32_t *offsets, *starts;
+  void *k_out, *v_out;
+  uint32_t rows, span;
+};
+
+// A wave per (span of packed rows, kv head's K or V), blocks as in append_kernel. K: a lane dequantizes
+// one word, 8 dims of a row. V: a lane has one dim (two at head_dim 128) of the block's 8 rows.
+template <int D, class TO>
+__global__ __launch_bounds__(256) void read_kernel(ReadArgs a, Pool pool) {
+  constexpr uint32_t kGroups = D / 32, kPer = D / 64;
+  const uint32_t lane = threadIdx.x & 63u;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t task = blockIdx.y * 4 + wave, kvh = pool.kv_heads;
+  if (task >= 2 * kvh) return;
+  const bool is_k = task < kvh;
+  const uint32_t head = is_k ? task : task - kvh;
+  TO* dst = static_cast<TO*>(is_k ? a.k_out : a.v_out);
+  const Layout at = layout<D>(1u << pool.page_shift);
+  for_blocks(a.offsets, a.starts, pool.sequences, a.rows, blockIdx.x * a.span, a.span,
+             [&](uint32_t seq, uint32_t row, uint32_t position, uint32_t n) {
+    const uint32_t page = pool.page_of(seq, position);
+    const bool have = page < pool.pages;
+    const uint8_t* block = pool.block(have ? page : 0, head, at.head_bytes);
+    const uint32_t slot = position & ((1u << pool.page_shift) - 1u);
+    const uint16_t* scales = reinterpret_cast<const uint16_t*>(block + (is_k ? at.k_scales : at.v_scales));
+    TO* out = dst + ((size_t)row * kvh + head) * D;
+    if (is_k) {
+#pragma unroll
+      for (uint32_t j = 0; j < kPer; j++) {
+        const uint32_t i = (64 * j + lane) / (D / 8), w = lane % (D / 8);  // row of the block, word of the row
+        if (i >= n) continue;
+        uint32_t word = 0x88888888u;
+        float s = 0.f;
+        const uint32_t part = w / kGroups, group = w % kGroups;
+        if (have) {
+          word = reinterpret_cast<const uint32_t*>(block)[(slot + i) * (D / 8) + w];
+          s = egd::half_to_float(scales[(group << pool.page_shift) + slot + i]);
+        }
+        TO* to = out + (size_t)i * kvh * D + 32 * group + 8 * part;
+#pragma unroll
+        for (uint32_t e = 0; e < 8; e++) to[e] = from_f32<TO>((float)((int)((word >> (4 * e)) & 15u) - 8) * s);
+      }
+    } else {
+#pragma unroll
+      for (uint32_t j = 0; j < kPer; j++) {
+        const uint32_t d = 64 * j + lane;
+        uint32_t word = 0x88888888u;
+        if (have) word = reinterpret_cast<const uint32_t*>(block + at.v_codes)[(slot >> 3) * D + d];
+        for (uint32_t i = 0; i < n; i++) {
+          const float s = have ? egd::half_to_float(scales[((d / 32) << pool.page_shift) + slot + i]) : 0.f;
+          out[(size_t)i * kvh * D + d] = from_f32<TO>((float)((int)((word >> (4 * ((slot + i) & 7u))) & 15u) - 8) * s);
+        }
+      }
+    }
+  });
+}
+
+// 16 KiB of a page per workgroup, four 16-byte words a thread, all read before any is written.
+constexpr uint32_t kCopyWords = 4, kCopyBytes = kThreads * kCopyWords * 16;
+__global__ __launch_bounds__(256) void copy_pages_kernel(uint8_t* pool, const uint32_t* pairs, uint32_t pages,
+                                                         uint64_t stride, uint32_t parts) {
+  const uint32_t pair = blockIdx.x / parts, part = blockIdx.x % parts;
+  const uint32_t from = pairs[2 * (size_t)pair], to = pairs[2 * (size_t)pair + 1];
+  if (from >= pages || to >= pages) return;
+  const uint64_t begin = (uint64_t)part * kCopyBytes + 16u * threadIdx.x;
+  const uint8_t* src = pool + from * stride;
+  uint8_t* dst = pool + to * stride;
+  uint4 v[kCopyWords];
+#pragma unroll
+  for (uint32_t i = 0; i < kCopyWords; i++) {
+    const uint64_t o = begin + 16u * kThreads * i;
+    if (o < stride) v[i] = *reinterpret_cast<const uint4*>(src + o);
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < kCopyWords; i++) {
+    const uint64_t o = begin + 16u * kThreads * i;
+    if (o < stride) *reinterpret_cast<uint4*>(dst + o) = v[i];
+  }
+}
+
+bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// Rows per wave: one where the rows are few (a decode batch's rows are blocks of their own, and a
+// wave would take them one after another), else a block's 8.
+uint32_t span_for(uint32_t rows) { return rows <= 2048u ? 1u : 8u; }
+
+}  // namespace
+
+int eg_kv4::check_dims(eg_context* ctx, const char* op, const eg_kv4_dims* d, const void* pool) {
+  if (!d || !pool) return eg::fail(ctx, EG_ERR_INVALID, "%s: NULL argument", op);
+  if (d->head_dim != 64 && d->head_dim != 128)
+    return eg::fail(ctx, EG_ERR_INVALID, "%s: head_dim %u is not supported (64, 128)", op, d->head_dim);
+  if (d->page_size != 32 && d->page_size != 64 && d->page_size != 128 && d->page_size != 256)
+    return eg::fail(ctx, EG_ERR_INVALID, "%s: page_size %u is not supported (32, 64, 128, 256)", op, d->page_size);
+  if (d->kv_heads == 0 || d->kv_heads > 1024)
+    return eg::fail(ctx, EG_ERR_INVALID, "%s: %u kv heads (1 to 1024)", op, d->kv_heads);
+  if (d->pages == 0) return eg::fail(ctx, EG_ERR_INVALID, "%s: a pool of no pages", op);
+  if (d->page_stride % 16 != 0 || d->page_stride < eg_kv4::page_bytes(*d))
+    return eg::fail(ctx, EG_ERR_INVALID, "%s: page_stride %llu is not a multiple of 16 of at least %llu bytes", op,
+                    (unsigned long long)d->page_stride, (unsigned long long)eg_kv4::page_bytes(*d));
+  if (!aligned(pool)) return eg::fail(ctx, EG_ERR_INVALID, "%s: the pool must be 16-byte aligned", op);
+  if ((uint64_t)d->max_pages * d->page_size >= (1ull << 31))
+    return eg::fail(ctx, EG_ERR_RANGE, "%s: %u pages of %u positions per sequence (under 2^31 positions)", op,
+                    d->max_pages, d->page_size);
+  if (d->sequences > (1u << 20))
+    return eg::fail(ctx, EG_ERR_RANGE, "%s: %u sequences (at most 2^20)", op, d->sequences);
+  return EG_OK;
+}
+
+extern "C" {
+
+int eg_kv4_page_bytes(const eg_kv4_dims* dims, uint64_t* out_bytes) {
+  if (!dims || !out_bytes) return eg::fail(nullptr, EG_ERR_INVALID, "kv4_page_bytes: NULL argument");
+  *out_bytes = eg_kv4::page_bytes(*dims);
+  return EG_OK;
+}
+
+int eg_kv4_append(eg_context* ctx, const void* q, const void* k, const void* v, const float* rope,
+                  const uint32_t* offsets, const uint32_t* starts, const uint32_t* table, void* pool, void* q_out,
+                  void* k_out, void* v_out, const eg_kv4_dims* dims, const eg_kv4_append_dims* append) {
+  const char* op = "kv4_append";
+  if (!ctx) return eg::fail(nullptr, EG_ERR_INVALID, "%s: ctx is NULL", op);
+  const int st = eg_kv4::check_dims(ctx, op, dims, pool);
+  if (st != EG_OK) return st;
+  if (!append || !k || !v || !offsets || !starts || !table)
+    return eg::fail(ctx, EG_ERR_INVALID, "%s: NULL argument", op);
+  const eg_kv4_append_dims& d = *append;
+  if (!known_type(d.in_type) || !known_type(d.out_type))
+    return eg::fail(ctx, EG_ERR_INVALID, "%s: in_type %d, out_type %d (eg_element)", op, d.in_type, d.out_type);
+  if ((q == nullptr) != (q_out == nullptr) || (q == nullptr) != (d.heads == 0))
+    return eg::fail(ctx, EG_ERR_INVALID, "%s: q, q_out and heads go together", op);
+  if (d.heads > 65535) return eg::fail(ctx, EG_ERR_RANGE, "%s: %u heads (at most 65535)", op, d.heads);
+  const uint32_t width = dims->kv_heads * dims->head_dim, q_width = d.heads * dims->head_dim;
+  AppendArgs a{q, k, v, reinterpret_cast<const float2*>(rope), offsets, starts, q_out, k_out, v_out, d.rows, d.heads,
+               d.q_stride ? d.q_stride : q_width, d.k_stride ? d.k_stride : width,
+               d.v_stride ? d.v_stride : width, d.rope_positions, span_for(d.rows)};
+  if (a.q_stride < q_width || a.k_stride < width || a.v_stride < width || (a.q_stride | a.k_stride | a.v_stride) % 4)
+    return eg::fail(ctx, EG_ERR_INVALID, "%s: row strides %u, %u, %u (multiples of 4, at least a row)", op, a.q_stride,
+                    a.k_stride, a.v_stride);
+  if (!aligned(q) || !aligned(k) || !aligned(v) || !aligned(rope) || !aligned(q_out) || !aligned(k_out) ||
+      !aligned(v_out))
+    return eg::fail(ctx, EG_ERR_INVALID, "%s: q, k, v, rope and the outputs must be 16-byte aligned", op);
+  if (d.rows == 0 || dims->sequences == 0) return EG_OK;
+  if (d.rows >= (1u << 30)) return eg::fail(ctx, EG_ERR_RANGE, "%s: %u rows (under 2^30)", op, d.rows);
+  const eg_kv4::Pool p = eg_kv4::pool_of(*dims, pool, table);
+  const dim3 grid((d.rows + a.span - 1) / a.span, (2 * dims->kv_heads + d.heads + 3) / 4);
+  with_type(d.in_type, [&](auto ti) {
+    with_type(d.out_type, [&](auto to) {
+      if (dims->head_dim == 64)
+        hipLaunchKernelGGL((append_kernel<64, decltype(ti), decltype(to)>), grid, dim3(kThreads), 0, ctx->stream, a, p);
+      else
+        hipLaunchKernelGGL((append_kernel<128, decltype(ti), decltype(to)>), grid, dim3(kThreads), 0, ctx->stream, a, p);
+    });
+  });
+  return eg::check_launch(ctx, op);
+}
+
+int eg_kv4_read(eg_context* ctx, const uint32_t* offsets, const uint32_t* starts, const uint32_t* table,
+                const void* pool, void* k_out, void* v_out, uint32_t rows, int out_type, const eg_kv4_dims* dims) {
+  const char* op = "kv4_read";
+  if (!ctx) return eg::fail(nullptr, EG_ERR_INVALID, "%s: ctx is NULL", op);
+  const int st = eg_kv4::check_dims(ctx, op, dims, pool);
+  if (st != EG_OK) return st;
+  if (!offsets || !starts || !table || !k_out || !v_out) return eg::fail(ctx, EG_ERR_INVALID, "%s: NULL argument", op);
+  if (!known_type(out_type)) return eg::fail(ctx, EG_ERR_INVALID, "%s: out_type %d (eg_element)", op, out_type);
+  if (!aligned(k_out) || !aligned(v_out))
+    return eg::fail(ctx, EG_ERR_INVALID, "%s: the outputs must be 16-byte aligned", op);
+  if (rows == 0 || dims->sequences == 0) return EG_OK;
+  if (rows >= (1u << 30)) return eg::fail(ctx, EG_ERR_RANGE, "%s: %u rows (under 2^30)", op, rows);
+  const ReadArgs a{offsets, starts, k_out, v_out, rows, span_for(rows)};
+  const eg_kv4::Pool p = eg_kv4::pool_of(*dims, pool, table);
+  const dim3 grid((rows + a.span - 1) / a.span, (2 * dims->kv_heads + 3) / 4);
+  with_type(out_type, [&](auto to) {
+    if (dims->head_dim == 64)
+      hipLaunchKernelGGL((read_kernel<64, decltype(to)>), grid, dim3(kThreads), 0, ctx->stream, a, p);
+    else
+      hipLaunchKernelGGL((read_kernel<128, decltype(to)>), grid, dim3(kThreads), 0, ctx->stream, a, p);
+  });
+  return eg::check_launch(ctx, op);
+}
+
+int eg_kv4_copy_pages(eg_context* ctx, void* pool, const uint32_t* pairs, uint32_t count, const eg_kv4_dims* dims) {
+  const char* op = "kv4_copy_pages";
+  if (!ctx) return eg::fail(nullptr, EG_ERR_INVALID, "%s: ctx is NULL", op);
+  const int st = eg_kv4::check_dims(ctx, op, dims, pool);
+  if (st != EG_OK) return st;
+  if (count == 0) return EG_OK;
+  if (!pairs) return eg::fail(ctx, EG_ERR_INVALID, "%s: NULL argument", op);
+  const uint64_t parts = (dims->page_stride + kCopyBytes - 1) / kCopyBytes;
+  if (parts * count >= (1ull << 31) / kThreads)
+    return eg::fail(ctx, EG_ERR_RANGE, "%s: %u pages of %llu bytes over the grid limit", op, count,
+                    (unsigned long long)dims->page_stride);
+  hipLaunchKernelGGL(copy_pages_kernel, dim3((uint32_t)(parts * count)), dim3(kThreads), 0, ctx->stream,
+                     static_cast<uint8_t*>(pool), pairs, dims->pages, dims->page_stride, (uint32_t)parts);
+  return eg::check_launch(ctx, op);
+}
+
+}  // extern "C"

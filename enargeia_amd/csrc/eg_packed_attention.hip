@@ -1,0 +1,349 @@
+// Causal attention over packed sequences of different lengths (eg_attention_packed).
+//
+//   out[i][h] = sum_j p_j V[j] / sum_j p_j,  p_j = exp(scale q[i][h] . K[j] - max_j),  j <= nk - nq + i
+//
+// One pass over the keys with the running max and sum of the softmax. A workgroup takes 128 queries of
+// one head, a wave 32 of them; key tiles of 64 go through LDS, the next one's loads under way while
+// this one is multiplied. Both products run on v_mfma_f32_32x32x16 in the transposed form S^T = K Q^T,
+// O^T = V^T P^T: a lane holds one query's scores (rows of S^T: 4 consecutive keys of every 8), which
+// are the second product's B operand where they lie, with V^T read from LDS transposed.
+#include <algorithm>
+
+#include "eg_kv4.hpp"
+
+namespace {
+
+using eg_kv4::bf16;
+using eg_kv4::from_f32;
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+using egd::u32x4;
+
+constexpr uint32_t kThreads = 256, kWaves = 4;
+constexpr uint32_t kQueries = 32 * kWaves;  // per workgroup
+constexpr uint32_t kKeys = 64;              // per tile
+constexpr float kLog2e = 1.44269504088896340736f;
+
+struct Args {
+  const void *q, *k, *v;
+  void* out;
+  const uint32_t *q_offsets, *k_offsets;
+  uint32_t sequences, rows, key_rows, heads, group, q_stride, k_stride, v_stride, out_stride;
+  float scale;  // times log2 e
+};
+
+template <class T>
+__device__ __forceinline__ f32x16 multiply(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (std::is_same<T, _Float16>::value)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+template <class T>
+__device__ __forceinline__ uint32_t pack(float a, float b) {
+  if constexpr (std::is_same<T, _Float16>::value) {
+    typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, half2v{(_Float16)a, (_Float16)b});
+  } else {
+    return egd::pack_bf16(a, b);
+  }
+}
+
+// Max over the 2 lanes that hold a query (lane % 32).
+__device__ __forceinline__ float max_of_query(float x) {
+  const uint32_t a = __float_as_uint(x);
+  const auto r = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// Whether any of 8 f16 (bf16) values is an infinity or a NaN; those replaced by zeros.
+template <class T>
+__device__ __forceinline__ bool clean(u32x4& v) {
+  constexpr uint32_t kExponent = std::is_same<T, _Float16>::value ? 0x7C00u : 0x7F80u;
+  bool any = false;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const bool lo = (v[i] & kExponent) == kExponent, hi = ((v[i] >> 16) & kExponent) == kExponent;
+    any |= lo || hi;
+    v[i] &= (lo ? 0xFFFF0000u : 0xFFFFFFFFu) & (hi ? 0xFFFFu : 0xFFFFFFFFu);
+  }
+  return any;
+}
+
+// Query block `id` of all sequences' blocks, counted from the last sequence's last one: the blocks
+// with the most keys of a sequence start first. False past the last.
+__device__ __forceinline__ bool find_block(const Args& a, uint32_t id, uint32_t& seq, uint32_t& block) {
+  const uint32_t lane = threadIdx.x & 63u;
+  const uint32_t last = (a.sequences - 1) / 64 * 64;
+  for (uint32_t i0 = last;; i0 -= 64) {
+    const uint32_t s = i0 + (63u - lane);  // later sequences in lower lanes
+    uint32_t n = 0;
+    if (s < a.sequences) {
+      const uint32_t b = min(a.q_offsets[s], a.rows), e = min(a.q_offsets[s + 1], a.rows);
+      n = e > b ? (e - b + kQueries - 1) / kQueries : 0;
+    }
+    uint32_t upto = n;  // blocks of lanes 0 .. this one
+#pragma unroll
+    for (uint32_t d = 1; d < 64; d <<= 1) {
+      const uint32_t t = __shfl_up(upto, d, 64);
+      if (lane >= d) upto += t;
+    }
+    const uint64_t past = __ballot(upto > id);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)upto, l);
+      seq = i0 + (63u - (uint32_t)l);
+      block = total - 1 - id;  // the sequence's last block first
+      return true;
+    }
+    id -= (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+    if (i0 == 0) return false;
+  }
+}
+
+template <int D, class T, class TO>
+__global__ __launch_bounds__(256) void packed_kernel(Args a) {
+  constexpr uint32_t kSlots = D / 8;                  // 16-byte slots of a row
+  constexpr uint32_t kRow = D * 2, kTile = kKeys * kRow;  // bytes
+  constexpr int kSteps = D / 16, kBlocks = D / 32;    // depth steps of S^T; blocks of 32 dims of O^T
+  constexpr uint32_t kLoads = kTile / (kThreads * 16);
+  __shared__ __attribute__((aligned(16))) uint8_t tiles[4 * kTile];  // [buffer][K or V]
+  const uint32_t tid = threadIdx.x, lane = tid & 63u;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t lq = lane & 31u, lh = lane >> 5;  // MFMA lane coordinates
+  const uint32_t h = blockIdx.x % a.heads, kv = h / a.group;
+  uint32_t seq, block;
+  if (!find_block(a, blockIdx.x / a.heads, seq, block)) return;
+  const uint32_t q_begin = min(a.q_offsets[seq], a.rows), nq = min(a.q_offsets[seq + 1], a.rows) - q_begin;
+  const uint32_t k_begin = min(a.k_offsets[seq], a.key_rows);
+  const uint32_t nk = max(min(a.k_offsets[seq + 1], a.key_rows), k_begin) - k_begin;
+  const uint32_t q0 = block * kQueries, query = q0 + wave * 32 + lq;
+  const T* q = static_cast<const T*>(a.q);
+  const uint8_t* kbase = reinterpret_cast<const uint8_t*>(static_cast<const T*>(a.k) + (size_t)k_begin * a.k_stride + kv * D);
+  const uint8_t* vbase = reinterpret_cast<const uint8_t*>(static_cast<const T*>(a.v) + (size_t)k_begin * a.v_stride + kv * D);
+
+  // Keys that query i sees: those below nk - nq + i + 1 (none where that is not positive).
+  const int shift = (int)(nk - nq) + 1;
+  const int last = shift + (int)min(q0 + kQueries, nq) - 1;  // of the workgroup's last query
+  const uint32_t key_end = last > 0 ? min((uint32_t)last, nk) : 0;
+  const int limit = shift + (int)query;                       // of this lane's query
+  const int open = shift + (int)(q0 + wave * 32);             // of the wave's first query
+  const uint32_t ntiles = (key_end + kKeys - 1) / kKeys;
+
+  // Q^T, B operand: query lq, dims 16 s + 8 lh .. +8.
+  u32x4 qf[kSteps];
+  {
+    const bool in = query < nq;
+    const u32x4* src = reinterpret_cast<const u32x4*>(q + (size_t)(q_begin + (in ? query : 0)) * a.q_stride + h * D + 8 * lh);
+#pragma unroll
+    for (int s = 0; s < kSteps; s++) qf[s] = in ? src[2 * s] : u32x4{0, 0, 0, 0};
+  }
+  f32x16 o[kBlocks];
+#pragma unroll
+  for (int n = 0; n < kBlocks; n++)
+#pragma unroll
+    for (int e = 0; e < 16; e++) o[n][e] = 0.f;
+  float m = -INFINITY, l = 0.f;  // running max before the scale; this lane's share of the sum
+
+  // K's and V's rows go to LDS 16 bytes a lane, row r's slot j at j ^ swizzle(r): 16 rows of K's
+  // operand reads, and the 4 rows of V's transposed ones, then lie in different banks.
+  const uint32_t lrow = tid / kSlots, slot = tid % kSlots;
+  const auto kswz = [](uint32_t r) { return D == 64 ? (r >> 1) & 7u : r & 15u; };
+  const auto vswz = [](uint32_t r) { return D == 64 ? 4u * ((r >> 1) & 1u) : 4u * (r & 3u); };
+  const auto load_tile = [&](uint32_t t, uint32_t buf) {
+    const uint32_t j0 = t * kKeys, left = min(kKeys, key_end - j0);
+    const auto kr = egd::buffer(kbase + (size_t)j0 * a.k_stride * 2, (left - 1) * a.k_stride * 2 + kRow);
+    const auto vr = egd::buffer(vbase + (size_t)j0 * a.v_stride * 2, (left - 1) * a.v_stride * 2 + kRow);
+#pragma unroll
+    for (uint32_t i = 0; i < kLoads; i++) {
+      const uint32_t r = lrow + i * (kThreads / kSlots);
+      uint8_t* at = tiles + 2 * kTile * buf + (i * kThreads + wave * 64) * 16;
+      // (rows past the last key: an offset past the resource, zeros)
+      egd::load_to_lds(kr, at, r < left ? r * a.k_stride * 2 + 16 * (slot ^ kswz(r)) : 0x7FFFFFF0u);
+      egd::load_to_lds(vr, at + kTile, r < left ? r * a.v_stride * 2 + 16 * (slot ^ vswz(r)) : 0x7FFFFFF0u);
+    }
+  };
+  const auto settle = [&]() {
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt 0: the memory-to-LDS loads have landed
+    __syncthreads();
+  };
+  // V^T operand reads: 4 keys x 16 dims a group of 16 lanes; lane i points at key i / 4, dims 4 (i % 4).
+  const uint32_t li = lane & 15u, vrow = 4 * lh + (li >> 2);
+  uint32_t vat[kBlocks];
+#pragma unroll
+  for (uint32_t n = 0; n < (uint32_t)kBlocks; n++)
+    vat[n] = kTile + vrow * kRow + 16 * ((4 * n + 2 * ((lane >> 4) & 1u) + ((li & 3u) >> 1)) ^ vswz(vrow)) + 8 * (li & 1u);
+
+  if (ntiles) load_tile(0, 0);
+  settle();
+  for (uint32_t t = 0; t < ntiles; t++) {
+    const uint32_t j0 = t * kKeys, buf = t & 1u;
+    const uint8_t* tile = tiles + 2 * kTile * buf;
+    if (t + 1 < ntiles) load_tile(t + 1, buf ^ 1u);
+    // A masked weight is 0, but 0 times an infinity or NaN is not: in the tiles with masked keys such
+    // values of V are taken out of the product, and added at the end to the queries that see them.
+    bool unclean = false;
+    if ((int)(j0 + kKeys) > shift + (int)q0) {
+#pragma unroll
+      for (uint32_t i = 0; i < kLoads; i++) {
+        u32x4* at = reinterpret_cast<u32x4*>(tiles + 2 * kTile * buf + kTile + (i * kThreads + tid) * 16);
+        u32x4 v = *at;
+        if (clean<T>(v)) {
+          *at = v;
+          unclean = true;
+        }
+      }
+      unclean = __syncthreads_or(unclean);
+    }
+    // (a wave whose queries all end before this tile has nothing to do in it)
+    if ((int)j0 < open + 31) {
+      f32x16 s[2];
+#pragma unroll
+      for (uint32_t n = 0; n < 2; n++) {
+#pragma unroll
+        for (int e = 0; e < 16; e++) s[n][e] = 0.f;
+        const uint32_t r = 32 * n + lq;
+#pragma unroll
+        for (uint32_t d = 0; d < (uint32_t)kSteps; d++) {
+          const u32x4 ka = *reinterpret_cast<const u32x4*>(tile + r * kRow + 16 * ((2 * d + lh) ^ kswz(r)));
+          s[n] = multiply<T>(ka, qf[d], s[n]);
+        }
+      }
+      // register e of block n is key j0 + 32 n + 8 (e / 4) + 4 lh + e % 4
+      if ((int)(j0 + kKeys) > open) {
+#pragma unroll
+        for (int n = 0; n < 2; n++)
+#pragma unroll
+          for (int e = 0; e < 16; e++)
+            if ((int)(j0 + 32 * n + 8 * (e / 4) + 4 * lh + e % 4) >= limit) s[n][e] = -INFINITY;
+      }
+      float top = m;
+#pragma unroll
+      for (int n = 0; n < 2; n++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) top = fmaxf(top, s[n][e]);
+      top = max_of_query(top);
+      if (__builtin_amdgcn_ballot_w64(top > m) != 0) {
+        const float alpha = top > m ? __builtin_amdgcn_exp2f((m - top) * a.scale) : 1.f;
+        l *= alpha;
+#pragma unroll
+        for (int n = 0; n < kBlocks; n++) o[n] *= alpha;
+        m = top;
+      }
+      const float off = m == -INFINITY ? 0.f : m * a.scale;
+#pragma unroll
+      for (int n = 0; n < 2; n++) {
+        uint32_t pb[8];
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+          const float x = __builtin_amdgcn_exp2f(fmaf(s[n][e], a.scale, -off));
+          const float y = __builtin_amdgcn_exp2f(fmaf(s[n][e + 1], a.scale, -off));
+          l += x + y;
+          pb[e / 2] = pack<T>(x, y);
+        }
+#pragma unroll
+        for (int kk = 0; kk < 2; kk++) {
+          const u32x4 p{pb[4 * kk], pb[4 * kk + 1], pb[4 * kk + 2], pb[4 * kk + 3]};
+#pragma unroll
+          for (int b = 0; b < kBlocks; b++) {
+            const uint8_t* at = tile + vat[b] + (32 * n + 16 * kk) * kRow;
+            const egd::s16x4 lo = egd::lds_read_transposed(at), hi = egd::lds_read_transposed(at + 8 * kRow);
+            const u32x4 va = __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+            o[b] = multiply<T>(va, p, o[b]);
+          }
+        }
+      }
+      if (unclean) {
+        for (uint32_t j = 0; j < kKeys && (int)(j0 + j) < limit && j0 + j < key_end; j++) {
+          const T* row = reinterpret_cast<const T*>(vbase) + (size_t)(j0 + j) * a.v_stride;
+#pragma unroll
+          for (int n = 0; n < kBlocks; n++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+              const float v = eg_kv4::to_f32(row[32 * n + 8 * (e / 4) + 4 * lh + e % 4]);
+              if (!(fabsf(v) < INFINITY)) o[n][e] += v;
+            }
+        }
+      }
+    }
+    settle();
+  }
+
+  l += __shfl_xor(l, 32, 64);
+  if (query >= nq) return;
+  const float r = limit > 0 ? 1.0f / l : 0.f;  // (no key seen: zeros)
+  TO* out = static_cast<TO*>(a.out) + (size_t)(q_begin + query) * a.out_stride + h * D;
+#pragma unroll
+  for (int n = 0; n < kBlocks; n++)
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      TO* to = out + 32 * n + 8 * (e / 4) + 4 * lh;
+      if constexpr (std::is_same<TO, float>::value)
+        *reinterpret_cast<float4*>(to) = make_float4(o[n][e] * r, o[n][e + 1] * r, o[n][e + 2] * r, o[n][e + 3] * r);
+      else
+        *reinterpret_cast<uint2*>(to) = make_uint2(pack<TO>(o[n][e] * r, o[n][e + 1] * r), pack<TO>(o[n][e + 2] * r, o[n][e + 3] * r));
+    }
+}
+
+}  // namespace
+
+extern "C" int eg_attention_packed(eg_context* ctx, const void* q, const void* k, const void* v,
+                                   const uint32_t* q_offsets, const uint32_t* k_offsets, void* out,
+                                   const eg_attention_packed_dims* dims) {
+  const char* op = "attention_packed";
+  if (!ctx) return eg::fail(nullptr, EG_ERR_INVALID, "%s: ctx is NULL", op);
+  if (!dims || !q || !k || !v || !q_offsets || !k_offsets || !out)
+    return eg::fail(ctx, EG_ERR_INVALID, "%s: NULL argument", op);
+  const eg_attention_packed_dims& d = *dims;
+  if (d.head_dim != 64 && d.head_dim != 128)
+    return eg::fail(ctx, EG_ERR_INVALID, "%s: head_dim %u is not supported (64, 128)", op, d.head_dim);
+  if (d.kv_heads == 0 || d.heads == 0 || d.heads % d.kv_heads != 0 || d.heads > 65535)
+    return eg::fail(ctx, EG_ERR_INVALID, "%s: heads %u are not a multiple of kv_heads %u (at most 65535)", op, d.heads,
+                    d.kv_heads);
+  if (d.type != EG_ELEMENT_F16 && d.type != EG_ELEMENT_BF16)
+    return eg::fail(ctx, EG_ERR_INVALID, "%s: type %d (f16 or bf16)", op, d.type);
+  if (d.out_type != d.type && d.out_type != EG_ELEMENT_F32)
+    return eg::fail(ctx, EG_ERR_INVALID, "%s: out_type %d (the type %d, or f32)", op, d.out_type, d.type);
+  if (!(d.scale >= 0.f) || d.scale > 1e6f) return eg::fail(ctx, EG_ERR_INVALID, "%s: scale %g (0 to 1e6)", op, d.scale);
+  const uint32_t width = d.heads * d.head_dim, kv_width = d.kv_heads * d.head_dim;
+  Args a{q, k, v, out, q_offsets, k_offsets, d.sequences, d.rows, d.key_rows, d.heads, d.heads / d.kv_heads,
+         d.q_stride ? d.q_stride : width, d.k_stride ? d.k_stride : kv_width, d.v_stride ? d.v_stride : kv_width,
+         d.out_stride ? d.out_stride : width,
+         (d.scale > 0.f ? d.scale : 1.0f / sqrtf((float)d.head_dim)) * kLog2e};
+  if (a.q_stride < width || a.out_stride < width || a.k_stride < kv_width || a.v_stride < kv_width ||
+      (a.q_stride | a.k_stride | a.v_stride | a.out_stride) % 8)
+    return eg::fail(ctx, EG_ERR_INVALID, "%s: strides %u, %u, %u, %u (multiples of 8, at least a row)", op, a.q_stride,
+                    a.k_stride, a.v_stride, a.out_stride);
+  if (a.k_stride > (1u << 23) || a.v_stride > (1u << 23))
+    return eg::fail(ctx, EG_ERR_RANGE, "%s: key strides %u, %u (at most 2^23 elements)", op, a.k_stride, a.v_stride);
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
+       reinterpret_cast<uintptr_t>(out)) & 15u)
+    return eg::fail(ctx, EG_ERR_INVALID, "%s: q, k, v and out must be 16-byte aligned", op);
+  if (d.sequences > (1u << 20))
+    return eg::fail(ctx, EG_ERR_RANGE, "%s: %u sequences (at most 2^20)", op, d.sequences);
+  if (d.rows >= (1u << 30) || d.key_rows >= (1u << 30))
+    return eg::fail(ctx, EG_ERR_RANGE, "%s: %u rows, %u key rows (under 2^30)", op, d.rows, d.key_rows);
+  if (d.rows == 0 || d.sequences == 0) return EG_OK;
+  // at most this many query blocks, whatever the lengths
+  const uint64_t blocks = (uint64_t)d.rows / kQueries + std::min<uint64_t>(d.sequences, d.rows);
+  if (blocks * d.heads >= (1ull << 31) / kThreads)
+    return eg::fail(ctx, EG_ERR_RANGE, "%s: %u rows of %u heads over the grid limit", op, d.rows, d.heads);
+  const dim3 grid((uint32_t)(blocks * d.heads));
+  const auto go = [&](auto t, auto to) {
+    if (d.head_dim == 64)
+      hipLaunchKernelGGL((packed_kernel<64, decltype(t), decltype(to)>), grid, dim3(kThreads), 0, ctx->stream, a);
+    else
+      hipLaunchKernelGGL((packed_kernel<128, decltype(t), decltype(to)>), grid, dim3(kThreads), 0, ctx->stream, a);
+  };
+  if (d.type == EG_ELEMENT_F16) {
+    if (d.out_type == EG_ELEMENT_F32) go(_Float16{}, float{});
+    else go(_Float16{}, _Float16{});
+  } else {
+    if (d.out_type == EG_ELEMENT_F32) go(bf16{}, float{});
+    else go(bf16{}, bf16{});
+  }
+  return eg::check_launch(ctx, op);
+}

@@ -518,6 +518,108 @@ EG_API int eg_attention_prefill_f32(eg_context* ctx, const float* q, const float
                                     float* v_cache, float* q_rope, float* out,
                                     const eg_attention_prefill_dims* dims);
 
+/* ---- several sequences over a paged cache held in 4 bits (no counterpart in the reference, whose
+ * cache is one sequence's contiguous f16 or f32 rows) -------------------------------------------
+ *
+ * The cache format kv4. A row is the head_dim (64 or 128) values of one position and kv head, of K
+ * or of V, in groups of 32. A group's scale is absmax / 7 as f16, rounded half up to 8 significant
+ * bits, at most 9344; a code is the value over the scale, rounded to nearest (even) and clamped to
+ * -7..7; the value held is code * scale, exact in f16. A group with an infinity or a NaN has the
+ * scale NaN, and all its values read as NaN. The scale of a group below about 2^-19 is 0.
+ *
+ * A pool is `pages` pages, page_stride bytes apart (one page may hold several layers: the pool
+ * pointer of layer l is the first page's base + l * page bytes, page_stride all layers' bytes). A page holds
+ * page_size positions, per kv head one block after another of
+ *   K codes   [page_size][4][head_dim / 32] words: word (l, g) of a row has dims 32 g + 8 l .. +8
+ *   V codes   [page_size / 8][head_dim] words: word (b, d) has positions 8 b .. +8 of dim d
+ *   K scales  [head_dim / 32][page_size] f16
+ *   V scales  [head_dim / 32][page_size] f16
+ * with codes as code + 8 in 4 bits, the first in the lowest bits of its word: page_size *
+ * (head_dim + head_dim / 8) bytes per kv head. Position p of sequence s is slot p % page_size of
+ * page table[s * max_pages + p / page_size]. An entry that is not below `pages` is no page: rows
+ * there are not stored, are read as zeros and are not attended to.
+ *
+ * Where several sequences' rows are packed one sequence after another, offsets[sequences + 1] (device
+ * memory, ascending) says where: sequence s has rows offsets[s] .. offsets[s + 1]. Rows outside
+ * them are neither read nor written. All tables, offsets, starts and lengths are read on the
+ * device when the launch runs, so a captured graph follows them. */
+
+/* Element types of rows. */
+typedef enum eg_element { EG_ELEMENT_F32 = 0, EG_ELEMENT_F16 = 1, EG_ELEMENT_BF16 = 2 } eg_element;
+
+typedef struct eg_kv4_dims {
+  uint32_t kv_heads, head_dim;   /* head_dim 64 or 128                                          */
+  uint32_t page_size, pages;     /* page_size 32, 64, 128 or 256                                */
+  uint64_t page_stride;          /* bytes from page to page: a multiple of 16, >= a page's      */
+  uint32_t sequences, max_pages; /* the page table is [sequences][max_pages]                    */
+} eg_kv4_dims;
+
+/* Bytes of one layer's page (kv_heads, head_dim and page_size of dims). */
+EG_API int eg_kv4_page_bytes(const eg_kv4_dims* dims, uint64_t* out_bytes);
+
+/* A batch's new rows into the cache. Row r of sequence s is at position starts[s] + r - offsets[s];
+ * no two rows of a call share a position of a page. With `rope` ([rope_positions][head_dim / 2]
+ * pairs (cos, sin) of f32) q and k are rotated by their position's row in half-rotation pairing,
+ * each product rounded on its own; k (rotated) and v go into the pages. The outputs are packed rows
+ * in out_type: q_out [rows][heads][head_dim] (q rotated), k_out and v_out [rows][kv_heads][head_dim]
+ * (k rotated, v as it is: unquantized). q and q_out go together and may be NULL, k_out and v_out each may be;
+ * rope may be NULL (no rotation). A row whose position the table or the rope does not reach is
+ * skipped: nothing of it is written. Positions of a page that no row names keep their values. */
+typedef struct eg_kv4_append_dims {
+  uint32_t rows, heads;                  /* rows of q, k and v; query heads (0 without q)        */
+  uint32_t q_stride, k_stride, v_stride; /* elements from row to row, multiples of 4; 0: dense   */
+  uint32_t rope_positions;
+  int in_type, out_type; /* eg_element of q, k, v and of the outputs                             */
+} eg_kv4_append_dims;
+EG_API int eg_kv4_append(eg_context* ctx, const void* q, const void* k, const void* v, const float* rope,
+                         const uint32_t* offsets, const uint32_t* starts, const uint32_t* table, void* pool,
+                         void* q_out, void* k_out, void* v_out, const eg_kv4_dims* dims,
+                         const eg_kv4_append_dims* append);
+
+/* Cached rows as packed rows of out_type: k_out and v_out [rows][kv_heads][head_dim], row r of
+ * sequence s the values at position starts[s] + r - offsets[s] (zeros where the table has no page). */
+EG_API int eg_kv4_read(eg_context* ctx, const uint32_t* offsets, const uint32_t* starts, const uint32_t* table,
+                       const void* pool, void* k_out, void* v_out, uint32_t rows, int out_type,
+                       const eg_kv4_dims* dims);
+
+/* Pages copied within the pool, page_stride bytes each (all layers): pair i copies page
+ * pairs[2 i] to page pairs[2 i + 1] (device memory). A pair with a page not below `pages` is
+ * skipped. No page may be the target of two pairs, or the source of one and the target of another. */
+EG_API int eg_kv4_copy_pages(eg_context* ctx, void* pool, const uint32_t* pairs, uint32_t count,
+                             const eg_kv4_dims* dims);
+
+/* Attention of one token per sequence over the cache: out[s][h] = sum_j p_j V[j] / sum_j p_j, p_j =
+ * exp(scale q[s][h] . K[j] - max), j < lengths[s] (at most max_pages * page_size), head h reading kv
+ * head h / (heads / kv_heads). A sequence with no position to attend to gives zeros. q and out are [sequences][heads]
+ * [head_dim] of `type`; sums and softmax statistics are f32; for EG_ELEMENT_F32 q and the
+ * softmax weights enter the matrix products as two f16 each (22 bits), for the others as one. A
+ * long cache is split over workgroups whose partials meet in the context's workspace. */
+typedef struct eg_attention_kv4_dims {
+  uint32_t heads;
+  uint32_t q_stride, out_stride; /* elements from sequence to sequence, multiples of 8; 0: dense */
+  int type;                      /* eg_element of q and out                                      */
+  float scale;                   /* 0: 1 / sqrt(head_dim)                                        */
+} eg_attention_kv4_dims;
+EG_API int eg_attention_decode_kv4(eg_context* ctx, const void* q, const uint32_t* lengths, const uint32_t* table,
+                                   const void* pool, void* out, const eg_kv4_dims* dims,
+                                   const eg_attention_kv4_dims* attention);
+
+/* Causal attention over packed sequences: sequence s has queries q_offsets[s] .. q_offsets[s + 1] of
+ * q and keys k_offsets[s] .. k_offsets[s + 1] of k and v, aligned at their ends: query i of nq sees
+ * keys j <= nk - nq + i of nk (nk = nq: a whole prompt; nk > nq: a chunk after earlier rows). A
+ * query that sees no key gives zeros. Matrix products of f16 or bf16 operands with f32 sums, the
+ * softmax in f32, its weights rounded to the operands' type. */
+typedef struct eg_attention_packed_dims {
+  uint32_t sequences, rows, key_rows; /* rows of q and out, of k and v                           */
+  uint32_t heads, kv_heads, head_dim; /* head_dim 64 or 128                                      */
+  uint32_t q_stride, k_stride, v_stride, out_stride; /* elements, multiples of 8; 0: dense       */
+  int type, out_type; /* EG_ELEMENT_F16 or _BF16; out: the same, or EG_ELEMENT_F32               */
+  float scale;        /* 0: 1 / sqrt(head_dim)                                                   */
+} eg_attention_packed_dims;
+EG_API int eg_attention_packed(eg_context* ctx, const void* q, const void* k, const void* v,
+                               const uint32_t* q_offsets, const uint32_t* k_offsets, void* out,
+                               const eg_attention_packed_dims* dims);
+
 /* ---- the .enargeia container (enargeia.ts:1-50, 112-240; WeightStore.loadQuantized,
  * weights.ts:299-471) ------------------------------------------------------------------------
  * eg_container_open parses the prefix and JSON header on the host and applies the reference's

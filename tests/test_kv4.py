@@ -1,0 +1,114 @@
+"""The 4-bit cache's format and the host's bookkeeping of its pages, without a GPU."""
+
+import numpy as np
+import pytest
+
+from enargeia_amd import kv4
+from enargeia_amd._lib import EgError, EgRangeError
+from kv4_reference import Pages, held, quantize, random_pages, scale_of
+
+
+def test_page_bytes():
+    assert kv4.page_bytes(2, 64, 64) == 2 * 64 * 72
+    assert kv4.page_bytes(8, 128, 256) == 8 * 256 * 144
+
+
+def test_values_are_exact_in_f16_and_within_half_a_step():
+    rng = np.random.default_rng(1)
+    for spread in (1e-6, 1e-3, 1.0, 300.0, 6e4):
+        x = np.asarray(rng.standard_normal((500, 64)) * spread, np.float32)
+        y = held(x)
+        assert np.array_equal(y, y.astype(np.float16).astype(np.float64))
+        s = scale_of(np.abs(x.reshape(500, 2, 32)).max(-1)).astype(np.float64)
+        off = np.abs(y - x).reshape(500, 2, 32)
+        # a code is at most half a step off, and one clamped at 7 by what the scale was rounded down:
+        # half a step of 8 significant bits (2^-8) of absmax = 7 steps, within half a step
+        # (values over 65408 saturate)
+        inside = np.abs(x).reshape(500, 2, 32) <= 65408
+        assert np.all((off <= 0.5001 * s[..., None] + 2.0 ** -19)[inside])
+
+
+def test_not_finite_groups_are_nan():
+    x = np.ones((1, 64), np.float32)
+    x[0, 3] = np.inf
+    assert np.isnan(held(x)[0, :32]).all() and np.array_equal(held(x)[0, 32:], held(np.ones((1, 64), np.float32))[0, 32:])
+
+
+def test_reference_places_what_it_reads():
+    rng = np.random.default_rng(2)
+    for d, page in ((64, 32), (128, 64)):
+        P, k, v = random_pages(rng, 3, 2, d, page)
+        Q = Pages(3, 2, d, page, fill=0xA5)
+        for p in range(3):
+            for slot in range(page):
+                for h in range(2):
+                    got = P.get(p, slot, h)
+                    assert np.array_equal(got[0], k[p, slot, h]) and np.array_equal(got[1], v[p, slot, h])
+                    Q.put(p, slot, h, k[p, slot, h], v[p, slot, h])
+        c, _ = quantize(np.asarray(k, np.float32))
+        assert c.min() >= 1 and c.max() <= 15
+        for p, slot, h in ((0, 0, 0), (2, page - 1, 1), (1, 13, 0)):
+            assert np.array_equal(Q.get(p, slot, h)[0], held(np.asarray(k[p, slot, h], np.float32)))
+
+
+def test_pages_grow_fork_free_compact():
+    t = kv4.PageTable(8, 32)
+    a = t.create()
+    assert t.grow(a, 40) == 0 and t.held[a] == [0, 1] and t.free_pages == 6
+    b = t.fork(a)  # one whole page shared, the partial one copied
+    assert t.held[b] == [0, 2] and t.users[:3] == [2, 1, 1]
+    c = t.fork(b)  # the copy is still pending: from where its rows come
+    assert t.copies == [(1, 2), (1, 3)] and t.users[0] == 3
+    t.free(a)
+    assert t.users[:4] == [2, 0, 1, 1]
+    d = t.create()
+    t.grow(d, 1)
+    assert t.held[d] == [4]  # not page 1: it is still to be copied from
+    assert np.array_equal(t.take_copies(), np.array([[1, 2], [1, 3]], np.uint32)) and t.copies == []
+    assert t.grow(b, 60) == 40 and t.held[b] == [0, 2, 1, 5]
+    t.free(d)
+    t.free(b)
+    assert t.compact() == 2 and t.held[c] == [0, 1]
+    assert np.array_equal(t.take_copies(), np.array([[3, 1]], np.uint32))
+    assert t.free_pages == 6 and t.users[:3] == [1, 1, 0]
+    assert np.array_equal(t.table([c], 3), np.array([[0, 1, kv4.NO_PAGE]], np.uint32))
+    assert t.lengths([c])[0] == 40
+
+
+def test_whole_pages_fork_without_a_copy():
+    t = kv4.PageTable(4, 32)
+    a = t.create()
+    t.grow(a, 64)
+    b = t.fork(a)
+    assert t.held[b] == t.held[a] and t.copies == []
+    t.grow(a, 1)
+    t.grow(b, 1)
+    assert t.held[a][2] != t.held[b][2]
+
+
+def test_page_table_refusals():
+    t = kv4.PageTable(2, 32)
+    a = t.create()
+    with pytest.raises(EgRangeError, match="3 pages wanted, 2 of 2 free"):
+        t.grow(a, 65)
+    assert t.lengths([a])[0] == 0 and t.held[a] == [] and t.free_pages == 2
+    t.grow(a, 33)
+    with pytest.raises(EgRangeError, match="1 pages wanted, 0 of 2 free"):
+        t.fork(a)
+    assert t.users == [1, 1]
+    with pytest.raises(EgRangeError, match="has 2 pages, the table 1"):
+        t.table([a], 1)
+    with pytest.raises(EgError, match="page_size 48"):
+        kv4.PageTable(2, 48)
+    t.free(a)
+    b = t.create()
+    t.grow(b, 3)
+    t.fork(b)
+    with pytest.raises(EgError, match="copies of forks are pending"):
+        t.compact()
+
+
+def test_element_types_have_names():
+    with pytest.raises(EgError, match="element type 'f8'"):
+        kv4.attention_packed(None, 0, 0, 0, 0, 0, 0, sequences=1, rows=1, key_rows=1, heads=1, kv_heads=1,
+                             head_dim=64, type="f8")
