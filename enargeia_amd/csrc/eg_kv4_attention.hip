@@ -14,7 +14,8 @@
 //
 // K codes go into the first product as they are: four bits at the bottom of an f16 are a denormal,
 // code * 2^-24 (2^-20 for the nibble above, whose queries are divided by 16), which the matrix cores
-// multiply exactly. A group of 32 dims is one product's depth, so its accumulator, started at -8 times
+// multiply exactly. (For f32 rows as code - 8 in f16, 9 instructions per word: what the sum and its start
+// at -8 times the queries leave of each other is off by 2e-6 of the result, these by 2e-7.) A group of 32 dims is one product's depth, so its accumulator, started at -8 times
 // the sum of the queries, is sum q (code - 8), and the scale is applied to it: 5 vector instructions
 // per word of 8 codes. V's scale differs along the second product's depth, so V is dequantized: (1024 +
 // code) - 1032 in f16, times the scale - exact by the format - 13 instructions per word.
@@ -35,6 +36,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 using egd::u32x4;
 
 constexpr uint32_t kThreads = 256, kWaves = 4;
+constexpr uint64_t kInfinityCache = 256u << 20;  // bytes
 constexpr float kLog2e = 1.44269504088896340736f;
 // slot of an 8-deep operand -> nibble of a word, as the two masks below deliver them
 constexpr uint32_t kOrder[8] = {0, 4, 1, 5, 2, 6, 3, 7};
@@ -70,20 +72,39 @@ __device__ __forceinline__ half8 as_half8(uint32_t a, uint32_t b, uint32_t c, ui
 __device__ __forceinline__ half2v halves(uint32_t v) { return __builtin_bit_cast(half2v, v); }
 __device__ __forceinline__ uint32_t bits(half2v v) { return __builtin_bit_cast(uint32_t, v); }
 
-// 8 codes as the matrix cores take them: slots 0, 1, 4, 5 code * 2^-24, slots 2, 3, 6, 7 code * 2^-20.
-__device__ __forceinline__ half8 codes(uint32_t w) {
+// Bits put over four of a word's nibbles: one v_and_or_b32 where they are in a register (as a literal,
+// beside the mask, they take an instruction of their own).
+struct Magic {
+  uint32_t lo, hi;  // f16 1024 (a nibble at the bottom: 1024 + code), f16 64 (the next one: 64 + code)
+};
+__device__ __forceinline__ Magic magic() {
+  Magic m{0x64006400u, 0x54005400u};
+  asm("" : "+v"(m.lo), "+v"(m.hi));
+  return m;
+}
+
+// 8 codes as the first product takes them: slots 0, 1, 4, 5 code * 2^-24, slots 2, 3, 6, 7 code * 2^-20
+// (code is value + 8 here); or, kSigned, the values -7 .. 7 themselves.
+template <bool kSigned>
+__device__ __forceinline__ half8 codes(uint32_t w, const Magic& m) {
   const uint32_t y = w >> 8;
-  return as_half8(w & 0x000F000Fu, w & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u);
+  if constexpr (kSigned) {
+    const half2v lo = {(_Float16)-1032.f, (_Float16)-1032.f}, hi = {(_Float16)-72.f, (_Float16)-72.f};
+    return as_half8(bits(halves((w & 0x000F000Fu) | m.lo) + lo), bits(halves((w & 0x00F000F0u) | m.hi) + hi),
+                    bits(halves((y & 0x000F000Fu) | m.lo) + lo), bits(halves((y & 0x00F000F0u) | m.hi) + hi));
+  } else {
+    return as_half8(w & 0x000F000Fu, w & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u);
+  }
 }
 
 // 8 codes of one dim at 8 positions, times the positions' scales (pairs in kOrder's order).
-__device__ __forceinline__ half8 values(uint32_t w, const half2v (&s)[4]) {
+__device__ __forceinline__ half8 values(uint32_t w, const half2v (&s)[4], const Magic& m) {
   const uint32_t y = w >> 8;
   const half2v lo = {(_Float16)-1032.f, (_Float16)-1032.f}, hi = {(_Float16)-72.f, (_Float16)-72.f};
-  const half2v a = (halves((w & 0x000F000Fu) | 0x64006400u) + lo) * s[0];  // 1024 + code
-  const half2v b = (halves((w & 0x00F000F0u) | 0x54005400u) + hi) * s[1];  // 64 + code
-  const half2v c = (halves((y & 0x000F000Fu) | 0x64006400u) + lo) * s[2];
-  const half2v d = (halves((y & 0x00F000F0u) | 0x54005400u) + hi) * s[3];
+  const half2v a = (halves((w & 0x000F000Fu) | m.lo) + lo) * s[0];  // 1024 + code
+  const half2v b = (halves((w & 0x00F000F0u) | m.hi) + hi) * s[1];  // 64 + code
+  const half2v c = (halves((y & 0x000F000Fu) | m.lo) + lo) * s[2];
+  const half2v d = (halves((y & 0x00F000F0u) | m.hi) + hi) * s[3];
   return as_half8(bits(a), bits(b), bits(c), bits(d));
 }
 
@@ -111,9 +132,15 @@ __device__ __forceinline__ u32x4 first_halves(u32x4 v, int n) {
 // tile lane / 8 % 2: each tile's product has zeros in the other's columns, both add into the same
 // accumulators, and the softmax of two tiles costs one's instructions - for groups of up to 8 heads, where half
 // of the columns would be empty. T = 1: 16 heads. kParts: f16 parts of a query and of a weight.
-template <int D, int T, int kParts, class TQ>
-__global__ __launch_bounds__(256) void decode_kernel(Args a, Pool pool) {
+// (Two waves per SIMD: their registers hold two steps' operands each, one step's loads under way while
+// the other is multiplied.)
+// kStream: codes are read past the caches' retention (non-temporal), for a cache larger than the Infinity
+// Cache: 32 sequences of 16384 (32 / 8 heads of 128) 96.9 us for 106.6, but 16 of up to 8192 27.3 for 25.7.
+template <int D, int T, int kParts, bool kStream, class TQ>
+__global__ __launch_bounds__(256, 2) void decode_kernel(Args a, Pool pool) {
   constexpr int kGroups = D / 32, kBlocks = D / 16;  // dim groups of K; blocks of 16 dims of O^T
+  constexpr bool kSigned = kParts == 2;
+  constexpr int kAux = kStream ? egd::kNonTemporal : 0;
   constexpr uint32_t kTile = 32 * T, kHeads = 16 / T;
   constexpr int kVWords = D / 16;  // V words of a lane: its dims D / 16 * (lane % 16) + 0 ..
   const uint32_t tid = threadIdx.x, lane = tid & 63u;
@@ -132,6 +159,7 @@ __global__ __launch_bounds__(256) void decode_kernel(Args a, Pool pool) {
   const uint32_t begin = split * chunk, end = min(length, begin + chunk);
   if (split != 0 && begin >= length) return;
   const uint32_t heads = min(kHeads, a.group - ht * kHeads), head0 = kv * a.group + ht * kHeads;
+  const Magic bits_over = magic();
 
   const uint32_t page_size = 1u << pool.page_shift;
   const Layout at = layout<D>(page_size);
@@ -160,18 +188,18 @@ __global__ __launch_bounds__(256) void decode_kernel(Args a, Pool pool) {
       for (int n = 0; n < 2; n++) {  // positions 2 apart: kOrder[4 + e] = kOrder[e] + 2
         const uint32_t o = k_row0 + 2 * n * (D / 2);
         if constexpr (kGroups == 2) {
-          const uint64_t w = egd::load_b64(r, o, s * (D / 2));
-          t.k[i][n][0] = (uint32_t)w;
-          t.k[i][n][1] = (uint32_t)(w >> 32);
+          const auto w = __builtin_amdgcn_raw_buffer_load_b64(r, o, s * (D / 2), kAux);
+          t.k[i][n][0] = w[0];
+          t.k[i][n][1] = w[1];
         } else {
-          const u32x4 w = egd::load_b128(r, o, s * (D / 2));
+          const u32x4 w = egd::load_b128_p<kAux>(r, o, s * (D / 2));
 #pragma unroll
           for (int g = 0; g < kGroups; g++) t.k[i][n][g] = w[g];
         }
       }
 #pragma unroll
       for (int j = 0; j < kVWords; j += 4) {
-        const u32x4 w = egd::load_b128(r, v_off + 4 * j, (s / 8) * (D * 4));
+        const u32x4 w = egd::load_b128_p<kAux>(r, v_off + 4 * j, (s / 8) * (D * 4));
 #pragma unroll
         for (int e = 0; e < 4; e++) t.v[i][j + e] = w[e];
       }
@@ -181,22 +209,18 @@ __global__ __launch_bounds__(256) void decode_kernel(Args a, Pool pool) {
     for (int g = 0; g < kGroups; g++) t.ks[g] = egd::load_b128(r, ks_off, ((g << pool.page_shift) + slot) * 2);
   };
 
-  // The pages of this wave's next 64 steps, one a lane.
-  const uint32_t steps = begin < end ? (end - begin + kTile - 1) / kTile : 0;  // of the chunk
+  const uint32_t steps = begin < end ? (end - begin + kTile - 1) / kTile : 0;
+  const uint32_t mine = steps > wave ? (steps - wave + kWaves - 1) / kWaves : 0;  // steps of this wave
+  // The pages of this wave's next 64 steps, one a lane, from its step i0 on.
   const auto pages_of = [&](uint32_t i0) {
     const uint32_t step = wave + kWaves * (i0 + lane);
     return step < steps ? pool.page_of(seq, begin + step * kTile) : 0xFFFFFFFFu;
   };
-  const uint32_t mine = steps > wave ? (steps - wave + kWaves - 1) / kWaves : 0;  // steps of this wave
-  uint32_t ids = pages_of(0);
-  const auto fetch = [&](Tile& t, uint32_t i) {
-    if (i >= mine) return;
-    if (i != 0 && i % 64 == 0) ids = pages_of(i);
-    load(t, (uint32_t)__builtin_amdgcn_readlane((int)ids, (int)(i % 64)),
-         (begin + (wave + kWaves * i) * kTile) & (page_size - 1u));
+  const auto fetch = [&](Tile& t, uint32_t ids, uint32_t i0, uint32_t i) {
+    load(t, (uint32_t)__builtin_amdgcn_readlane((int)ids, (int)i),
+         (begin + (wave + kWaves * (i0 + i)) * kTile) & (page_size - 1u));
   };
-  Tile tiles[2];
-  fetch(tiles[0], 0);
+  uint32_t ids = pages_of(0);
 
   // The queries, B operand: lane group g has dims 32 grp + 8 g + kOrder[slot] of head `col`.
   half8 qf[T][kGroups][kParts];
@@ -207,16 +231,21 @@ __global__ __launch_bounds__(256) void decode_kernel(Args a, Pool pool) {
     const bool in = col < heads;
     const TQ* src = static_cast<const TQ*>(a.q) + (size_t)seq * a.q_stride + (size_t)(head0 + (in ? col : 0)) * D;
 #pragma unroll
-    for (int g = 0; g < kGroups; g++)
+    for (int g = 0; g < kGroups; g++) {
+      struct alignas(16) Eight {
+        TQ v[8];
+      };
+      const Eight e = *reinterpret_cast<const Eight*>(src + 32 * g + 8 * lg);
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        x[g][i] = in ? to_f32(src[32 * g + 8 * lg + kOrder[i]]) : 0.f;
+        x[g][i] = in ? to_f32(e.v[kOrder[i]]) : 0.f;
         top = fmaxf(top, fabsf(x[g][i]));
       }
+    }
     top = max_of_head(top);
     int e = top > 0.f ? 14 - ((int)(__float_as_uint(top) >> 23) - 127) : 0;
     e = max(-100, min(110, e));
-    f = ldexpf(a.scale, 24 - e);
+    f = ldexpf(a.scale, kSigned ? -e : 24 - e);
 #pragma unroll
     for (int g = 0; g < kGroups; g++) {
       half8 part[kParts];
@@ -227,14 +256,14 @@ __global__ __launch_bounds__(256) void decode_kernel(Args a, Pool pool) {
         for (int p = 0; p < kParts; p++) {
           const _Float16 h = (_Float16)y;
           y -= (float)h;
-          part[p][i] = (i & 2) ? h * (_Float16)0.0625f : h;
+          part[p][i] = !kSigned && (i & 2) ? h * (_Float16)0.0625f : h;
         }
       }
       const half8 eight = as_half8(0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u);
       start[g] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int p = 0; p < kParts; p++) {
-        start[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(eight, part[p], start[g], 0, 0, 0);
+        if constexpr (!kSigned) start[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(eight, part[p], start[g], 0, 0, 0);
 #pragma unroll
         for (int i = 0; i < T; i++)
           qf[i][g][p] = T == 1 || half == (uint32_t)i ? part[p] : half8{0, 0, 0, 0, 0, 0, 0, 0};
@@ -258,7 +287,7 @@ __global__ __launch_bounds__(256) void decode_kernel(Args a, Pool pool) {
         f32x4 acc = start[g];
 #pragma unroll
         for (int b = 0; b < T; b++) {
-          const half8 kc = codes(t.k[b][n][g]);
+          const half8 kc = codes<kSigned>(t.k[b][n][g], bits_over);
 #pragma unroll
           for (int p = 0; p < kParts; p++) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, qf[b][g][p], acc, 0, 0, 0);
         }
@@ -314,19 +343,27 @@ __global__ __launch_bounds__(256) void decode_kernel(Args a, Pool pool) {
         w[k] = T == 1 || half == (uint32_t)b ? pb[k] : half8{0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
       for (int n = 0; n < kBlocks; n++) {
-        const half8 va = values(t.v[b][n], pairs);
+        const half8 va = values(t.v[b][n], pairs, bits_over);
 #pragma unroll
         for (int k = 0; k < kParts; k++) o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, w[k], o[n], 0, 0, 0);
       }
     }
   };
 
-  for (uint32_t i = 0; i < mine; i += 2) {
-    fetch(tiles[1], i + 1);
-    compute(tiles[0], i);
-    if (i + 1 < mine) {
-      fetch(tiles[0], i + 2);
-      compute(tiles[1], i + 1);
+  // (The page ids are read outside the loop over their 64 steps: a wait for them inside would be a wait
+  // for the tiles under way.)
+  for (uint32_t i0 = 0; i0 < mine; i0 += 64) {
+    if (i0) ids = pages_of(i0);
+    const uint32_t n = min(64u, mine - i0);
+    Tile tiles[2];
+    fetch(tiles[0], ids, i0, 0);
+    for (uint32_t i = 0; i < n; i += 2) {
+      if (i + 1 < n) fetch(tiles[1], ids, i0, i + 1);
+      compute(tiles[0], i0 + i);
+      if (i + 1 < n) {
+        if (i + 2 < n) fetch(tiles[0], ids, i0, i + 2);
+        compute(tiles[1], i0 + i + 1);
+      }
     }
   }
 
@@ -413,14 +450,14 @@ __global__ __launch_bounds__(256) void join_kernel(Args a) {
   }
 }
 
-template <int D, class TQ>
-void launch(eg_context* ctx, const Args& a, const Pool& p, bool pair, uint64_t blocks) {
+template <int D, int T, class TQ>
+void launch(eg_context* ctx, const Args& a, const Pool& p, bool stream, uint64_t blocks) {
   constexpr int kParts = std::is_same<TQ, float>::value ? 2 : 1;
-  const dim3 grid((uint32_t)blocks);
-  if (pair) hipLaunchKernelGGL((decode_kernel<D, 2, kParts, TQ>), grid, dim3(kThreads), 0, ctx->stream, a, p);
-  else hipLaunchKernelGGL((decode_kernel<D, 1, kParts, TQ>), grid, dim3(kThreads), 0, ctx->stream, a, p);
+  const dim3 grid((uint32_t)blocks), threads(kThreads);
+  if (stream) hipLaunchKernelGGL((decode_kernel<D, T, kParts, true, TQ>), grid, threads, 0, ctx->stream, a, p);
+  else hipLaunchKernelGGL((decode_kernel<D, T, kParts, false, TQ>), grid, threads, 0, ctx->stream, a, p);
   if (a.splits > 1)
-    hipLaunchKernelGGL((join_kernel<D, TQ>), dim3(p.sequences * a.heads), dim3(kThreads), 0, ctx->stream, a);
+    hipLaunchKernelGGL((join_kernel<D, TQ>), dim3(p.sequences * a.heads), threads, 0, ctx->stream, a);
 }
 
 }  // namespace
@@ -459,11 +496,16 @@ extern "C" int eg_attention_decode_kv4(eg_context* ctx, const void* q, const uin
   // Two key tiles a step where the heads leave room for them (and a step's 64 positions lie in one page).
   const bool pair = a.group <= 8 && dims->page_size >= 64;
   a.head_tiles = pair ? 1 : (a.group + 15) / 16;
-  a.min_chunk = pair ? 256 : 128;
+  // Splits: as many as the device holds at once (two workgroups per CU), of at least min_chunk positions, and
+  // none for tables that reach 1024. A workgroup's first loads wait for each other (length, page, rows) and
+  // the join is a launch, so more and shorter chunks cost more than they balance: 16 sequences of up to
+  // 8192 (28 / 4 heads of 128, f32) 28.9 us in 512 workgroups, 39.4 in 1024; 48 of 2048 (14 / 2 of 64) 11.2
+  // in chunks of 512, 13.1 in 256, 13.9 in 1024; 4 of 65536 (16 / 1 of 128, f16) 19.9 in chunks of 1024, 23.0 in
+  // 512; 1 of 517 6.8 whole, 9.0 in two (the second launch).
+  a.min_chunk = pair ? 512 : 1024;
   const uint64_t rows = (uint64_t)dims->sequences * dims->kv_heads * a.head_tiles;
-  const uint64_t target = (uint64_t)ctx->cu_count * 8;
-  uint64_t splits = std::max<uint64_t>(1, std::min<uint64_t>((target + rows - 1) / rows,
-                                                             (a.capacity + a.min_chunk - 1) / a.min_chunk));
+  const uint64_t room = 2ull * ctx->cu_count / rows, most = (a.capacity + a.min_chunk - 1) / a.min_chunk;
+  uint64_t splits = a.capacity <= 1024 ? 1 : std::max<uint64_t>(1, std::min(room, most));
   const uint64_t per_split = (uint64_t)dims->sequences * d.heads * (dims->head_dim + 2) * 4;
   splits = std::max<uint64_t>(1, std::min<uint64_t>(splits, (eg::kPartialsBytes - 64) / per_split));
   a.splits = (uint32_t)splits;
@@ -472,9 +514,16 @@ extern "C" int eg_attention_decode_kv4(eg_context* ctx, const void* q, const uin
   a.ml = reinterpret_cast<float*>(eg::partials(ctx));
   a.o = a.ml + (((size_t)dims->sequences * d.heads * splits * 2 + 3) & ~(size_t)3);
   const Pool p = eg_kv4::pool_of(*dims, pool, table);
+  // The most that the call can read: what the tables reach, and what the pool holds.
+  const uint64_t reach = std::min<uint64_t>((uint64_t)dims->sequences * dims->max_pages, dims->pages) * eg_kv4::page_bytes(*dims);
+  const bool stream = reach > kInfinityCache;
   with_type(d.type, [&](auto t) {
-    if (dims->head_dim == 64) launch<64, decltype(t)>(ctx, a, p, pair, rows * splits);
-    else launch<128, decltype(t)>(ctx, a, p, pair, rows * splits);
+    using TQ = decltype(t);
+    const uint64_t blocks = rows * splits;
+    if (dims->head_dim == 64)
+      pair ? launch<64, 2, TQ>(ctx, a, p, stream, blocks) : launch<64, 1, TQ>(ctx, a, p, stream, blocks);
+    else
+      pair ? launch<128, 2, TQ>(ctx, a, p, stream, blocks) : launch<128, 1, TQ>(ctx, a, p, stream, blocks);
   });
   return eg::check_launch(ctx, op);
 }
