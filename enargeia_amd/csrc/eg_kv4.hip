@@ -1,11 +1,11 @@
 // The paged 4-bit cache (enargeia_hip.h): rows appended, rows read back, pages copied. All three move
 // bytes: their floor is what they read and write once at the memory's rate.
 //
-// Append and read go by blocks of 8 positions of a page: a V code word holds 8 positions of one dim,
-// so a block's V words are written by one wave from its 8 rows, whole - or, where the batch has only
-// some of the 8, merged into what is there (one wave per block and kv head: no race). Packed rows
+// Append and read go by blocks of positions of a page (8, or 32): a V code word holds 8 positions of one
+// dim, so a block's V words are written by one wave from its 8 rows, whole - or, where the batch has
+// only some of the 8, merged into what is there (one wave per block and kv head: no race). Packed rows
 // and blocks do not align, so a wave that owns `span` packed rows takes the blocks whose first row
-// of this call lies among them, up to 7 rows past its span.
+// of this call lies among them, rows past its span included.
 #include <algorithm>
 
 #include "eg_kv4.hpp"
@@ -16,9 +16,9 @@ using namespace eg_kv4;
 
 constexpr uint32_t kThreads = 256;
 
-// The runs of rows that lie in one 8-position block, for the packed rows [r0, r0 + span):
+// The runs of rows that lie in one block of kBlock positions, for the packed rows [r0, r0 + span):
 // f(sequence, first row, its position, rows).
-template <class F>
+template <uint32_t kBlock, class F>
 __device__ __forceinline__ void for_blocks(const uint32_t* offsets, const uint32_t* starts, uint32_t sequences,
                                            uint32_t rows, uint32_t r0, uint32_t span, F&& f) {
   uint32_t r = r0, seq = 0, first = 0, end = 0, start = 0;
@@ -35,8 +35,8 @@ __device__ __forceinline__ void for_blocks(const uint32_t* offsets, const uint32
       have = true;
       start = starts[seq];
     }
-    const uint32_t position = start + (r - first), in_block = position & 7u;
-    const uint32_t n = min(min(8u - in_block, end - r), rows - r);
+    const uint32_t position = start + (r - first), in_block = position & (kBlock - 1u);
+    const uint32_t n = min(min(kBlock - in_block, end - r), rows - r);
     if (in_block == 0 || r == first) f(seq, r, position, n);
     r += n;
   }
@@ -82,31 +82,131 @@ struct AppendArgs {
   const float2* rope;
   const uint32_t *offsets, *starts;
   void *q_out, *k_out, *v_out;
-  uint32_t rows, heads, q_stride, k_stride, v_stride, rope_positions, span;
+  uint32_t rows, heads, q_stride, k_stride, v_stride, rope_positions;
+  uint32_t span, q_span, kv_groups;  // packed rows per wave, per workgroup of queries; workgroups of kv heads
 };
 
-// A wave per (span of packed rows, kv head's K, kv head's V or query head). A lane holds dim `lane`
-// of up to 8 rows (and dim lane + 64 at head_dim 128), all read at once. Bound by latency where the
-// rows are few, by memory where they are many.
+// The positions of rows r0 + lane (kNowhere for those of no sequence).
+constexpr uint32_t kNowhere = 0xFFFFFFFFu;
+__device__ __forceinline__ uint32_t position_of(const uint32_t* offsets, const uint32_t* starts, uint32_t sequences,
+                                                uint32_t r) {
+  uint32_t lo = 0, hi = sequences + 1, first = 0;  // offsets[lo - 1] <= r < offsets[hi], as far as known
+  if (sequences < 64) {  // all offsets in the wave's lanes
+    const uint32_t mine = offsets[min(threadIdx.x & 63u, sequences)];
+    while (__ballot(lo < hi)) {
+      const uint32_t mid = (lo + hi) / 2, v = (uint32_t)__shfl((int)mine, (int)min(mid, sequences), 64);
+      if (lo < hi) {
+        if (v <= r) {
+          lo = mid + 1;
+          first = v;
+        } else {
+          hi = mid;
+        }
+      }
+    }
+  } else {
+    while (lo < hi) {
+      const uint32_t mid = (lo + hi) / 2, v = offsets[mid];
+      if (v <= r) {
+        lo = mid + 1;
+        first = v;
+      } else {
+        hi = mid;
+      }
+    }
+  }
+  return lo == 0 || lo > sequences ? kNowhere : starts[lo - 1] + (r - first);
+}
+
+// 4 consecutive elements.
+template <class T>
+__device__ __forceinline__ float4 load4(const T* p) {
+  if constexpr (std::is_same<T, float>::value) {
+    return *reinterpret_cast<const float4*>(p);
+  } else {
+    struct alignas(8) Four {
+      T v[4];
+    };
+    const Four f = *reinterpret_cast<const Four*>(p);
+    return make_float4(to_f32(f.v[0]), to_f32(f.v[1]), to_f32(f.v[2]), to_f32(f.v[3]));
+  }
+}
+template <class T>
+__device__ __forceinline__ void store4(T* p, float4 v) {
+  if constexpr (std::is_same<T, float>::value) {
+    *reinterpret_cast<float4*>(p) = v;
+  } else {
+    struct alignas(8) Four {
+      T v[4];
+    };
+    *reinterpret_cast<Four*>(p) = Four{{from_f32<T>(v.x), from_f32<T>(v.y), from_f32<T>(v.z), from_f32<T>(v.w)}};
+  }
+}
+
+// The queries of `rows` packed rows from r0 on, rotated: a thread has 4 dims of a head's first half and the
+// 4 of its second that pair with them. A row is skipped where its position is out of reach.
+template <int D, class TI, class TO>
+__device__ __forceinline__ void rotate_queries(const AppendArgs& a, const Pool& pool, uint32_t r0, uint32_t rows) {
+#pragma clang fp contract(off)
+  constexpr uint32_t kQuads = D / 8;
+  __shared__ uint32_t position[64];
+  const uint32_t tid = threadIdx.x;
+  if (tid < 64) {
+    uint32_t p = position_of(a.offsets, a.starts, pool.sequences, r0 + tid);
+    if (p != kNowhere && ((p >> pool.page_shift) >= pool.max_pages || (a.rope && p >= a.rope_positions))) p = kNowhere;
+    position[tid] = p;
+  }
+  __syncthreads();
+  const TI* q = static_cast<const TI*>(a.q);
+  TO* out = static_cast<TO*>(a.q_out);
+  const uint32_t per_row = a.heads * kQuads, items = rows * per_row;
+#pragma unroll 4
+  for (uint32_t i = tid; i < items; i += kThreads) {
+    const uint32_t r = i / per_row, in_row = i % per_row, p = position[r];
+    if (p == kNowhere) continue;
+    const uint32_t quad = in_row % kQuads, at = in_row / kQuads * D + 4 * quad;
+    const TI* src = q + (size_t)(r0 + r) * a.q_stride + at;
+    float4 u = load4(src), w = load4(src + D / 2);
+    if (a.rope) {
+      const float4* cs = reinterpret_cast<const float4*>(a.rope + (size_t)p * (D / 2) + 4 * quad);
+      const float4 x = cs[0], y = cs[1];  // (cos, sin) of two pairs each
+      const float4 s = u;
+      u = make_float4(s.x * x.x - w.x * x.y, s.y * x.z - w.y * x.w, s.z * y.x - w.z * y.y, s.w * y.z - w.w * y.w);
+      w = make_float4(w.x * x.x + s.x * x.y, w.y * x.z + s.y * x.w, w.z * y.x + s.z * y.y, w.w * y.z + s.w * y.w);
+    }
+    TO* to = out + (size_t)(r0 + r) * (a.heads * D) + at;
+    store4(to, u);
+    store4(to + D / 2, w);
+  }
+}
+
+// Workgroups of blockIdx.y < kv_groups: a wave per (span of packed rows, kv head's K or V). A lane holds dim
+// `lane` of up to 8 rows (and dim lane + 64 at head_dim 128), all read at once. The others: the span's
+// queries. Bound by latency where the rows are few, by memory where they are many.
 template <int D, class TI, class TO>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a, Pool pool) {
   constexpr int kPer = D / 64;  // dims per lane
+  const uint32_t kvh = pool.kv_heads;
+  if (blockIdx.y >= a.kv_groups) {
+    const uint32_t r0 = blockIdx.x * a.q_span;
+    if (r0 < a.rows) rotate_queries<D, TI, TO>(a, pool, r0, min(a.q_span, a.rows - r0));
+    return;
+  }
   const uint32_t lane = threadIdx.x & 63u;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t task = blockIdx.y * 4 + wave, kvh = pool.kv_heads;
-  if (task >= 2 * kvh + a.heads) return;
-  const bool is_k = task < kvh, is_v = !is_k && task < 2 * kvh;
-  const uint32_t head = is_k ? task : is_v ? task - kvh : task - 2 * kvh;
-  const TI* src = static_cast<const TI*>(is_k ? a.k : is_v ? a.v : a.q);
-  TO* dst = static_cast<TO*>(is_k ? a.k_out : is_v ? a.v_out : a.q_out);
-  const uint32_t stride = is_k ? a.k_stride : is_v ? a.v_stride : a.q_stride;
-  const uint32_t out_stride = (is_k || is_v ? kvh : a.heads) * D;
+  const uint32_t task = blockIdx.y * 4 + wave;
+  if (task >= 2 * kvh || blockIdx.x * a.span >= a.rows) return;
+  const bool is_k = task < kvh;
+  const uint32_t head = is_k ? task : task - kvh;
+  const TI* src = static_cast<const TI*>(is_k ? a.k : a.v);
+  TO* dst = static_cast<TO*>(is_k ? a.k_out : a.v_out);
+  const uint32_t stride = is_k ? a.k_stride : a.v_stride, out_stride = kvh * D;
   const Layout at = layout<D>(1u << pool.page_shift);
 
-  for_blocks(a.offsets, a.starts, pool.sequences, a.rows, blockIdx.x * a.span, a.span,
-             [&](uint32_t seq, uint32_t row, uint32_t position, uint32_t n) {
-    const uint32_t page = pool.page_of(seq, position);
+  for_blocks<8>(a.offsets, a.starts, pool.sequences, a.rows, blockIdx.x * a.span, a.span,
+                [&](uint32_t seq, uint32_t row, uint32_t position, uint32_t n) {
     if ((position >> pool.page_shift) >= pool.max_pages) return;
+    const uint32_t page = pool.page_of(seq, position);
     if (a.rope) {  // rows that the rope does not reach are skipped
       if (position >= a.rope_positions) return;
       n = min(n, a.rope_positions - position);
@@ -119,10 +219,10 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a, Pool pool) {
 #pragma unroll
       for (int j = 0; j < kPer; j++) x[i][j] = to_f32(src[(size_t)r * stride + head * D + 64 * j + lane]);
       cs[i] = make_float2(1.f, 0.f);
-      if (a.rope && !is_v)
+      if (a.rope && is_k)
         cs[i] = a.rope[(size_t)(position + min(i, n - 1)) * (D / 2) + (D == 64 ? lane & 31u : lane)];
     }
-    if (a.rope && !is_v) {
+    if (a.rope && is_k) {
 #pragma clang fp contract(off)
 #pragma unroll
       for (uint32_t i = 0; i < 8; i++) {
@@ -146,7 +246,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a, Pool pool) {
             dst[(size_t)(row + i) * out_stride + head * D + 64 * j + lane] = from_f32<TO>(x[i][j]);
         }
     }
-    if ((!is_k && !is_v) || page >= pool.pages) return;
+    if (page >= pool.pages) return;
     uint8_t* block = pool.block(page, head, at.head_bytes);
     const uint32_t slot = position & ((1u << pool.page_shift) - 1u), mine = lane & 7u;
 #pragma unroll
@@ -189,11 +289,35 @@ struct ReadArgs {
   uint32_t rows, span;
 };
 
-// A wave per (span of packed rows, kv head's K or V), blocks as in append_kernel. K: a lane dequantizes
-// one word, 8 dims of a row. V: a lane has one dim (two at head_dim 128) of the block's 8 rows.
-template <int D, class TO>
+template <class T>
+__device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
+  if constexpr (std::is_same<T, float>::value) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+  } else {
+    struct alignas(16) Eight {
+      T v[8];
+    };
+    Eight e;
+#pragma unroll
+    for (int i = 0; i < 8; i++) e.v[i] = from_f32<T>(v[i]);
+    *reinterpret_cast<Eight*>(p) = e;
+  }
+}
+template <class T>
+__device__ __forceinline__ void store2(T* p, float a, float b) {
+  struct alignas(2 * sizeof(T)) Two {
+    T v[2];
+  };
+  *reinterpret_cast<Two*>(p) = Two{{from_f32<T>(a), from_f32<T>(b)}};
+}
+
+// A wave per (span of packed rows, kv head's K or V), blocks of kBlock positions. K: a lane dequantizes
+// words, 8 dims of a row each, stored in one. V: a lane has 2 dims (the wave 128: a block's 8 rows, or at
+// head_dim 64 every other one). All of a block's words are read before any value is stored.
+template <int D, uint32_t kBlock, class TO>
 __global__ __launch_bounds__(256) void read_kernel(ReadArgs a, Pool pool) {
-  constexpr uint32_t kGroups = D / 32, kPer = D / 64;
+  constexpr uint32_t kGroups = D / 32, kWords = D / 8;
   const uint32_t lane = threadIdx.x & 63u;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t task = blockIdx.y * 4 + wave, kvh = pool.kv_heads;
@@ -202,8 +326,9 @@ __global__ __launch_bounds__(256) void read_kernel(ReadArgs a, Pool pool) {
   const uint32_t head = is_k ? task : task - kvh;
   TO* dst = static_cast<TO*>(is_k ? a.k_out : a.v_out);
   const Layout at = layout<D>(1u << pool.page_shift);
-  for_blocks(a.offsets, a.starts, pool.sequences, a.rows, blockIdx.x * a.span, a.span,
-             [&](uint32_t seq, uint32_t row, uint32_t position, uint32_t n) {
+  const auto value = [](uint32_t word, uint32_t i, float s) { return (float)((int)((word >> (4 * i)) & 15u) - 8) * s; };
+  for_blocks<kBlock>(a.offsets, a.starts, pool.sequences, a.rows, blockIdx.x * a.span, a.span,
+                     [&](uint32_t seq, uint32_t row, uint32_t position, uint32_t n) {
     const uint32_t page = pool.page_of(seq, position);
     const bool have = page < pool.pages;
     const uint8_t* block = pool.block(have ? page : 0, head, at.head_bytes);
@@ -211,32 +336,48 @@ __global__ __launch_bounds__(256) void read_kernel(ReadArgs a, Pool pool) {
     const uint16_t* scales = reinterpret_cast<const uint16_t*>(block + (is_k ? at.k_scales : at.v_scales));
     TO* out = dst + ((size_t)row * kvh + head) * D;
     if (is_k) {
+      constexpr uint32_t kEach = kBlock * kWords / 64;
+      uint32_t word[kEach];
+      float s[kEach];
+      const uint32_t w = lane % kWords, group = w / 4, part = w % 4;  // dims 8 w .. +8
 #pragma unroll
-      for (uint32_t j = 0; j < kPer; j++) {
-        const uint32_t i = (64 * j + lane) / (D / 8), w = lane % (D / 8);  // row of the block, word of the row
+      for (uint32_t j = 0; j < kEach; j++) {
+        const uint32_t i = min((64 * j + lane) / kWords, n - 1);  // (rows past n: the last one, not stored)
+        word[j] = reinterpret_cast<const uint32_t*>(block)[(slot + i) * kWords + part * kGroups + group];
+        s[j] = egd::half_to_float(scales[(group << pool.page_shift) + slot + i]);
+      }
+#pragma unroll
+      for (uint32_t j = 0; j < kEach; j++) {
+        const uint32_t i = (64 * j + lane) / kWords;
         if (i >= n) continue;
-        uint32_t word = 0x88888888u;
-        float s = 0.f;
-        const uint32_t part = w / kGroups, group = w % kGroups;
-        if (have) {
-          word = reinterpret_cast<const uint32_t*>(block)[(slot + i) * (D / 8) + w];
-          s = egd::half_to_float(scales[(group << pool.page_shift) + slot + i]);
-        }
-        TO* to = out + (size_t)i * kvh * D + 32 * group + 8 * part;
+        float v[8];
 #pragma unroll
-        for (uint32_t e = 0; e < 8; e++) to[e] = from_f32<TO>((float)((int)((word >> (4 * e)) & 15u) - 8) * s);
+        for (uint32_t e = 0; e < 8; e++) v[e] = have ? value(word[j], e, s[j]) : 0.f;
+        store8(out + (size_t)i * kvh * D + 8 * w, v);
       }
     } else {
+      constexpr uint32_t kRows = 128 / D;  // rows at a time
+      const uint32_t p = lane % (D / 2), first = slot >> 3;
+      uint2 word[kBlock / 8];
+      uint4 s[kBlock / 8];
 #pragma unroll
-      for (uint32_t j = 0; j < kPer; j++) {
-        const uint32_t d = 64 * j + lane;
-        uint32_t word = 0x88888888u;
-        if (have) word = reinterpret_cast<const uint32_t*>(block + at.v_codes)[(slot >> 3) * D + d];
-        for (uint32_t i = 0; i < n; i++) {
-          const float s = have ? egd::half_to_float(scales[((d / 32) << pool.page_shift) + slot + i]) : 0.f;
-          out[(size_t)i * kvh * D + d] = from_f32<TO>((float)((int)((word >> (4 * ((slot + i) & 7u))) & 15u) - 8) * s);
-        }
+      for (uint32_t j = 0; j < kBlock / 8; j++) {
+        const uint32_t b = min(first + j, (slot + n - 1) >> 3);
+        word[j] = reinterpret_cast<const uint2*>(block + at.v_codes)[b * (D / 2) + p];
+        s[j] = *reinterpret_cast<const uint4*>(scales + ((p / 16) << pool.page_shift) + 8 * b);
       }
+#pragma unroll
+      for (uint32_t j = 0; j < kBlock / 8; j++)
+#pragma unroll
+        for (uint32_t e = 0; e < 8; e += kRows) {
+          const uint32_t f = e + (D == 64 ? lane >> 5 : 0);  // position of the 8
+          const uint32_t i = 8 * (first + j) + f - slot;     // row (before the first: past n)
+          const uint32_t pair[4] = {s[j].x, s[j].y, s[j].z, s[j].w};
+          const float scale = egd::half_to_float((uint16_t)(pair[e / 2] >> (16 * (f & 1u))));
+          if (i < n)
+            store2(out + (size_t)i * kvh * D + 2 * p, have ? value(word[j].x, f, scale) : 0.f,
+                   have ? value(word[j].y, f, scale) : 0.f);
+        }
     }
   });
 }
@@ -266,9 +407,9 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(uint8_t* pool, const ui
 
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-// Rows per wave: one where the rows are few (a decode batch's rows are blocks of their own, and a
-// wave would take them one after another), else a block's 8.
-uint32_t span_for(uint32_t rows) { return rows <= 2048u ? 1u : 8u; }
+// Where the rows are at most this many a wave has one row (a decode batch's rows are blocks of their own, and
+// a wave would take them one after another) and a workgroup one row's queries; else a block.
+constexpr uint32_t kFewRows = 2048;
 
 }  // namespace
 
@@ -319,7 +460,8 @@ int eg_kv4_append(eg_context* ctx, const void* q, const void* k, const void* v, 
   const uint32_t width = dims->kv_heads * dims->head_dim, q_width = d.heads * dims->head_dim;
   AppendArgs a{q, k, v, reinterpret_cast<const float2*>(rope), offsets, starts, q_out, k_out, v_out, d.rows, d.heads,
                d.q_stride ? d.q_stride : q_width, d.k_stride ? d.k_stride : width,
-               d.v_stride ? d.v_stride : width, d.rope_positions, span_for(d.rows)};
+               d.v_stride ? d.v_stride : width, d.rope_positions, d.rows <= kFewRows ? 1u : 8u, d.rows <= kFewRows ? 1u : 16u,
+               (2 * dims->kv_heads + 3) / 4};
   if (a.q_stride < q_width || a.k_stride < width || a.v_stride < width || (a.q_stride | a.k_stride | a.v_stride) % 4)
     return eg::fail(ctx, EG_ERR_INVALID, "%s: row strides %u, %u, %u (multiples of 4, at least a row)", op, a.q_stride,
                     a.k_stride, a.v_stride);
@@ -329,7 +471,7 @@ int eg_kv4_append(eg_context* ctx, const void* q, const void* k, const void* v, 
   if (d.rows == 0 || dims->sequences == 0) return EG_OK;
   if (d.rows >= (1u << 30)) return eg::fail(ctx, EG_ERR_RANGE, "%s: %u rows (under 2^30)", op, d.rows);
   const eg_kv4::Pool p = eg_kv4::pool_of(*dims, pool, table);
-  const dim3 grid((d.rows + a.span - 1) / a.span, (2 * dims->kv_heads + d.heads + 3) / 4);
+  const dim3 grid((d.rows + a.span - 1) / a.span, a.kv_groups + (d.heads ? 1 : 0));
   with_type(d.in_type, [&](auto ti) {
     with_type(d.out_type, [&](auto to) {
       if (dims->head_dim == 64)
@@ -353,14 +495,15 @@ int eg_kv4_read(eg_context* ctx, const uint32_t* offsets, const uint32_t* starts
     return eg::fail(ctx, EG_ERR_INVALID, "%s: the outputs must be 16-byte aligned", op);
   if (rows == 0 || dims->sequences == 0) return EG_OK;
   if (rows >= (1u << 30)) return eg::fail(ctx, EG_ERR_RANGE, "%s: %u rows (under 2^30)", op, rows);
-  const ReadArgs a{offsets, starts, k_out, v_out, rows, span_for(rows)};
+  const bool few = rows <= kFewRows;
+  const ReadArgs a{offsets, starts, k_out, v_out, rows, few ? 1u : 32u};
   const eg_kv4::Pool p = eg_kv4::pool_of(*dims, pool, table);
   const dim3 grid((rows + a.span - 1) / a.span, (2 * dims->kv_heads + 3) / 4);
   with_type(out_type, [&](auto to) {
-    if (dims->head_dim == 64)
-      hipLaunchKernelGGL((read_kernel<64, decltype(to)>), grid, dim3(kThreads), 0, ctx->stream, a, p);
-    else
-      hipLaunchKernelGGL((read_kernel<128, decltype(to)>), grid, dim3(kThreads), 0, ctx->stream, a, p);
+    using TO = decltype(to);
+    const auto kernel = dims->head_dim == 64 ? (few ? read_kernel<64, 8, TO> : read_kernel<64, 32, TO>)
+                                             : (few ? read_kernel<128, 8, TO> : read_kernel<128, 32, TO>);
+    hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, ctx->stream, a, p);
   });
   return eg::check_launch(ctx, op);
 }
