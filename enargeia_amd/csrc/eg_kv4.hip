@@ -83,7 +83,8 @@ struct AppendArgs {
   const uint32_t *offsets, *starts;
   void *q_out, *k_out, *v_out;
   uint32_t rows, heads, q_stride, k_stride, v_stride, rope_positions;
-  uint32_t span, q_span, kv_groups;  // packed rows per wave, per workgroup of queries; workgroups of kv heads
+  uint32_t span, q_span;          // packed rows per wave of a kv head, per workgroup of queries
+  uint32_t kv_groups, kv_blocks;  // workgroups of the kv heads: per span, in all; those of the queries follow
 };
 
 // The positions of rows r0 + lane (kNowhere for those of no sequence).
@@ -148,54 +149,67 @@ __device__ __forceinline__ void store4(T* p, float4 v) {
 template <int D, class TI, class TO>
 __device__ __forceinline__ void rotate_queries(const AppendArgs& a, const Pool& pool, uint32_t r0, uint32_t rows) {
 #pragma clang fp contract(off)
-  constexpr uint32_t kQuads = D / 8;
+  constexpr uint32_t kQuads = D / 8, kAhead = 2;
   __shared__ uint32_t position[64];
   const uint32_t tid = threadIdx.x;
+  const TI* q = static_cast<const TI*>(a.q);
+  TO* out = static_cast<TO*>(a.q_out);
+  const uint32_t per_row = a.heads * kQuads, items = rows * per_row;
+  const auto at_of = [&](uint32_t i) { return (i % per_row) / kQuads * D + 4 * (i % kQuads); };  // (kQuads divides per_row)
+  const auto read = [&](uint32_t i, float4& u, float4& w) {
+    const TI* src = q + (size_t)(r0 + i / per_row) * a.q_stride + at_of(i);
+    u = load4(src);
+    w = load4(src + D / 2);
+  };
+  const auto finish = [&](uint32_t i, float4 u, float4 w) {
+    const uint32_t r = i / per_row, p = position[r];
+    if (p == kNowhere) return;
+    if (a.rope) {
+      const float4* cs = reinterpret_cast<const float4*>(a.rope + (size_t)p * (D / 2) + 4 * (i % kQuads));
+      const float4 x = cs[0], y = cs[1];  // (cos, sin) of two pairs each
+      const float4 s = u;
+      u = make_float4(s.x * x.x - w.x * x.y, s.y * x.z - w.y * x.w, s.z * y.x - w.z * y.y, s.w * y.z - w.w * y.w);
+      w = make_float4(w.x * x.x + s.x * x.y, w.y * x.z + s.y * x.w, w.z * y.x + s.z * y.y, w.w * y.z + s.w * y.w);
+    }
+    TO* to = out + (size_t)(r0 + r) * (a.heads * D) + at_of(i);
+    store4(to, u);
+    store4(to + D / 2, w);
+  };
+  // What a thread takes first is under way while the positions are found.
+  float4 u[kAhead], w[kAhead];
+#pragma unroll
+  for (uint32_t j = 0; j < kAhead; j++) read(min(tid + j * kThreads, items - 1), u[j], w[j]);
   if (tid < 64) {
     uint32_t p = position_of(a.offsets, a.starts, pool.sequences, r0 + tid);
     if (p != kNowhere && ((p >> pool.page_shift) >= pool.max_pages || (a.rope && p >= a.rope_positions))) p = kNowhere;
     position[tid] = p;
   }
   __syncthreads();
-  const TI* q = static_cast<const TI*>(a.q);
-  TO* out = static_cast<TO*>(a.q_out);
-  const uint32_t per_row = a.heads * kQuads, items = rows * per_row;
-#pragma unroll 4
-  for (uint32_t i = tid; i < items; i += kThreads) {
-    const uint32_t r = i / per_row, in_row = i % per_row, p = position[r];
-    if (p == kNowhere) continue;
-    const uint32_t quad = in_row % kQuads, at = in_row / kQuads * D + 4 * quad;
-    const TI* src = q + (size_t)(r0 + r) * a.q_stride + at;
-    float4 u = load4(src), w = load4(src + D / 2);
-    if (a.rope) {
-      const float4* cs = reinterpret_cast<const float4*>(a.rope + (size_t)p * (D / 2) + 4 * quad);
-      const float4 x = cs[0], y = cs[1];  // (cos, sin) of two pairs each
-      const float4 s = u;
-      u = make_float4(s.x * x.x - w.x * x.y, s.y * x.z - w.y * x.w, s.z * y.x - w.z * y.y, s.w * y.z - w.w * y.w);
-      w = make_float4(w.x * x.x + s.x * x.y, w.y * x.z + s.y * x.w, w.z * y.x + s.z * y.y, w.w * y.z + s.w * y.w);
-    }
-    TO* to = out + (size_t)(r0 + r) * (a.heads * D) + at;
-    store4(to, u);
-    store4(to + D / 2, w);
+#pragma unroll
+  for (uint32_t j = 0; j < kAhead; j++)
+    if (tid + j * kThreads < items) finish(tid + j * kThreads, u[j], w[j]);
+  for (uint32_t i = tid + kAhead * kThreads; i < items; i += kThreads) {
+    read(i, u[0], w[0]);
+    finish(i, u[0], w[0]);
   }
 }
 
-// Workgroups of blockIdx.y < kv_groups: a wave per (span of packed rows, kv head's K or V). A lane holds dim
+// The first kv_blocks workgroups: a wave per (span of packed rows, kv head's K or V). A lane holds dim
 // `lane` of up to 8 rows (and dim lane + 64 at head_dim 128), all read at once. The others: the span's
 // queries. Bound by latency where the rows are few, by memory where they are many.
 template <int D, class TI, class TO>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a, Pool pool) {
   constexpr int kPer = D / 64;  // dims per lane
   const uint32_t kvh = pool.kv_heads;
-  if (blockIdx.y >= a.kv_groups) {
-    const uint32_t r0 = blockIdx.x * a.q_span;
-    if (r0 < a.rows) rotate_queries<D, TI, TO>(a, pool, r0, min(a.q_span, a.rows - r0));
+  if (blockIdx.x >= a.kv_blocks) {
+    const uint32_t r0 = (blockIdx.x - a.kv_blocks) * a.q_span;
+    rotate_queries<D, TI, TO>(a, pool, r0, min(a.q_span, a.rows - r0));
     return;
   }
   const uint32_t lane = threadIdx.x & 63u;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t task = blockIdx.y * 4 + wave;
-  if (task >= 2 * kvh || blockIdx.x * a.span >= a.rows) return;
+  const uint32_t task = blockIdx.x % a.kv_groups * 4 + wave, r0 = blockIdx.x / a.kv_groups * a.span;
+  if (task >= 2 * kvh) return;
   const bool is_k = task < kvh;
   const uint32_t head = is_k ? task : task - kvh;
   const TI* src = static_cast<const TI*>(is_k ? a.k : a.v);
@@ -203,7 +217,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a, Pool pool) {
   const uint32_t stride = is_k ? a.k_stride : a.v_stride, out_stride = kvh * D;
   const Layout at = layout<D>(1u << pool.page_shift);
 
-  for_blocks<8>(a.offsets, a.starts, pool.sequences, a.rows, blockIdx.x * a.span, a.span,
+  for_blocks<8>(a.offsets, a.starts, pool.sequences, a.rows, r0, a.span,
                 [&](uint32_t seq, uint32_t row, uint32_t position, uint32_t n) {
     if ((position >> pool.page_shift) >= pool.max_pages) return;
     const uint32_t page = pool.page_of(seq, position);
@@ -382,8 +396,10 @@ __global__ __launch_bounds__(256) void read_kernel(ReadArgs a, Pool pool) {
   });
 }
 
-// 16 KiB of a page per workgroup, four 16-byte words a thread, all read before any is written.
-constexpr uint32_t kCopyWords = 4, kCopyBytes = kThreads * kCopyWords * 16;
+// A part of a page per workgroup, kCopyWords 16-byte words a thread, all read before any is written, past the
+// caches' retention. 2000 pages of 221,184 bytes: 167.2 us (5.29 TB/s; 175.4 with ordinary accesses; with 4
+// words a thread 168.9 and with 8 172.2).
+constexpr uint32_t kCopyWords = 2, kCopyBytes = kThreads * kCopyWords * 16;
 __global__ __launch_bounds__(256) void copy_pages_kernel(uint8_t* pool, const uint32_t* pairs, uint32_t pages,
                                                          uint64_t stride, uint32_t parts) {
   const uint32_t pair = blockIdx.x / parts, part = blockIdx.x % parts;
@@ -392,16 +408,16 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(uint8_t* pool, const ui
   const uint64_t begin = (uint64_t)part * kCopyBytes + 16u * threadIdx.x;
   const uint8_t* src = pool + from * stride;
   uint8_t* dst = pool + to * stride;
-  uint4 v[kCopyWords];
+  egd::u32x4 v[kCopyWords];
 #pragma unroll
-  for (uint32_t i = 0; i < kCopyWords; i++) {
+  for (uint32_t i = 0; i < kCopyWords; i++) {  // (past the page: its last word again, not written)
     const uint64_t o = begin + 16u * kThreads * i;
-    if (o < stride) v[i] = *reinterpret_cast<const uint4*>(src + o);
+    v[i] = __builtin_nontemporal_load(reinterpret_cast<const egd::u32x4*>(src + (o < stride ? o : stride - 16)));
   }
 #pragma unroll
   for (uint32_t i = 0; i < kCopyWords; i++) {
     const uint64_t o = begin + 16u * kThreads * i;
-    if (o < stride) *reinterpret_cast<uint4*>(dst + o) = v[i];
+    if (o < stride) __builtin_nontemporal_store(v[i], reinterpret_cast<egd::u32x4*>(dst + o));
   }
 }
 
@@ -410,6 +426,13 @@ bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0
 // Where the rows are at most this many a wave has one row (a decode batch's rows are blocks of their own, and
 // a wave would take them one after another) and a workgroup one row's queries; else a block.
 constexpr uint32_t kFewRows = 2048;
+
+// Rows of queries per workgroup of a long append: about two items of 8 elements a thread, what it reads
+// ahead. 16384 rows of 14 heads of 64 (f32 to f16, with the read back) 30.2 us in 4s, 32.4 in 2s, 31.9 in 8s; 4000
+// of 40 heads of 128 (bf16) 37.1 us in 1s, 40.3 in 4s.
+uint32_t query_span(uint32_t rows, uint32_t width) {
+  return rows <= kFewRows || width == 0 ? 1u : std::max(1u, std::min(8u, 4096u / width));
+}
 
 }  // namespace
 
@@ -460,8 +483,8 @@ int eg_kv4_append(eg_context* ctx, const void* q, const void* k, const void* v, 
   const uint32_t width = dims->kv_heads * dims->head_dim, q_width = d.heads * dims->head_dim;
   AppendArgs a{q, k, v, reinterpret_cast<const float2*>(rope), offsets, starts, q_out, k_out, v_out, d.rows, d.heads,
                d.q_stride ? d.q_stride : q_width, d.k_stride ? d.k_stride : width,
-               d.v_stride ? d.v_stride : width, d.rope_positions, d.rows <= kFewRows ? 1u : 8u, d.rows <= kFewRows ? 1u : 16u,
-               (2 * dims->kv_heads + 3) / 4};
+               d.v_stride ? d.v_stride : width, d.rope_positions, d.rows <= kFewRows ? 1u : 8u, query_span(d.rows, q_width),
+               (2 * dims->kv_heads + 3) / 4, 0};
   if (a.q_stride < q_width || a.k_stride < width || a.v_stride < width || (a.q_stride | a.k_stride | a.v_stride) % 4)
     return eg::fail(ctx, EG_ERR_INVALID, "%s: row strides %u, %u, %u (multiples of 4, at least a row)", op, a.q_stride,
                     a.k_stride, a.v_stride);
@@ -471,7 +494,12 @@ int eg_kv4_append(eg_context* ctx, const void* q, const void* k, const void* v, 
   if (d.rows == 0 || dims->sequences == 0) return EG_OK;
   if (d.rows >= (1u << 30)) return eg::fail(ctx, EG_ERR_RANGE, "%s: %u rows (under 2^30)", op, d.rows);
   const eg_kv4::Pool p = eg_kv4::pool_of(*dims, pool, table);
-  const dim3 grid((d.rows + a.span - 1) / a.span, a.kv_groups + (d.heads ? 1 : 0));
+  const uint64_t kv_blocks = (uint64_t)((d.rows + a.span - 1) / a.span) * a.kv_groups;
+  const uint64_t blocks = kv_blocks + (d.heads ? (d.rows + a.q_span - 1) / a.q_span : 0);
+  if (blocks >= (1ull << 31) / kThreads)
+    return eg::fail(ctx, EG_ERR_RANGE, "%s: %u rows of %u kv heads over the grid limit", op, d.rows, dims->kv_heads);
+  a.kv_blocks = (uint32_t)kv_blocks;
+  const dim3 grid((uint32_t)blocks);
   with_type(d.in_type, [&](auto ti) {
     with_type(d.out_type, [&](auto to) {
       if (dims->head_dim == 64)

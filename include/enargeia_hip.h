@@ -541,7 +541,7 @@ EG_API int eg_attention_prefill_f32(eg_context* ctx, const float* q, const float
  *
  * Where several sequences' rows are packed one sequence after another, offsets[sequences + 1] (device
  * memory, ascending) says where: sequence s has rows offsets[s] .. offsets[s + 1]. Rows outside
- * them are neither read nor written. All tables, offsets, starts and lengths are read on the
+ * them are not used and not written. All tables, offsets, starts and lengths are read on the
  * device when the launch runs, so a captured graph follows them. */
 
 /* Element types of rows. */
