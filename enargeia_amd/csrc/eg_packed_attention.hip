@@ -24,6 +24,7 @@ using egd::u32x4;
 constexpr uint32_t kThreads = 256, kWaves = 4;
 constexpr uint32_t kQueries = 32 * kWaves;  // per workgroup
 constexpr uint32_t kKeys = 64;              // per tile
+constexpr float kLag = 8.f;
 constexpr float kLog2e = 1.44269504088896340736f;
 
 struct Args {
@@ -31,6 +32,7 @@ struct Args {
   void* out;
   const uint32_t *q_offsets, *k_offsets;
   uint32_t sequences, rows, key_rows, heads, group, q_stride, k_stride, v_stride, out_stride;
+  uint32_t xcds;  // XCDs a kv head, where kv heads are 1, 2 or 4; else 0
   float scale;  // times log2 e
 };
 
@@ -59,33 +61,58 @@ __device__ __forceinline__ float max_of_query(float x) {
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-// Whether any of 8 f16 (bf16) values is an infinity or a NaN; those replaced by zeros.
 template <class T>
-__device__ __forceinline__ bool clean(u32x4& v) {
-  constexpr uint32_t kExponent = std::is_same<T, _Float16>::value ? 0x7C00u : 0x7F80u;
-  bool any = false;
+constexpr uint32_t kExponent = std::is_same<T, _Float16>::value ? 0x7C00u : 0x7F80u;
+
+// Infinities and NaN among 8 values replaced by zeros.
+template <class T>
+__device__ __forceinline__ void clean(u32x4& v) {
 #pragma unroll
   for (int i = 0; i < 4; i++) {
-    const bool lo = (v[i] & kExponent) == kExponent, hi = ((v[i] >> 16) & kExponent) == kExponent;
-    any |= lo || hi;
+    const bool lo = (v[i] & kExponent<T>) == kExponent<T>, hi = ((v[i] >> 16) & kExponent<T>) == kExponent<T>;
     v[i] &= (lo ? 0xFFFF0000u : 0xFFFFFFFFu) & (hi ? 0xFFFFu : 0xFFFFFFFFu);
   }
-  return any;
 }
 
-// Query block `id` of all sequences' blocks, counted from the last sequence's last one: the blocks
-// with the most keys of a sequence start first. False past the last.
+// Sum over the wave, in every lane.
+__device__ __forceinline__ uint32_t sum_of_wave(uint32_t v) {
+#pragma unroll
+  for (int d = 32; d; d >>= 1) v += (uint32_t)__shfl_xor((int)v, d, 64);
+  return v;
+}
+
+// Query block `id` of all sequences' blocks, those with the most blocks of their sequence before them (so,
+// about, the most keys) first: ranks go down through the levels, a level being the sequences' blocks of one
+// index. The level is the largest with no more than `id` blocks above it, by bisection; the sequences' counts
+// are in the wave's lanes. More than 64 sequences: from the last one's last block on. False past the last.
 __device__ __forceinline__ bool find_block(const Args& a, uint32_t id, uint32_t& seq, uint32_t& block) {
   const uint32_t lane = threadIdx.x & 63u;
+  const auto blocks_of = [&](uint32_t s) {
+    if (s >= a.sequences) return 0u;
+    const uint32_t b = min(a.q_offsets[s], a.rows), e = min(a.q_offsets[s + 1], a.rows);
+    return e > b ? (e - b + kQueries - 1) / kQueries : 0u;
+  };
+  if (a.sequences <= 64) {
+    const uint32_t n = blocks_of(lane);
+    const auto from_level = [&](uint32_t level) {  // blocks of this level and above
+      return __builtin_amdgcn_readfirstlane(sum_of_wave(n > level ? n - level : 0u));
+    };
+    uint32_t lo = 0, hi = a.rows / kQueries + 1;  // from_level(lo) > id >= from_level(hi)
+    if (from_level(0) <= id) return false;
+    while (hi - lo > 1) {
+      const uint32_t mid = (lo + hi) / 2;
+      if (from_level(mid) > id) lo = mid;
+      else hi = mid;
+    }
+    uint64_t have = __ballot(n > lo);
+    for (uint32_t skip = id - from_level(lo + 1); skip; skip--) have &= have - 1;
+    seq = (uint32_t)__builtin_ctzll(have);
+    block = lo;
+    return true;
+  }
   const uint32_t last = (a.sequences - 1) / 64 * 64;
   for (uint32_t i0 = last;; i0 -= 64) {
-    const uint32_t s = i0 + (63u - lane);  // later sequences in lower lanes
-    uint32_t n = 0;
-    if (s < a.sequences) {
-      const uint32_t b = min(a.q_offsets[s], a.rows), e = min(a.q_offsets[s + 1], a.rows);
-      n = e > b ? (e - b + kQueries - 1) / kQueries : 0;
-    }
-    uint32_t upto = n;  // blocks of lanes 0 .. this one
+    uint32_t upto = blocks_of(i0 + (63u - lane));  // blocks of lanes 0 .. this one, later sequences in lower lanes
 #pragma unroll
     for (uint32_t d = 1; d < 64; d <<= 1) {
       const uint32_t t = __shfl_up(upto, d, 64);
@@ -104,8 +131,27 @@ __device__ __forceinline__ bool find_block(const Args& a, uint32_t id, uint32_t&
   }
 }
 
+// The query block (its rank) and head of this workgroup. Workgroups go to the 8 XCDs in turn, each with its own L2:
+// a kv head's keys and values are read by one XCD (of fewer than 8 kv heads, by 8 / kv_heads), its query
+// heads and blocks in ranks' order there.
+__device__ __forceinline__ void work_of(const Args& a, uint32_t& rank, uint32_t& h) {
+  const uint32_t kv_heads = a.heads / a.group, id = blockIdx.x, xcd = id % 8u, turn = id / 8u;
+  if (a.xcds) {
+    const uint32_t item = turn * a.xcds + xcd % a.xcds;
+    rank = item / a.group;
+    h = xcd / a.xcds * a.group + item % a.group;
+  } else if (kv_heads % 8u == 0) {
+    const uint32_t mine = a.heads / 8u, i = turn % mine;
+    rank = turn / mine;
+    h = (xcd + 8u * (i / a.group)) * a.group + i % a.group;
+  } else {
+    rank = id / a.heads;
+    h = id % a.heads;
+  }
+}
+
 template <int D, class T, class TO>
-__global__ __launch_bounds__(256) void packed_kernel(Args a) {
+__global__ __launch_bounds__(256, 2) void packed_kernel(Args a) {
   constexpr uint32_t kSlots = D / 8;                  // 16-byte slots of a row
   constexpr uint32_t kRow = D * 2, kTile = kKeys * kRow;  // bytes
   constexpr int kSteps = D / 16, kBlocks = D / 32;    // depth steps of S^T; blocks of 32 dims of O^T
@@ -114,9 +160,10 @@ __global__ __launch_bounds__(256) void packed_kernel(Args a) {
   const uint32_t tid = threadIdx.x, lane = tid & 63u;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t lq = lane & 31u, lh = lane >> 5;  // MFMA lane coordinates
-  const uint32_t h = blockIdx.x % a.heads, kv = h / a.group;
-  uint32_t seq, block;
-  if (!find_block(a, blockIdx.x / a.heads, seq, block)) return;
+  uint32_t rank, h, seq, block;
+  work_of(a, rank, h);
+  const uint32_t kv = h / a.group;
+  if (!find_block(a, rank, seq, block)) return;
   const uint32_t q_begin = min(a.q_offsets[seq], a.rows), nq = min(a.q_offsets[seq + 1], a.rows) - q_begin;
   const uint32_t k_begin = min(a.k_offsets[seq], a.key_rows);
   const uint32_t nk = max(min(a.k_offsets[seq + 1], a.key_rows), k_begin) - k_begin;
@@ -141,13 +188,6 @@ __global__ __launch_bounds__(256) void packed_kernel(Args a) {
 #pragma unroll
     for (int s = 0; s < kSteps; s++) qf[s] = in ? src[2 * s] : u32x4{0, 0, 0, 0};
   }
-  f32x16 o[kBlocks];
-#pragma unroll
-  for (int n = 0; n < kBlocks; n++)
-#pragma unroll
-    for (int e = 0; e < 16; e++) o[n][e] = 0.f;
-  float m = -INFINITY, l = 0.f;  // running max before the scale; this lane's share of the sum
-
   // K's and V's rows go to LDS 16 bytes a lane, row r's slot j at j ^ swizzle(r): 16 rows of K's
   // operand reads, and the 4 rows of V's transposed ones, then lie in different banks.
   const uint32_t lrow = tid / kSlots, slot = tid % kSlots;
@@ -172,48 +212,60 @@ __global__ __launch_bounds__(256) void packed_kernel(Args a) {
   };
   // V^T operand reads: 4 keys x 16 dims a group of 16 lanes; lane i points at key i / 4, dims 4 (i % 4).
   const uint32_t li = lane & 15u, vrow = 4 * lh + (li >> 2);
+  constexpr uint32_t kVTile = kTile;
   uint32_t vat[kBlocks];
 #pragma unroll
   for (uint32_t n = 0; n < (uint32_t)kBlocks; n++)
-    vat[n] = kTile + vrow * kRow + 16 * ((4 * n + 2 * ((lane >> 4) & 1u) + ((li & 3u) >> 1)) ^ vswz(vrow)) + 8 * (li & 1u);
+    vat[n] = kVTile + vrow * kRow + 16 * ((4 * n + 2 * ((lane >> 4) & 1u) + ((li & 3u) >> 1)) ^ vswz(vrow)) + 8 * (li & 1u);
 
+  f32x16 o[kBlocks];
+  float m, l;  // running max before the scale; this lane's share of the sum
+  const auto run = [&](auto careful) {
+#pragma unroll
+  for (int n = 0; n < kBlocks; n++)
+#pragma unroll
+    for (int e = 0; e < 16; e++) o[n][e] = 0.f;
+  m = -INFINITY;
+  l = 0.f;
   if (ntiles) load_tile(0, 0);
   settle();
   for (uint32_t t = 0; t < ntiles; t++) {
     const uint32_t j0 = t * kKeys, buf = t & 1u;
     const uint8_t* tile = tiles + 2 * kTile * buf;
     if (t + 1 < ntiles) load_tile(t + 1, buf ^ 1u);
-    // A masked weight is 0, but 0 times an infinity or NaN is not: in the tiles with masked keys such
-    // values of V are taken out of the product, and added at the end to the queries that see them.
-    bool unclean = false;
-    if ((int)(j0 + kKeys) > shift + (int)q0) {
-#pragma unroll
-      for (uint32_t i = 0; i < kLoads; i++) {
-        u32x4* at = reinterpret_cast<u32x4*>(tiles + 2 * kTile * buf + kTile + (i * kThreads + tid) * 16);
-        u32x4 v = *at;
-        if (clean<T>(v)) {
-          *at = v;
-          unclean = true;
-        }
-      }
-      unclean = __syncthreads_or(unclean);
-    }
     // (a wave whose queries all end before this tile has nothing to do in it)
     if ((int)j0 < open + 31) {
       f32x16 s[2];
 #pragma unroll
-      for (uint32_t n = 0; n < 2; n++) {
+      for (uint32_t n = 0; n < 2; n++)
 #pragma unroll
         for (int e = 0; e < 16; e++) s[n][e] = 0.f;
+      const auto key = [&](uint32_t d, uint32_t n) {
         const uint32_t r = 32 * n + lq;
+        return *reinterpret_cast<const u32x4*>(tile + r * kRow + 16 * ((2 * d + lh) ^ kswz(r)));
+      };
+      u32x4 ka[3][2];
 #pragma unroll
-        for (uint32_t d = 0; d < (uint32_t)kSteps; d++) {
-          const u32x4 ka = *reinterpret_cast<const u32x4*>(tile + r * kRow + 16 * ((2 * d + lh) ^ kswz(r)));
-          s[n] = multiply<T>(ka, qf[d], s[n]);
-        }
+      for (uint32_t d = 0; d < 2; d++)
+#pragma unroll
+        for (uint32_t n = 0; n < 2; n++) ka[d][n] = key(d, n);
+#pragma unroll
+      for (uint32_t d = 0; d < (uint32_t)kSteps; d++) {
+        if (d + 2 < (uint32_t)kSteps)
+#pragma unroll
+          for (uint32_t n = 0; n < 2; n++) ka[(d + 2) % 3][n] = key(d + 2, n);
+#pragma unroll
+        for (uint32_t n = 0; n < 2; n++) s[n] = multiply<T>(ka[d % 3][n], qf[d], s[n]);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+      for (uint32_t d = 0; d < (uint32_t)kSteps; d++) {
+        if (d + 2 < (uint32_t)kSteps) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
       }
       // register e of block n is key j0 + 32 n + 8 (e / 4) + 4 lh + e % 4
-      if ((int)(j0 + kKeys) > open) {
+      const bool masked = (int)(j0 + kKeys) > open;
+      if (masked) {
 #pragma unroll
         for (int n = 0; n < 2; n++)
 #pragma unroll
@@ -226,7 +278,9 @@ __global__ __launch_bounds__(256) void packed_kernel(Args a) {
 #pragma unroll
         for (int e = 0; e < 16; e++) top = fmaxf(top, s[n][e]);
       top = max_of_query(top);
-      if (__builtin_amdgcn_ballot_w64(top > m) != 0) {
+      // The weights are relative to a max that may lag 2^kLag behind: the accumulators are rescaled only
+      // where a score passes that (or is a query's first).
+      if (__builtin_amdgcn_ballot_w64((top - m) * a.scale > kLag) != 0) {
         const float alpha = top > m ? __builtin_amdgcn_exp2f((m - top) * a.scale) : 1.f;
         l *= alpha;
 #pragma unroll
@@ -234,29 +288,44 @@ __global__ __launch_bounds__(256) void packed_kernel(Args a) {
         m = top;
       }
       const float off = m == -INFINITY ? 0.f : m * a.scale;
+      const auto add_values = [&](auto cleaned) {
+        const auto weights = [&](int k) {  // of keys 16 k .. +16 of the tile, as far as this lane has them
+          u32x4 p;
 #pragma unroll
-      for (int n = 0; n < 2; n++) {
-        uint32_t pb[8];
-#pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-          const float x = __builtin_amdgcn_exp2f(fmaf(s[n][e], a.scale, -off));
-          const float y = __builtin_amdgcn_exp2f(fmaf(s[n][e + 1], a.scale, -off));
-          l += x + y;
-          pb[e / 2] = pack<T>(x, y);
-        }
-#pragma unroll
-        for (int kk = 0; kk < 2; kk++) {
-          const u32x4 p{pb[4 * kk], pb[4 * kk + 1], pb[4 * kk + 2], pb[4 * kk + 3]};
-#pragma unroll
-          for (int b = 0; b < kBlocks; b++) {
-            const uint8_t* at = tile + vat[b] + (32 * n + 16 * kk) * kRow;
-            const egd::s16x4 lo = egd::lds_read_transposed(at), hi = egd::lds_read_transposed(at + 8 * kRow);
-            const u32x4 va = __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-            o[b] = multiply<T>(va, p, o[b]);
+          for (int e = 0; e < 8; e += 2) {
+            const float x = __builtin_amdgcn_exp2f(fmaf(s[k / 2][8 * (k & 1) + e], a.scale, -off));
+            const float y = __builtin_amdgcn_exp2f(fmaf(s[k / 2][8 * (k & 1) + e + 1], a.scale, -off));
+            l += x + y;
+            p[e / 2] = pack<T>(x, y);
           }
+          return p;
+        };
+        const auto value = [&](int k, int b) {
+          const uint8_t* at = tile + vat[b] + 16 * k * kRow;
+          const egd::s16x4 lo = egd::lds_read_transposed(at), hi = egd::lds_read_transposed(at + 8 * kRow);
+          u32x4 va = __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+          if constexpr (decltype(cleaned)::value) clean<T>(va);
+          return va;
+        };
+        u32x4 va[2][kBlocks], p[2];
+        p[0] = weights(0);
+#pragma unroll
+        for (int b = 0; b < kBlocks; b++) va[0][b] = value(0, b);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          if (k < 3) {
+#pragma unroll
+            for (int b = 0; b < kBlocks; b++) va[(k + 1) & 1][b] = value(k + 1, b);
+            p[(k + 1) & 1] = weights(k + 1);
+          }
+#pragma unroll
+          for (int b = 0; b < kBlocks; b++) o[b] = multiply<T>(va[k & 1][b], p[k & 1], o[b]);
         }
-      }
-      if (unclean) {
+      };
+      if (!decltype(careful)::value || !masked) {
+        add_values(std::false_type{});
+      } else if constexpr (decltype(careful)::value) {
+        add_values(std::true_type{});
         for (uint32_t j = 0; j < kKeys && (int)(j0 + j) < limit && j0 + j < key_end; j++) {
           const T* row = reinterpret_cast<const T*>(vbase) + (size_t)(j0 + j) * a.v_stride;
 #pragma unroll
@@ -273,6 +342,23 @@ __global__ __launch_bounds__(256) void packed_kernel(Args a) {
   }
 
   l += __shfl_xor(l, 32, 64);
+  };
+  run(std::false_type{});
+  // A masked weight is 0, but 0 times an infinity or NaN in V is NaN: where a result is not finite the
+  // workgroup goes through its keys again, with care in the tiles that have masked ones.
+  float check = 0.f;
+#pragma unroll
+  for (int n = 0; n < kBlocks; n++)
+#pragma unroll
+    for (int e = 0; e < 16; e++) check = fmaf(o[n][e], 0.f, check);
+  const bool again = __builtin_amdgcn_ballot_w64(query < nq && check != 0.f) != 0;
+  uint32_t* votes = reinterpret_cast<uint32_t*>(tiles);  // (the tiles have been read)
+  votes[wave] = again;
+  __syncthreads();
+  if (votes[0] | votes[1] | votes[2] | votes[3]) {
+    __syncthreads();
+    run(std::true_type{});
+  }
   if (query >= nq) return;
   const float r = limit > 0 ? 1.0f / l : 0.f;  // (no key seen: zeros)
   TO* out = static_cast<TO*>(a.out) + (size_t)(q_begin + query) * a.out_stride + h * D;
@@ -312,6 +398,7 @@ extern "C" int eg_attention_packed(eg_context* ctx, const void* q, const void* k
   Args a{q, k, v, out, q_offsets, k_offsets, d.sequences, d.rows, d.key_rows, d.heads, d.heads / d.kv_heads,
          d.q_stride ? d.q_stride : width, d.k_stride ? d.k_stride : kv_width, d.v_stride ? d.v_stride : kv_width,
          d.out_stride ? d.out_stride : width,
+         d.kv_heads <= 4 && d.kv_heads != 3 ? 8 / d.kv_heads : 0,
          (d.scale > 0.f ? d.scale : 1.0f / sqrtf((float)d.head_dim)) * kLog2e};
   if (a.q_stride < width || a.out_stride < width || a.k_stride < kv_width || a.v_stride < kv_width ||
       (a.q_stride | a.k_stride | a.v_stride | a.out_stride) % 8)
@@ -329,9 +416,11 @@ extern "C" int eg_attention_packed(eg_context* ctx, const void* q, const void* k
   if (d.rows == 0 || d.sequences == 0) return EG_OK;
   // at most this many query blocks, whatever the lengths
   const uint64_t blocks = (uint64_t)d.rows / kQueries + std::min<uint64_t>(d.sequences, d.rows);
-  if (blocks * d.heads >= (1ull << 31) / kThreads)
+  // (a kv head's items rounded up to its XCDs)
+  const uint64_t items = a.xcds ? (blocks * a.group + a.xcds - 1) / a.xcds * 8 : blocks * d.heads;
+  if (items >= (1ull << 31) / kThreads)
     return eg::fail(ctx, EG_ERR_RANGE, "%s: %u rows of %u heads over the grid limit", op, d.rows, d.heads);
-  const dim3 grid((uint32_t)(blocks * d.heads));
+  const dim3 grid((uint32_t)items);
   const auto go = [&](auto t, auto to) {
     if (d.head_dim == 64)
       hipLaunchKernelGGL((packed_kernel<64, decltype(t), decltype(to)>), grid, dim3(kThreads), 0, ctx->stream, a);
