@@ -7,6 +7,15 @@
 // this one is multiplied. Both products run on v_mfma_f32_32x32x16 in the transposed form S^T = K Q^T,
 // O^T = V^T P^T: a lane holds one query's scores (rows of S^T: 4 consecutive keys of every 8), which
 // are the second product's B operand where they lie, with V^T read from LDS transposed.
+//
+// Bound by the SIMDs' issue of both units. A wave and tile of 64 keys take 1024 (head_dim 128) or 512 (64)
+// cycles of the matrix cores and about 700 of vector instructions (32 exponentials of 8 cycles, the rest 4 each);
+// run together, a product holds back about 13 cycles of vector instructions. MI355X: a prompt of 8192, 32 / 8
+// heads of 128, bf16: 514 us, 1070 TFLOP/s (a library product of 8192 reaches 1435 on the card), the
+// matrix cores busy 55% of 960,000 cycles and the vector units 52%; 14 heads of 64, f16: 156 us, 770 TFLOP/s; 8
+// prompts of up to 2048, 14 heads of 64: 52 us. Tried and slower at 8192: two groups of four waves half a
+// step apart, one at its products while the other is at its softmax (550 us); the next tile's scores
+// before this one's softmax (832, for the registers); row sums by a product with ones or by dot products (528, 518).
 #include <algorithm>
 
 #include "eg_kv4.hpp"
@@ -24,6 +33,7 @@ using egd::u32x4;
 constexpr uint32_t kThreads = 256, kWaves = 4;
 constexpr uint32_t kQueries = 32 * kWaves;  // per workgroup
 constexpr uint32_t kKeys = 64;              // per tile
+constexpr uint32_t kSplitTiles = 8, kLeastSplits = 3;
 constexpr float kLag = 8.f;
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -33,6 +43,9 @@ struct Args {
   const uint32_t *q_offsets, *k_offsets;
   uint32_t sequences, rows, key_rows, heads, group, q_stride, k_stride, v_stride, out_stride;
   uint32_t xcds;  // XCDs a kv head, where kv heads are 1, 2 or 4; else 0
+  // Keys split over workgroups: partials [row][head][split][D], unnormalised, and (max times scale, sum).
+  uint32_t splits, items;
+  float *o, *ml;
   float scale;  // times log2 e
 };
 
@@ -134,8 +147,8 @@ __device__ __forceinline__ bool find_block(const Args& a, uint32_t id, uint32_t&
 // The query block (its rank) and head of this workgroup. Workgroups go to the 8 XCDs in turn, each with its own L2:
 // a kv head's keys and values are read by one XCD (of fewer than 8 kv heads, by 8 / kv_heads), its query
 // heads and blocks in ranks' order there.
-__device__ __forceinline__ void work_of(const Args& a, uint32_t& rank, uint32_t& h) {
-  const uint32_t kv_heads = a.heads / a.group, id = blockIdx.x, xcd = id % 8u, turn = id / 8u;
+__device__ __forceinline__ void work_of(const Args& a, uint32_t id, uint32_t& rank, uint32_t& h) {
+  const uint32_t kv_heads = a.heads / a.group, xcd = id % 8u, turn = id / 8u;
   if (a.xcds) {
     const uint32_t item = turn * a.xcds + xcd % a.xcds;
     rank = item / a.group;
@@ -150,7 +163,38 @@ __device__ __forceinline__ void work_of(const Args& a, uint32_t& rank, uint32_t&
   }
 }
 
-template <int D, class T, class TO>
+// A workgroup's queries and keys.
+struct Work {
+  uint32_t head, split, q0, nq, q_begin, k_begin;
+  int shift;          // query i sees the keys below shift + i
+  uint32_t key_end;   // of the workgroup's last query
+  uint32_t first, stop;  // its key tiles [first, stop)
+  uint32_t per_split;    // key tiles of a split
+};
+// (The splits of an item lie `items` apart: an item's workgroups are on one XCD, items being a multiple of 8.)
+__device__ __forceinline__ bool find_work(const Args& a, uint32_t id, Work& w) {
+  uint32_t rank, seq, block;
+  w.split = a.splits > 1 ? id / a.items : 0;
+  work_of(a, a.splits > 1 ? id % a.items : id, rank, w.head);
+  if (!find_block(a, rank, seq, block)) return false;
+  w.q_begin = min(a.q_offsets[seq], a.rows);
+  w.nq = min(a.q_offsets[seq + 1], a.rows) - w.q_begin;
+  w.k_begin = min(a.k_offsets[seq], a.key_rows);
+  const uint32_t nk = max(min(a.k_offsets[seq + 1], a.key_rows), w.k_begin) - w.k_begin;
+  w.q0 = block * kQueries;
+  w.shift = (int)(nk - w.nq) + 1;
+  const int last = w.shift + (int)min(w.q0 + kQueries, w.nq) - 1;
+  w.key_end = last > 0 ? min((uint32_t)last, nk) : 0;
+  const uint32_t tiles = (w.key_end + kKeys - 1) / kKeys;
+  w.per_split = ((nk + kKeys - 1) / kKeys + a.splits - 1) / a.splits;
+  w.first = min(w.split * w.per_split, tiles);
+  w.stop = min(w.first + w.per_split, tiles);
+  return true;
+}
+
+// LDS is one array: with a second one the compiler has the reads of K wait for the loads into the other
+// buffer (as it does with stores to LDS in the loop). The reads run two steps ahead of their products.
+template <int D, bool kSplit, class T, class TO>
 __global__ __launch_bounds__(256, 2) void packed_kernel(Args a) {
   constexpr uint32_t kSlots = D / 8;                  // 16-byte slots of a row
   constexpr uint32_t kRow = D * 2, kTile = kKeys * kRow;  // bytes
@@ -160,25 +204,17 @@ __global__ __launch_bounds__(256, 2) void packed_kernel(Args a) {
   const uint32_t tid = threadIdx.x, lane = tid & 63u;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t lq = lane & 31u, lh = lane >> 5;  // MFMA lane coordinates
-  uint32_t rank, h, seq, block;
-  work_of(a, rank, h);
-  const uint32_t kv = h / a.group;
-  if (!find_block(a, rank, seq, block)) return;
-  const uint32_t q_begin = min(a.q_offsets[seq], a.rows), nq = min(a.q_offsets[seq + 1], a.rows) - q_begin;
-  const uint32_t k_begin = min(a.k_offsets[seq], a.key_rows);
-  const uint32_t nk = max(min(a.k_offsets[seq + 1], a.key_rows), k_begin) - k_begin;
-  const uint32_t q0 = block * kQueries, query = q0 + wave * 32 + lq;
+  Work w;
+  if (!find_work(a, blockIdx.x, w)) return;
+  if (kSplit && w.split != 0 && w.first >= w.stop) return;
+  const uint32_t h = w.head, kv = h / a.group, q_begin = w.q_begin, nq = w.nq, key_end = w.key_end;
+  const uint32_t query = w.q0 + wave * 32 + lq;
   const T* q = static_cast<const T*>(a.q);
-  const uint8_t* kbase = reinterpret_cast<const uint8_t*>(static_cast<const T*>(a.k) + (size_t)k_begin * a.k_stride + kv * D);
-  const uint8_t* vbase = reinterpret_cast<const uint8_t*>(static_cast<const T*>(a.v) + (size_t)k_begin * a.v_stride + kv * D);
-
-  // Keys that query i sees: those below nk - nq + i + 1 (none where that is not positive).
-  const int shift = (int)(nk - nq) + 1;
-  const int last = shift + (int)min(q0 + kQueries, nq) - 1;  // of the workgroup's last query
-  const uint32_t key_end = last > 0 ? min((uint32_t)last, nk) : 0;
-  const int limit = shift + (int)query;                       // of this lane's query
-  const int open = shift + (int)(q0 + wave * 32);             // of the wave's first query
-  const uint32_t ntiles = (key_end + kKeys - 1) / kKeys;
+  const uint8_t* kbase = reinterpret_cast<const uint8_t*>(static_cast<const T*>(a.k) + (size_t)w.k_begin * a.k_stride + kv * D);
+  const uint8_t* vbase = reinterpret_cast<const uint8_t*>(static_cast<const T*>(a.v) + (size_t)w.k_begin * a.v_stride + kv * D);
+  const int limit = w.shift + (int)query;                 // the keys this lane's query sees are below
+  const int open = w.shift + (int)(w.q0 + wave * 32);     // and those the wave's first query does
+  const uint32_t first = kSplit ? w.first : 0, stop = kSplit ? w.stop : (key_end + kKeys - 1) / kKeys;
 
   // Q^T, B operand: query lq, dims 16 s + 8 lh .. +8.
   u32x4 qf[kSteps];
@@ -227,12 +263,12 @@ __global__ __launch_bounds__(256, 2) void packed_kernel(Args a) {
     for (int e = 0; e < 16; e++) o[n][e] = 0.f;
   m = -INFINITY;
   l = 0.f;
-  if (ntiles) load_tile(0, 0);
+  if (first < stop) load_tile(first, first & 1u);
   settle();
-  for (uint32_t t = 0; t < ntiles; t++) {
+  for (uint32_t t = first; t < stop; t++) {
     const uint32_t j0 = t * kKeys, buf = t & 1u;
     const uint8_t* tile = tiles + 2 * kTile * buf;
-    if (t + 1 < ntiles) load_tile(t + 1, buf ^ 1u);
+    if (t + 1 < stop) load_tile(t + 1, buf ^ 1u);
     // (a wave whose queries all end before this tile has nothing to do in it)
     if ((int)j0 < open + 31) {
       f32x16 s[2];
@@ -360,6 +396,17 @@ __global__ __launch_bounds__(256, 2) void packed_kernel(Args a) {
     run(std::true_type{});
   }
   if (query >= nq) return;
+  if constexpr (kSplit) {
+    const size_t row = ((size_t)(q_begin + query) * a.heads + h) * a.splits + w.split;
+#pragma unroll
+    for (int n = 0; n < kBlocks; n++)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4)
+        *reinterpret_cast<float4*>(a.o + row * D + 32 * n + 8 * (e / 4) + 4 * lh) =
+            make_float4(o[n][e], o[n][e + 1], o[n][e + 2], o[n][e + 3]);
+    if (lh == 0) *reinterpret_cast<float2*>(a.ml + 2 * row) = make_float2(m * a.scale, l);
+    return;
+  }
   const float r = limit > 0 ? 1.0f / l : 0.f;  // (no key seen: zeros)
   TO* out = static_cast<TO*>(a.out) + (size_t)(q_begin + query) * a.out_stride + h * D;
 #pragma unroll
@@ -372,6 +419,42 @@ __global__ __launch_bounds__(256, 2) void packed_kernel(Args a) {
       else
         *reinterpret_cast<uint2*>(to) = make_uint2(pack<TO>(o[n][e] * r, o[n][e + 1] * r), pack<TO>(o[n][e + 2] * r, o[n][e + 3] * r));
     }
+}
+
+// The splits of a query block joined, in their order: 4 dims of a query a thread, kThreads / (D / 4) queries a
+// workgroup.
+template <int D, class T, class TO>
+__global__ __launch_bounds__(256) void join_kernel(Args a) {
+  constexpr uint32_t kEach = kThreads / (D / 4), kParts = kQueries / kEach;
+  Args all = a;
+  all.splits = 1;
+  Work w;
+  if (!find_work(all, blockIdx.x / kParts, w)) return;
+  const uint32_t per_split = (w.per_split + a.splits - 1) / a.splits;  // (of one split: all the sequence's tiles)
+  const uint32_t count = max(1u, per_split ? (w.stop + per_split - 1) / per_split : 1u);
+  const uint32_t query = w.q0 + blockIdx.x % kParts * kEach + threadIdx.x / (D / 4), d = 4 * (threadIdx.x % (D / 4));
+  if (query < w.nq) {
+    const size_t row = ((size_t)(w.q_begin + query) * a.heads + w.head) * a.splits;
+    float top = -INFINITY;
+    for (uint32_t c = 0; c < count; c++) top = fmaxf(top, a.ml[2 * (row + c)]);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
+#pragma unroll 4
+    for (uint32_t c = 0; c < count; c++) {
+      const float2 ml = *reinterpret_cast<const float2*>(a.ml + 2 * (row + c));
+      const float4 v = *reinterpret_cast<const float4*>(a.o + (row + c) * D + d);
+      // (a split of which the query sees no key has nothing but zeros; its max, of none, is below all)
+      const float f = ml.x == -INFINITY && ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - top);
+      sum = fmaf(f, ml.y, sum);
+      acc = make_float4(fmaf(f, v.x, acc.x), fmaf(f, v.y, acc.y), fmaf(f, v.z, acc.z), fmaf(f, v.w, acc.w));
+    }
+    const float r = w.shift + (int)query > 0 ? 1.0f / sum : 0.f;
+    TO* to = static_cast<TO*>(a.out) + (size_t)(w.q_begin + query) * a.out_stride + w.head * D + d;
+    if constexpr (std::is_same<TO, float>::value)
+      *reinterpret_cast<float4*>(to) = make_float4(acc.x * r, acc.y * r, acc.z * r, acc.w * r);
+    else
+      *reinterpret_cast<uint2*>(to) = make_uint2(pack<TO>(acc.x * r, acc.y * r), pack<TO>(acc.z * r, acc.w * r));
+  }
 }
 
 }  // namespace
@@ -398,7 +481,7 @@ extern "C" int eg_attention_packed(eg_context* ctx, const void* q, const void* k
   Args a{q, k, v, out, q_offsets, k_offsets, d.sequences, d.rows, d.key_rows, d.heads, d.heads / d.kv_heads,
          d.q_stride ? d.q_stride : width, d.k_stride ? d.k_stride : kv_width, d.v_stride ? d.v_stride : kv_width,
          d.out_stride ? d.out_stride : width,
-         d.kv_heads <= 4 && d.kv_heads != 3 ? 8 / d.kv_heads : 0,
+         d.kv_heads <= 4 && d.kv_heads != 3 ? 8 / d.kv_heads : 0, 1, 0, nullptr, nullptr,
          (d.scale > 0.f ? d.scale : 1.0f / sqrtf((float)d.head_dim)) * kLog2e};
   if (a.q_stride < width || a.out_stride < width || a.k_stride < kv_width || a.v_stride < kv_width ||
       (a.q_stride | a.k_stride | a.v_stride | a.out_stride) % 8)
@@ -420,12 +503,32 @@ extern "C" int eg_attention_packed(eg_context* ctx, const void* q, const void* k
   const uint64_t items = a.xcds ? (blocks * a.group + a.xcds - 1) / a.xcds * 8 : blocks * d.heads;
   if (items >= (1ull << 31) / kThreads)
     return eg::fail(ctx, EG_ERR_RANGE, "%s: %u rows of %u heads over the grid limit", op, d.rows, d.heads);
-  const dim3 grid((uint32_t)items);
+  // Few query blocks leave the device idle over long keys: each block's keys are then split over workgroups, as
+  // many as make two workgroups a CU, of at least kSplitTiles of a sequence's tiles. 14 / 2 heads of 64: 256
+  // queries after 1792 rows 28.9 -> 17.0 us, twice 64 after 6000 75 -> 24.5; but for what the join costs, a prompt
+  // of 1024 in two splits takes 19.4 us for 17.7, and 4 of 500 after 2000 in two or three 40.4 for 36.3.
+  const uint64_t resident = 2ull * ctx->cu_count;
+  const uint64_t tiles = (uint64_t)d.key_rows / d.sequences / kKeys, row_bytes = (uint64_t)d.rows * d.heads * (d.head_dim + 2) * 4;
+  const uint64_t splits = std::min({resident / (blocks * d.heads), tiles / kSplitTiles, (eg::kPartialsBytes - 64) / row_bytes});
+  if (splits >= kLeastSplits) {
+    a.splits = (uint32_t)splits;
+    a.items = (uint32_t)((items + 7) / 8 * 8);
+    a.ml = reinterpret_cast<float*>(eg::partials(ctx));
+    a.o = a.ml + (((size_t)d.rows * d.heads * splits * 2 + 3) & ~(size_t)3);
+  }
   const auto go = [&](auto t, auto to) {
-    if (d.head_dim == 64)
-      hipLaunchKernelGGL((packed_kernel<64, decltype(t), decltype(to)>), grid, dim3(kThreads), 0, ctx->stream, a);
-    else
-      hipLaunchKernelGGL((packed_kernel<128, decltype(t), decltype(to)>), grid, dim3(kThreads), 0, ctx->stream, a);
+    using T = decltype(t);
+    using TO = decltype(to);
+    const dim3 whole((uint32_t)items), threads(kThreads);
+    if (a.splits > 1) {
+      hipLaunchKernelGGL((d.head_dim == 64 ? packed_kernel<64, true, T, TO> : packed_kernel<128, true, T, TO>),
+                         dim3(a.items * a.splits), threads, 0, ctx->stream, a);
+      hipLaunchKernelGGL((d.head_dim == 64 ? join_kernel<64, T, TO> : join_kernel<128, T, TO>),
+                         dim3((uint32_t)items * d.head_dim / 8), threads, 0, ctx->stream, a);
+    } else {
+      hipLaunchKernelGGL((d.head_dim == 64 ? packed_kernel<64, false, T, TO> : packed_kernel<128, false, T, TO>), whole,
+                         threads, 0, ctx->stream, a);
+    }
   };
   if (d.type == EG_ELEMENT_F16) {
     if (d.out_type == EG_ELEMENT_F32) go(_Float16{}, float{});

@@ -470,6 +470,18 @@ def test_packed_chunks_after_earlier_rows_and_rows_that_see_nothing(device, up, 
         check_packed(device, up, np.random.default_rng(21), nq, nk, 4, 2, d, kind)
 
 
+@pytest.mark.parametrize("kind,out_kind", [("f16", "f16"), ("bf16", "bf16"), ("f16", "f32"), ("bf16", "f32")])
+def test_packed_few_queries_over_long_keys(device, up, kind, out_kind):
+    """The keys split over workgroups and joined: sequences of very different lengths, some shorter than a
+    split, blocks whose last splits are empty, queries that see nothing."""
+    rng = np.random.default_rng(27)
+    for heads, kv, d in ((3, 1, 64), (4, 4, 128), (6, 3, 64)):
+        print(f"packed few queries, {heads}/{kv} x {d}, {kind} {out_kind}", flush=True)
+        check_packed(device, up, rng, [130, 3, 1], [5000, 1100, 40], heads, kv, d, kind, out_kind, before=2, after=1)
+        check_packed(device, up, rng, [200, 0, 70], [100, 9, 4200], heads, kv, d, kind, out_kind)
+        check_packed(device, up, rng, [2500], [2500], heads, kv, d, kind, out_kind)
+
+
 def test_packed_strides_types_and_rows_outside(device, up):
     rng = np.random.default_rng(22)
     check_packed(device, up, rng, [40, 90], [40, 90], 14, 2, 64, "f16", "f32", before=3, after=5, pad=8)
@@ -523,12 +535,15 @@ def test_packed_not_finite_values_stay_with_who_sees_them(device, up, what, valu
     assert np.isfinite(g[:at]).all()
 
 
-def test_packed_value_before_the_poisoned_row_is_clean(device, up):
-    def change(q, k, v):
-        v[70, 5] = np.nan
-        v[100, 6] = np.inf
+@pytest.mark.parametrize("nq,nk", [(150, 150), (150, 4000)])
+def test_packed_value_before_the_poisoned_row_is_clean(device, up, nq, nk):
+    at = nk - nq  # the first query's own position
 
-    (g, qi, ki, vi), = check_packed(device, up, np.random.default_rng(25), [150], [150], 2, 1, 128, "bf16", change=change)
+    def change(q, k, v):
+        v[at + 70, 5] = np.nan
+        v[at + 100, 6] = np.inf
+
+    (g, qi, ki, vi), = check_packed(device, up, np.random.default_rng(25), [nq], [nk], 2, 1, 128, "bf16", change=change)
     assert np.isfinite(g[:70]).all() and np.isnan(g[70:, :, 5]).all()
     assert np.isfinite(g[:100, :, 6]).all() and not np.isfinite(g[100:, :, 6]).any()
 
