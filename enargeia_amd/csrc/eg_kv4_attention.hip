@@ -37,6 +37,7 @@ using egd::u32x4;
 
 constexpr uint32_t kThreads = 256, kWaves = 4;
 constexpr uint64_t kInfinityCache = 256u << 20;  // bytes
+constexpr float kLargest = 0x1p20f;
 constexpr float kLog2e = 1.44269504088896340736f;
 // slot of an 8-deep operand -> nibble of a word, as the two masks below deliver them
 constexpr uint32_t kOrder[8] = {0, 4, 1, 5, 2, 6, 3, 7};
@@ -311,7 +312,16 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(Args a, Pool pool) {
 #pragma unroll
       for (int e = 0; e < 4; e++) top = fmaxf(top, s[n][e]);
     top = max_of_head(top);
-    const float shift = top == -INFINITY ? 0.f : fmaf(top, f, -15.f);
+    float shift = top == -INFINITY ? 0.f : fmaf(top, f, -15.f);
+    // (past kLargest the max's own rounding would put weights out of f16's range: there it is taken from the
+    // scores instead, which leaves the largest exactly 0)
+    if (__builtin_amdgcn_ballot_w64(fabsf(shift) > kLargest) != 0) {
+#pragma unroll
+      for (int n = 0; n < 2; n++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[n][e] -= top;
+      shift = -15.f;
+    }
     if (__builtin_amdgcn_ballot_w64(top > m) != 0) {
       const float alpha = top > m ? __builtin_amdgcn_exp2f((m - top) * f) : 1.f;
       l *= alpha;

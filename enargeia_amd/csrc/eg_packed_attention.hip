@@ -34,7 +34,7 @@ constexpr uint32_t kThreads = 256, kWaves = 4;
 constexpr uint32_t kQueries = 32 * kWaves;  // per workgroup
 constexpr uint32_t kKeys = 64;              // per tile
 constexpr uint32_t kSplitTiles = 8, kLeastSplits = 3;
-constexpr float kLag = 8.f;
+constexpr float kLag = 8.f, kLargest = 0x1p20f;
 constexpr float kLog2e = 1.44269504088896340736f;
 
 struct Args {
@@ -87,11 +87,16 @@ __device__ __forceinline__ void clean(u32x4& v) {
   }
 }
 
-// Sum over the wave, in every lane.
+// Sum over the wave, in every lane, by DPP.
 __device__ __forceinline__ uint32_t sum_of_wave(uint32_t v) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) v += (uint32_t)__shfl_xor((int)v, d, 64);
-  return v;
+  const auto add = [&](int moved) { v += (uint32_t)moved; };
+  add(__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true));    // quad_perm [1,0,3,2]
+  add(__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true));    // quad_perm [2,3,0,1]
+  add(__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, true));   // row_half_mirror
+  add(__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, true));   // row_mirror
+  add(__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false));  // row_bcast:15 into rows 1 and 3
+  add(__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false));  // row_bcast:31 into rows 2 and 3
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 
 // Query block `id` of all sequences' blocks, those with the most blocks of their sequence before them (so,
@@ -108,7 +113,7 @@ __device__ __forceinline__ bool find_block(const Args& a, uint32_t id, uint32_t&
   if (a.sequences <= 64) {
     const uint32_t n = blocks_of(lane);
     const auto from_level = [&](uint32_t level) {  // blocks of this level and above
-      return __builtin_amdgcn_readfirstlane(sum_of_wave(n > level ? n - level : 0u));
+      return sum_of_wave(n > level ? n - level : 0u);
     };
     uint32_t lo = 0, hi = a.rows / kQueries + 1;  // from_level(lo) > id >= from_level(hi)
     if (from_level(0) <= id) return false;
@@ -323,7 +328,17 @@ __global__ __launch_bounds__(256, 2) void packed_kernel(Args a) {
         for (int n = 0; n < kBlocks; n++) o[n] *= alpha;
         m = top;
       }
-      const float off = m == -INFINITY ? 0.f : m * a.scale;
+      float off = m == -INFINITY ? 0.f : m * a.scale;
+      // (past kLargest the max's own rounding would put weights out of range: there it is taken from the scores
+      // instead)
+      if (__builtin_amdgcn_ballot_w64(fabsf(off) > kLargest) != 0) {
+        const float from = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int n = 0; n < 2; n++)
+#pragma unroll
+          for (int e = 0; e < 16; e++) s[n][e] -= from;
+        off = 0.f;
+      }
       const auto add_values = [&](auto cleaned) {
         const auto weights = [&](int k) {  // of keys 16 k .. +16 of the tile, as far as this lane has them
           u32x4 p;

@@ -60,6 +60,13 @@ _ATTENTION_KV4_DIMS = struct.Struct("3Iif").pack  # heads, q_stride, out_stride,
 _ATTENTION_PACKED_DIMS = struct.Struct("10I2if").pack
 
 
+def _packed(pack, *values) -> bytes:
+    try:
+        return pack(*values)
+    except struct.error as e:
+        raise EgRangeError(EG_ERR_RANGE, f"kv4: a dimension out of range ({e})") from None
+
+
 def page_bytes(kv_heads: int, head_dim: int, page_size: int) -> int:
     """Bytes of one layer's page."""
     out = ctypes.c_uint64()
@@ -78,6 +85,8 @@ class Kv4Cache:
         self.layer_bytes = page_bytes(kv_heads, head_dim, page_size)
         self.dims = Kv4Dims(kv_heads, head_dim, page_size, pages, self.layer_bytes * layers, 0, 0)
         self._dims = ctypes.byref(self.dims)
+        lib = _lib.load()  # (bound once: a small call's time is its host path)
+        self._append, self._read, self._attend = lib.eg_kv4_append, lib.eg_kv4_read, lib.eg_attention_decode_kv4
         self.layers = layers
         self.owned = device.buffer(self.dims.page_stride * pages, "kv4 pool") if pool is None else None
         self.pool = self.owned if pool is None else pool
@@ -98,29 +107,34 @@ class Kv4Cache:
                v_stride: int = 0) -> None:
         """eg_kv4_append: the batch's new rows rotated and stored."""
         ctx = self.device.ctx
-        check(_lib.load().eg_kv4_append(
+        status = self._append(
             ctx, _address(q), _address(k), _address(v), _address(rope), _address(offsets), _address(starts),
             _address(table), self._at(layer), _address(q_out), _address(k_out), _address(v_out),
             self._for(sequences, max_pages),
-            _APPEND_DIMS(rows, heads, q_stride, k_stride, v_stride, rope_positions, _element(in_type),
-                         _element(out_type))), ctx)
+            _packed(_APPEND_DIMS, rows, heads, q_stride, k_stride, v_stride, rope_positions, _element(in_type),
+                    _element(out_type)))
+        if status:
+            check(status, ctx)
 
     def read(self, k_out, v_out, offsets, starts, table, *, rows: int, sequences: int, max_pages: int,
              layer: int = 0, out_type: str = "f16") -> None:
         """eg_kv4_read: cached rows as packed rows."""
         ctx = self.device.ctx
-        check(_lib.load().eg_kv4_read(ctx, _address(offsets), _address(starts), _address(table), self._at(layer),
-                                      _address(k_out), _address(v_out), rows, _element(out_type),
-                                      self._for(sequences, max_pages)), ctx)
+        status = self._read(ctx, _address(offsets), _address(starts), _address(table), self._at(layer),
+                            _address(k_out), _address(v_out), rows, _element(out_type),
+                            self._for(sequences, max_pages))
+        if status:
+            check(status, ctx)
 
     def attend(self, q, lengths, table, out, *, heads: int, sequences: int, max_pages: int, layer: int = 0,
                type: str = "f32", scale: float = 0.0, q_stride: int = 0, out_stride: int = 0) -> None:
         """eg_attention_decode_kv4: one token per sequence against its cached positions."""
         ctx = self.device.ctx
-        check(_lib.load().eg_attention_decode_kv4(ctx, _address(q), _address(lengths), _address(table),
-                                                  self._at(layer), _address(out), self._for(sequences, max_pages),
-                                                  _ATTENTION_KV4_DIMS(heads, q_stride, out_stride, _element(type),
-                                                                      scale)), ctx)
+        status = self._attend(ctx, _address(q), _address(lengths), _address(table), self._at(layer), _address(out),
+                              self._for(sequences, max_pages),
+                              _packed(_ATTENTION_KV4_DIMS, heads, q_stride, out_stride, _element(type), scale))
+        if status:
+            check(status, ctx)
 
     def copy_pages(self, pairs, count: int) -> None:
         """eg_kv4_copy_pages: page pairs[i][0] to page pairs[i][1], all layers."""
@@ -142,8 +156,8 @@ def attention_packed(device: Device, q, k, v, out, q_offsets, k_offsets, *, sequ
     ctx = device.ctx
     check(_lib.load().eg_attention_packed(
         ctx, _address(q), _address(k), _address(v), _address(q_offsets), _address(k_offsets), _address(out),
-        _ATTENTION_PACKED_DIMS(sequences, rows, key_rows, heads, kv_heads, head_dim, q_stride, k_stride, v_stride,
-                               out_stride, t, t if out_type is None else _element(out_type), scale)), ctx)
+        _packed(_ATTENTION_PACKED_DIMS, sequences, rows, key_rows, heads, kv_heads, head_dim, q_stride, k_stride,
+                v_stride, out_stride, t, t if out_type is None else _element(out_type), scale)), ctx)
 
 
 class PageTable:

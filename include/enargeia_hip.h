@@ -542,7 +542,8 @@ EG_API int eg_attention_prefill_f32(eg_context* ctx, const float* q, const float
  * Where several sequences' rows are packed one sequence after another, offsets[sequences + 1] (device
  * memory, ascending) says where: sequence s has rows offsets[s] .. offsets[s + 1]. Rows outside
  * them are not used and not written. All tables, offsets, starts and lengths are read on the
- * device when the launch runs, so a captured graph follows them. */
+ * device when the launch runs, so a captured graph follows them. Outputs overlap no input. Pointers to rows,
+ * pools and rope tables are 16-byte aligned. */
 
 /* Element types of rows. */
 typedef enum eg_element { EG_ELEMENT_F32 = 0, EG_ELEMENT_F16 = 1, EG_ELEMENT_BF16 = 2 } eg_element;
@@ -558,13 +559,14 @@ typedef struct eg_kv4_dims {
 EG_API int eg_kv4_page_bytes(const eg_kv4_dims* dims, uint64_t* out_bytes);
 
 /* A batch's new rows into the cache. Row r of sequence s is at position starts[s] + r - offsets[s];
- * no two rows of a call share a position of a page. With `rope` ([rope_positions][head_dim / 2]
+ * a page that rows go to is one sequence's alone in the call (pages that forks share are only read). With `rope` ([rope_positions][head_dim / 2]
  * pairs (cos, sin) of f32) q and k are rotated by their position's row in half-rotation pairing,
  * each product rounded on its own; k (rotated) and v go into the pages. The outputs are packed rows
  * in out_type: q_out [rows][heads][head_dim] (q rotated), k_out and v_out [rows][kv_heads][head_dim]
  * (k rotated, v as it is: unquantized). q and q_out go together and may be NULL, k_out and v_out each may be;
  * rope may be NULL (no rotation). A row whose position the table or the rope does not reach is
- * skipped: nothing of it is written. Positions of a page that no row names keep their values. */
+ * skipped: nothing of it is written; one whose table entry is no page has its outputs, but is not stored.
+ * Positions of a page that no row names keep their values. */
 typedef struct eg_kv4_append_dims {
   uint32_t rows, heads;                  /* rows of q, k and v; query heads (0 without q)        */
   uint32_t q_stride, k_stride, v_stride; /* elements from row to row, multiples of 4; 0: dense   */

@@ -288,6 +288,29 @@ def test_decode_splits(device, up, lengths, extra, kind):
         check_decode(device, up, np.random.default_rng(11), lengths, heads, kv, d, page, kind, extra=extra)
 
 
+def test_decode_many_sequences(device, up):
+    """More rows than the device holds at once, most of them of a position or none."""
+    rng = np.random.default_rng(37)
+    lengths = [int(n) for n in rng.integers(0, 3, 900)] + [100]
+    check_decode(device, up, rng, lengths, 4, 2, 64, 64, "f32")
+    check_decode(device, up, rng, lengths[600:], 3, 1, 128, 32, "f16")
+
+
+def test_decode_tables_of_no_pages(device, up):
+    """max_pages 0: no position is within reach, so nothing is attended to, stored or read."""
+    P = Pages(1, 1, 64, 32)
+    cache = kv4.Kv4Cache(device, 1, 64, 1, 32, pool=up(P.pool))
+    x = np.ones((2, 64), np.float32)
+    out, tb, two = up(np.full((2, 64), 7.0, np.float32)), up(np.zeros(2, np.uint32)), up(np.array([5, 9], np.uint32))
+    cache.attend(up(x), two, tb, out, heads=1, sequences=2, max_pages=0)
+    assert not device.read_array(out, np.float32, 128).any()
+    off = up(np.array([0, 1, 2], np.uint32))
+    cache.append(up(x), up(x), off, up(np.zeros(2, np.uint32)), tb, rows=2, sequences=2, max_pages=0)
+    cache.read(out, out, off, up(np.zeros(2, np.uint32)), tb, rows=2, sequences=2, max_pages=0, out_type="f32")
+    assert not device.read_array(out, np.float32, 128).any()
+    assert not device.read_array(cache.pool, np.uint8, P.pool.size).any()
+
+
 def test_decode_strides_scale_and_holes(device, up):
     rng = np.random.default_rng(12)
     check_decode(device, up, rng, [100, 300], 14, 2, 64, 64, "f32", pad=8, scale=0.3)
@@ -303,6 +326,53 @@ def test_decode_query_sizes(device, up, factor):
     q = (rng.standard_normal((2, 14, 64)) * factor).astype(np.float32)
     q[:, ::2] *= np.float32(1e-3)
     check_decode(device, up, rng, [90, 500], 14, 2, 64, 64, "f32", q_of=q.reshape(2, -1))
+
+
+def one_position_takes_all(s, v, got, half):
+    """Rows of scores s [.., n] whose largest leads by far more than f32 rounds a score by: the result is its
+    value, to the output's half step."""
+    order = np.sort(s, -1)
+    clear = order[..., -1] - order[..., -2] > 2.0 ** -18 * np.abs(s).max(-1) + 100.0
+    assert clear.any()
+    want = v[np.argmax(s, -1)]
+    assert np.all(np.abs(got - want)[clear] <= (half + 2.0 ** -20) * np.abs(want)[clear])
+
+
+@pytest.mark.parametrize("factor", [1e6, 1e9, 1e20])
+def test_decode_scores_past_what_f32_resolves(device, up, factor):
+    """Scores so large that a rounding of one is more than all exponents hold: still finite, the largest
+    position's value."""
+    rng = np.random.default_rng(35)
+    heads, d, page, n = 4, 64, 64, 300
+    P, k, v = random_pages(rng, 6, 1, d, page)
+    table = rng.permutation(6)[None].astype(np.uint32)
+    q = (rng.standard_normal((1, heads, d)) * factor).astype(np.float32)
+    out = up(q.nbytes)
+    cache = kv4.Kv4Cache(device, 1, d, 6, page, pool=up(P.pool))
+    cache.attend(up(q), up(np.array([n], np.uint32)), up(table), out, heads=heads, sequences=1, max_pages=6)
+    got = device.read_array(out, np.float32, q.size).reshape(heads, d)
+    kk, vv = (x[table[0]].reshape(-1, d)[:n] for x in (k, v))
+    assert np.isfinite(got).all()
+    one_position_takes_all(q[0].astype(np.float64) @ kk.T / 8, vv, got, HALF_STEP["f32"])
+
+
+@pytest.mark.parametrize("kind,factor", [("f16", 2e4), ("bf16", 1e6), ("bf16", 1e18)])
+def test_packed_scores_past_what_f32_resolves(device, up, kind, factor):
+    rng = np.random.default_rng(36)
+    n, d = 200, 64
+
+    def change(q, k, v):
+        q *= np.float32(factor)
+        if kind == "f16":
+            q[:] = np.clip(q, -6e4, 6e4)
+            k *= np.float32(1e4)
+
+    (g, qi, ki, vi), = check_packed(device, up, rng, [1], [n], 2, 1, d, kind, change=change)
+    assert np.isfinite(g).all()
+    for h in range(2):
+        # (its weight, not 1 where the running max lags, is rounded for the product and not for the sum: half a
+        # step of it, and the output's)
+        one_position_takes_all(qi[:, h] @ ki[:, 0].T / 8, vi[:, 0], g[:, h], 2 * HALF_STEP[kind])
 
 
 def test_decode_not_finite_queries_and_rows_stay_where_they_are(device, up):

@@ -112,3 +112,16 @@ def test_element_types_have_names():
     with pytest.raises(EgError, match="element type 'f8'"):
         kv4.attention_packed(None, 0, 0, 0, 0, 0, 0, sequences=1, rows=1, key_rows=1, heads=1, kv_heads=1,
                              head_dim=64, type="f8")
+
+
+def test_dimensions_out_of_range():
+    class Device:
+        ctx = None
+
+    with pytest.raises(EgRangeError, match="a dimension out of range"):
+        kv4.attention_packed(Device, 0, 0, 0, 0, 0, 0, sequences=-1, rows=1, key_rows=1, heads=1, kv_heads=1, head_dim=64)
+    cache = kv4.Kv4Cache(Device, 1, 64, 4, 32, pool=1 << 20)
+    with pytest.raises(EgRangeError, match="a dimension out of range"):
+        cache.attend(0, 0, 0, 0, heads=1 << 32, sequences=1, max_pages=1)
+    with pytest.raises(EgRangeError, match="layer 1 of 1"):
+        cache.read(0, 0, 0, 0, 0, rows=1, sequences=1, max_pages=1, layer=1)
