@@ -9,11 +9,11 @@
 // are the second product's B operand where they lie, with V^T read from LDS transposed.
 //
 // Bound by the SIMDs' issue of both units. A wave and tile of 64 keys take 1024 (head_dim 128) or 512 (64)
-// cycles of the matrix cores and about 700 of vector instructions (32 exponentials of 8 cycles, the rest 4 each);
+// cycles of the matrix cores and 700 to 750 of vector instructions (32 exponentials of 8 cycles, the rest 4 each);
 // run together, a product holds back about 13 cycles of vector instructions. MI355X: a prompt of 8192, 32 / 8
-// heads of 128, bf16: 514 us, 1070 TFLOP/s (a library product of 8192 reaches 1435 on the card), the
-// matrix cores busy 55% of 960,000 cycles and the vector units 52%; 14 heads of 64, f16: 156 us, 770 TFLOP/s; 8
-// prompts of up to 2048, 14 heads of 64: 52 us. Tried and slower at 8192: two groups of four waves half a
+// heads of 128, bf16: 504 us, 1090 TFLOP/s (a library product of 8192 reaches 1435 on the card), the
+// matrix cores busy 55% of 960,000 cycles and the vector units 52%; 14 heads of 64, f16: 153 us, 780 TFLOP/s; 8
+// prompts of up to 2048, 14 heads of 64: 50 us. Tried and slower at 8192: two groups of four waves half a
 // step apart, one at its products while the other is at its softmax (550 us); the next tile's scores
 // before this one's softmax (832, for the registers); row sums by a product with ones or by dot products (528, 518).
 #include <algorithm>
@@ -234,17 +234,23 @@ __global__ __launch_bounds__(256, 2) void packed_kernel(Args a) {
   const uint32_t lrow = tid / kSlots, slot = tid % kSlots;
   const auto kswz = [](uint32_t r) { return D == 64 ? (r >> 1) & 7u : r & 15u; };
   const auto vswz = [](uint32_t r) { return D == 64 ? 4u * ((r >> 1) & 1u) : 4u * (r & 3u); };
+  uint32_t kfrom[kLoads], vfrom[kLoads];  // byte offsets in a tile, of rows kThreads / kSlots apart
+#pragma unroll
+  for (uint32_t i = 0; i < kLoads; i++) {
+    const uint32_t r = lrow + i * (kThreads / kSlots);
+    kfrom[i] = r * a.k_stride * 2 + 16 * (slot ^ kswz(r));
+    vfrom[i] = r * a.v_stride * 2 + 16 * (slot ^ vswz(r));
+  }
   const auto load_tile = [&](uint32_t t, uint32_t buf) {
     const uint32_t j0 = t * kKeys, left = min(kKeys, key_end - j0);
+    // (the resources end with the last key's row: past it, zeros)
     const auto kr = egd::buffer(kbase + (size_t)j0 * a.k_stride * 2, (left - 1) * a.k_stride * 2 + kRow);
     const auto vr = egd::buffer(vbase + (size_t)j0 * a.v_stride * 2, (left - 1) * a.v_stride * 2 + kRow);
 #pragma unroll
     for (uint32_t i = 0; i < kLoads; i++) {
-      const uint32_t r = lrow + i * (kThreads / kSlots);
       uint8_t* at = tiles + 2 * kTile * buf + (i * kThreads + wave * 64) * 16;
-      // (rows past the last key: an offset past the resource, zeros)
-      egd::load_to_lds(kr, at, r < left ? r * a.k_stride * 2 + 16 * (slot ^ kswz(r)) : 0x7FFFFFF0u);
-      egd::load_to_lds(vr, at + kTile, r < left ? r * a.v_stride * 2 + 16 * (slot ^ vswz(r)) : 0x7FFFFFF0u);
+      egd::load_to_lds(kr, at, kfrom[i]);
+      egd::load_to_lds(vr, at + kTile, vfrom[i]);
     }
   };
   const auto settle = [&]() {
@@ -520,8 +526,8 @@ extern "C" int eg_attention_packed(eg_context* ctx, const void* q, const void* k
     return eg::fail(ctx, EG_ERR_RANGE, "%s: %u rows of %u heads over the grid limit", op, d.rows, d.heads);
   // Few query blocks leave the device idle over long keys: each block's keys are then split over workgroups, as
   // many as make two workgroups a CU, of at least kSplitTiles of a sequence's tiles. 14 / 2 heads of 64: 256
-  // queries after 1792 rows 28.9 -> 17.0 us, twice 64 after 6000 75 -> 24.5; but for what the join costs, a prompt
-  // of 1024 in two splits takes 19.4 us for 17.7, and 4 of 500 after 2000 in two or three 40.4 for 36.3.
+  // queries after 1792 rows 28.9 -> 15.8 us, twice 64 after 6000 75 -> 23.3; but for what the join costs, a prompt
+  // of 1024 in two splits takes 19.4 us for 17.5, and 4 of 500 after 2000 in two or three 40.4 for 36.3.
   const uint64_t resident = 2ull * ctx->cu_count;
   const uint64_t tiles = (uint64_t)d.key_rows / d.sequences / kKeys, row_bytes = (uint64_t)d.rows * d.heads * (d.head_dim + 2) * 4;
   const uint64_t splits = std::min({resident / (blocks * d.heads), tiles / kSplitTiles, (eg::kPartialsBytes - 64) / row_bytes});
