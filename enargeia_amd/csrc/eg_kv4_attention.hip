@@ -246,7 +246,7 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(Args a, Pool pool) {
     top = max_of_head(top);
     int e = top > 0.f ? 14 - ((int)(__float_as_uint(top) >> 23) - 127) : 0;
     e = max(-100, min(110, e));
-    f = ldexpf(a.scale, kSigned ? -e : 24 - e);
+    f = fmaxf(ldexpf(a.scale, kSigned ? -e : 24 - e), 0x1p-126f);  // (not 0: -inf times it is -inf)
 #pragma unroll
     for (int g = 0; g < kGroups; g++) {
       half8 part[kParts];
@@ -316,10 +316,11 @@ __global__ __launch_bounds__(256, 2) void decode_kernel(Args a, Pool pool) {
     // (past kLargest the max's own rounding would put weights out of f16's range: there it is taken from the
     // scores instead, which leaves the largest exactly 0)
     if (__builtin_amdgcn_ballot_w64(fabsf(shift) > kLargest) != 0) {
+      const float from = top == -INFINITY ? 0.f : top;  // (a half without a position yet)
 #pragma unroll
       for (int n = 0; n < 2; n++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) s[n][e] -= top;
+        for (int e = 0; e < 4; e++) s[n][e] -= from;
       shift = -15.f;
     }
     if (__builtin_amdgcn_ballot_w64(top > m) != 0) {

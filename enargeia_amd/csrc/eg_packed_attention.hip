@@ -503,7 +503,7 @@ extern "C" int eg_attention_packed(eg_context* ctx, const void* q, const void* k
          d.q_stride ? d.q_stride : width, d.k_stride ? d.k_stride : kv_width, d.v_stride ? d.v_stride : kv_width,
          d.out_stride ? d.out_stride : width,
          d.kv_heads <= 4 && d.kv_heads != 3 ? 8 / d.kv_heads : 0, 1, 0, nullptr, nullptr,
-         (d.scale > 0.f ? d.scale : 1.0f / sqrtf((float)d.head_dim)) * kLog2e};
+         std::max((d.scale > 0.f ? d.scale : 1.0f / sqrtf((float)d.head_dim)) * kLog2e, 0x1p-126f)};
   if (a.q_stride < width || a.out_stride < width || a.k_stride < kv_width || a.v_stride < kv_width ||
       (a.q_stride | a.k_stride | a.v_stride | a.out_stride) % 8)
     return eg::fail(ctx, EG_ERR_INVALID, "%s: strides %u, %u, %u, %u (multiples of 8, at least a row)", op, a.q_stride,

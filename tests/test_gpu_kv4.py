@@ -356,6 +356,36 @@ def test_decode_scores_past_what_f32_resolves(device, up, factor):
     one_position_takes_all(q[0].astype(np.float64) @ kk.T / 8, vv, got, HALF_STEP["f32"])
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n", [20, 32, 80, 200])
+def test_decode_large_scores_where_half_a_step_has_no_position(device, up, n, d):
+    """Steps of 64 positions of which a wave's first ends within the first 32."""
+    rng = np.random.default_rng(37)
+    heads, page = 4, 64
+    P, k, v = random_pages(rng, 4, 1, d, page)
+    table = rng.permutation(4)[None].astype(np.uint32)
+    q = (rng.standard_normal((1, heads, d)) * 1e8).astype(np.float32)
+    out = up(q.nbytes)
+    cache = kv4.Kv4Cache(device, 1, d, 4, page, pool=up(P.pool))
+    cache.attend(up(q), up(np.array([n], np.uint32)), up(table), out, heads=heads, sequences=1, max_pages=4)
+    got = device.read_array(out, np.float32, q.size).reshape(heads, d)
+    kk, vv = (x[table[0]].reshape(-1, d)[:n] for x in (k, v))
+    assert np.isfinite(got).all()
+    one_position_takes_all(q[0].astype(np.float64) @ kk.T / np.sqrt(d), vv, got, HALF_STEP["f32"])
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+def test_decode_smallest_scale_and_queries(device, up, kind):
+    """A scale and queries whose product is below f32: all positions alike, none past the end."""
+    rng = np.random.default_rng(38)
+    q = (rng.standard_normal((2, 4 * 64)) * 1e-35).astype(np.float32)
+    check_decode(device, up, rng, [20, 300], 4, 1, 64, 64, kind, q_of=q, scale=1e-35)
+
+
+def test_packed_smallest_scale(device, up):
+    check_packed(device, up, np.random.default_rng(39), [70, 3], [70, 90], 2, 1, 64, "bf16", scale=1e-45)
+
+
 @pytest.mark.parametrize("kind,factor", [("f16", 2e4), ("bf16", 1e6), ("bf16", 1e18)])
 def test_packed_scores_past_what_f32_resolves(device, up, kind, factor):
     rng = np.random.default_rng(36)
