@@ -33,7 +33,7 @@ __device__ __forceinline__ void for_blocks(const uint32_t* offsets, const uint32
         continue;
       }
       have = true;
-      start = starts[seq];
+      start = start_of(starts, seq);
     }
     const uint32_t position = start + (r - first), in_block = position & (kBlock - 1u);
     const uint32_t n = min(min(kBlock - in_block, end - r), rows - r);
@@ -116,7 +116,7 @@ __device__ __forceinline__ uint32_t position_of(const uint32_t* offsets, const u
       }
     }
   }
-  return lo == 0 || lo > sequences ? kNowhere : starts[lo - 1] + (r - first);
+  return lo == 0 || lo > sequences ? kNowhere : start_of(starts, lo - 1) + (r - first);
 }
 
 // 4 consecutive elements.
@@ -527,6 +527,8 @@ int eg_kv4_read(eg_context* ctx, const uint32_t* offsets, const uint32_t* starts
   const ReadArgs a{offsets, starts, k_out, v_out, rows, few ? 1u : 32u};
   const eg_kv4::Pool p = eg_kv4::pool_of(*dims, pool, table);
   const dim3 grid((rows + a.span - 1) / a.span, (2 * dims->kv_heads + 3) / 4);
+  if (grid.x >= (1u << 31) / kThreads)
+    return eg::fail(ctx, EG_ERR_RANGE, "%s: %u rows over the grid limit", op, rows);
   with_type(out_type, [&](auto to) {
     using TO = decltype(to);
     const auto kernel = dims->head_dim == 64 ? (few ? read_kernel<64, 8, TO> : read_kernel<64, 32, TO>)
@@ -544,7 +546,7 @@ int eg_kv4_copy_pages(eg_context* ctx, void* pool, const uint32_t* pairs, uint32
   if (count == 0) return EG_OK;
   if (!pairs) return eg::fail(ctx, EG_ERR_INVALID, "%s: NULL argument", op);
   const uint64_t parts = (dims->page_stride + kCopyBytes - 1) / kCopyBytes;
-  if (parts * count >= (1ull << 31) / kThreads)
+  if (parts > ((1ull << 31) / kThreads - 1) / count)
     return eg::fail(ctx, EG_ERR_RANGE, "%s: %u pages of %llu bytes over the grid limit", op, count,
                     (unsigned long long)dims->page_stride);
   hipLaunchKernelGGL(copy_pages_kernel, dim3((uint32_t)(parts * count)), dim3(kThreads), 0, ctx->stream,

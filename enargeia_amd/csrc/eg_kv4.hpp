@@ -87,7 +87,10 @@ __device__ __forceinline__ bool find_sequence(const uint32_t* offsets, uint32_t 
   seq = below - 1;
   first = offsets[seq];
   end = offsets[seq + 1];
-  return true;
+  return first <= r && r < end;  // (always, of ascending offsets)
 }
+
+// A sequence's first position, kept where adding any row index to it stays past every table's reach.
+__device__ __forceinline__ uint32_t start_of(const uint32_t* starts, uint32_t seq) { return min(starts[seq], 1u << 31); }
 
 }  // namespace eg_kv4

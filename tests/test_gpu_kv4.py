@@ -208,6 +208,45 @@ def test_rows_that_the_table_the_pages_or_the_rope_do_not_reach(device, up):
     np.testing.assert_array_equal(got[n:n + 12], held(x[n:n + 12]))
 
 
+def test_starts_past_every_table(device, up):
+    """Positions that no table reaches and whose sum with a row's index passes 32 bits: skipped, zeros."""
+    rng = np.random.default_rng(40)
+    d, page, n = 64, 32, 12
+    x = rng.standard_normal((2 * n, d)).astype(np.float32)
+    P = Pages(3, 1, d, page, fill=0x3C)
+    pool = up(P.pool.copy())
+    b, off, tb = up(x), up(np.array([0, n, 2 * n], np.uint32)), up(np.array([[2, 1], [0, 1]], np.uint32))
+    st = up(np.array([0xFFFFFFFC, 0x7FFFFFFE], np.uint32))
+    cs = up(np.ones((64, d // 2, 2), np.float32))
+    ko, qo = (up(np.full((2 * n, d), 9.0, np.float32)) for _ in range(2))
+    cache = kv4.Kv4Cache(device, 1, d, 3, page, pool=pool)
+    for rope in (None, cs):
+        cache.append(b, b, off, st, tb, rows=2 * n, sequences=2, max_pages=2, q=b, q_out=qo, heads=1, k_out=ko, rope=rope,
+                     rope_positions=64)
+        for o in (ko, qo):
+            assert np.all(device.read_array(o, np.float32, x.size) == 9.0)
+    np.testing.assert_array_equal(device.read_array(pool, np.uint8, P.pool.size).reshape(P.pool.shape), P.pool)
+    cache.read(ko, qo, off, st, tb, rows=2 * n, sequences=2, max_pages=2, out_type="f32")
+    for o in (ko, qo):
+        assert not device.read_array(o, np.float32, x.size).any()
+
+
+def test_offsets_that_do_not_ascend_end(device, up):
+    """What they select is not said, but the calls end and keep to the rows and the sequences' pages."""
+    d, page, n = 64, 32, 12
+    b = up(np.ones((n, d), np.float32))
+    off, st, tb = up(np.array([0, 5, 3, 10], np.uint32)), up(np.zeros(3, np.uint32)), up(np.array([[0], [1], [2]], np.uint32))
+    P = Pages(4, 1, d, page, fill=0x3C)
+    pool, out = up(P.pool.copy()), up(np.full((n, d), 9.0, np.float32))
+    cache = kv4.Kv4Cache(device, 1, d, 4, page, pool=pool)
+    cache.append(b, b, off, st, tb, rows=n, sequences=3, max_pages=1, q=b, q_out=out, heads=1, k_out=up(b.size))
+    cache.read(out, up(b.size), off, st, tb, rows=n, sequences=3, max_pages=1, out_type="f32")
+    kv4.attention_packed(device, b, b, b, up(b.size), off, off, sequences=3, rows=n, key_rows=n, heads=1, kv_heads=1,
+                         head_dim=64)
+    assert np.all(device.read_array(out, np.float32, n * d).reshape(n, d)[10:] == 9.0)
+    assert np.all(device.read_array(pool, np.uint8, P.pool.size).reshape(P.pool.shape)[3] == 0x3C)
+
+
 # ---- decode attention -------------------------------------------------------------------------------
 
 
@@ -710,6 +749,11 @@ def test_refusals(device, up):
     fails("NULL argument", lambda: cache.read(b, None, b, b, b, **ok))
     fails("layer 1 of 1", lambda: cache.read(b, b, b, b, b, layer=1, **ok), _lib.EgRangeError)
     fails("NULL argument", lambda: cache.copy_pages(None, 1))
+    fails("rows over the grid limit", lambda: cache.read(b, b, b, b, b, rows=1 << 29, sequences=1, max_pages=1),
+          _lib.EgRangeError)
+    cache.dims.page_stride = 1 << 50  # (times the count, past 64 bits)
+    fails("over the grid limit", lambda: cache.copy_pages(b, 1 << 27), _lib.EgRangeError)
+    cache.dims.page_stride = kv4.page_bytes(2, 64, 64)
     pk = dict(sequences=1, rows=1, key_rows=1, heads=2, kv_heads=1, head_dim=64)
     call = lambda **change: kv4.attention_packed(device, b, b, b, b, b, b, **{**pk, **change})  # noqa: E731
     fails("head_dim 80 is not supported", lambda: call(head_dim=80))
