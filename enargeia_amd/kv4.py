@@ -22,8 +22,8 @@ import struct
 import numpy as np
 
 from . import _lib
-from ._lib import EG_ERR_INVALID, EG_ERR_RANGE, EgError, EgRangeError, check
-from .kernels import Device, _ptr
+from ._lib import EG_ERR_INVALID, EG_ERR_RANGE, EG_ERR_STATE, EgError, EgRangeError, check
+from .kernels import Buffer, Device, _ptr
 
 ELEMENTS = {"f32": 0, "f16": 1, "bf16": 2}  # eg_element
 NO_PAGE = 0xFFFFFFFF
@@ -81,6 +81,8 @@ class Kv4Cache:
 
     def __init__(self, device: Device, kv_heads: int, head_dim: int, pages: int, page_size: int = 64,
                  layers: int = 1, pool=None):
+        if pages < 1 or layers < 1:
+            raise EgRangeError(EG_ERR_RANGE, f"kv4: a pool of {pages} pages of {layers} layers")
         self.device = device
         self.layer_bytes = page_bytes(kv_heads, head_dim, page_size)
         self.dims = Kv4Dims(kv_heads, head_dim, page_size, pages, self.layer_bytes * layers, 0, 0)
@@ -88,13 +90,20 @@ class Kv4Cache:
         lib = _lib.load()  # (bound once: a small call's time is its host path)
         self._append, self._read, self._attend = lib.eg_kv4_append, lib.eg_kv4_read, lib.eg_attention_decode_kv4
         self.layers = layers
-        self.owned = device.buffer(self.dims.page_stride * pages, "kv4 pool") if pool is None else None
+        size = self.dims.page_stride * pages
+        held = pool.size if isinstance(pool, Buffer) else getattr(pool, "nbytes", None)
+        if held is not None and held < size:
+            raise EgRangeError(EG_ERR_RANGE, f"kv4: a pool of {held} bytes for {pages} pages of {self.dims.page_stride}")
+        self.owned = device.buffer(size, "kv4 pool") if pool is None else None
         self.pool = self.owned if pool is None else pool
 
     def _at(self, layer: int) -> int:
         if not 0 <= layer < self.layers:
             raise EgRangeError(EG_ERR_RANGE, f"kv4: layer {layer} of {self.layers}")
-        return _address(self.pool) + layer * self.layer_bytes
+        base = _address(self.pool)
+        if not base:  # (an offset from nowhere would not be NULL)
+            raise EgError(EG_ERR_STATE, "kv4: the pool has been released")
+        return base + layer * self.layer_bytes
 
     def _for(self, sequences: int, max_pages: int):
         d = self.dims
@@ -144,7 +153,7 @@ class Kv4Cache:
     def release(self) -> None:
         if self.owned is not None:
             self.owned.release()
-            self.owned = None
+            self.owned = self.pool = None
 
 
 def attention_packed(device: Device, q, k, v, out, q_offsets, k_offsets, *, sequences: int, rows: int, key_rows: int,
@@ -229,7 +238,7 @@ class PageTable:
     def compact(self) -> int:
         """The used pages moved together at the pool's beginning (into `copies`); how many they are."""
         if self.copies:
-            raise EgError(_lib.EG_ERR_STATE, "kv4: copies of forks are pending (take_copies first)")
+            raise EgError(EG_ERR_STATE, "kv4: copies of forks are pending (take_copies first)")
         used = [p for p, n in enumerate(self.users) if n]
         holes = [p for p in range(len(used)) if not self.users[p]]
         moved = dict(zip([p for p in used if p >= len(used)], holes))

@@ -5,6 +5,7 @@ import pytest
 
 from enargeia_amd import kv4
 from enargeia_amd._lib import EgError, EgRangeError
+from enargeia_amd.kernels import Buffer
 from kv4_reference import Pages, held, quantize, random_pages, scale_of
 
 
@@ -125,3 +126,32 @@ def test_dimensions_out_of_range():
         cache.attend(0, 0, 0, 0, heads=1 << 32, sequences=1, max_pages=1)
     with pytest.raises(EgRangeError, match="layer 1 of 1"):
         cache.read(0, 0, 0, 0, 0, rows=1, sequences=1, max_pages=1, layer=1)
+
+
+def test_pools_too_small_or_released():
+    class Device:
+        ctx = None
+
+        def buffer(self, size, label=""):
+            return Buffer(self, 1 << 20, size, label)
+
+    size = 4 * kv4.page_bytes(1, 64, 32) * 2
+    with pytest.raises(EgRangeError, match=f"a pool of {size - 1} bytes for 4 pages of {size // 4}"):
+        kv4.Kv4Cache(Device(), 1, 64, 4, 32, layers=2, pool=Buffer(Device(), 1 << 20, size - 1))
+    with pytest.raises(EgRangeError, match="a pool of"):
+        kv4.Kv4Cache(Device(), 1, 64, 4, 32, layers=2, pool=np.zeros(size - 1, np.uint8))
+    with pytest.raises(EgRangeError, match="a pool of 0 pages of 2 layers"):
+        kv4.Kv4Cache(Device(), 1, 64, 0, 32, layers=2)
+    pool = Buffer(Device(), 1 << 20, size)
+    cache = kv4.Kv4Cache(Device(), 1, 64, 4, 32, layers=2, pool=pool)
+    pool.ptr = 0  # released by its owner
+    for call in (lambda: cache.read(0, 0, 0, 0, 0, rows=1, sequences=1, max_pages=1, layer=1),
+                 lambda: cache.append(0, 0, 0, 0, 0, rows=1, sequences=1, max_pages=1, layer=1),
+                 lambda: cache.attend(0, 0, 0, 0, heads=1, sequences=1, max_pages=1, layer=1)):
+        with pytest.raises(EgError, match="the pool has been released"):
+            call()
+    owner = kv4.Kv4Cache(Device(), 1, 64, 4, 32, layers=2)
+    owner.owned.ptr = 0  # (nothing of a device to free)
+    owner.release()
+    with pytest.raises(EgError, match="the pool has been released"):
+        owner.read(0, 0, 0, 0, 0, rows=1, sequences=1, max_pages=1, layer=1)
