@@ -472,12 +472,13 @@ int eg_kv4_append(eg_context* ctx, const void* q, const void* k, const void* v, 
   if (!ctx) return eg::fail(nullptr, EG_ERR_INVALID, "%s: ctx is NULL", op);
   const int st = eg_kv4::check_dims(ctx, op, dims, pool);
   if (st != EG_OK) return st;
-  if (!append || !k || !v || !offsets || !starts || !table)
+  const bool some = append && append->rows != 0 && dims->sequences != 0;
+  if (!append || (some && (!k || !v || !offsets || !starts || !table)))
     return eg::fail(ctx, EG_ERR_INVALID, "%s: NULL argument", op);
   const eg_kv4_append_dims& d = *append;
   if (!known_type(d.in_type) || !known_type(d.out_type))
     return eg::fail(ctx, EG_ERR_INVALID, "%s: in_type %d, out_type %d (eg_element)", op, d.in_type, d.out_type);
-  if ((q == nullptr) != (q_out == nullptr) || (q == nullptr) != (d.heads == 0))
+  if (some && ((q == nullptr) != (q_out == nullptr) || (q == nullptr) != (d.heads == 0)))
     return eg::fail(ctx, EG_ERR_INVALID, "%s: q, q_out and heads go together", op);
   if (d.heads > 65535) return eg::fail(ctx, EG_ERR_RANGE, "%s: %u heads (at most 65535)", op, d.heads);
   const uint32_t width = dims->kv_heads * dims->head_dim, q_width = d.heads * dims->head_dim;
@@ -491,7 +492,7 @@ int eg_kv4_append(eg_context* ctx, const void* q, const void* k, const void* v, 
   if (!aligned(q) || !aligned(k) || !aligned(v) || !aligned(rope) || !aligned(q_out) || !aligned(k_out) ||
       !aligned(v_out))
     return eg::fail(ctx, EG_ERR_INVALID, "%s: q, k, v, rope and the outputs must be 16-byte aligned", op);
-  if (d.rows == 0 || dims->sequences == 0) return EG_OK;
+  if (!some) return EG_OK;
   if (d.rows >= (1u << 30)) return eg::fail(ctx, EG_ERR_RANGE, "%s: %u rows (under 2^30)", op, d.rows);
   const eg_kv4::Pool p = eg_kv4::pool_of(*dims, pool, table);
   const uint64_t kv_blocks = (uint64_t)((d.rows + a.span - 1) / a.span) * a.kv_groups;
@@ -500,6 +501,7 @@ int eg_kv4_append(eg_context* ctx, const void* q, const void* k, const void* v, 
     return eg::fail(ctx, EG_ERR_RANGE, "%s: %u rows of %u kv heads over the grid limit", op, d.rows, dims->kv_heads);
   a.kv_blocks = (uint32_t)kv_blocks;
   const dim3 grid((uint32_t)blocks);
+  const OnDevice on(ctx);
   with_type(d.in_type, [&](auto ti) {
     with_type(d.out_type, [&](auto to) {
       if (dims->head_dim == 64)
@@ -517,11 +519,13 @@ int eg_kv4_read(eg_context* ctx, const uint32_t* offsets, const uint32_t* starts
   if (!ctx) return eg::fail(nullptr, EG_ERR_INVALID, "%s: ctx is NULL", op);
   const int st = eg_kv4::check_dims(ctx, op, dims, pool);
   if (st != EG_OK) return st;
-  if (!offsets || !starts || !table || !k_out || !v_out) return eg::fail(ctx, EG_ERR_INVALID, "%s: NULL argument", op);
+  const bool some = rows != 0 && dims->sequences != 0;
+  if (some && (!offsets || !starts || !table || !k_out || !v_out))
+    return eg::fail(ctx, EG_ERR_INVALID, "%s: NULL argument", op);
   if (!known_type(out_type)) return eg::fail(ctx, EG_ERR_INVALID, "%s: out_type %d (eg_element)", op, out_type);
   if (!aligned(k_out) || !aligned(v_out))
     return eg::fail(ctx, EG_ERR_INVALID, "%s: the outputs must be 16-byte aligned", op);
-  if (rows == 0 || dims->sequences == 0) return EG_OK;
+  if (!some) return EG_OK;
   if (rows >= (1u << 30)) return eg::fail(ctx, EG_ERR_RANGE, "%s: %u rows (under 2^30)", op, rows);
   const bool few = rows <= kFewRows;
   const ReadArgs a{offsets, starts, k_out, v_out, rows, few ? 1u : 32u};
@@ -529,6 +533,7 @@ int eg_kv4_read(eg_context* ctx, const uint32_t* offsets, const uint32_t* starts
   const dim3 grid((rows + a.span - 1) / a.span, (2 * dims->kv_heads + 3) / 4);
   if (grid.x >= (1u << 31) / kThreads)
     return eg::fail(ctx, EG_ERR_RANGE, "%s: %u rows over the grid limit", op, rows);
+  const OnDevice on(ctx);
   with_type(out_type, [&](auto to) {
     using TO = decltype(to);
     const auto kernel = dims->head_dim == 64 ? (few ? read_kernel<64, 8, TO> : read_kernel<64, 32, TO>)
@@ -549,6 +554,7 @@ int eg_kv4_copy_pages(eg_context* ctx, void* pool, const uint32_t* pairs, uint32
   if (parts > ((1ull << 31) / kThreads - 1) / count)
     return eg::fail(ctx, EG_ERR_RANGE, "%s: %u pages of %llu bytes over the grid limit", op, count,
                     (unsigned long long)dims->page_stride);
+  const OnDevice on(ctx);
   hipLaunchKernelGGL(copy_pages_kernel, dim3((uint32_t)(parts * count)), dim3(kThreads), 0, ctx->stream,
                      static_cast<uint8_t*>(pool), pairs, dims->pages, dims->page_stride, (uint32_t)parts);
   return eg::check_launch(ctx, op);

@@ -44,6 +44,23 @@ inline uint64_t page_bytes(const eg_kv4_dims& d) {
   return (uint64_t)d.kv_heads * d.page_size * (d.head_dim + d.head_dim / 8);
 }
 
+// The context's device as the current one while a call launches.
+class OnDevice {
+ public:
+  explicit OnDevice(const eg_context* ctx) {
+    int now = ctx->device;
+    if (hipGetDevice(&now) == hipSuccess && now != ctx->device && hipSetDevice(ctx->device) == hipSuccess) before_ = now;
+  }
+  ~OnDevice() {
+    if (before_ >= 0) (void)hipSetDevice(before_);
+  }
+  OnDevice(const OnDevice&) = delete;
+  OnDevice& operator=(const OnDevice&) = delete;
+
+ private:
+  int before_ = -1;
+};
+
 // The checks every entry point over a pool makes.
 int check_dims(eg_context* ctx, const char* op, const eg_kv4_dims* dims, const void* pool);
 

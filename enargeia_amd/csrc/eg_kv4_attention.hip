@@ -480,7 +480,8 @@ extern "C" int eg_attention_decode_kv4(eg_context* ctx, const void* q, const uin
   if (!ctx) return eg::fail(nullptr, EG_ERR_INVALID, "%s: ctx is NULL", op);
   const int st = eg_kv4::check_dims(ctx, op, dims, pool);
   if (st != EG_OK) return st;
-  if (!attention || !q || !lengths || !table || !out) return eg::fail(ctx, EG_ERR_INVALID, "%s: NULL argument", op);
+  if (!attention || (dims->sequences != 0 && (!q || !lengths || !out || (dims->max_pages != 0 && !table))))
+    return eg::fail(ctx, EG_ERR_INVALID, "%s: NULL argument", op);
   const eg_attention_kv4_dims& d = *attention;
   if (!known_type(d.type)) return eg::fail(ctx, EG_ERR_INVALID, "%s: type %d (eg_element)", op, d.type);
   if (d.heads == 0 || d.heads % dims->kv_heads != 0 || d.heads > 65535)
@@ -528,6 +529,7 @@ extern "C" int eg_attention_decode_kv4(eg_context* ctx, const void* q, const uin
   // The most that the call can read: what the tables reach, and what the pool holds.
   const uint64_t reach = std::min<uint64_t>((uint64_t)dims->sequences * dims->max_pages, dims->pages) * eg_kv4::page_bytes(*dims);
   const bool stream = reach > kInfinityCache;
+  const OnDevice on(ctx);
   with_type(d.type, [&](auto t) {
     using TQ = decltype(t);
     const uint64_t blocks = rows * splits;

@@ -485,7 +485,8 @@ extern "C" int eg_attention_packed(eg_context* ctx, const void* q, const void* k
                                    const eg_attention_packed_dims* dims) {
   const char* op = "attention_packed";
   if (!ctx) return eg::fail(nullptr, EG_ERR_INVALID, "%s: ctx is NULL", op);
-  if (!dims || !q || !k || !v || !q_offsets || !k_offsets || !out)
+  const bool some = dims && dims->rows != 0 && dims->sequences != 0;
+  if (!dims || (some && (!q || !q_offsets || !k_offsets || !out || (dims->key_rows != 0 && (!k || !v)))))
     return eg::fail(ctx, EG_ERR_INVALID, "%s: NULL argument", op);
   const eg_attention_packed_dims& d = *dims;
   if (d.head_dim != 64 && d.head_dim != 128)
@@ -517,7 +518,7 @@ extern "C" int eg_attention_packed(eg_context* ctx, const void* q, const void* k
     return eg::fail(ctx, EG_ERR_RANGE, "%s: %u sequences (at most 2^20)", op, d.sequences);
   if (d.rows >= (1u << 30) || d.key_rows >= (1u << 30))
     return eg::fail(ctx, EG_ERR_RANGE, "%s: %u rows, %u key rows (under 2^30)", op, d.rows, d.key_rows);
-  if (d.rows == 0 || d.sequences == 0) return EG_OK;
+  if (!some) return EG_OK;
   // at most this many query blocks, whatever the lengths
   const uint64_t blocks = (uint64_t)d.rows / kQueries + std::min<uint64_t>(d.sequences, d.rows);
   // (a kv head's items rounded up to its XCDs)
@@ -551,6 +552,7 @@ extern "C" int eg_attention_packed(eg_context* ctx, const void* q, const void* k
                          threads, 0, ctx->stream, a);
     }
   };
+  const eg_kv4::OnDevice on(ctx);
   if (d.type == EG_ELEMENT_F16) {
     if (d.out_type == EG_ELEMENT_F32) go(_Float16{}, float{});
     else go(_Float16{}, _Float16{});

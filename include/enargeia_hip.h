@@ -543,7 +543,7 @@ EG_API int eg_attention_prefill_f32(eg_context* ctx, const float* q, const float
  * memory, ascending) says where: sequence s has rows offsets[s] .. offsets[s + 1]. Rows outside
  * them are not used and not written. All tables, offsets, starts and lengths are read on the
  * device when the launch runs, so a captured graph follows them. Outputs overlap no input. Pointers to rows,
- * pools and rope tables are 16-byte aligned. */
+ * pools and rope tables are 16-byte aligned; those of arrays without an element may be NULL. */
 
 /* Element types of rows. */
 typedef enum eg_element { EG_ELEMENT_F32 = 0, EG_ELEMENT_F16 = 1, EG_ELEMENT_BF16 = 2 } eg_element;

@@ -771,6 +771,17 @@ def test_refusals(device, up):
     cache.append(b, b, b, b, b, rows=0, sequences=1, max_pages=1)
     cache.attend(b, b, b, b, heads=2, sequences=0, max_pages=0)
     cache.copy_pages(None, 0)
+    # nor are the pointers of arrays without an element
+    kv4.attention_packed(device, None, None, None, None, b, b, **{**pk, "rows": 0})
+    cache.append(None, None, b, b, b, heads=2, rows=0, sequences=1, max_pages=1)
+    cache.read(None, None, None, None, None, rows=0, sequences=0, max_pages=0)
+    cache.attend(None, None, None, None, heads=2, sequences=0, max_pages=0)
+    fails("NULL argument", lambda: kv4.attention_packed(device, b, None, None, b, b, b, **pk))
+    zeros, one = up(np.zeros(2, np.uint32)), up(np.array([0, 1], np.uint32))
+    out = up(np.full((2, 128), 9.0, np.float16))
+    kv4.attention_packed(device, b, None, None, out, one, zeros, **{**pk, "key_rows": 0})
+    cache.attend(b, zeros, None, K.Binding(out, 256), heads=2, sequences=1, max_pages=0, type="f16")
+    assert not device.read_array(out, np.float16, 256).any()
     device.sync()
 
 
