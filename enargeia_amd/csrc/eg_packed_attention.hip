@@ -44,7 +44,7 @@ struct Args {
   uint32_t sequences, rows, key_rows, heads, group, q_stride, k_stride, v_stride, out_stride;
   uint32_t xcds;  // XCDs a kv head, where kv heads are 1, 2 or 4; else 0
   // Keys split over workgroups: partials [row][head][split][D], unnormalised, and (max times scale, sum).
-  uint32_t splits, items;
+  uint32_t splits, items, xcd_cus;
   float *o, *ml;
   float scale;  // times log2 e
 };
@@ -153,7 +153,9 @@ __device__ __forceinline__ bool find_block(const Args& a, uint32_t id, uint32_t&
 // a kv head's keys and values are read by one XCD (of fewer than 8 kv heads, by 8 / kv_heads), its query
 // heads and blocks in ranks' order there.
 __device__ __forceinline__ void work_of(const Args& a, uint32_t id, uint32_t& rank, uint32_t& h) {
-  const uint32_t kv_heads = a.heads / a.group, xcd = id % 8u, turn = id / 8u;
+  const uint32_t kv_heads = a.heads / a.group, xcd = id % 8u;
+  uint32_t turn = id / 8u;
+  if (turn < a.xcd_cus && a.items >= 8u * a.xcd_cus) turn = a.xcd_cus - 1 - turn;
   if (a.xcds) {
     const uint32_t item = turn * a.xcds + xcd % a.xcds;
     rank = item / a.group;
@@ -163,8 +165,8 @@ __device__ __forceinline__ void work_of(const Args& a, uint32_t id, uint32_t& ra
     rank = turn / mine;
     h = (xcd + 8u * (i / a.group)) * a.group + i % a.group;
   } else {
-    rank = id / a.heads;
-    h = id % a.heads;
+    rank = (8u * turn + xcd) / a.heads;
+    h = (8u * turn + xcd) % a.heads;
   }
 }
 
@@ -266,14 +268,16 @@ __global__ __launch_bounds__(256, 2) void packed_kernel(Args a) {
     vat[n] = kVTile + vrow * kRow + 16 * ((4 * n + 2 * ((lane >> 4) & 1u) + ((li & 3u) >> 1)) ^ vswz(vrow)) + 8 * (li & 1u);
 
   f32x16 o[kBlocks];
-  float m, l;  // running max before the scale; this lane's share of the sum
+  float m, l, off;  // running max before the scale; this lane's share of the sum; the max after the scale
+  bool large;       // some query's is past kLargest: off is 0
   const auto run = [&](auto careful) {
 #pragma unroll
   for (int n = 0; n < kBlocks; n++)
 #pragma unroll
     for (int e = 0; e < 16; e++) o[n][e] = 0.f;
   m = -INFINITY;
-  l = 0.f;
+  l = off = 0.f;
+  large = false;
   if (first < stop) load_tile(first, first & 1u);
   settle();
   for (uint32_t t = first; t < stop; t++) {
@@ -319,31 +323,32 @@ __global__ __launch_bounds__(256, 2) void packed_kernel(Args a) {
           for (int e = 0; e < 16; e++)
             if ((int)(j0 + 32 * n + 8 * (e / 4) + 4 * lh + e % 4) >= limit) s[n][e] = -INFINITY;
       }
+      // The weights are relative to a max that may lag 2^kLag behind: it is taken up, and the accumulators
+      // rescaled, only where a score passes that (or is a query's first).
       float top = m;
 #pragma unroll
       for (int n = 0; n < 2; n++)
 #pragma unroll
         for (int e = 0; e < 16; e++) top = fmaxf(top, s[n][e]);
-      top = max_of_query(top);
-      // The weights are relative to a max that may lag 2^kLag behind: the accumulators are rescaled only
-      // where a score passes that (or is a query's first).
       if (__builtin_amdgcn_ballot_w64((top - m) * a.scale > kLag) != 0) {
+        top = max_of_query(top);
         const float alpha = top > m ? __builtin_amdgcn_exp2f((m - top) * a.scale) : 1.f;
         l *= alpha;
 #pragma unroll
         for (int n = 0; n < kBlocks; n++) o[n] *= alpha;
         m = top;
+        off = m == -INFINITY ? 0.f : m * a.scale;
+        large = __builtin_amdgcn_ballot_w64(fabsf(off) > kLargest) != 0;
+        if (large) off = 0.f;
       }
-      float off = m == -INFINITY ? 0.f : m * a.scale;
       // (past kLargest the max's own rounding would put weights out of range: there it is taken from the scores
       // instead)
-      if (__builtin_amdgcn_ballot_w64(fabsf(off) > kLargest) != 0) {
+      if (large) {
         const float from = m == -INFINITY ? 0.f : m;
 #pragma unroll
         for (int n = 0; n < 2; n++)
 #pragma unroll
           for (int e = 0; e < 16; e++) s[n][e] -= from;
-        off = 0.f;
       }
       const auto add_values = [&](auto cleaned) {
         const auto weights = [&](int k) {  // of keys 16 k .. +16 of the tile, as far as this lane has them
@@ -503,7 +508,7 @@ extern "C" int eg_attention_packed(eg_context* ctx, const void* q, const void* k
   Args a{q, k, v, out, q_offsets, k_offsets, d.sequences, d.rows, d.key_rows, d.heads, d.heads / d.kv_heads,
          d.q_stride ? d.q_stride : width, d.k_stride ? d.k_stride : kv_width, d.v_stride ? d.v_stride : kv_width,
          d.out_stride ? d.out_stride : width,
-         d.kv_heads <= 4 && d.kv_heads != 3 ? 8 / d.kv_heads : 0, 1, 0, nullptr, nullptr,
+         d.kv_heads <= 4 && d.kv_heads != 3 ? 8 / d.kv_heads : 0, 1, 0, (uint32_t)ctx->cu_count / 8, nullptr, nullptr,
          std::max((d.scale > 0.f ? d.scale : 1.0f / sqrtf((float)d.head_dim)) * kLog2e, 0x1p-126f)};
   if (a.q_stride < width || a.out_stride < width || a.k_stride < kv_width || a.v_stride < kv_width ||
       (a.q_stride | a.k_stride | a.v_stride | a.out_stride) % 8)
@@ -532,21 +537,21 @@ extern "C" int eg_attention_packed(eg_context* ctx, const void* q, const void* k
   const uint64_t resident = 2ull * ctx->cu_count;
   const uint64_t tiles = (uint64_t)d.key_rows / d.sequences / kKeys, row_bytes = (uint64_t)d.rows * d.heads * (d.head_dim + 2) * 4;
   const uint64_t splits = std::min({resident / (blocks * d.heads), tiles / kSplitTiles, (eg::kPartialsBytes - 64) / row_bytes});
+  a.items = (uint32_t)((items + 7) / 8 * 8);
   if (splits >= kLeastSplits) {
     a.splits = (uint32_t)splits;
-    a.items = (uint32_t)((items + 7) / 8 * 8);
     a.ml = reinterpret_cast<float*>(eg::partials(ctx));
     a.o = a.ml + (((size_t)d.rows * d.heads * splits * 2 + 3) & ~(size_t)3);
   }
   const auto go = [&](auto t, auto to) {
     using T = decltype(t);
     using TO = decltype(to);
-    const dim3 whole((uint32_t)items), threads(kThreads);
+    const dim3 whole(a.items), threads(kThreads);
     if (a.splits > 1) {
       hipLaunchKernelGGL((d.head_dim == 64 ? packed_kernel<64, true, T, TO> : packed_kernel<128, true, T, TO>),
                          dim3(a.items * a.splits), threads, 0, ctx->stream, a);
       hipLaunchKernelGGL((d.head_dim == 64 ? join_kernel<64, T, TO> : join_kernel<128, T, TO>),
-                         dim3((uint32_t)items * d.head_dim / 8), threads, 0, ctx->stream, a);
+                         dim3(a.items * d.head_dim / 8), threads, 0, ctx->stream, a);
     } else {
       hipLaunchKernelGGL((d.head_dim == 64 ? packed_kernel<64, false, T, TO> : packed_kernel<128, false, T, TO>), whole,
                          threads, 0, ctx->stream, a);
