@@ -8,14 +8,16 @@
 // O^T = V^T P^T: a lane holds one query's scores (rows of S^T: 4 consecutive keys of every 8), which
 // are the second product's B operand where they lie, with V^T read from LDS transposed.
 //
-// Bound by the SIMDs' issue of both units. A wave and tile of 64 keys take 1024 (head_dim 128) or 512 (64)
-// cycles of the matrix cores and 700 to 750 of vector instructions (32 exponentials of 8 cycles, the rest 4 each);
-// run together, a product holds back about 13 cycles of vector instructions. MI355X: a prompt of 8192, 32 / 8
-// heads of 128, bf16: 504 us, 1090 TFLOP/s (a library product of 8192 reaches 1435 on the card), the
-// matrix cores busy 55% of 960,000 cycles and the vector units 52%; 14 heads of 64, f16: 153 us, 780 TFLOP/s; 8
-// prompts of up to 2048, 14 heads of 64: 50 us. Tried and slower at 8192: two groups of four waves half a
-// step apart, one at its products while the other is at its softmax (550 us); the next tile's scores
-// before this one's softmax (832, for the registers); row sums by a product with ones or by dot products (528, 518).
+// Bound by the SIMDs' issue of both units, and at length by power: the clock falls from 2.4 to 1.9 GHz. A wave and
+// tile of 64 keys take 1024 (head_dim 128) or 512 (64) cycles of the matrix cores and 750 to 780 of vector
+// instructions (32 exponentials of 8 cycles, the rest 4 each), together 2050 (two waves a SIMD) and 1220 (three).
+// MI355X: a prompt of 8192, 32 / 8 heads of 128, bf16: 514 us, 1070 TFLOP/s (a library product of 8192 reaches 1435
+// on the card), the matrix cores busy 53% of 1,000,000 cycles; 14 heads of 64, f16: 147 us, 820 TFLOP/s; 8 prompts of
+// up to 2048, 14 heads of 64: 49 us. Tried and slower at 8192: two groups of four waves half a step apart, one at its
+// products while the other is at its softmax (550 us); the next tile's scores among this one's softmax (832, and 950
+// with one wave a SIMD); 64 queries a wave (head_dim 64, 206 us); row sums by a product with ones or by dot products
+// (528, 518). Reading V before the softmax, or keeping the reads of V from waiting for the other buffer's loads,
+// changes 1% either way.
 #include <algorithm>
 
 #include "eg_kv4.hpp"
@@ -44,7 +46,8 @@ struct Args {
   uint32_t sequences, rows, key_rows, heads, group, q_stride, k_stride, v_stride, out_stride;
   uint32_t xcds;  // XCDs a kv head, where kv heads are 1, 2 or 4; else 0
   // Keys split over workgroups: partials [row][head][split][D], unnormalised, and (max times scale, sum).
-  uint32_t splits, items, xcd_cus;
+  uint32_t splits, items;
+  uint32_t xcd_cus;  // CUs of an XCD
   float *o, *ml;
   float scale;  // times log2 e
 };
@@ -151,7 +154,9 @@ __device__ __forceinline__ bool find_block(const Args& a, uint32_t id, uint32_t&
 
 // The query block (its rank) and head of this workgroup. Workgroups go to the 8 XCDs in turn, each with its own L2:
 // a kv head's keys and values are read by one XCD (of fewer than 8 kv heads, by 8 / kv_heads), its query
-// heads and blocks in ranks' order there.
+// heads and blocks in ranks' order there - but for the first, one a CU, which go the other way: the workgroups after
+// them go to the same CUs in the same order, so the CU with the fewest keys of the first gets the most of the
+// second. A prompt of 8192, 14 heads of 64: 147 us for 157, 32 heads of 128 and 2048: 46.9 for 50.0.
 __device__ __forceinline__ void work_of(const Args& a, uint32_t id, uint32_t& rank, uint32_t& h) {
   const uint32_t kv_heads = a.heads / a.group, xcd = id % 8u;
   uint32_t turn = id / 8u;
