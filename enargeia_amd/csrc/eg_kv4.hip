@@ -216,6 +216,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a, Pool pool) {
   TO* dst = static_cast<TO*>(is_k ? a.k_out : a.v_out);
   const uint32_t stride = is_k ? a.k_stride : a.v_stride, out_stride = kvh * D;
   const Layout at = layout<D>(1u << pool.page_shift);
+  const uint32_t scales_at = is_k ? at.k_scales : at.v_scales;  // (chosen in the lambda it goes through memory)
 
   for_blocks<8>(a.offsets, a.starts, pool.sequences, a.rows, r0, a.span,
                 [&](uint32_t seq, uint32_t row, uint32_t position, uint32_t n) {
@@ -291,7 +292,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a, Pool pool) {
         *word = vword;
       }
       if ((lane & 31u) < n)
-        reinterpret_cast<uint16_t*>(block + (is_k ? at.k_scales : at.v_scales))
+        reinterpret_cast<uint16_t*>(block + scales_at)
             [(group << pool.page_shift) + slot + (lane & 31u)] = (uint16_t)my_scale;
     }
   });
