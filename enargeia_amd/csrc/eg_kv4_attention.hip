@@ -15,10 +15,11 @@
 // K codes go into the first product as they are: four bits at the bottom of an f16 are a denormal,
 // code * 2^-24 (2^-20 for the nibble above, whose queries are divided by 16), which the matrix cores
 // multiply exactly. (For f32 rows as code - 8 in f16, 9 instructions per word: what the sum and its start
-// at -8 times the queries leave of each other is off by 2e-6 of the result, these by 2e-7.) A group of 32 dims is one product's depth, so its accumulator, started at -8 times
-// the sum of the queries, is sum q (code - 8), and the scale is applied to it: 5 vector instructions
-// per word of 8 codes. V's scale differs along the second product's depth, so V is dequantized: (1024 +
-// code) - 1032 in f16, times the scale - exact by the format - 13 instructions per word.
+// at -8 times the queries leave of each other is off by 2e-6 of the result, these by 2e-7.) A group of
+// 32 dims is one product's depth, so its accumulator, started at -8 times the sum of the queries, is
+// sum q (code - 8), and the scale is applied to it: 5 vector instructions per word of 8 codes. V's scale
+// differs along the second product's depth, so V is dequantized: (1024 + code) - 1032 in f16, times the
+// scale - exact by the format - 13 instructions per word.
 //
 // Queries are scaled by a power of two that puts a head's largest into [2^14, 2^15), weights by 2^15:
 // an f16 and the f16 of what it leaves (kParts 2, for f32 rows) then hold 22 bits of them.
