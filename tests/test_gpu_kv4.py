@@ -602,6 +602,16 @@ def test_packed_prompts(device, up, nq, heads, kv, d, kind):
     check_packed(device, up, np.random.default_rng(sum(nq) + d), nq, nq, heads, kv, d, kind)
 
 
+@pytest.mark.parametrize("heads,kv", [(14, 2), (16, 16), (24, 3), (20, 5), (12, 1), (16, 4)])
+@pytest.mark.parametrize("sequences", [24, 70])
+def test_packed_more_workgroups_than_cus(device, up, sequences, heads, kv):
+    """Every query block is some workgroup's, however heads and blocks are laid over the XCDs."""
+    rng = np.random.default_rng(41)
+    nq = [int(n) for n in rng.integers(1, 60, sequences)]
+    nq[3], nq[5] = 300, 0
+    check_packed(device, up, rng, nq, nq, heads, kv, 64, "f16")
+
+
 @pytest.mark.parametrize("nq,nk", [([5], [300]), ([64, 1], [65, 1000]), ([200, 130], [330, 128]), ([3, 4], [0, 2]),
                                    ([300], [40])])
 def test_packed_chunks_after_earlier_rows_and_rows_that_see_nothing(device, up, nq, nk):
