@@ -559,14 +559,14 @@ typedef struct eg_kv4_dims {
 EG_API int eg_kv4_page_bytes(const eg_kv4_dims* dims, uint64_t* out_bytes);
 
 /* A batch's new rows into the cache. Row r of sequence s is at position starts[s] + r - offsets[s];
- * a page that rows go to is one sequence's alone in the call (pages that forks share are only read). With `rope` ([rope_positions][head_dim / 2]
- * pairs (cos, sin) of f32) q and k are rotated by their position's row in half-rotation pairing,
- * each product rounded on its own; k (rotated) and v go into the pages. The outputs are packed rows
- * in out_type: q_out [rows][heads][head_dim] (q rotated), k_out and v_out [rows][kv_heads][head_dim]
- * (k rotated, v as it is: unquantized). q and q_out go together and may be NULL, k_out and v_out each may be;
- * rope may be NULL (no rotation). A row whose position the table or the rope does not reach is
- * skipped: nothing of it is written; one whose table entry is no page has its outputs, but is not stored.
- * Positions of a page that no row names keep their values. */
+ * a page that rows go to is one sequence's alone in the call (pages that forks share are only read).
+ * With `rope` ([rope_positions][head_dim / 2] pairs (cos, sin) of f32) q and k are rotated by their
+ * position's row in half-rotation pairing, each product rounded on its own; k (rotated) and v go into
+ * the pages. The outputs are packed rows in out_type: q_out [rows][heads][head_dim] (q rotated), k_out
+ * and v_out [rows][kv_heads][head_dim] (k rotated, v as it is: unquantized). q and q_out go together
+ * and may be NULL, k_out and v_out each may be; rope may be NULL (no rotation). A row whose position
+ * the table or the rope does not reach is skipped: nothing of it is written; one whose table entry is
+ * no page has its outputs, but is not stored. Positions of a page that no row names keep their values. */
 typedef struct eg_kv4_append_dims {
   uint32_t rows, heads;                  /* rows of q, k and v; query heads (0 without q)        */
   uint32_t q_stride, k_stride, v_stride; /* elements from row to row, multiples of 4; 0: dense   */
