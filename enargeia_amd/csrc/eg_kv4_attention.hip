@@ -137,7 +137,7 @@ __device__ __forceinline__ u32x4 first_halves(u32x4 v, int n) {
 // (Two waves per SIMD: their registers hold two steps' operands each, one step's loads under way while
 // the other is multiplied.)
 // kStream: codes are read past the caches' retention (non-temporal), for a cache larger than the Infinity
-// Cache: 32 sequences of 16384 (32 / 8 heads of 128) 96.9 us for 106.6, but 16 of up to 8192 27.3 for 25.7.
+// Cache: 32 sequences of 16384 (32 / 8 heads of 128) 94.4 us for 106.5, but 16 of up to 8192 26.0 for 24.6.
 template <int D, int T, int kParts, bool kStream, class TQ>
 __global__ __launch_bounds__(256, 2) void decode_kernel(Args a, Pool pool) {
   constexpr int kGroups = D / 32, kBlocks = D / 16;  // dim groups of K; blocks of 16 dims of O^T
@@ -509,15 +509,16 @@ extern "C" int eg_attention_decode_kv4(eg_context* ctx, const void* q, const uin
   // Two key tiles a step where the heads leave room for them (and a step's 64 positions lie in one page).
   const bool pair = a.group <= 8 && dims->page_size >= 64;
   a.head_tiles = pair ? 1 : (a.group + 15) / 16;
-  // Splits: as many as the device holds at once (two workgroups per CU), of at least min_chunk positions, and
-  // none for tables that reach 1024. A workgroup's first loads wait for each other (length, page, rows) and
-  // the join is a launch, so more and shorter chunks cost more than they balance: 16 sequences of up to
-  // 8192 (28 / 4 heads of 128, f32) 28.9 us in 512 workgroups, 39.4 in 1024; 48 of 2048 (14 / 2 of 64) 11.2
-  // in chunks of 512, 13.1 in 256, 13.9 in 1024; 4 of 65536 (16 / 1 of 128, f16) 19.9 in chunks of 1024, 23.0 in
-  // 512; 1 of 517 6.8 whole, 9.0 in two (the second launch).
-  a.min_chunk = pair ? 512 : 1024;
-  const uint64_t rows = (uint64_t)dims->sequences * dims->kv_heads * a.head_tiles;
-  const uint64_t room = 2ull * ctx->cu_count / rows, most = (a.capacity + a.min_chunk - 1) / a.min_chunk;
+  // Splits, none for tables that reach 1024: chunks of at least two steps a wave. A workgroup's first loads wait for
+  // each other (length, page, rows) and the join is a launch, so shorter chunks cost more than they balance: 48
+  // sequences of 2048 (14 / 2 heads of 64) 11.1 us in chunks of 512, 13.9 in 1024, 13.1 in 256; 5 of 4000 (32 / 2 of 64,
+  // f16) 9.2 in 256, 9.9 in 512, 11.6 in 1024; 1 of 517 6.5 whole, 9.0 in two. Workgroups: two a CU, as the device
+  // holds at once (16 of up to 8192, 28 / 4 of 128, f32: 24.6 us, in twice as many 29.7), but of T = 1's one where the
+  // tables do not reach 1024 positions for each of two (4 of 65536, 16 / 1 of 128: 19.5 us, in a few more 21.8).
+  a.min_chunk = pair ? 512 : 256;
+  const uint64_t rows = (uint64_t)dims->sequences * dims->kv_heads * a.head_tiles, twice = 2ull * ctx->cu_count / rows;
+  const uint64_t room = pair || a.capacity >= 1024 * twice ? twice : ctx->cu_count / rows;
+  const uint64_t most = (a.capacity + a.min_chunk - 1) / a.min_chunk;
   uint64_t splits = a.capacity <= 1024 ? 1 : std::max<uint64_t>(1, std::min(room, most));
   const uint64_t per_split = (uint64_t)dims->sequences * d.heads * (dims->head_dim + 2) * 4;
   splits = std::max<uint64_t>(1, std::min<uint64_t>(splits, (eg::kPartialsBytes - 64) / per_split));
