@@ -35,7 +35,7 @@ using egd::u32x4;
 constexpr uint32_t kThreads = 256, kWaves = 4;
 constexpr uint32_t kQueries = 32 * kWaves;  // per workgroup
 constexpr uint32_t kKeys = 64;              // per tile
-constexpr uint32_t kSplitTiles = 8, kLeastSplits = 3;
+constexpr uint32_t kSplitTiles = 6, kLeastSplits = 3;
 constexpr float kLag = 8.f, kLargest = 0x1p20f;
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -537,8 +537,9 @@ extern "C" int eg_attention_packed(eg_context* ctx, const void* q, const void* k
     return eg::fail(ctx, EG_ERR_RANGE, "%s: %u rows of %u heads over the grid limit", op, d.rows, d.heads);
   // Few query blocks leave the device idle over long keys: each block's keys are then split over workgroups, as
   // many as make two workgroups a CU, of at least kSplitTiles of a sequence's tiles. 14 / 2 heads of 64: 256
-  // queries after 1792 rows 28.9 -> 15.8 us, twice 64 after 6000 75 -> 23.3; but for what the join costs, a prompt
-  // of 1024 in two splits takes 19.4 us for 17.5, and 4 of 500 after 2000 in two or three 40.4 for 36.3.
+  // queries after 1792 rows 28.9 -> 15.7 us, twice 64 after 6000 75 -> 21.6 (of at least 8 tiles 23.0; of 4 the first
+  // takes 16.6, and a prompt of 1024 18.8 for 15.9). Two splits, where no more fit, cost more in the join than they
+  // gain: 4 of 500 after 2000 37.6 for 33.9.
   const uint64_t resident = 2ull * ctx->cu_count;
   const uint64_t tiles = (uint64_t)d.key_rows / d.sequences / kKeys, row_bytes = (uint64_t)d.rows * d.heads * (d.head_dim + 2) * 4;
   const uint64_t splits = std::min({resident / (blocks * d.heads), tiles / kSplitTiles, (eg::kPartialsBytes - 64) / row_bytes});
