@@ -27,6 +27,7 @@ from .kernels import Buffer, Device, _ptr
 
 ELEMENTS = {"f32": 0, "f16": 1, "bf16": 2}  # eg_element
 NO_PAGE = 0xFFFFFFFF
+_MOST = 0xFFFFFFFF  # of a u32
 
 
 def _element(name: str) -> int:
@@ -67,8 +68,16 @@ def _packed(pack, *values) -> bytes:
         raise EgRangeError(EG_ERR_RANGE, f"kv4: a dimension out of range ({e})") from None
 
 
+def _fits(bits: int = 32, **values: int) -> None:
+    """Refuses what does not fit its field (ctypes would keep the low bits of it)."""
+    for name, x in values.items():
+        if not 0 <= x < 1 << bits:
+            raise EgRangeError(EG_ERR_RANGE, f"kv4: a dimension out of range ({name} {x}: 0 to 2^{bits} - 1)")
+
+
 def page_bytes(kv_heads: int, head_dim: int, page_size: int) -> int:
     """Bytes of one layer's page."""
+    _fits(kv_heads=kv_heads, head_dim=head_dim, page_size=page_size)
     out = ctypes.c_uint64()
     check(_lib.load().eg_kv4_page_bytes(ctypes.byref(Kv4Dims(kv_heads, head_dim, page_size, 0, 0, 0, 0)),
                                         ctypes.byref(out)), None)
@@ -85,6 +94,8 @@ class Kv4Cache:
             raise EgRangeError(EG_ERR_RANGE, f"kv4: a pool of {pages} pages of {layers} layers")
         self.device = device
         self.layer_bytes = page_bytes(kv_heads, head_dim, page_size)
+        _fits(pages=pages)
+        _fits(64, pool_bytes=self.layer_bytes * layers * pages)
         self.dims = Kv4Dims(kv_heads, head_dim, page_size, pages, self.layer_bytes * layers, 0, 0)
         self._dims = ctypes.byref(self.dims)
         lib = _lib.load()  # (bound once: a small call's time is its host path)
@@ -106,6 +117,8 @@ class Kv4Cache:
         return base + layer * self.layer_bytes
 
     def _for(self, sequences: int, max_pages: int):
+        if not (0 <= sequences <= _MOST and 0 <= max_pages <= _MOST):
+            _fits(sequences=sequences, max_pages=max_pages)
         d = self.dims
         d.sequences, d.max_pages = sequences, max_pages
         return self._dims
@@ -129,6 +142,8 @@ class Kv4Cache:
              layer: int = 0, out_type: str = "f16") -> None:
         """eg_kv4_read: cached rows as packed rows."""
         ctx = self.device.ctx
+        if not 0 <= rows <= _MOST:
+            _fits(rows=rows)
         status = self._read(ctx, _address(offsets), _address(starts), _address(table), self._at(layer),
                             _address(k_out), _address(v_out), rows, _element(out_type),
                             self._for(sequences, max_pages))
@@ -148,6 +163,7 @@ class Kv4Cache:
     def copy_pages(self, pairs, count: int) -> None:
         """eg_kv4_copy_pages: page pairs[i][0] to page pairs[i][1], all layers."""
         ctx = self.device.ctx
+        _fits(count=count)
         check(_lib.load().eg_kv4_copy_pages(ctx, self._at(0), _address(pairs), count, self._for(0, 0)), ctx)
 
     def release(self) -> None:

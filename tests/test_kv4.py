@@ -155,3 +155,41 @@ def test_pools_too_small_or_released():
     owner.release()
     with pytest.raises(EgError, match="the pool has been released"):
         owner.read(0, 0, 0, 0, 0, rows=1, sequences=1, max_pages=1, layer=1)
+
+
+def test_sizes_past_32_bits_are_refused():
+    """Not taken modulo 2^32, which is a call that returns with nothing done."""
+    class Device:
+        ctx = None
+
+    cache = kv4.Kv4Cache(Device, 1, 64, 4, 32, pool=1 << 20)
+    some = dict(rows=1, sequences=1, max_pages=1)
+    calls = [lambda **c: cache.read(0, 0, 0, 0, 0, **{**some, **c}), lambda **c: cache.append(0, 0, 0, 0, 0, **{**some, **c})]
+    for name in some:
+        for size in (1 << 32, (1 << 32) + 1, -1):
+            for call in calls:
+                with pytest.raises(EgRangeError, match="a dimension out of range"):
+                    call(**{name: size})
+    for name in ("sequences", "max_pages"):
+        with pytest.raises(EgRangeError, match=f"a dimension out of range .{name} 4294967296"):
+            cache.attend(0, 0, 0, 0, **{"heads": 1, "sequences": 1, "max_pages": 1, name: 1 << 32})
+    for count in (1 << 32, -1):
+        with pytest.raises(EgRangeError, match="a dimension out of range"):
+            cache.copy_pages(0, count)
+    # (the largest that fit are the library's to judge)
+    with pytest.raises(EgError, match="ctx is NULL"):
+        cache.read(0, 0, 0, 0, 0, rows=(1 << 32) - 1, sequences=(1 << 32) - 1, max_pages=(1 << 32) - 1)
+
+
+def test_pools_past_64_bits_are_refused():
+    class Device:
+        ctx = None
+
+    for change in (dict(kv_heads=(1 << 32) + 1), dict(head_dim=(1 << 32) + 64), dict(page_size=(1 << 32) + 32)):
+        with pytest.raises(EgRangeError, match="a dimension out of range"):
+            kv4.page_bytes(**{"kv_heads": 1, "head_dim": 64, "page_size": 32, **change})
+    size = kv4.page_bytes(1, 64, 32)
+    with pytest.raises(EgRangeError, match="pages 4294967300"):
+        kv4.Kv4Cache(Device, 1, 64, (1 << 32) + 4, 32, pool=1 << 20)
+    with pytest.raises(EgRangeError, match="pool_bytes"):  # (its stride modulo 2^64 is one layer's)
+        kv4.Kv4Cache(Device, 1, 64, 4, 32, layers=(1 << 64) // 256 + 1, pool=np.zeros(4 * size, np.uint8))
