@@ -221,7 +221,10 @@ class PageTable:
         return seq
 
     def grow(self, seq: int, rows: int) -> int:
-        """Room for `rows` more positions; the first one's position."""
+        """Room for `rows` more positions; the first one's position. (A sequence never shrinks: its next rows
+        could then lie in a page that a fork shares.)"""
+        if rows < 0:
+            raise EgRangeError(EG_ERR_RANGE, f"kv4: sequence {seq} cannot grow by {rows} rows")
         start = self.length[seq]
         need = -(-(start + rows) // self.page_size) - len(self.held[seq])
         if need > 0:

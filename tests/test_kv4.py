@@ -193,3 +193,17 @@ def test_pools_past_64_bits_are_refused():
         kv4.Kv4Cache(Device, 1, 64, (1 << 32) + 4, 32, pool=1 << 20)
     with pytest.raises(EgRangeError, match="pool_bytes"):  # (its stride modulo 2^64 is one layer's)
         kv4.Kv4Cache(Device, 1, 64, 4, 32, layers=(1 << 64) // 256 + 1, pool=np.zeros(4 * size, np.uint8))
+
+
+def test_sequences_do_not_shrink():
+    """Grown by fewer than no rows, a sequence kept its pages, and a fork of it shared one that both then wrote."""
+    t = kv4.PageTable(8, 32)
+    a = t.create()
+    t.grow(a, 64)
+    with pytest.raises(EgRangeError, match="cannot grow by -40 rows"):
+        t.grow(a, -40)
+    assert t.length[a] == 64 and t.held[a] == [0, 1] and t.grow(a, 0) == 64
+    b = t.fork(a)
+    t.grow(a, 1)
+    t.grow(b, 1)
+    assert t.held[a] == [0, 1, 2] and t.held[b] == [0, 1, 3]
