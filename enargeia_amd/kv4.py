@@ -203,11 +203,15 @@ class PageTable:
 
     @property
     def free_pages(self) -> int:
-        return self.users.count(0)
+        """Pages that can be given out now: the sources of pending copies are not, until those are taken."""
+        return len(self._free())
+
+    def _free(self) -> list[int]:
+        sources = {a for a, _ in self.copies}  # (still to be read, whoever held them)
+        return [p for p, n in enumerate(self.users) if n == 0 and p not in sources]
 
     def _take(self, count: int) -> list[int]:
-        sources = {a for a, _ in self.copies}  # (still to be read, whoever held them)
-        free = [p for p, n in enumerate(self.users) if n == 0 and p not in sources][:count]
+        free = self._free()[:count]
         if len(free) < count:
             raise EgRangeError(EG_ERR_RANGE, f"kv4: {count} pages wanted, {len(free)} of {self.pages} free")
         for p in free:

@@ -207,3 +207,19 @@ def test_sequences_do_not_shrink():
     t.grow(a, 1)
     t.grow(b, 1)
     assert t.held[a] == [0, 1, 2] and t.held[b] == [0, 1, 3]
+
+
+def test_free_pages_are_those_that_can_be_taken():
+    t = kv4.PageTable(3, 32)
+    a = t.create()
+    t.grow(a, 40)
+    t.fork(a)
+    t.free(a)  # its second page is free, but still to be copied from
+    c = t.create()
+    assert t.free_pages == 0
+    with pytest.raises(EgRangeError, match="1 pages wanted, 0 of 3 free"):
+        t.grow(c, 1)
+    t.take_copies()
+    assert t.free_pages == 1
+    t.grow(c, 1)
+    assert t.held[c] == [1] and t.free_pages == 0
