@@ -440,14 +440,21 @@ uint32_t query_span(uint32_t rows, uint32_t width) {
 
 }  // namespace
 
-int eg_kv4::check_dims(eg_context* ctx, const char* op, const eg_kv4_dims* d, const void* pool) {
-  if (!d || !pool) return eg::fail(ctx, EG_ERR_INVALID, "%s: NULL argument", op);
+// What a page's size follows from.
+static int check_format(eg_context* ctx, const char* op, const eg_kv4_dims* d) {
   if (d->head_dim != 64 && d->head_dim != 128)
     return eg::fail(ctx, EG_ERR_INVALID, "%s: head_dim %u is not supported (64, 128)", op, d->head_dim);
   if (d->page_size != 32 && d->page_size != 64 && d->page_size != 128 && d->page_size != 256)
     return eg::fail(ctx, EG_ERR_INVALID, "%s: page_size %u is not supported (32, 64, 128, 256)", op, d->page_size);
   if (d->kv_heads == 0 || d->kv_heads > 1024)
     return eg::fail(ctx, EG_ERR_INVALID, "%s: %u kv heads (1 to 1024)", op, d->kv_heads);
+  return EG_OK;
+}
+
+int eg_kv4::check_dims(eg_context* ctx, const char* op, const eg_kv4_dims* d, const void* pool) {
+  if (!d || !pool) return eg::fail(ctx, EG_ERR_INVALID, "%s: NULL argument", op);
+  const int st = check_format(ctx, op, d);
+  if (st != EG_OK) return st;
   if (d->pages == 0) return eg::fail(ctx, EG_ERR_INVALID, "%s: a pool of no pages", op);
   if (d->page_stride % 16 != 0 || d->page_stride < eg_kv4::page_bytes(*d))
     return eg::fail(ctx, EG_ERR_INVALID, "%s: page_stride %llu is not a multiple of 16 of at least %llu bytes", op,
@@ -465,6 +472,8 @@ extern "C" {
 
 int eg_kv4_page_bytes(const eg_kv4_dims* dims, uint64_t* out_bytes) {
   if (!dims || !out_bytes) return eg::fail(nullptr, EG_ERR_INVALID, "kv4_page_bytes: NULL argument");
+  const int st = check_format(nullptr, "kv4_page_bytes", dims);
+  if (st != EG_OK) return st;
   *out_bytes = eg_kv4::page_bytes(*dims);
   return EG_OK;
 }

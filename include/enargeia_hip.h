@@ -555,7 +555,7 @@ typedef struct eg_kv4_dims {
   uint32_t sequences, max_pages; /* the page table is [sequences][max_pages]                    */
 } eg_kv4_dims;
 
-/* Bytes of one layer's page (kv_heads, head_dim and page_size of dims). */
+/* Bytes of one layer's page (kv_heads, 1 to 1024, head_dim and page_size of dims; the rest is not looked at). */
 EG_API int eg_kv4_page_bytes(const eg_kv4_dims* dims, uint64_t* out_bytes);
 
 /* A batch's new rows into the cache. Row r of sequence s is at position starts[s] + r - offsets[s];

@@ -223,3 +223,20 @@ def test_free_pages_are_those_that_can_be_taken():
     assert t.free_pages == 1
     t.grow(c, 1)
     assert t.held[c] == [1] and t.free_pages == 0
+
+
+def test_formats_that_no_call_takes_have_no_size():
+    class Device:
+        ctx = None
+
+        def buffer(self, size, label=""):
+            raise AssertionError("a pool of an unknown format was allocated")
+
+    for match, change in (("head_dim 96 is not supported", dict(head_dim=96)), ("page_size 48 is not supported", dict(page_size=48)),
+                          ("0 kv heads", dict(kv_heads=0)), ("1025 kv heads", dict(kv_heads=1025))):
+        dims = {"kv_heads": 2, "head_dim": 64, "page_size": 32, **change}
+        with pytest.raises(EgError, match=match):
+            kv4.page_bytes(**dims)
+        with pytest.raises(EgError, match=match):
+            kv4.Kv4Cache(Device(), pages=4, **dims)
+    assert kv4.page_bytes(1024, 128, 256) == 1024 * 256 * 144
