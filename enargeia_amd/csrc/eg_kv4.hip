@@ -63,6 +63,8 @@ __device__ __forceinline__ uint32_t or_of_8(uint32_t v) {
 
 // The code (0..15) of this lane's value and the f16 bits of its group's scale; a group is 32 lanes.
 // The absmax is taken over the values' bits, which order magnitudes and put infinities and NaN on top.
+// Products with reciprocals, not divisions: they are what the format says (a division of f32 is some ten
+// instructions, and takes a value halfway between two codes to the other one now and then).
 __device__ __forceinline__ uint32_t quantize(float x, uint32_t& scale) {
 #pragma clang fp contract(off)
   const uint32_t top = max_of_32(__float_as_uint(x) & 0x7FFFFFFFu);

@@ -522,10 +522,13 @@ EG_API int eg_attention_prefill_f32(eg_context* ctx, const float* q, const float
  * cache is one sequence's contiguous f16 or f32 rows) -------------------------------------------
  *
  * The cache format kv4. A row is the head_dim (64 or 128) values of one position and kv head, of K
- * or of V, in groups of 32. A group's scale is absmax / 7 as f16, rounded half up to 8 significant
- * bits, at most 9344; a code is the value over the scale, rounded to nearest (even) and clamped to
- * -7..7; the value held is code * scale, exact in f16. A group with an infinity or a NaN has the
- * scale NaN, and all its values read as NaN. The scale of a group below about 2^-19 is 0.
+ * or of V, in groups of 32. A group's scale: its absmax times the f32 nearest to 1/7, rounded to f32,
+ * at most 9344, rounded to f16 (nearest, even), then half up to 8 significant bits (to a multiple of
+ * 2^-21 where that is coarser). A code: the value times the scale's reciprocal, both rounded to f32,
+ * rounded to the nearest integer (even) and clamped to -7..7. So a value halfway between two codes gets
+ * the one that its product falls to, which for about one scale in four is not the even one. The value held is
+ * code * scale, exact in f16. A group with an infinity or a NaN has the scale NaN, and all its values
+ * read as NaN. The scale of a group below about 2^-19 is 0, and so are its values.
  *
  * A pool is `pages` pages, page_stride bytes apart (one page may hold several layers: the pool
  * pointer of layer l is the first page's base + l * page bytes, page_stride all layers' bytes). A page holds

@@ -1,6 +1,8 @@
 """The 4-bit cache's format and the operators over it in numpy float64, written from their
 definitions (include/enargeia_hip.h), for the tests of the kernels."""
 
+from fractions import Fraction
+
 import numpy as np
 
 NO_PAGE = 0xFFFFFFFF
@@ -37,6 +39,47 @@ def rotate(x, cs):
     a, b = x[..., :h].astype(np.float32), x[..., h:].astype(np.float32)
     c, s = cs[:, None, :, 0], cs[:, None, :, 1]
     return np.concatenate([a * c - b * s, b * c + a * s], -1)
+
+
+def _nearest(x, bits, least):
+    """x (a Fraction) to `bits` significant bits, or to a multiple of 2^least where that is coarser: to
+    nearest, ties to even."""
+    if x == 0:
+        return x
+    e = abs(x).numerator.bit_length() - abs(x).denominator.bit_length()
+    if abs(x) < Fraction(2) ** e:
+        e -= 1
+    step = Fraction(2) ** max(e + 1 - bits, least)
+    return round(x / step) * step  # (round() of a Fraction takes ties to even)
+
+
+def by_the_text(group):
+    """Codes (0..15) and scale of 32 finite values by the header's words, in rational arithmetic."""
+    x = [Fraction(float(v)) for v in group]
+    f32 = lambda v: _nearest(v, 24, -149)  # noqa: E731
+    t = min(f32(max(abs(v) for v in x) * f32(Fraction(1, 7))), Fraction(9344))
+    t = _nearest(t, 11, -24)
+    step = Fraction(1, 1 << 21)
+    while t >= 256 * step:
+        step *= 2
+    s = (t / step + Fraction(1, 2)).__floor__() * step
+    if s == 0:
+        return [8] * len(x), 0.0
+    r = f32(1 / s)
+    return [max(-7, min(7, round(f32(v * r)))) + 8 for v in x], float(s)
+
+
+def halfway(rng):
+    """Groups of 32 values (f32) of every significand of a scale, with all the values halfway between two of
+    its codes, and that scale's codes by an exact division."""
+    significands = [(128 + i) / 128 for i in range(128)]
+    groups, divided = [], []
+    for i, m in enumerate(significands * 2):
+        s = m * 2.0 ** int(rng.integers(-12, 12) if i >= 128 else 0)
+        ties = np.array([c + 0.5 for c in range(-7, 7)] * 2 + [7.0, -7.0, 3.0, 0.0])
+        groups.append(np.asarray(ties * s, np.float32))
+        divided.append(np.rint(ties) + 8)
+    return np.stack(groups), np.stack(divided).astype(np.uint8)
 
 
 class Pages:

@@ -1,15 +1,40 @@
 """The operators over the paged 4-bit cache in the forms that only large or uneven calls take, against the
 same float64 references and bounds as tests/test_gpu_kv4.py: codes read past the caches (a reach over 256
-MiB), more steps than a wave holds page ids for, appends and reads of more than 2048 rows."""
+MiB), more steps than a wave holds page ids for, appends and reads of more than 2048 rows. And scales and
+codes by the header's words."""
 
 import numpy as np
 import pytest
 
 from enargeia_amd import kv4
-from kv4_reference import NO_PAGE, as_type, attend, from_type, random_pages
+from kv4_reference import NO_PAGE, as_type, attend, by_the_text, from_type, halfway, random_pages
 from test_gpu_kv4 import check_append, check_decode, decode_bound, kv4_size, up  # noqa: F401 (a fixture)
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+def test_scales_and_codes_by_the_headers_words(device, up, kind):  # noqa: F811
+    """Values halfway between two codes, of every scale's significand."""
+    ties, divided = halfway(np.random.default_rng(3))
+    d, page = 64, 64
+    x = ties.reshape(-1, d)
+    n = len(x)
+    raw, values = as_type(x, kind)
+    pages = -(-n // page)
+    cache = kv4.Kv4Cache(device, 1, d, pages, page, pool=up(pages * kv4.page_bytes(1, d, page)))
+    off, st, tb = up(np.array([0, n], np.uint32)), up(np.zeros(1, np.uint32)), up(np.arange(pages, dtype=np.uint32)[None])
+    b, k, v = up(raw), up(n * d * 4), up(n * d * 4)
+    cache.append(b, b, off, st, tb, rows=n, sequences=1, max_pages=pages, in_type=kind)
+    cache.read(k, v, off, st, tb, rows=n, sequences=1, max_pages=pages, out_type="f32")
+    want, by_division = [], []
+    for group, other in zip(values.reshape(-1, 32), divided):
+        codes, scale = by_the_text(group)
+        want.append((np.array(codes) - 8.0) * scale)
+        by_division.append((other - 8.0) * scale)
+    assert kind != "f32" or np.any(np.stack(want) != np.stack(by_division))
+    for o in (k, v):
+        np.testing.assert_array_equal(device.read_array(o, np.float32, n * d).reshape(-1, 32), np.stack(want))
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])

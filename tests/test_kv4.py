@@ -6,7 +6,7 @@ import pytest
 from enargeia_amd import kv4
 from enargeia_amd._lib import EgError, EgRangeError
 from enargeia_amd.kernels import Buffer
-from kv4_reference import Pages, held, quantize, random_pages, scale_of
+from kv4_reference import Pages, by_the_text, halfway, held, quantize, random_pages, scale_of
 
 
 def test_page_bytes():
@@ -240,3 +240,24 @@ def test_formats_that_no_call_takes_have_no_size():
         with pytest.raises(EgError, match=match):
             kv4.Kv4Cache(Device(), pages=4, **dims)
     assert kv4.page_bytes(1024, 128, 256) == 1024 * 256 * 144
+
+
+def test_scales_and_codes_by_the_headers_words():
+    """The arithmetic that the header states, in exact rationals: values halfway between two codes, values of
+    each type, the smallest and the largest scales."""
+    rng = np.random.default_rng(3)
+    ties, divided = halfway(rng)
+    groups = [ties]
+    for spread in (2.0 ** -20, 2.0 ** -18, 1e-3, 1.0, 300.0, 3e4, 1e9):
+        x = np.asarray(rng.standard_normal((60, 32)) * spread, np.float32)
+        with np.errstate(over="ignore"):
+            h = x.astype(np.float16).astype(np.float32)
+        groups += [x, h[np.isfinite(h).all(1)], (x.view(np.uint32) & 0xFFFF0000).view(np.float32)]
+    x = np.concatenate(groups)
+    codes, scales = quantize(x)
+    for row, c, s in zip(x, codes, scales[:, 0].astype(np.float64)):
+        want, scale = by_the_text(row)
+        assert s == scale and c.tolist() == want
+    # a value over its scale is another format: about one scale in four has ties that fall to the odd code
+    other = (codes[: len(ties)] != divided).any(1).mean()
+    assert 0.1 < other < 0.5, other
