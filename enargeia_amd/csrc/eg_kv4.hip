@@ -334,7 +334,8 @@ __device__ __forceinline__ void store2(T* p, float a, float b) {
 // head_dim 64 every other one). All of a block's words are read before any value is stored. 16 x 4096 rows of 8 heads
 // of 128 (bf16) 74.0 us (4.65 TB/s) in blocks of 32, 88.6 of 16, 123.8 of 8. (Stored past the caches' retention they
 // take 55.1, but the attention that reads the rows next pays for it: 512 queries each over them 570 us in all for 556,
-// 500 each over 4 x 2000 rows of 2 heads of 64 39.3 for 34.3.)
+// 500 each over 4 x 2000 rows of 2 heads of 64 39.3 for 34.3.) Of few kv heads blocks of 32 are few waves: 16384 rows of
+// 2 heads of 64 are one block for each of two waves a SIMD, so one latency is the launch: 7.1 us for 11 MB.
 template <int D, uint32_t kBlock, class TO>
 __global__ __launch_bounds__(256) void read_kernel(ReadArgs a, Pool pool) {
   constexpr uint32_t kGroups = D / 32, kWords = D / 8;

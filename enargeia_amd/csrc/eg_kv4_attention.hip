@@ -136,8 +136,9 @@ __device__ __forceinline__ u32x4 first_halves(u32x4 v, int n) {
 // of the columns would be empty. T = 1: 16 heads. kParts: f16 parts of a query and of a weight.
 // (Two waves per SIMD: their registers hold two steps' operands each, one step's loads under way while
 // the other is multiplied.)
-// kStream: codes are read past the caches' retention (non-temporal), for a cache larger than the Infinity
-// Cache: 32 sequences of 16384 (32 / 8 heads of 128) 94.4 us for 106.5, but 16 of up to 8192 26.0 for 24.6.
+// kStream: codes are read past the caches' retention (non-temporal), where the call's reach is larger than the
+// Infinity Cache: 32 sequences of 16384 (32 / 8 heads of 128) 94.4 us for 106.5, but 16 of up to 8192 26.0 for
+// 24.6 (calls on one layer that follow each other: what lies in the caches is from the call before).
 template <int D, int T, int kParts, bool kStream, class TQ>
 __global__ __launch_bounds__(256, 2) void decode_kernel(Args a, Pool pool) {
   constexpr int kGroups = D / 32, kBlocks = D / 16;  // dim groups of K; blocks of 16 dims of O^T
@@ -515,6 +516,9 @@ extern "C" int eg_attention_decode_kv4(eg_context* ctx, const void* q, const uin
   // f16) 9.2 in 256, 9.9 in 512, 11.6 in 1024; 1 of 517 6.5 whole, 9.0 in two. Workgroups: two a CU, as the device
   // holds at once (16 of up to 8192, 28 / 4 of 128, f32: 24.6 us, in twice as many 29.7), but of T = 1's one where the
   // tables do not reach 1024 positions for each of two (4 of 65536, 16 / 1 of 128: 19.5 us, in a few more 21.8).
+  // All of this goes by counts, the lengths being on the device: with more (sequence, kv head) rows than CUs nothing
+  // is split, and a sequence far longer than the others holds the launch up (one of 65536 beside 63 of 512, 32 / 8 of
+  // 128, bf16: 340 us, alone 24; 64 of 512: 12.5).
   a.min_chunk = pair ? 512 : 256;
   const uint64_t rows = (uint64_t)dims->sequences * dims->kv_heads * a.head_tiles, twice = 2ull * ctx->cu_count / rows;
   const uint64_t room = pair || a.capacity >= 1024 * twice ? twice : ctx->cu_count / rows;
@@ -528,7 +532,8 @@ extern "C" int eg_attention_decode_kv4(eg_context* ctx, const void* q, const uin
   a.ml = reinterpret_cast<float*>(eg::partials(ctx));
   a.o = a.ml + (((size_t)dims->sequences * d.heads * splits * 2 + 3) & ~(size_t)3);
   const Pool p = eg_kv4::pool_of(*dims, pool, table);
-  // The most that the call can read: what the tables reach, and what the pool holds.
+  // The most that the call can read: what the tables reach, and what the pool holds, of its one layer. (The other
+  // layers of a step are not counted, though they too pass through the caches before this one is read again.)
   const uint64_t reach = std::min<uint64_t>((uint64_t)dims->sequences * dims->max_pages, dims->pages) * eg_kv4::page_bytes(*dims);
   const bool stream = reach > kInfinityCache;
   const OnDevice on(ctx);

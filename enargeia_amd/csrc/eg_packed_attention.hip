@@ -9,10 +9,10 @@
 // are the second product's B operand where they lie, with V^T read from LDS transposed.
 //
 // Bound by the SIMDs' issue of both units, and at length by power: the clock falls from 2.4 to 1.9 GHz. A wave and
-// tile of 64 keys take 1024 (head_dim 128) or 512 (64) cycles of the matrix cores and 750 to 780 of vector
+// tile of 64 keys take 1024 (head_dim 128) or 512 (64) cycles of the matrix cores and about 750 of vector
 // instructions (32 exponentials of 8 cycles, the rest 4 each), together 2050 (two waves a SIMD) and 1220 (three).
 // MI355X: a prompt of 8192, 32 / 8 heads of 128, bf16: 514 us, 1070 TFLOP/s (a library product of 8192 reaches 1435
-// on the card), the matrix cores busy 53% of 1,000,000 cycles; 14 heads of 64, f16: 147 us, 820 TFLOP/s; 8 prompts of
+// on the card), the matrix cores busy 55% of 956,000 cycles; 14 heads of 64, f16: 147 us, 820 TFLOP/s; 8 prompts of
 // up to 2048, 14 heads of 64: 49 us. Tried and slower at 8192: two groups of four waves half a step apart, one at its
 // products while the other is at its softmax (550 us); the next tile's scores among this one's softmax (832, and 950
 // with one wave a SIMD); 64 queries a wave (head_dim 64, 206 us); row sums by a product with ones or by dot products
@@ -539,7 +539,9 @@ extern "C" int eg_attention_packed(eg_context* ctx, const void* q, const void* k
   // many as make two workgroups a CU, of at least kSplitTiles of a sequence's tiles. 14 / 2 heads of 64: 256
   // queries after 1792 rows 28.9 -> 15.7 us, twice 64 after 6000 75 -> 21.6 (of at least 8 tiles 23.0; of 4 the first
   // takes 16.6, and a prompt of 1024 18.8 for 15.9). Two splits, where no more fit, cost more in the join than they
-  // gain: 4 of 500 after 2000 37.6 for 33.9.
+  // gain: 4 of 500 after 2000 37.6 for 33.9. What stays: a workgroup is 128 queries of one head, so of 64 queries two
+  // of its waves go through all keys for none, and every head of a kv head loads the same keys (twice 64 after 6000:
+  // 21.3 us with 4.6 in the join, where the products they need take 1.8).
   const uint64_t resident = 2ull * ctx->cu_count;
   const uint64_t tiles = (uint64_t)d.key_rows / d.sequences / kKeys, row_bytes = (uint64_t)d.rows * d.heads * (d.head_dim + 2) * 4;
   const uint64_t splits = std::min({resident / (blocks * d.heads), tiles / kSplitTiles, (eg::kPartialsBytes - 64) / row_bytes});
