@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import ctypes
 import struct
+from operator import index
 
 import numpy as np
 
@@ -92,6 +93,7 @@ class Kv4Cache:
                  layers: int = 1, pool=None):
         if pages < 1 or layers < 1:
             raise EgRangeError(EG_ERR_RANGE, f"kv4: a pool of {pages} pages of {layers} layers")
+        pages, layers = index(pages), index(layers)  # (numpy's would wrap in the products below)
         self.device = device
         self.layer_bytes = page_bytes(kv_heads, head_dim, page_size)
         _fits(pages=pages)
@@ -114,7 +116,7 @@ class Kv4Cache:
         base = _address(self.pool)
         if not base:  # (an offset from nowhere would not be NULL)
             raise EgError(EG_ERR_STATE, "kv4: the pool has been released")
-        return base + layer * self.layer_bytes
+        return base + index(layer) * self.layer_bytes
 
     def _for(self, sequences: int, max_pages: int):
         if not (0 <= sequences <= _MOST and 0 <= max_pages <= _MOST):

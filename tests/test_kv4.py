@@ -261,3 +261,22 @@ def test_scales_and_codes_by_the_headers_words():
     # a value over its scale is another format: about one scale in four has ties that fall to the odd code
     other = (codes[: len(ties)] != divided).any(1).mean()
     assert 0.1 < other < 0.5, other
+
+
+def test_pool_sizes_of_numpy_integers_do_not_wrap():
+    """A pool that is allocated for pages counted in 32 bits holds all of them."""
+    sizes = []
+
+    class Device:
+        ctx = None
+
+        def buffer(self, size, label=""):
+            sizes.append(size)
+            return Buffer(self, 1 << 20, size, label)
+
+    stride = kv4.page_bytes(8, 128, 64)
+    cache = kv4.Kv4Cache(Device(), 8, 128, np.int32(60000), 64, layers=np.int32(1))
+    kv4.Kv4Cache(Device(), 8, 128, 60000, 64, layers=np.int32(60000))
+    assert sizes == [60000 * stride, 60000 * 60000 * stride] and cache.dims.pages == 60000
+    large = kv4.Kv4Cache(Device(), 1024, 128, 4, 256, layers=64)
+    assert large._at(np.int32(63)) == (1 << 20) + 63 * kv4.page_bytes(1024, 128, 256)
