@@ -229,6 +229,7 @@ class PageTable:
     def grow(self, seq: int, rows: int) -> int:
         """Room for `rows` more positions; the first one's position. (A sequence never shrinks: its next rows
         could then lie in a page that a fork shares.)"""
+        rows = index(rows)  # (of an unsigned numpy integer the rounding up below would wrap)
         if rows < 0:
             raise EgRangeError(EG_ERR_RANGE, f"kv4: sequence {seq} cannot grow by {rows} rows")
         start = self.length[seq]

@@ -280,3 +280,15 @@ def test_pool_sizes_of_numpy_integers_do_not_wrap():
     assert sizes == [60000 * stride, 60000 * 60000 * stride] and cache.dims.pages == 60000
     large = kv4.Kv4Cache(Device(), 1024, 128, 4, 256, layers=64)
     assert large._at(np.int32(63)) == (1 << 20) + 63 * kv4.page_bytes(1024, 128, 256)
+
+
+@pytest.mark.parametrize("kind", [np.uint32, np.int32, np.uint64, np.uint8])
+def test_sequences_grow_by_numpy_integers(kind):
+    """As `lengths` gives them."""
+    t = kv4.PageTable(12, 32)
+    a = t.create()
+    assert t.grow(a, kind(200)) == 0 and len(t.held[a]) == 7
+    assert t.grow(a, kind(100)) == 200 and len(t.held[a]) == 10 and t.length[a] == 300
+    b = t.create()
+    t.grow(b, t.lengths([b])[0])
+    assert t.held[b] == [] and t.lengths([a, b]).tolist() == [300, 0]
