@@ -176,7 +176,7 @@ def test_sizes_past_32_bits_are_refused():
     for count in (1 << 32, -1):
         with pytest.raises(EgRangeError, match="a dimension out of range"):
             cache.copy_pages(0, count)
-    # (the largest that fit are the library's to judge)
+    # (the largest that fit are the library's to check)
     with pytest.raises(EgError, match="ctx is NULL"):
         cache.read(0, 0, 0, 0, 0, rows=(1 << 32) - 1, sequences=(1 << 32) - 1, max_pages=(1 << 32) - 1)
 
