@@ -77,6 +77,11 @@ SIGNATURES: dict[str, tuple] = {
     "eg_kv4_copy_pages": (_i, [_vp, _vp, _vp, ctypes.c_uint32, _vp]),
     "eg_attention_decode_kv4": (_i, [_vp] * 8),
     "eg_attention_packed": (_i, [_vp] * 8),
+    "eg_rope_table": (_i, [_vp] * 3),
+    "eg_rope": (_i, [_vp] * 10),
+    "eg_attention_tree_kv4": (_i, [_vp] * 10),
+    "eg_verify_drafts": (_i, [_vp] * 13),
+    "eg_kv4_keep_rows": (_i, [_vp] * 9 + [ctypes.c_uint32, ctypes.c_uint32]),
     "eg_container_open": (_i, [_vp, ctypes.c_char_p, ctypes.POINTER(_vp)]),
     "eg_container_close": (_i, [_vp]),
     "eg_container_header_get": (_i, [_vp, _vp]),

@@ -47,7 +47,8 @@ HIP_FLAGS = [
 # The decode attention over the 4-bit cache has registers to spare for the scheduler that goes
 # for instruction-level parallelism: 2 to 4% off its time (the others, short of registers, spill).
 FILE_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form"]
-              for name in ("eg_prefill_attention.hip", "eg_packed_attention.hip", "eg_kv4_attention.hip")}
+              for name in ("eg_prefill_attention.hip", "eg_packed_attention.hip", "eg_kv4_attention.hip",
+                           "eg_kv4_tree.hip")}
 FILE_FLAGS["eg_kv4_attention.hip"] += ["-mllvm", "-amdgpu-sched-strategy=max-ilp"]
 
 

@@ -1,0 +1,522 @@
+// Attention of a tree of drafted rows per sequence over the paged 4-bit cache (eg_attention_tree_kv4).
+//
+//   out[r][h] = sum_j p_j V[j] / sum_j p_j,  p_j = exp(scale q[r][h] . K[j] - max_j),  j of those that row r sees
+//
+// The decode attention (eg_kv4_attention.hip) with more columns: a kv head's columns are all its query heads of all
+// the sequence's rows, in blocks of 16, and a tile of 32 positions, dequantized once, is multiplied with kBlocks of
+// them. One pass over the cache with the running max and sum of the softmax; a workgroup's waves take a chunk's
+// tiles in turn and meet in LDS, chunks meet in a second launch. Which of the last positions a column sees is
+// its row's ancestors, as 64 bits; tiles before them have no mask.
+#include <algorithm>
+
+#include "eg_kv4_operands.hpp"
+
+namespace {
+
+using namespace eg_kv4;
+
+constexpr uint32_t kThreads = 256, kWaves = 4, kMostRows = 64;
+
+struct Args {
+  const void* q;
+  const uint32_t *offsets, *parents, *lengths;
+  void* out;
+  float* o;   // partials [row][head][split][D], unnormalised
+  float* ml;  // [row][head][split] (max, sum)
+  uint32_t rows, max_rows, heads, group, tiles, q_stride, out_stride, splits, min_chunk, capacity;
+  float scale;  // times log2 e
+};
+
+// Positions per chunk: the same in the attention and the launch that joins its partials.
+__device__ __forceinline__ uint32_t chunk_of(const Args& a, uint32_t length) {
+  const uint32_t even = (length + a.splits - 1) / a.splits;
+  return max(a.min_chunk, (even + 63u) & ~63u);
+}
+
+// Whether a sequence's rows, packed rows first .. last, are computed.
+__device__ __forceinline__ bool computed(const Args& a, uint32_t first, uint32_t last) {
+  return first <= last && last <= a.rows && last - first <= a.max_rows;
+}
+
+// What a row of a sequence sees of its rows, itself among them: lane i of a wave gets row i's bits. Each turn
+// adds what the row at the end of the chain so far has, and moves that end to its own: 6 turns reach 64.
+__device__ __forceinline__ uint64_t ancestors(const uint32_t* parents, uint32_t first, uint32_t n) {
+  const uint32_t lane = threadIdx.x & 63u;
+  if (!parents) return ~0ull >> (63u - lane);
+  uint32_t end = lane;
+  if (lane < n) {
+    const uint32_t p = parents[first + lane];
+    if (p < lane) end = p;
+  }
+  uint32_t lo = lane < 32 ? 1u << lane : 0u, hi = lane < 32 ? 0u : 1u << (lane - 32);
+#pragma unroll
+  for (int i = 0; i < 6; i++) {
+    lo |= (uint32_t)__shfl((int)lo, (int)end, 64);
+    hi |= (uint32_t)__shfl((int)hi, (int)end, 64);
+    end = (uint32_t)__shfl((int)end, (int)end, 64);
+  }
+  return (uint64_t)hi << 32 | lo;
+}
+
+// D: head_dim. kBlocks: blocks of 16 columns a wave multiplies a tile with. kParts: f16 parts of a query and of a
+// weight (2 for f32 rows).
+template <int D, int kBlocks, int kParts, class TQ>
+__global__ __launch_bounds__(256, 2) void tree_kernel(Args a, Pool pool) {
+  constexpr int kGroups = D / 32, kDims = D / 16;  // dim groups of K; blocks of 16 dims of O^T
+  constexpr bool kSigned = kParts == 2;
+  constexpr uint32_t kTile = 32, kColumns = 16 * kBlocks;
+  constexpr int kVWords = D / 16;  // V words of a lane: its dims D / 16 * (lane % 16) + 0 ..
+  const uint32_t tid = threadIdx.x, lane = tid & 63u;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t lr = lane & 15u, lg = lane >> 4;
+
+  uint32_t id = blockIdx.x;
+  const uint32_t split = id % a.splits;
+  id /= a.splits;
+  const uint32_t tile = id % a.tiles;
+  id /= a.tiles;
+  const uint32_t kv = id % pool.kv_heads, seq = id / pool.kv_heads;
+
+  const uint32_t first = a.offsets[seq], last = a.offsets[seq + 1], n = last - first, length = a.lengths[seq];
+  if (!computed(a, first, last) || tile * kColumns >= n * a.group) return;
+  const uint32_t reach = min(length, a.capacity), chunk = chunk_of(a, reach), begin = split * chunk;
+  if (split != 0 && begin >= reach) return;
+  const bool fits = n <= length;  // (else the rows give zeros)
+  const uint32_t base = fits ? length - n : 0, end = fits ? min(reach, begin + chunk) : 0;
+  const Magic bits_over = magic();
+
+  // This lane's columns: row and head of each block's.
+  uint32_t row[kBlocks], head[kBlocks];
+  bool in[kBlocks];
+#pragma unroll
+  for (int b = 0; b < kBlocks; b++) {
+    const uint32_t c = tile * kColumns + 16 * b + lr;
+    in[b] = c < n * a.group;
+    row[b] = in[b] ? c / a.group : 0;
+    head[b] = kv * a.group + (in[b] ? c % a.group : 0);
+  }
+
+  const uint32_t page_size = 1u << pool.page_shift;
+  const Layout at = layout<D>(page_size);
+  const uint32_t e_off = lr & 3u;  // row e of a lane's K operand: positions kOrder[e] and kOrder[4 + e]
+  const uint32_t k_row0 = (8 * (lr >> 2) + (e_off == 0 ? 0u : e_off == 1 ? 4u : e_off == 2 ? 1u : 5u)) * (D / 2) +
+                          lg * (kGroups * 4);
+  const uint32_t v_off = at.v_codes + (lg * D + lr * kVWords) * 4;
+  const uint32_t ks_off = at.k_scales + 8 * lg * 2;
+  const uint32_t vs_off = at.v_scales + (((lr * kVWords) / 32) << (pool.page_shift + 1)) + 16 * lg;
+
+  // A step's operands as they come from memory.
+  struct Tile {
+    uint32_t k[2][kGroups];
+    uint32_t v[kVWords];
+    u32x4 ks[kGroups], vs;
+    bool have;
+  };
+  const auto load = [&](Tile& t, uint32_t page, uint32_t slot) {
+    t.have = page < pool.pages;
+    // (no page: a resource of no bytes, whose loads return zeros)
+    const auto r = egd::buffer(pool.block(t.have ? page : 0, kv, at.head_bytes), t.have ? at.head_bytes : 0);
+#pragma unroll
+    for (int m = 0; m < 2; m++) {  // positions 2 apart: kOrder[4 + e] = kOrder[e] + 2
+      const uint32_t o = k_row0 + 2 * m * (D / 2);
+      if constexpr (kGroups == 2) {
+        const auto w = __builtin_amdgcn_raw_buffer_load_b64(r, o, slot * (D / 2), 0);
+        t.k[m][0] = w[0];
+        t.k[m][1] = w[1];
+      } else {
+        const u32x4 w = egd::load_b128(r, o, slot * (D / 2));
+#pragma unroll
+        for (int g = 0; g < kGroups; g++) t.k[m][g] = w[g];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kVWords; j += 4) {
+      const u32x4 w = egd::load_b128(r, v_off + 4 * j, (slot / 8) * (D * 4));
+#pragma unroll
+      for (int e = 0; e < 4; e++) t.v[j + e] = w[e];
+    }
+    t.vs = egd::load_b128(r, vs_off, slot * 2);
+#pragma unroll
+    for (int g = 0; g < kGroups; g++) t.ks[g] = egd::load_b128(r, ks_off, ((g << pool.page_shift) + slot) * 2);
+  };
+
+  const uint32_t steps = begin < end ? (end - begin + kTile - 1) / kTile : 0;
+  const uint32_t mine = steps > wave ? (steps - wave + kWaves - 1) / kWaves : 0;  // steps of this wave
+  // The pages of this wave's next 64 steps, one a lane, from its step i0 on.
+  const auto pages_of = [&](uint32_t i0) {
+    const uint32_t step = wave + kWaves * (i0 + lane);
+    return step < steps ? pool.page_of(seq, begin + step * kTile) : 0xFFFFFFFFu;
+  };
+  const auto fetch = [&](Tile& t, uint32_t ids, uint32_t i0, uint32_t i) {
+    load(t, (uint32_t)__builtin_amdgcn_readlane((int)ids, (int)i),
+         (begin + (wave + kWaves * (i0 + i)) * kTile) & (page_size - 1u));
+  };
+  uint32_t ids = pages_of(0);
+
+  // What each column sees of the sequence's rows.
+  uint64_t sees[kBlocks];
+  if (end > base) {
+    const uint64_t all = ancestors(a.parents, first, n);
+#pragma unroll
+    for (int b = 0; b < kBlocks; b++)
+      sees[b] = (uint64_t)(uint32_t)__shfl((int)(uint32_t)(all >> 32), (int)row[b], 64) << 32 |
+                (uint32_t)__shfl((int)(uint32_t)all, (int)row[b], 64);
+  }
+
+  // The queries, B operand: lane group g has dims 32 grp + 8 g + kOrder[slot] of column lr.
+  half8 qf[kBlocks][kGroups][kParts];
+  f32x4 start[kBlocks][kGroups];  // -8 sum q per group: what makes codes of code - 8
+  float f[kBlocks];
+#pragma unroll
+  for (int b = 0; b < kBlocks; b++) {
+    float x[kGroups][8], top = 0.f;
+    const TQ* src = static_cast<const TQ*>(a.q) + (size_t)(first + row[b]) * a.q_stride + (size_t)head[b] * D;
+#pragma unroll
+    for (int g = 0; g < kGroups; g++) {
+      struct alignas(16) Eight {
+        TQ v[8];
+      };
+      const Eight e = *reinterpret_cast<const Eight*>(src + 32 * g + 8 * lg);
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        x[g][i] = in[b] ? to_f32(e.v[kOrder[i]]) : 0.f;
+        top = fmaxf(top, fabsf(x[g][i]));
+      }
+    }
+    top = max_of_head(top);
+    int e = top > 0.f ? 14 - ((int)(__float_as_uint(top) >> 23) - 127) : 0;
+    e = max(-100, min(110, e));
+    f[b] = fmaxf(ldexpf(a.scale, kSigned ? -e : 24 - e), 0x1p-126f);  // (not 0: -inf times it is -inf)
+#pragma unroll
+    for (int g = 0; g < kGroups; g++) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        float y = ldexpf(x[g][i], e);
+#pragma unroll
+        for (int p = 0; p < kParts; p++) {
+          const _Float16 h = (_Float16)y;
+          y -= (float)h;
+          qf[b][g][p][i] = !kSigned && (i & 2) ? h * (_Float16)0.0625f : h;
+        }
+      }
+      const half8 eight = as_half8(0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u);
+      start[b][g] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if constexpr (!kSigned) {
+#pragma unroll
+        for (int p = 0; p < kParts; p++)
+          start[b][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(eight, qf[b][g][p], start[b][g], 0, 0, 0);
+      }
+    }
+  }
+
+  f32x4 o[kBlocks][kDims];
+  float m[kBlocks], l[kBlocks];  // running max of the scores before f; this lane's share of the sum
+#pragma unroll
+  for (int b = 0; b < kBlocks; b++) {
+    m[b] = -INFINITY;
+    l[b] = 0.f;
+#pragma unroll
+    for (int i = 0; i < kDims; i++) o[b][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  const auto compute = [&](Tile& t, uint32_t i) {
+    const uint32_t j0 = begin + (wave + kWaves * i) * kTile;
+    f32x4 s[kBlocks][2];
+#pragma unroll
+    for (int b = 0; b < kBlocks; b++)
+#pragma unroll
+      for (int k = 0; k < 2; k++) s[b][k] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < 2; k++)
+#pragma unroll
+      for (int g = 0; g < kGroups; g++) {
+        const half8 kc = codes<kSigned>(t.k[k][g], bits_over);
+#pragma unroll
+        for (int b = 0; b < kBlocks; b++) {
+          f32x4 acc = start[b][g];
+#pragma unroll
+          for (int p = 0; p < kParts; p++) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, qf[b][g][p], acc, 0, 0, 0);
+#pragma unroll
+          for (int e = 0; e < 4; e++) s[b][k][e] = fmaf(half_of(t.ks[g], kOrder[4 * k + e]), acc[e], s[b][k][e]);
+        }
+      }
+    uint32_t poison = 0;  // blocks whose column sees a value that is not a number
+    if (j0 + kTile > base || !t.have) {
+      // positions past the end: no score, values of zero; of the sequence's rows what the column sees
+      const int seen = t.have ? (int)(end - j0) : 0;  // of the tile
+      t.vs = first_halves(t.vs, max(0, min(8, seen - (int)(8 * lg))));
+      uint32_t visible[kBlocks];  // of this tile's 32 positions
+#pragma unroll
+      for (int b = 0; b < kBlocks; b++) {
+        uint32_t v = j0 >= base ? (uint32_t)(sees[b] >> (j0 - base)) : 0;
+        if (j0 < base) v = base - j0 >= 32 ? 0xFFFFFFFFu : (uint32_t)(sees[b] << (base - j0)) | ((1u << (base - j0)) - 1u);
+        visible[b] = seen >= 32 ? v : seen <= 0 ? 0 : v & ((1u << seen) - 1u);
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            if (!(visible[b] >> (8 * lg + kOrder[4 * k + e]) & 1u)) s[b][k][e] = -INFINITY;
+      }
+      // A scale that is not a number (its values are none then) would reach, times a weight of 0, the columns that do
+      // not see its position: it is taken out of the product, and put into the sums of those that do.
+      uint32_t bad = 0;  // of this lane's 8 positions
+#pragma unroll
+      for (int h = 0; h < 8; h++) {
+        const uint32_t x = t.vs[h / 2] >> (16 * (h & 1)) & 0x7FFFu;
+        if (x >= 0x7C00u) bad |= 1u << h;
+      }
+      if (__builtin_amdgcn_ballot_w64(bad != 0) != 0) {
+#pragma unroll
+        for (int h = 0; h < 8; h++)
+          if (bad >> h & 1u) t.vs[h / 2] &= h & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+        // The dims of this lane's sums (D / 16 (4 lg + e) + n) are all of group D lg / 128, whose scales the lanes of
+        // columns 2 D lg / 128 * 16 / D .. hold: the first of them, of each four positions' lane group.
+        const uint32_t holder = lg * D / 128 * 32 / kVWords;
+        uint32_t mask = 0;
+#pragma unroll
+        for (uint32_t x = 0; x < 4; x++) mask |= (uint32_t)__shfl((int)bad, (int)(16 * x + holder), 64) << (8 * x);
+#pragma unroll
+        for (int b = 0; b < kBlocks; b++)
+          if (visible[b] & mask) poison |= 1u << b;
+      }
+    }
+    half8 pb[kBlocks][kParts];
+#pragma unroll
+    for (int b = 0; b < kBlocks; b++) {
+      float top = m[b];
+#pragma unroll
+      for (int k = 0; k < 2; k++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) top = fmaxf(top, s[b][k][e]);
+      top = max_of_head(top);
+      float shift = top == -INFINITY ? 0.f : fmaf(top, f[b], -15.f);
+      // (past kLargest the max's own rounding would put weights out of f16's range: there it is taken from the
+      // scores instead, which leaves the largest exactly 0)
+      if (__builtin_amdgcn_ballot_w64(fabsf(shift) > kLargest) != 0) {
+        const float from = top == -INFINITY ? 0.f : top;  // (a column without a position yet)
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) s[b][k][e] -= from;
+        shift = -15.f;
+      }
+      if (__builtin_amdgcn_ballot_w64(top > m[b]) != 0) {
+        const float alpha = top > m[b] ? __builtin_amdgcn_exp2f((m[b] - top) * f[b]) : 1.f;
+        l[b] *= alpha;
+#pragma unroll
+        for (int i = 0; i < kDims; i++) o[b][i] *= alpha;
+        m[b] = top;
+      }
+#pragma unroll
+      for (int k = 0; k < 2; k++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          float p = __builtin_amdgcn_exp2f(fmaf(s[b][k][e], f[b], -shift));
+          l[b] += p;
+#pragma unroll
+          for (int x = 0; x < kParts; x++) {
+            const _Float16 h = (_Float16)p;
+            pb[b][x][4 * k + e] = h;
+            p -= (float)h;
+          }
+        }
+      if (poison >> b & 1u) {
+#pragma unroll
+        for (int i = 0; i < kDims; i++) o[b][i] += __builtin_nanf("");
+      }
+    }
+    half2v pairs[4];
+    scale_pairs(t.vs, pairs);
+#pragma unroll
+    for (int i = 0; i < kDims; i++) {
+      const half8 va = values(t.v[i], pairs, bits_over);
+#pragma unroll
+      for (int b = 0; b < kBlocks; b++)
+#pragma unroll
+        for (int x = 0; x < kParts; x++) o[b][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pb[b][x], o[b][i], 0, 0, 0);
+    }
+  };
+
+  // (The page ids are read outside the loop over their 64 steps: a wait for them inside would be a wait
+  // for the tiles under way.)
+  for (uint32_t i0 = 0; i0 < mine; i0 += 64) {
+    if (i0) ids = pages_of(i0);
+    const uint32_t count = min(64u, mine - i0);
+    Tile tiles[2];
+    fetch(tiles[0], ids, i0, 0);
+    for (uint32_t i = 0; i < count; i += 2) {
+      if (i + 1 < count) fetch(tiles[1], ids, i0, i + 1);
+      compute(tiles[0], i0 + i);
+      if (i + 1 < count) {
+        if (i + 2 < count) fetch(tiles[0], ids, i0, i + 2);
+        compute(tiles[1], i0 + i + 1);
+      }
+    }
+  }
+
+  // The waves meet in LDS, a block of columns at a time.
+  __shared__ float top_of[kWaves][16], sum_of[kWaves][16];
+  __shared__ __attribute__((aligned(16))) float part_of[kWaves][16][D];
+  const bool whole = chunk >= reach;  // no other chunk: the result itself
+#pragma unroll
+  for (int b = 0; b < kBlocks; b++) {
+    const uint32_t c0 = tile * kColumns + 16 * b;
+    if (c0 >= n * a.group) break;
+    if (b) __syncthreads();
+    float sum_l = l[b];
+    sum_l += __shfl_xor(sum_l, 16, 64);
+    sum_l += __shfl_xor(sum_l, 32, 64);
+    if (lg == 0) {
+      top_of[wave][lr] = m[b] == -INFINITY ? -INFINITY : m[b] * f[b];
+      sum_of[wave][lr] = sum_l;
+    }
+    // row 4 lg + e of block i is dim D / 16 (4 lg + e) + i
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+#pragma unroll
+      for (int i = 0; i < kDims; i += 4)
+        *reinterpret_cast<float4*>(&part_of[wave][lr][kDims * (4 * lg + e) + i]) =
+            make_float4(o[b][i][e], o[b][i + 1][e], o[b][i + 2][e], o[b][i + 3][e]);
+    __syncthreads();
+    const uint32_t columns = min(16u, n * a.group - c0);
+    for (uint32_t i = tid; i < columns * (D / 4); i += kThreads) {
+      const uint32_t h = i / (D / 4), d = 4 * (i % (D / 4));
+      float top = -INFINITY;
+#pragma unroll
+      for (uint32_t w = 0; w < kWaves; w++) top = fmaxf(top, top_of[w][h]);
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      float sum = 0.f;
+#pragma unroll
+      for (uint32_t w = 0; w < kWaves; w++) {
+        const float c = top_of[w][h] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top_of[w][h] - top);
+        const float4 v = *reinterpret_cast<const float4*>(&part_of[w][h][d]);
+        sum = fmaf(c, sum_of[w][h], sum);
+        acc = make_float4(fmaf(c, v.x, acc.x), fmaf(c, v.y, acc.y), fmaf(c, v.z, acc.z), fmaf(c, v.w, acc.w));
+      }
+      const uint32_t r = first + (c0 + h) / a.group, hd = kv * a.group + (c0 + h) % a.group;
+      if (whole) {
+        const float x = sum == 0.f ? 0.f : 1.f / sum;
+        TQ* to = static_cast<TQ*>(a.out) + (size_t)r * a.out_stride + (size_t)hd * D + d;
+        to[0] = from_f32<TQ>(acc.x * x);
+        to[1] = from_f32<TQ>(acc.y * x);
+        to[2] = from_f32<TQ>(acc.z * x);
+        to[3] = from_f32<TQ>(acc.w * x);
+      } else {
+        const size_t at_row = ((size_t)r * a.heads + hd) * a.splits + split;
+        *reinterpret_cast<float4*>(a.o + at_row * D + d) = acc;
+        if (d == 0) *reinterpret_cast<float2*>(a.ml + 2 * at_row) = make_float2(top, sum);
+      }
+    }
+  }
+}
+
+// A row's chunks joined: a workgroup per (row, head), its waves taking the chunks in turn.
+template <int D, class TQ>
+__global__ __launch_bounds__(256) void join_kernel(Args a, uint32_t sequences) {
+  constexpr uint32_t kPer = D / 64;
+  const uint32_t head = blockIdx.x % a.heads, r = blockIdx.x / a.heads, tid = threadIdx.x;
+  const uint32_t lane = tid & 63u, wave = tid >> 6;
+  uint32_t seq, first, last;
+  if (!find_sequence(a.offsets, sequences, r, seq, first, last)) return;
+  const uint32_t reach = min(a.lengths[seq], a.capacity), chunk = chunk_of(a, reach);
+  if (!computed(a, first, last) || chunk >= reach) return;  // (one chunk: it wrote the result)
+  const uint32_t count = (reach + chunk - 1) / chunk;
+  const size_t at_row = ((size_t)r * a.heads + head) * a.splits;
+  const float* ml = a.ml + 2 * at_row;
+  float top = -INFINITY;
+  for (uint32_t c = lane; c < count; c += 64) top = fmaxf(top, ml[2 * c]);
+  top = egd::team_allmax<64>(top);
+  float acc[kPer] = {}, sum = 0.f;
+#pragma unroll 4
+  for (uint32_t c = wave; c < count; c += kWaves) {
+    const float w = ml[2 * c] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[2 * c] - top);
+    sum = fmaf(w, ml[2 * c + 1], sum);
+#pragma unroll
+    for (uint32_t j = 0; j < kPer; j++) acc[j] = fmaf(w, a.o[(at_row + c) * D + 64 * j + lane], acc[j]);
+  }
+  __shared__ float part[kWaves][D], sums[kWaves];
+#pragma unroll
+  for (uint32_t j = 0; j < kPer; j++) part[wave][64 * j + lane] = acc[j];
+  if (lane == 0) sums[wave] = sum;
+  __syncthreads();
+  if (tid < D) {
+    const float total = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    const float v = (part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid]);
+    static_cast<TQ*>(a.out)[(size_t)r * a.out_stride + (size_t)head * D + tid] =
+        from_f32<TQ>(total == 0.f ? 0.f : v / total);
+  }
+}
+
+template <int D, class TQ>
+void launch(eg_context* ctx, const Args& a, const Pool& p, uint32_t blocks_of_columns, uint64_t blocks) {
+  constexpr int kParts = std::is_same<TQ, float>::value ? 2 : 1;
+  const dim3 grid((uint32_t)blocks), threads(kThreads);
+  if (blocks_of_columns == 1) hipLaunchKernelGGL((tree_kernel<D, 1, kParts, TQ>), grid, threads, 0, ctx->stream, a, p);
+  else hipLaunchKernelGGL((tree_kernel<D, 2, kParts, TQ>), grid, threads, 0, ctx->stream, a, p);
+  if (a.splits > 1)
+    hipLaunchKernelGGL((join_kernel<D, TQ>), dim3(a.rows * a.heads), threads, 0, ctx->stream, a, p.sequences);
+}
+
+}  // namespace
+
+extern "C" int eg_attention_tree_kv4(eg_context* ctx, const void* q, const uint32_t* offsets, const uint32_t* parents,
+                                     const uint32_t* lengths, const uint32_t* table, const void* pool, void* out,
+                                     const eg_kv4_dims* dims, const eg_attention_tree_dims* attention) {
+  const char* op = "attention_tree_kv4";
+  if (!ctx) return eg::fail(nullptr, EG_ERR_INVALID, "%s: ctx is NULL", op);
+  const int st = eg_kv4::check_dims(ctx, op, dims, pool);
+  if (st != EG_OK) return st;
+  const bool some = attention && attention->rows != 0 && attention->max_rows != 0 && dims->sequences != 0;
+  if (!attention || (some && (!q || !offsets || !lengths || !out || (dims->max_pages != 0 && !table))))
+    return eg::fail(ctx, EG_ERR_INVALID, "%s: NULL argument", op);
+  const eg_attention_tree_dims& d = *attention;
+  if (!known_type(d.type)) return eg::fail(ctx, EG_ERR_INVALID, "%s: type %d (eg_element)", op, d.type);
+  if (d.heads == 0 || d.heads % dims->kv_heads != 0 || d.heads > 65535)
+    return eg::fail(ctx, EG_ERR_INVALID, "%s: heads %u are not a multiple of kv_heads %u (at most 65535)", op, d.heads,
+                    dims->kv_heads);
+  if (d.max_rows > kMostRows) return eg::fail(ctx, EG_ERR_RANGE, "%s: max_rows %u (at most %u)", op, d.max_rows, kMostRows);
+  if (!(d.scale >= 0.f) || d.scale > 1e6f) return eg::fail(ctx, EG_ERR_INVALID, "%s: scale %g (0 to 1e6)", op, d.scale);
+  const uint32_t width = d.heads * dims->head_dim;
+  Args a{};
+  a.q = q;
+  a.offsets = offsets;
+  a.parents = parents;
+  a.lengths = lengths;
+  a.out = out;
+  a.rows = d.rows;
+  a.max_rows = d.max_rows;
+  a.heads = d.heads;
+  a.group = d.heads / dims->kv_heads;
+  a.q_stride = d.q_stride ? d.q_stride : width;
+  a.out_stride = d.out_stride ? d.out_stride : width;
+  if (a.q_stride < width || a.out_stride < width || (a.q_stride | a.out_stride) % 8)
+    return eg::fail(ctx, EG_ERR_INVALID, "%s: strides %u, %u (multiples of 8, at least a row)", op, a.q_stride,
+                    a.out_stride);
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15u)
+    return eg::fail(ctx, EG_ERR_INVALID, "%s: q and out must be 16-byte aligned", op);
+  if (!some) return EG_OK;
+  a.scale = (d.scale > 0.f ? d.scale : 1.0f / sqrtf((float)dims->head_dim)) * kLog2e;
+  const uint32_t columns = std::min(d.max_rows, d.rows) * a.group, per_tile = columns <= 16 ? 1 : 2;
+  a.tiles = (columns + 16 * per_tile - 1) / (16 * per_tile);
+  // Splits: workgroups for two a CU, of chunks of at least two steps a wave.
+  a.min_chunk = 256;
+  a.capacity = dims->max_pages * dims->page_size;
+  const uint64_t tiles = (uint64_t)dims->sequences * dims->kv_heads * a.tiles;
+  const uint64_t most = ((uint64_t)a.capacity + a.min_chunk - 1) / a.min_chunk, per_split = (uint64_t)d.rows * d.heads * (dims->head_dim + 2) * 4;
+  uint64_t splits = std::max<uint64_t>(1, std::min<uint64_t>(2ull * ctx->cu_count / tiles, most));
+  splits = std::max<uint64_t>(1, std::min<uint64_t>(splits, (eg::kPartialsBytes - 64) / per_split));
+  a.splits = (uint32_t)splits;
+  if (tiles * splits >= (1ull << 31) / kThreads || (uint64_t)d.rows * d.heads >= (1ull << 31) / kThreads)
+    return eg::fail(ctx, EG_ERR_RANGE, "%s: %u rows of %u heads in %u sequences over the grid limit", op, d.rows, d.heads,
+                    dims->sequences);
+  a.ml = reinterpret_cast<float*>(eg::partials(ctx));
+  a.o = a.ml + (((size_t)d.rows * d.heads * splits * 2 + 3) & ~(size_t)3);
+  const Pool p = eg_kv4::pool_of(*dims, pool, table);
+  const OnDevice on(ctx);
+  with_type(d.type, [&](auto t) {
+    using TQ = decltype(t);
+    if (dims->head_dim == 64) launch<64, TQ>(ctx, a, p, per_tile, tiles * splits);
+    else launch<128, TQ>(ctx, a, p, per_tile, tiles * splits);
+  });
+  return eg::check_launch(ctx, op);
+}

@@ -11,7 +11,7 @@ in device memory, read when the launch runs.
 A prompt: ``append`` (q, k, v of the packed rows; q rotated comes back, and k and v in the operands'
 type if asked for), then ``attention_packed``. A chunk after earlier rows: ``append``, ``read`` all of
 the sequences' rows, ``attention_packed`` with more keys than queries. A decode step: ``append`` one row
-per sequence, ``attend``.
+per sequence, ``attend``. A step of drafted tokens: drafts.py, with ``attend_tree`` and ``keep`` here.
 """
 
 from __future__ import annotations
@@ -55,9 +55,10 @@ class Kv4Dims(ctypes.Structure):
                 ("max_pages", ctypes.c_uint32)]
 
 
-# eg_kv4_append_dims, eg_attention_kv4_dims, eg_attention_packed_dims, field by field
+# eg_kv4_append_dims, eg_attention_kv4_dims, eg_attention_tree_dims, eg_attention_packed_dims, field by field
 _APPEND_DIMS = struct.Struct("6I2i").pack  # rows, heads, q_stride, k_stride, v_stride, rope_positions, in_type, out_type
 _ATTENTION_KV4_DIMS = struct.Struct("3Iif").pack  # heads, q_stride, out_stride, type, scale
+_ATTENTION_TREE_DIMS = struct.Struct("5Iif").pack  # rows, max_rows, heads, q_stride, out_stride, type, scale
 # sequences, rows, key_rows, heads, kv_heads, head_dim, q_stride, k_stride, v_stride, out_stride, type, out_type, scale
 _ATTENTION_PACKED_DIMS = struct.Struct("10I2if").pack
 
@@ -102,6 +103,7 @@ class Kv4Cache:
         self._dims = ctypes.byref(self.dims)
         lib = _lib.load()  # (bound once: a small call's time is its host path)
         self._append, self._read, self._attend = lib.eg_kv4_append, lib.eg_kv4_read, lib.eg_attention_decode_kv4
+        self._attend_tree, self._keep_rows = lib.eg_attention_tree_kv4, lib.eg_kv4_keep_rows
         self.layers = layers
         size = self.dims.page_stride * pages
         held = pool.size if isinstance(pool, Buffer) else getattr(pool, "nbytes", None)
@@ -159,6 +161,31 @@ class Kv4Cache:
         status = self._attend(ctx, _address(q), _address(lengths), _address(table), self._at(layer), _address(out),
                               self._for(sequences, max_pages),
                               _packed(_ATTENTION_KV4_DIMS, heads, q_stride, out_stride, _element(type), scale))
+        if status:
+            check(status, ctx)
+
+    def attend_tree(self, q, offsets, lengths, table, out, *, heads: int, rows: int, max_rows: int, sequences: int,
+                    max_pages: int, parents=None, layer: int = 0, type: str = "f32", scale: float = 0.0,
+                    q_stride: int = 0, out_stride: int = 0) -> None:
+        """eg_attention_tree_kv4: a tree (without parents a chain) of rows per sequence, which lie last in the
+        cache, each against the positions before them, its ancestors and itself."""
+        ctx = self.device.ctx
+        status = self._attend_tree(ctx, _address(q), _address(offsets), _address(parents), _address(lengths),
+                                   _address(table), self._at(layer), _address(out), self._for(sequences, max_pages),
+                                   _packed(_ATTENTION_TREE_DIMS, rows, max_rows, heads, q_stride, out_stride,
+                                           _element(type), scale))
+        if status:
+            check(status, ctx)
+
+    def keep(self, path, counts, offsets, lengths, table, new_lengths, *, max_rows: int, sequences: int,
+             max_pages: int) -> None:
+        """eg_kv4_keep_rows: the accepted rows of each sequence moved together, all layers."""
+        ctx = self.device.ctx
+        if not 0 <= max_rows <= _MOST:
+            _fits(max_rows=max_rows)
+        status = self._keep_rows(ctx, _address(path), _address(counts), _address(offsets), _address(lengths),
+                                 _address(table), self._at(0), _address(new_lengths), self._for(sequences, max_pages),
+                                 self.layers, max_rows)
         if status:
             check(status, ctx)
 
@@ -238,6 +265,24 @@ class PageTable:
             self.held[seq] += self._take(need)
         self.length[seq] = start + rows
         return start
+
+    def shrink(self, seq: int, rows: int) -> int:
+        """The last `rows` positions given back (a step's drafts that were not accepted), and the pages that hold
+        none of the others; the first one's position. Refused where the next rows would lie in a page that a
+        fork shares."""
+        rows = index(rows)
+        length = self.length[seq] - rows
+        if rows < 0 or length < 0:
+            raise EgRangeError(EG_ERR_RANGE, f"kv4: sequence {seq} of {self.length[seq]} cannot shrink by {rows} rows")
+        held, keep = self.held[seq], -(-length // self.page_size)
+        if length % self.page_size and rows and self.users[held[keep - 1]] > 1:
+            raise EgError(EG_ERR_STATE, f"kv4: sequence {seq} cannot shrink to {length}: a fork shares that page")
+        for p in held[keep:]:
+            self.users[p] -= 1
+        del held[keep:]
+        self.length[seq] = length
+        self.copies = [(a, b) for a, b in self.copies if self.users[b]]
+        return length
 
     def fork(self, seq: int) -> int:
         """A sequence with the same positions: whole pages shared, the partial last one copied."""

@@ -625,6 +625,120 @@ EG_API int eg_attention_packed(eg_context* ctx, const void* q, const void* k, co
                                const uint32_t* q_offsets, const uint32_t* k_offsets, void* out,
                                const eg_attention_packed_dims* dims);
 
+/* ---- a speculative step over the 4-bit cache (no counterpart in the reference, which decodes one token at
+ * a time) -------------------------------------------------------------------------------------------
+ *
+ * Drafted tokens of several sequences are checked in one pass of the model. A sequence's rows, packed as above
+ * (offsets[sequences + 1]), are its last token - row 0, the root, which is decided but not yet cached - and its
+ * drafts. Rows are a tree: parents[r] is row r's parent, counted from its sequence's first row; a parent that is
+ * not before its row is none. Without parents they are a chain: each row's parent is the one before it. At
+ * most 64 rows a sequence. A step is
+ *   eg_rope                    q and k of the rows rotated at starts[s] + their depths
+ *   eg_kv4_append              k and v (no rope) at positions lengths[s] - rows .. lengths[s]
+ *   eg_attention_tree_kv4      the rows against the cache, per layer
+ *   eg_verify_drafts           from the rows' logits the accepted branch and the next token
+ *   eg_kv4_keep_rows           the branch's rows moved together in the pages, all layers; the new lengths
+ * where the next token is the next step's root. */
+
+/* RoPE tables: table[p][i] = amplitude * (cos, sin)((first + p) f_i) for p < positions, i < rotary_dim / 2, f32
+ * pairs, angles in 64 bits: what eg_kv4_append (rotary_dim = head_dim) and eg_rope take. f_i = theta^(-2 i /
+ * rotary_dim), and for longer contexts than a model was trained on
+ *   EG_ROPE_LINEAR     f_i / factor
+ *   EG_ROPE_BASE       theta * factor^(rotary_dim / (rotary_dim - 2)) for theta
+ *   EG_ROPE_TURNS      f_i (w + (1 - w) / factor), w = (t_i - low) / (high - low) clamped to 0..1, by the turns
+ *                      t_i = context f_i / (2 pi) that a pair makes in the trained context
+ *   EG_ROPE_LOG_TURNS  the same with w = log(t_i / low) / log(high / low): even steps from pair to pair. */
+typedef enum eg_rope_scaling {
+  EG_ROPE_PLAIN = 0,
+  EG_ROPE_LINEAR = 1,
+  EG_ROPE_BASE = 2,
+  EG_ROPE_TURNS = 3,
+  EG_ROPE_LOG_TURNS = 4
+} eg_rope_scaling;
+typedef struct eg_rope_table_dims {
+  uint32_t positions, first; /* together under 2^31                                           */
+  uint32_t rotary_dim;       /* a multiple of 8, to 512                                       */
+  int scaling;               /* eg_rope_scaling                                               */
+  double theta, factor;      /* above 0                                                       */
+  double context, low, high; /* of the turns: above 0, low below high                         */
+  double amplitude;          /* 0: 1                                                          */
+} eg_rope_table_dims;
+EG_API int eg_rope_table(eg_context* ctx, float* table, const eg_rope_table_dims* dims);
+
+/* Rows of q and k rotated by the table's row of their position, each product rounded on its own. A row of
+ * sequence s is at starts[s] + positions[r]; without positions at starts[s] + r - offsets[s]; without offsets
+ * (and starts, sequences) at positions[r]; without starts, as if those were 0. The first rotary_dim dims of a
+ * head are rotated, in pairs (i, i + rotary_dim / 2) or (2 i, 2 i + 1), the others pass as they are. Rows outside
+ * the sequences, and of a position that the table does not reach, are skipped: nothing is written. q, q_out and
+ * heads go together, as do k, k_out and kv_heads; either may be absent. An output may be its input, of the same type
+ * and stride. Rows are 16-byte aligned. */
+typedef enum eg_rope_layout { EG_ROPE_HALF = 0, EG_ROPE_INTERLEAVED = 1 } eg_rope_layout;
+typedef struct eg_rope_dims {
+  uint32_t rows, heads, kv_heads;
+  uint32_t head_dim, rotary_dim; /* multiples of 8, to 512; rotary_dim 0: head_dim               */
+  uint32_t q_stride, k_stride, q_out_stride, k_out_stride; /* elements, multiples of 8; 0: dense */
+  uint32_t table_positions, sequences;
+  int layout, in_type, out_type; /* eg_rope_layout, eg_element                                   */
+} eg_rope_dims;
+EG_API int eg_rope(eg_context* ctx, const void* q, const void* k, const float* table, const uint32_t* positions,
+                   const uint32_t* offsets, const uint32_t* starts, void* q_out, void* k_out,
+                   const eg_rope_dims* dims);
+
+/* Attention of a sequence's rows over the cache, where they lie last: row i of n at position lengths[s] - n + i.
+ * It sees the positions before lengths[s] - n, its ancestors and itself (not what is behind the table or on no
+ * page): softmax and values as eg_attention_decode_kv4, which is the case of one row. A row that sees nothing
+ * gives zeros; so do the rows of a sequence with fewer positions than rows. Rows outside the sequences, and those
+ * of a sequence of more than max_rows rows, are not written. q and out are [rows][heads][head_dim] of `type`. */
+typedef struct eg_attention_tree_dims {
+  uint32_t rows, max_rows;       /* rows of q and out; the most of a sequence, to 64              */
+  uint32_t heads;
+  uint32_t q_stride, out_stride; /* elements from row to row, multiples of 8; 0: dense            */
+  int type;                      /* eg_element of q and out                                       */
+  float scale;                   /* 0: 1 / sqrt(head_dim)                                         */
+} eg_attention_tree_dims;
+EG_API int eg_attention_tree_kv4(eg_context* ctx, const void* q, const uint32_t* offsets, const uint32_t* parents,
+                                 const uint32_t* lengths, const uint32_t* table, const void* pool, void* out,
+                                 const eg_kv4_dims* dims, const eg_attention_tree_dims* attention);
+
+/* Drafts against the target's probabilities. At an accepted row (the root first) with p = softmax(logits /
+ * temperatures[s]), the rows whose parent it is are tried in their order, row r with token x = tokens[r]:
+ *   without draft  accepted where accept[r] * S < p(x); S is 1 less the p of the tokens rejected at this row. (Drafts
+ *                  that are a choice: the likeliest, n-grams. A token that was rejected here is again.)
+ *   with draft     (a chain) accepted where accept[r] * q(x) < p(x), q the draft's probabilities at the parent,
+ *                  draft[parent] (x was drawn from them)
+ * and the first that is accepted is gone on from. Where none is, the next token is drawn: the lowest id whose
+ * running sum, in id order, of p without the rejected tokens (with draft: of max(p - q, 0) after a rejection) exceeds
+ * draws[s] times the sum over all. So the tokens come out distributed as if drawn from p one by one. At a
+ * temperature that is not above 0, and without temperatures, a row is accepted if it holds its parent's largest
+ * logit (the lowest id of them; 0 where none is above -inf), which else is the next token. Above 0, ids whose
+ * logit is -inf have p = 0, and a row with a NaN or +inf among its logits, or without one above -inf, accepts
+ * nothing, its next token as at 0. Probabilities and sums are 64 bits. Temperatures are finite.
+ * path [sequences][max_rows]: the accepted rows, counted from the sequence's first, then 0xFFFFFFFF; counts
+ * [sequences]: how many, the root among them; next [sequences]. A sequence of no rows, or of more than max_rows, has
+ * a count of 0 and 0xFFFFFFFF for the rest. logits are [rows][vocab] of `type`, draft f32 [rows][vocab]. accept
+ * (per row) and draws (per sequence), in [0, 1), may be NULL without temperatures. */
+typedef struct eg_verify_dims {
+  uint32_t sequences, rows, max_rows; /* max_rows to 64                                           */
+  uint32_t vocab;                     /* 1 to 2^20                                                */
+  uint32_t logits_stride, draft_stride; /* elements from row to row; 0: vocab                     */
+  int type;                             /* eg_element of the logits                               */
+} eg_verify_dims;
+EG_API int eg_verify_drafts(eg_context* ctx, const void* logits, const uint32_t* tokens, const uint32_t* offsets,
+                            const uint32_t* parents, const float* draft, const float* accept, const float* draws,
+                            const float* temperatures, uint32_t* path, uint32_t* counts, uint32_t* next,
+                            const eg_verify_dims* dims);
+
+/* The accepted rows moved together: for each sequence of n = offsets[s + 1] - offsets[s] rows, of which the cache
+ * holds row i at position lengths[s] - n + i, row path[s][i] goes to position lengths[s] - n + i for i < counts[s],
+ * as it is held (no rounding), in every layer; new_lengths[s] = lengths[s] - n + counts[s]. All are read before any is
+ * written. Positions from there on keep what they held, or what lay there before. The pool is that of layer 0, and a page
+ * holds `layers` layers. Entries of path that are not below n, and rows that come from or go to no page, are not
+ * moved; a count past n is n. A sequence of fewer positions than rows, or of more than max_rows rows, stays as it is.
+ * The pages that rows go to are one sequence's alone. */
+EG_API int eg_kv4_keep_rows(eg_context* ctx, const uint32_t* path, const uint32_t* counts, const uint32_t* offsets,
+                            const uint32_t* lengths, const uint32_t* table, void* pool, uint32_t* new_lengths,
+                            const eg_kv4_dims* dims, uint32_t layers, uint32_t max_rows);
+
 /* ---- the .enargeia container (enargeia.ts:1-50, 112-240; WeightStore.loadQuantized,
  * weights.ts:299-471) ------------------------------------------------------------------------
  * eg_container_open parses the prefix and JSON header on the host and applies the reference's
