@@ -410,6 +410,343 @@ __global__ __launch_bounds__(256, 2) void tree_kernel(Args a, Pool pool) {
   }
 }
 
+// Many columns: the waves share the tiles instead of taking them in turn. A step of 64 positions is dequantized
+// once, by all four waves, into LDS - K as what the first product takes (8 dims of a position), V as what the second takes
+// (8 positions of a dim), each code times its scale, exact in f16 - and each wave multiplies it with its own kBlocks
+// blocks of columns. So a word is unpacked once for 64 kBlocks columns, columns never meet, and one step's words are under
+// way and the next one's in the other half of LDS while this one is multiplied. Scores need no scale of their own.
+//
+// K lies as [8 dims][position], V as [8 positions][dim], so that a product's 16 rows are 16 consecutive operands of
+// 16 bytes; positions in the order of the first product's rows (row 16 k + 4 a + e of 32: position 8 a + kOrder[4 k + e]),
+// dims 4 q + j (2 q + j at head_dim 64) at 32 j + q, which is how a thread's words of neighbouring dims are
+// stored without bank conflicts.
+template <int D, int kBlocks, int kParts, class TQ>
+__global__ __launch_bounds__(256, 2) void wide_kernel(Args a, Pool pool) {
+  constexpr int kGroups = D / 32, kDims = D / 16, kWords = D / 32;  // kWords: of K and of V, a thread and step
+  constexpr uint32_t kStep = 64, kColumns = 64 * kBlocks, kPad = kStep + 1;
+  __shared__ half8 k_of[2][D / 8][kPad], v_of[2][8][D];
+  __shared__ __attribute__((aligned(8))) uint8_t bad_of[2][kGroups][8];  // of a tail step's V: positions (8 a byte) whose scale is no number
+  const uint32_t tid = threadIdx.x, lane = tid & 63u;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t lr = lane & 15u, lg = lane >> 4, half_step = wave >> 1;  // the 32 positions that this wave unpacks
+
+  uint32_t id = blockIdx.x;
+  const uint32_t split = id % a.splits;
+  id /= a.splits;
+  const uint32_t tile = id % a.tiles;
+  id /= a.tiles;
+  const uint32_t kv = id % pool.kv_heads, seq = id / pool.kv_heads;
+
+  const uint32_t first = a.offsets[seq], last = a.offsets[seq + 1], n = last - first, length = a.lengths[seq];
+  if (!computed(a, first, last) || tile * kColumns >= n * a.group) return;
+  const uint32_t reach = min(length, a.capacity), chunk = chunk_of(a, reach), begin = split * chunk;
+  if (split != 0 && begin >= reach) return;
+  const bool fits = n <= length;  // (else the rows give zeros)
+  const uint32_t base = fits ? length - n : 0, end = fits ? min(reach, begin + chunk) : 0;
+  const Magic bits_over = magic();
+  const uint32_t c0 = tile * kColumns + 16 * kBlocks * wave;  // the wave's first column
+  const bool active = c0 < n * a.group;
+
+  const uint32_t page_size = 1u << pool.page_shift;
+  const Layout at = layout<D>(page_size);
+  // K: a thread has position tid / 4 and words (tid % 4, 0 ..) of its row, and the scale of group tid % 4; V: 8
+  // positions tid / 32 and kWords dims.
+  const uint32_t position = (tid >> 2) & 31u, quad = tid & 3u, pairs_at = tid & 31u, eight = (tid >> 5) & 3u;
+  const uint32_t k_off = position * (D / 2) + quad * (kGroups * 4);
+  const uint32_t ks_off = at.k_scales + ((quad % kGroups) << (pool.page_shift + 1)) + position * 2;
+  const uint32_t v_off = at.v_codes + (eight * D + pairs_at * kWords) * 4;
+  const uint32_t v_group = pairs_at * kWords / 32;
+  const uint32_t vs_off = at.v_scales + (v_group << (pool.page_shift + 1)) + eight * 16;
+  const uint32_t j = ((position & 3u) << 1) | ((position >> 2) & 1u);  // kOrder[j] = position % 8
+  const uint32_t k_to = 32 * half_step + 16 * (j >> 2) + 4 * (position >> 3) + (j & 3u);
+
+  const uint32_t steps = begin < end ? (end - begin + kStep - 1) / kStep : 0;
+  // The pages of 64 halves of steps, one a lane, from step s0 on.
+  const auto pages_of = [&](uint32_t s0) {
+    const uint32_t p = begin + s0 * kStep + 32 * lane;
+    return p < end ? pool.page_of(seq, p) : 0xFFFFFFFFu;
+  };
+  uint32_t ids = pages_of(0), later = 0;  // `later`: of the 32 steps after those
+  const auto page_at = [&](uint32_t s, uint32_t half) {  // (ids of the step's 32; the next ones' from the second on)
+    return (uint32_t)__builtin_amdgcn_readlane((int)ids, (int)(2 * (s & 31u) + half));
+  };
+
+  struct Stage {
+    uint32_t k[kWords], v[kWords];
+    u32x4 vs;
+    uint32_t ks;
+  };
+  const auto load = [&](Stage& t, uint32_t page, uint32_t s) {
+    const bool have = page < pool.pages;
+    // (no page: a resource of no bytes, whose loads return zeros)
+    const auto r = egd::buffer(pool.block(have ? page : 0, kv, at.head_bytes), have ? at.head_bytes : 0);
+    const uint32_t slot = (begin + s * kStep + 32 * half_step) & (page_size - 1u);
+    if constexpr (kWords == 4) {
+      const u32x4 k = egd::load_b128(r, k_off, slot * (D / 2)), v = egd::load_b128(r, v_off, (slot / 8) * (D * 4));
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        t.k[i] = k[i];
+        t.v[i] = v[i];
+      }
+    } else {
+      const uint64_t k = egd::load_b64(r, k_off, slot * (D / 2)), v = egd::load_b64(r, v_off, (slot / 8) * (D * 4));
+      t.k[0] = (uint32_t)k;
+      t.k[1] = (uint32_t)(k >> 32);
+      t.v[0] = (uint32_t)v;
+      t.v[1] = (uint32_t)(v >> 32);
+    }
+    t.ks = __builtin_amdgcn_raw_buffer_load_b16(r, ks_off, slot * 2, 0);
+    t.vs = egd::load_b128(r, vs_off, slot * 2);
+  };
+  const auto put = [&](Stage& t, uint32_t s) {
+    const uint32_t buffer = s & 1u;
+    const uint32_t two = t.ks * 0x00010001u;  // (each group's by its quad of lanes)
+    const uint32_t scale[4] = {(uint32_t)__builtin_amdgcn_update_dpp(0, (int)two, 0x00, 0xF, 0xF, true),
+                               (uint32_t)__builtin_amdgcn_update_dpp(0, (int)two, 0x55, 0xF, 0xF, true),
+                               (uint32_t)__builtin_amdgcn_update_dpp(0, (int)two, 0xAA, 0xF, 0xF, true),
+                               (uint32_t)__builtin_amdgcn_update_dpp(0, (int)two, 0xFF, 0xF, 0xF, true)};
+#pragma unroll
+    for (int g = 0; g < kGroups; g++) {
+      const half2v x = halves(scale[g]);
+      const half2v same[4] = {x, x, x, x};
+      k_of[buffer][4 * g + quad][k_to] = values(t.k[g], same, bits_over);
+    }
+    const uint32_t j0 = begin + s * kStep + 32 * half_step + 8 * eight;  // of this thread's V
+    if (begin + (s + 1) * kStep > base) {
+      // positions past the end: values of zero. Scales that are no numbers (their values are none then) would reach, times
+      // a weight of 0, the columns that do not see their position: they are taken out of the product, and noted for the
+      // sums of those that do.
+      t.vs = first_halves(t.vs, max(0, min(8, (int)(end - j0))));
+      uint32_t bad = 0;
+#pragma unroll
+      for (int h = 0; h < 8; h++)
+        if ((t.vs[h / 2] >> (16 * (h & 1)) & 0x7FFFu) >= 0x7C00u) {
+          bad |= 1u << h;
+          t.vs[h / 2] &= h & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+        }
+      if (pairs_at % (32 / kWords) == 0) bad_of[buffer][v_group][4 * half_step + eight] = (uint8_t)bad;
+    }
+    half2v pairs[4];
+    scale_pairs(t.vs, pairs);
+#pragma unroll
+    for (int w = 0; w < kWords; w++) v_of[buffer][4 * half_step + eight][32 * w + pairs_at] = values(t.v[w], pairs, bits_over);
+  };
+
+  // This lane's columns, and what each sees of the sequence's rows.
+  half8 qf[kBlocks][kGroups][kParts];
+  float f[kBlocks];
+  uint64_t sees[kBlocks];
+  Stage stage;
+  if (steps != 0) load(stage, page_at(0, half_step), 0);
+  const uint64_t all = end > base ? ancestors(a.parents, first, n) : 0;
+#pragma unroll
+  for (int b = 0; b < kBlocks; b++) {
+    const uint32_t c = c0 + 16 * b + lr;
+    const bool in = c < n * a.group;
+    const uint32_t row = in ? c / a.group : 0, head = kv * a.group + (in ? c % a.group : 0);
+    sees[b] = (uint64_t)(uint32_t)__shfl((int)(uint32_t)(all >> 32), (int)row, 64) << 32 |
+              (uint32_t)__shfl((int)(uint32_t)all, (int)row, 64);
+    float x[kGroups][8], top = 0.f;
+    const TQ* src = static_cast<const TQ*>(a.q) + (size_t)(first + row) * a.q_stride + (size_t)head * D;
+#pragma unroll
+    for (int g = 0; g < kGroups; g++) {
+      struct alignas(16) Eight {
+        TQ v[8];
+      };
+      const Eight e = *reinterpret_cast<const Eight*>(src + 32 * g + 8 * lg);
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        x[g][i] = in ? to_f32(e.v[kOrder[i]]) : 0.f;
+        top = fmaxf(top, fabsf(x[g][i]));
+      }
+    }
+    top = max_of_head(top);
+    int e = top > 0.f ? 14 - ((int)(__float_as_uint(top) >> 23) - 127) : 0;
+    e = max(-100, min(110, e));
+    f[b] = fmaxf(ldexpf(a.scale, -e), 0x1p-126f);  // (not 0: -inf times it is -inf)
+#pragma unroll
+    for (int g = 0; g < kGroups; g++)
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        float y = ldexpf(x[g][i], e);
+#pragma unroll
+        for (int p = 0; p < kParts; p++) {
+          const _Float16 h = (_Float16)y;
+          y -= (float)h;
+          qf[b][g][p][i] = h;
+        }
+      }
+  }
+
+  f32x4 o[kBlocks][kDims];
+  float m[kBlocks], l[kBlocks];  // running max of the scores before f; this lane's share of the sum
+#pragma unroll
+  for (int b = 0; b < kBlocks; b++) {
+    m[b] = -INFINITY;
+    l[b] = 0.f;
+#pragma unroll
+    for (int i = 0; i < kDims; i++) o[b][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  const auto compute = [&](uint32_t step) {
+    const uint32_t buffer = step & 1u, j0 = begin + step * kStep;
+    f32x4 s[kBlocks][4];
+#pragma unroll
+    for (int b = 0; b < kBlocks; b++)
+#pragma unroll
+      for (int k = 0; k < 4; k++) s[b][k] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int g = 0; g < kGroups; g++)
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const half8 kc = k_of[buffer][4 * g + lg][16 * k + lr];
+#pragma unroll
+        for (int b = 0; b < kBlocks; b++)
+#pragma unroll
+          for (int p = 0; p < kParts; p++) s[b][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, qf[b][g][p], s[b][k], 0, 0, 0);
+      }
+    const bool have0 = page_at(step, 0) < pool.pages, have1 = page_at(step, 1) < pool.pages;
+    if (j0 + kStep > base || !have0 || !have1) {
+      // of the sequence's rows what the column sees; nothing past the end or on no page
+      uint64_t real = end - j0 >= 64 ? ~0ull : (1ull << (end - j0)) - 1u;
+      if (!have0) real &= 0xFFFFFFFF00000000ull;
+      if (!have1) real &= 0x00000000FFFFFFFFull;
+      const bool tail = j0 + kStep > base;
+#pragma unroll
+      for (int b = 0; b < kBlocks; b++) {
+        uint64_t visible = j0 >= base ? sees[b] >> (j0 - base) : ~0ull;
+        if (j0 < base && tail) visible = sees[b] << (base - j0) | ((1ull << (base - j0)) - 1u);
+        visible &= real;
+        const uint64_t mine = visible >> (8 * lg);
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            if (!(mine >> (32 * (k >> 1) + kOrder[4 * (k & 1) + e]) & 1u)) s[b][k][e] = -INFINITY;
+        if (tail) {
+          // this lane's sums are of dims 64 i + 16 lg .. +16 (32 i + 8 lg .. +8 at head_dim 64), i < 2
+#pragma unroll
+          for (int i = 0; i < 2; i++) {
+            const uint32_t group = D == 128 ? 2 * i + (lg >> 1) : i;
+            if (visible & *reinterpret_cast<const uint64_t*>(bad_of[buffer][group])) {
+#pragma unroll
+              for (int x = i; x < kDims; x += 2) o[b][x] += __builtin_nanf("");
+            }
+          }
+        }
+      }
+    }
+    half8 pb[kBlocks][2][kParts];
+#pragma unroll
+    for (int b = 0; b < kBlocks; b++) {
+      float top = m[b];
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) top = fmaxf(top, s[b][k][e]);
+      top = max_of_head(top);
+      float shift = top == -INFINITY ? 0.f : fmaf(top, f[b], -15.f);
+      // (past kLargest the max's own rounding would put weights out of f16's range: there it is taken from the
+      // scores instead, which leaves the largest exactly 0)
+      if (__builtin_amdgcn_ballot_w64(fabsf(shift) > kLargest) != 0) {
+        const float from = top == -INFINITY ? 0.f : top;  // (a column without a position yet)
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) s[b][k][e] -= from;
+        shift = -15.f;
+      }
+      if (__builtin_amdgcn_ballot_w64(top > m[b]) != 0) {
+        const float alpha = top > m[b] ? __builtin_amdgcn_exp2f((m[b] - top) * f[b]) : 1.f;
+        l[b] *= alpha;
+#pragma unroll
+        for (int i = 0; i < kDims; i++) o[b][i] *= alpha;
+        m[b] = top;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          float p = __builtin_amdgcn_exp2f(fmaf(s[b][k][e], f[b], -shift));
+          l[b] += p;
+#pragma unroll
+          for (int x = 0; x < kParts; x++) {
+            const _Float16 h = (_Float16)p;
+            pb[b][k >> 1][x][4 * (k & 1) + e] = h;
+            p -= (float)h;
+          }
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int i = 0; i < kDims; i++) {
+        const half8 va = v_of[buffer][4 * h + lg][16 * i + lr];
+#pragma unroll
+        for (int b = 0; b < kBlocks; b++)
+#pragma unroll
+          for (int x = 0; x < kParts; x++)
+            o[b][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pb[b][h][x], o[b][i], 0, 0, 0);
+      }
+  };
+
+  if (steps != 0) put(stage, 0);
+  if (steps > 1) load(stage, page_at(1, half_step), 1);
+  __syncthreads();
+  for (uint32_t s = 0; s < steps; s++) {
+    if (active) compute(s);
+    if (s + 1 < steps) put(stage, s + 1);
+    if ((s & 31u) == 31u) ids = later;  // (the next step's)
+    if ((s & 31u) == 29u) later = pages_of(s + 3);
+    if (s + 2 < steps) {
+      const uint32_t next = s + 2;
+      const uint32_t page = (next & 31u) == 0 && (s & 31u) == 30u ? (uint32_t)__builtin_amdgcn_readlane((int)later, (int)half_step)
+                                                                : page_at(next, half_step);
+      load(stage, page, next);
+    }
+    __syncthreads();
+  }
+
+  if (!active) return;
+  const bool whole = chunk >= reach;  // no other chunk: the result itself
+#pragma unroll
+  for (int b = 0; b < kBlocks; b++) {
+    const uint32_t c = c0 + 16 * b + lr;
+    float sum = l[b];
+    sum += __shfl_xor(sum, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+    if (c >= n * a.group) continue;
+    const uint32_t r = first + c / a.group, hd = kv * a.group + c % a.group;
+    const size_t at_row = ((size_t)r * a.heads + hd) * a.splits + split;
+    const float x = whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f;
+    if (!whole && lg == 0) *reinterpret_cast<float2*>(a.ml + 2 * at_row) = make_float2(m[b] == -INFINITY ? -INFINITY : m[b] * f[b], sum);
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        float y[kWords];
+#pragma unroll
+        for (int w = 0; w < kWords; w++) y[w] = o[b][i + 2 * w][e] * x;
+        const uint32_t d = (D / 2) * i + (4 * lg + e) * kWords;
+        if (whole) {
+          struct alignas(sizeof(TQ) * kWords) Several {
+            TQ v[kWords];
+          } to;
+#pragma unroll
+          for (int w = 0; w < kWords; w++) to.v[w] = from_f32<TQ>(y[w]);
+          *reinterpret_cast<Several*>(static_cast<TQ*>(a.out) + (size_t)r * a.out_stride + (size_t)hd * D + d) = to;
+        } else {
+          struct alignas(4 * kWords) Several {
+            float v[kWords];
+          } to;
+#pragma unroll
+          for (int w = 0; w < kWords; w++) to.v[w] = y[w];
+          *reinterpret_cast<Several*>(a.o + at_row * D + d) = to;
+        }
+      }
+  }
+}
+
 // A row's chunks joined: a workgroup per (row, head), its waves taking the chunks in turn.
 template <int D, class TQ>
 __global__ __launch_bounds__(256) void join_kernel(Args a, uint32_t sequences) {
@@ -451,8 +788,11 @@ template <int D, class TQ>
 void launch(eg_context* ctx, const Args& a, const Pool& p, uint32_t blocks_of_columns, uint64_t blocks) {
   constexpr int kParts = std::is_same<TQ, float>::value ? 2 : 1;
   const dim3 grid((uint32_t)blocks), threads(kThreads);
-  if (blocks_of_columns == 1) hipLaunchKernelGGL((tree_kernel<D, 1, kParts, TQ>), grid, threads, 0, ctx->stream, a, p);
-  else hipLaunchKernelGGL((tree_kernel<D, 2, kParts, TQ>), grid, threads, 0, ctx->stream, a, p);
+  const auto kernel = blocks_of_columns == 1   ? tree_kernel<D, 1, kParts, TQ>
+                      : blocks_of_columns == 2 ? tree_kernel<D, 2, kParts, TQ>
+                      : blocks_of_columns == 4 ? wide_kernel<D, 1, kParts, TQ>
+                                               : wide_kernel<D, 2, kParts, TQ>;
+  hipLaunchKernelGGL(kernel, grid, threads, 0, ctx->stream, a, p);
   if (a.splits > 1)
     hipLaunchKernelGGL((join_kernel<D, TQ>), dim3(a.rows * a.heads), threads, 0, ctx->stream, a, p.sequences);
 }
@@ -496,7 +836,7 @@ extern "C" int eg_attention_tree_kv4(eg_context* ctx, const void* q, const uint3
     return eg::fail(ctx, EG_ERR_INVALID, "%s: q and out must be 16-byte aligned", op);
   if (!some) return EG_OK;
   a.scale = (d.scale > 0.f ? d.scale : 1.0f / sqrtf((float)dims->head_dim)) * kLog2e;
-  const uint32_t columns = std::min(d.max_rows, d.rows) * a.group, per_tile = columns <= 16 ? 1 : 2;
+  const uint32_t columns = std::min(d.max_rows, d.rows) * a.group, per_tile = columns <= 16 ? 1 : columns <= 32 ? 2 : columns <= 64 ? 4 : 8;
   a.tiles = (columns + 16 * per_tile - 1) / (16 * per_tile);
   // Splits: workgroups for two a CU, of chunks of at least two steps a wave.
   a.min_chunk = 256;
