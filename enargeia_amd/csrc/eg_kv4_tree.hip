@@ -3,10 +3,10 @@
 //   out[r][h] = sum_j p_j V[j] / sum_j p_j,  p_j = exp(scale q[r][h] . K[j] - max_j),  j of those that row r sees
 //
 // The decode attention (eg_kv4_attention.hip) with more columns: a kv head's columns are all its query heads of all
-// the sequence's rows, in blocks of 16, and a tile of 32 positions, dequantized once, is multiplied with kBlocks of
-// them. One pass over the cache with the running max and sum of the softmax; a workgroup's waves take a chunk's
-// tiles in turn and meet in LDS, chunks meet in a second launch. Which of the last positions a column sees is
-// its row's ancestors, as 64 bits; tiles before them have no mask.
+// the sequence's rows, in blocks of 16, and a tile of positions serves as many of them as there are. One pass over the
+// cache with the running max and sum of the softmax; chunks of a sequence's positions meet in a second launch. Which of
+// the last positions a column sees is its row's ancestors, as 64 bits; tiles before them have no mask. Two kernels: few
+// columns bind by what a wave waits for and unpacks, many by issue (products and vector instructions hardly overlap).
 #include <algorithm>
 
 #include "eg_kv4_operands.hpp"
@@ -58,13 +58,57 @@ __device__ __forceinline__ uint64_t ancestors(const uint32_t* parents, uint32_t 
   return (uint64_t)hi << 32 | lo;
 }
 
-// D: head_dim. kBlocks: blocks of 16 columns a wave multiplies a tile with. kParts: f16 parts of a query and of a
-// weight (2 for f32 rows).
-template <int D, int kBlocks, int kParts, class TQ>
-__global__ __launch_bounds__(256, 2) void tree_kernel(Args a, Pool pool) {
+// Those bits of a row.
+__device__ __forceinline__ uint64_t of_row(uint64_t all, uint32_t row) {
+  return (uint64_t)(uint32_t)__shfl((int)(uint32_t)(all >> 32), (int)row, 64) << 32 |
+         (uint32_t)__shfl((int)(uint32_t)all, (int)row, 64);
+}
+
+// A column's query as the first product's B operand: lane group g has dims 32 grp + 8 g + kOrder[slot], times the
+// power of two that puts the largest of the column's into [2^14, 2^15), whose exponent is returned.
+template <int D, int kParts, class TQ>
+__device__ __forceinline__ int load_queries(const Args& a, uint32_t row, uint32_t head, bool in, uint32_t lg,
+                                            half8 (&qf)[D / 32][kParts]) {
+  struct alignas(16) Eight {
+    TQ v[8];
+  };
+  const TQ* src = static_cast<const TQ*>(a.q) + (size_t)row * a.q_stride + (size_t)head * D;
+  float x[D / 32][8], top = 0.f;
+#pragma unroll
+  for (int g = 0; g < D / 32; g++) {
+    const Eight e = *reinterpret_cast<const Eight*>(src + 32 * g + 8 * lg);
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      x[g][i] = in ? to_f32(e.v[kOrder[i]]) : 0.f;
+      top = fmaxf(top, fabsf(x[g][i]));
+    }
+  }
+  top = max_of_head(top);
+  const int up = max(-100, min(110, top > 0.f ? 14 - ((int)(__float_as_uint(top) >> 23) - 127) : 0));
+#pragma unroll
+  for (int g = 0; g < D / 32; g++)
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      float y = ldexpf(x[g][i], up);
+#pragma unroll
+      for (int p = 0; p < kParts; p++) {
+        const _Float16 h = (_Float16)y;
+        y -= (float)h;
+        qf[g][p][i] = h;
+      }
+    }
+  return up;
+}
+
+// Few columns: 16 a workgroup, whose waves take a chunk's tiles of 32 positions in turn and meet in LDS. D: head_dim. kParts:
+// f16 parts of a query and of a weight (2 for f32 rows). (With two blocks of columns a wave, 32 / 8 heads of 128 in
+// bf16: 16 sequences of up to 2048 with 8 rows 35.1 us for 22.9, 32 of up to 4096 62.3 for 54.8: half as many workgroups,
+// and no registers left for the next tile's words.)
+template <int D, int kParts, class TQ>
+__global__ __launch_bounds__(256, 2) void few_kernel(Args a, Pool pool) {
   constexpr int kGroups = D / 32, kDims = D / 16;  // dim groups of K; blocks of 16 dims of O^T
   constexpr bool kSigned = kParts == 2;
-  constexpr uint32_t kTile = 32, kColumns = 16 * kBlocks;
+  constexpr uint32_t kTile = 32, kColumns = 16;
   constexpr int kVWords = D / 16;  // V words of a lane: its dims D / 16 * (lane % 16) + 0 ..
   const uint32_t tid = threadIdx.x, lane = tid & 63u;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -85,16 +129,10 @@ __global__ __launch_bounds__(256, 2) void tree_kernel(Args a, Pool pool) {
   const uint32_t base = fits ? length - n : 0, end = fits ? min(reach, begin + chunk) : 0;
   const Magic bits_over = magic();
 
-  // This lane's columns: row and head of each block's.
-  uint32_t row[kBlocks], head[kBlocks];
-  bool in[kBlocks];
-#pragma unroll
-  for (int b = 0; b < kBlocks; b++) {
-    const uint32_t c = tile * kColumns + 16 * b + lr;
-    in[b] = c < n * a.group;
-    row[b] = in[b] ? c / a.group : 0;
-    head[b] = kv * a.group + (in[b] ? c % a.group : 0);
-  }
+  // This lane's column.
+  const uint32_t c0 = tile * kColumns, column = c0 + lr;
+  const bool in = column < n * a.group;
+  const uint32_t row = in ? column / a.group : 0, head = kv * a.group + (in ? column % a.group : 0);
 
   const uint32_t page_size = 1u << pool.page_shift;
   const Layout at = layout<D>(page_size);
@@ -153,110 +191,61 @@ __global__ __launch_bounds__(256, 2) void tree_kernel(Args a, Pool pool) {
   };
   uint32_t ids = pages_of(0);
 
-  // What each column sees of the sequence's rows.
-  uint64_t sees[kBlocks];
-  if (end > base) {
-    const uint64_t all = ancestors(a.parents, first, n);
-#pragma unroll
-    for (int b = 0; b < kBlocks; b++)
-      sees[b] = (uint64_t)(uint32_t)__shfl((int)(uint32_t)(all >> 32), (int)row[b], 64) << 32 |
-                (uint32_t)__shfl((int)(uint32_t)all, (int)row[b], 64);
-  }
+  const uint64_t sees = end > base ? of_row(ancestors(a.parents, first, n), row) : 0;
 
   // The queries, B operand: lane group g has dims 32 grp + 8 g + kOrder[slot] of column lr.
-  half8 qf[kBlocks][kGroups][kParts];
-  f32x4 start[kBlocks][kGroups];  // -8 sum q per group: what makes codes of code - 8
-  float f[kBlocks];
+  half8 qf[kGroups][kParts];
+  f32x4 start[kGroups];  // -8 sum q per group: what makes codes of code - 8
+  const int up = load_queries<D, kParts, TQ>(a, first + row, head, in, lg, qf);
+  const float f = fmaxf(ldexpf(a.scale, kSigned ? -up : 24 - up), 0x1p-126f);  // (not 0: -inf times it is -inf)
 #pragma unroll
-  for (int b = 0; b < kBlocks; b++) {
-    float x[kGroups][8], top = 0.f;
-    const TQ* src = static_cast<const TQ*>(a.q) + (size_t)(first + row[b]) * a.q_stride + (size_t)head[b] * D;
-#pragma unroll
-    for (int g = 0; g < kGroups; g++) {
-      struct alignas(16) Eight {
-        TQ v[8];
-      };
-      const Eight e = *reinterpret_cast<const Eight*>(src + 32 * g + 8 * lg);
-#pragma unroll
-      for (int i = 0; i < 8; i++) {
-        x[g][i] = in[b] ? to_f32(e.v[kOrder[i]]) : 0.f;
-        top = fmaxf(top, fabsf(x[g][i]));
-      }
-    }
-    top = max_of_head(top);
-    int e = top > 0.f ? 14 - ((int)(__float_as_uint(top) >> 23) - 127) : 0;
-    e = max(-100, min(110, e));
-    f[b] = fmaxf(ldexpf(a.scale, kSigned ? -e : 24 - e), 0x1p-126f);  // (not 0: -inf times it is -inf)
-#pragma unroll
-    for (int g = 0; g < kGroups; g++) {
-#pragma unroll
-      for (int i = 0; i < 8; i++) {
-        float y = ldexpf(x[g][i], e);
-#pragma unroll
-        for (int p = 0; p < kParts; p++) {
-          const _Float16 h = (_Float16)y;
-          y -= (float)h;
-          qf[b][g][p][i] = !kSigned && (i & 2) ? h * (_Float16)0.0625f : h;
-        }
-      }
+  for (int g = 0; g < kGroups; g++) {
+    start[g] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if constexpr (!kSigned) {
       const half8 eight = as_half8(0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u);
-      start[b][g] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if constexpr (!kSigned) {
 #pragma unroll
-        for (int p = 0; p < kParts; p++)
-          start[b][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(eight, qf[b][g][p], start[b][g], 0, 0, 0);
+      for (int p = 0; p < kParts; p++) {
+#pragma unroll
+        for (int i = 2; i < 8; i++)
+          if (i & 2) qf[g][p][i] *= (_Float16)0.0625f;
+        start[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(eight, qf[g][p], start[g], 0, 0, 0);
       }
     }
   }
 
-  f32x4 o[kBlocks][kDims];
-  float m[kBlocks], l[kBlocks];  // running max of the scores before f; this lane's share of the sum
+  f32x4 o[kDims];
 #pragma unroll
-  for (int b = 0; b < kBlocks; b++) {
-    m[b] = -INFINITY;
-    l[b] = 0.f;
-#pragma unroll
-    for (int i = 0; i < kDims; i++) o[b][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
+  for (int i = 0; i < kDims; i++) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;  // running max of the scores before f; this lane's share of the sum
 
   const auto compute = [&](Tile& t, uint32_t i) {
     const uint32_t j0 = begin + (wave + kWaves * i) * kTile;
-    f32x4 s[kBlocks][2];
-#pragma unroll
-    for (int b = 0; b < kBlocks; b++)
-#pragma unroll
-      for (int k = 0; k < 2; k++) s[b][k] = f32x4{0.f, 0.f, 0.f, 0.f};
+    f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
     for (int k = 0; k < 2; k++)
 #pragma unroll
       for (int g = 0; g < kGroups; g++) {
         const half8 kc = codes<kSigned>(t.k[k][g], bits_over);
+        f32x4 acc = start[g];
 #pragma unroll
-        for (int b = 0; b < kBlocks; b++) {
-          f32x4 acc = start[b][g];
+        for (int p = 0; p < kParts; p++) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, qf[g][p], acc, 0, 0, 0);
 #pragma unroll
-          for (int p = 0; p < kParts; p++) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, qf[b][g][p], acc, 0, 0, 0);
-#pragma unroll
-          for (int e = 0; e < 4; e++) s[b][k][e] = fmaf(half_of(t.ks[g], kOrder[4 * k + e]), acc[e], s[b][k][e]);
-        }
+        for (int e = 0; e < 4; e++) s[k][e] = fmaf(half_of(t.ks[g], kOrder[4 * k + e]), acc[e], s[k][e]);
       }
-    uint32_t poison = 0;  // blocks whose column sees a value that is not a number
+    bool poison = false;  // the column sees a value that is not a number
     if (j0 + kTile > base || !t.have) {
       // positions past the end: no score, values of zero; of the sequence's rows what the column sees
       const int seen = t.have ? (int)(end - j0) : 0;  // of the tile
       t.vs = first_halves(t.vs, max(0, min(8, seen - (int)(8 * lg))));
-      uint32_t visible[kBlocks];  // of this tile's 32 positions
+      uint32_t visible = 0xFFFFFFFFu;  // of the tile's 32 positions
+      if (j0 >= base) visible = (uint32_t)(sees >> (j0 - base));
+      else if (base - j0 < 32) visible = (uint32_t)(sees << (base - j0)) | ((1u << (base - j0)) - 1u);
+      if (seen < 32) visible &= seen <= 0 ? 0u : (1u << seen) - 1u;
 #pragma unroll
-      for (int b = 0; b < kBlocks; b++) {
-        uint32_t v = j0 >= base ? (uint32_t)(sees[b] >> (j0 - base)) : 0;
-        if (j0 < base) v = base - j0 >= 32 ? 0xFFFFFFFFu : (uint32_t)(sees[b] << (base - j0)) | ((1u << (base - j0)) - 1u);
-        visible[b] = seen >= 32 ? v : seen <= 0 ? 0 : v & ((1u << seen) - 1u);
+      for (int k = 0; k < 2; k++)
 #pragma unroll
-        for (int k = 0; k < 2; k++)
-#pragma unroll
-          for (int e = 0; e < 4; e++)
-            if (!(visible[b] >> (8 * lg + kOrder[4 * k + e]) & 1u)) s[b][k][e] = -INFINITY;
-      }
+        for (int e = 0; e < 4; e++)
+          if (!(visible >> (8 * lg + kOrder[4 * k + e]) & 1u)) s[k][e] = -INFINITY;
       // A scale that is not a number (its values are none then) would reach, times a weight of 0, the columns that do
       // not see its position: it is taken out of the product, and put into the sums of those that do.
       uint32_t bad = 0;  // of this lane's 8 positions
@@ -275,55 +264,50 @@ __global__ __launch_bounds__(256, 2) void tree_kernel(Args a, Pool pool) {
         uint32_t mask = 0;
 #pragma unroll
         for (uint32_t x = 0; x < 4; x++) mask |= (uint32_t)__shfl((int)bad, (int)(16 * x + holder), 64) << (8 * x);
-#pragma unroll
-        for (int b = 0; b < kBlocks; b++)
-          if (visible[b] & mask) poison |= 1u << b;
+        poison = (visible & mask) != 0;
       }
     }
-    half8 pb[kBlocks][kParts];
+    float top = m;
 #pragma unroll
-    for (int b = 0; b < kBlocks; b++) {
-      float top = m[b];
+    for (int k = 0; k < 2; k++)
 #pragma unroll
-      for (int k = 0; k < 2; k++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) top = fmaxf(top, s[b][k][e]);
-      top = max_of_head(top);
-      float shift = top == -INFINITY ? 0.f : fmaf(top, f[b], -15.f);
-      // (past kLargest the max's own rounding would put weights out of f16's range: there it is taken from the
-      // scores instead, which leaves the largest exactly 0)
-      if (__builtin_amdgcn_ballot_w64(fabsf(shift) > kLargest) != 0) {
-        const float from = top == -INFINITY ? 0.f : top;  // (a column without a position yet)
-#pragma unroll
-        for (int k = 0; k < 2; k++)
-#pragma unroll
-          for (int e = 0; e < 4; e++) s[b][k][e] -= from;
-        shift = -15.f;
-      }
-      if (__builtin_amdgcn_ballot_w64(top > m[b]) != 0) {
-        const float alpha = top > m[b] ? __builtin_amdgcn_exp2f((m[b] - top) * f[b]) : 1.f;
-        l[b] *= alpha;
-#pragma unroll
-        for (int i = 0; i < kDims; i++) o[b][i] *= alpha;
-        m[b] = top;
-      }
+      for (int e = 0; e < 4; e++) top = fmaxf(top, s[k][e]);
+    top = max_of_head(top);
+    float shift = top == -INFINITY ? 0.f : fmaf(top, f, -15.f);
+    // (past kLargest the max's own rounding would put weights out of f16's range: there it is taken from the
+    // scores instead, which leaves the largest exactly 0)
+    if (__builtin_amdgcn_ballot_w64(fabsf(shift) > kLargest) != 0) {
+      const float from = top == -INFINITY ? 0.f : top;  // (a column without a position yet)
 #pragma unroll
       for (int k = 0; k < 2; k++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          float p = __builtin_amdgcn_exp2f(fmaf(s[b][k][e], f[b], -shift));
-          l[b] += p;
+        for (int e = 0; e < 4; e++) s[k][e] -= from;
+      shift = -15.f;
+    }
+    if (__builtin_amdgcn_ballot_w64(top > m) != 0) {
+      const float alpha = top > m ? __builtin_amdgcn_exp2f((m - top) * f) : 1.f;
+      l *= alpha;
 #pragma unroll
-          for (int x = 0; x < kParts; x++) {
-            const _Float16 h = (_Float16)p;
-            pb[b][x][4 * k + e] = h;
-            p -= (float)h;
-          }
+      for (int i = 0; i < kDims; i++) o[i] *= alpha;
+      m = top;
+    }
+    half8 pb[kParts];
+#pragma unroll
+    for (int k = 0; k < 2; k++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        float p = __builtin_amdgcn_exp2f(fmaf(s[k][e], f, -shift));
+        l += p;
+#pragma unroll
+        for (int x = 0; x < kParts; x++) {
+          const _Float16 h = (_Float16)p;
+          pb[x][4 * k + e] = h;
+          p -= (float)h;
         }
-      if (poison >> b & 1u) {
-#pragma unroll
-        for (int i = 0; i < kDims; i++) o[b][i] += __builtin_nanf("");
       }
+    if (poison) {
+#pragma unroll
+      for (int i = 0; i < kDims; i++) o[i] += __builtin_nanf("");
     }
     half2v pairs[4];
     scale_pairs(t.vs, pairs);
@@ -331,9 +315,7 @@ __global__ __launch_bounds__(256, 2) void tree_kernel(Args a, Pool pool) {
     for (int i = 0; i < kDims; i++) {
       const half8 va = values(t.v[i], pairs, bits_over);
 #pragma unroll
-      for (int b = 0; b < kBlocks; b++)
-#pragma unroll
-        for (int x = 0; x < kParts; x++) o[b][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pb[b][x], o[b][i], 0, 0, 0);
+      for (int x = 0; x < kParts; x++) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pb[x], o[i], 0, 0, 0);
     }
   };
 
@@ -354,58 +336,51 @@ __global__ __launch_bounds__(256, 2) void tree_kernel(Args a, Pool pool) {
     }
   }
 
-  // The waves meet in LDS, a block of columns at a time.
+  // The waves meet in LDS.
   __shared__ float top_of[kWaves][16], sum_of[kWaves][16];
   __shared__ __attribute__((aligned(16))) float part_of[kWaves][16][D];
   const bool whole = chunk >= reach;  // no other chunk: the result itself
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  if (lg == 0) {
+    top_of[wave][lr] = m == -INFINITY ? -INFINITY : m * f;
+    sum_of[wave][lr] = l;
+  }
+  // row 4 lg + e of block i is dim D / 16 (4 lg + e) + i
 #pragma unroll
-  for (int b = 0; b < kBlocks; b++) {
-    const uint32_t c0 = tile * kColumns + 16 * b;
-    if (c0 >= n * a.group) break;
-    if (b) __syncthreads();
-    float sum_l = l[b];
-    sum_l += __shfl_xor(sum_l, 16, 64);
-    sum_l += __shfl_xor(sum_l, 32, 64);
-    if (lg == 0) {
-      top_of[wave][lr] = m[b] == -INFINITY ? -INFINITY : m[b] * f[b];
-      sum_of[wave][lr] = sum_l;
+  for (int e = 0; e < 4; e++)
+#pragma unroll
+    for (int i = 0; i < kDims; i += 4)
+      *reinterpret_cast<float4*>(&part_of[wave][lr][kDims * (4 * lg + e) + i]) =
+          make_float4(o[i][e], o[i + 1][e], o[i + 2][e], o[i + 3][e]);
+  __syncthreads();
+  const uint32_t columns = min(16u, n * a.group - c0);
+  for (uint32_t i = tid; i < columns * (D / 4); i += kThreads) {
+    const uint32_t h = i / (D / 4), d = 4 * (i % (D / 4));
+    float top = -INFINITY;
+#pragma unroll
+    for (uint32_t w = 0; w < kWaves; w++) top = fmaxf(top, top_of[w][h]);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
+#pragma unroll
+    for (uint32_t w = 0; w < kWaves; w++) {
+      const float c = top_of[w][h] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top_of[w][h] - top);
+      const float4 v = *reinterpret_cast<const float4*>(&part_of[w][h][d]);
+      sum = fmaf(c, sum_of[w][h], sum);
+      acc = make_float4(fmaf(c, v.x, acc.x), fmaf(c, v.y, acc.y), fmaf(c, v.z, acc.z), fmaf(c, v.w, acc.w));
     }
-    // row 4 lg + e of block i is dim D / 16 (4 lg + e) + i
-#pragma unroll
-    for (int e = 0; e < 4; e++)
-#pragma unroll
-      for (int i = 0; i < kDims; i += 4)
-        *reinterpret_cast<float4*>(&part_of[wave][lr][kDims * (4 * lg + e) + i]) =
-            make_float4(o[b][i][e], o[b][i + 1][e], o[b][i + 2][e], o[b][i + 3][e]);
-    __syncthreads();
-    const uint32_t columns = min(16u, n * a.group - c0);
-    for (uint32_t i = tid; i < columns * (D / 4); i += kThreads) {
-      const uint32_t h = i / (D / 4), d = 4 * (i % (D / 4));
-      float top = -INFINITY;
-#pragma unroll
-      for (uint32_t w = 0; w < kWaves; w++) top = fmaxf(top, top_of[w][h]);
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      float sum = 0.f;
-#pragma unroll
-      for (uint32_t w = 0; w < kWaves; w++) {
-        const float c = top_of[w][h] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top_of[w][h] - top);
-        const float4 v = *reinterpret_cast<const float4*>(&part_of[w][h][d]);
-        sum = fmaf(c, sum_of[w][h], sum);
-        acc = make_float4(fmaf(c, v.x, acc.x), fmaf(c, v.y, acc.y), fmaf(c, v.z, acc.z), fmaf(c, v.w, acc.w));
-      }
-      const uint32_t r = first + (c0 + h) / a.group, hd = kv * a.group + (c0 + h) % a.group;
-      if (whole) {
-        const float x = sum == 0.f ? 0.f : 1.f / sum;
-        TQ* to = static_cast<TQ*>(a.out) + (size_t)r * a.out_stride + (size_t)hd * D + d;
-        to[0] = from_f32<TQ>(acc.x * x);
-        to[1] = from_f32<TQ>(acc.y * x);
-        to[2] = from_f32<TQ>(acc.z * x);
-        to[3] = from_f32<TQ>(acc.w * x);
-      } else {
-        const size_t at_row = ((size_t)r * a.heads + hd) * a.splits + split;
-        *reinterpret_cast<float4*>(a.o + at_row * D + d) = acc;
-        if (d == 0) *reinterpret_cast<float2*>(a.ml + 2 * at_row) = make_float2(top, sum);
-      }
+    const uint32_t r = first + (c0 + h) / a.group, hd = kv * a.group + (c0 + h) % a.group;
+    if (whole) {
+      const float x = sum == 0.f ? 0.f : 1.f / sum;
+      TQ* to = static_cast<TQ*>(a.out) + (size_t)r * a.out_stride + (size_t)hd * D + d;
+      to[0] = from_f32<TQ>(acc.x * x);
+      to[1] = from_f32<TQ>(acc.y * x);
+      to[2] = from_f32<TQ>(acc.z * x);
+      to[3] = from_f32<TQ>(acc.w * x);
+    } else {
+      const size_t at_row = ((size_t)r * a.heads + hd) * a.splits + split;
+      *reinterpret_cast<float4*>(a.o + at_row * D + d) = acc;
+      if (d == 0) *reinterpret_cast<float2*>(a.ml + 2 * at_row) = make_float2(top, sum);
     }
   }
 }
@@ -423,6 +398,10 @@ __global__ __launch_bounds__(256, 2) void tree_kernel(Args a, Pool pool) {
 template <int D, int kBlocks, int kParts, class TQ>
 __global__ __launch_bounds__(256, 2) void wide_kernel(Args a, Pool pool) {
   constexpr int kGroups = D / 32, kDims = D / 16, kWords = D / 32;  // kWords: of K and of V, a thread and step
+  // The max is taken up only where it has grown by kLag (in powers of two): with 16-bit rows, whose weights are scaled by
+  // that much less, a column's sums are then rescaled about once (8 of up to 8192, 64 rows, 32 / 8 heads of 128, bf16: 92.6
+  // us, rescaled at every new max 98).
+  constexpr float kLag = kParts == 2 ? 0.f : 3.f, kShift = 15.f - kLag;
   constexpr uint32_t kStep = 64, kColumns = 64 * kBlocks, kPad = kStep + 1;
   __shared__ half8 k_of[2][D / 8][kPad], v_of[2][8][D];
   __shared__ __attribute__((aligned(8))) uint8_t bad_of[2][kGroups][8];  // of a tail step's V: positions (8 a byte) whose scale is no number
@@ -544,38 +523,9 @@ __global__ __launch_bounds__(256, 2) void wide_kernel(Args a, Pool pool) {
     const uint32_t c = c0 + 16 * b + lr;
     const bool in = c < n * a.group;
     const uint32_t row = in ? c / a.group : 0, head = kv * a.group + (in ? c % a.group : 0);
-    sees[b] = (uint64_t)(uint32_t)__shfl((int)(uint32_t)(all >> 32), (int)row, 64) << 32 |
-              (uint32_t)__shfl((int)(uint32_t)all, (int)row, 64);
-    float x[kGroups][8], top = 0.f;
-    const TQ* src = static_cast<const TQ*>(a.q) + (size_t)(first + row) * a.q_stride + (size_t)head * D;
-#pragma unroll
-    for (int g = 0; g < kGroups; g++) {
-      struct alignas(16) Eight {
-        TQ v[8];
-      };
-      const Eight e = *reinterpret_cast<const Eight*>(src + 32 * g + 8 * lg);
-#pragma unroll
-      for (int i = 0; i < 8; i++) {
-        x[g][i] = in ? to_f32(e.v[kOrder[i]]) : 0.f;
-        top = fmaxf(top, fabsf(x[g][i]));
-      }
-    }
-    top = max_of_head(top);
-    int e = top > 0.f ? 14 - ((int)(__float_as_uint(top) >> 23) - 127) : 0;
-    e = max(-100, min(110, e));
-    f[b] = fmaxf(ldexpf(a.scale, -e), 0x1p-126f);  // (not 0: -inf times it is -inf)
-#pragma unroll
-    for (int g = 0; g < kGroups; g++)
-#pragma unroll
-      for (int i = 0; i < 8; i++) {
-        float y = ldexpf(x[g][i], e);
-#pragma unroll
-        for (int p = 0; p < kParts; p++) {
-          const _Float16 h = (_Float16)y;
-          y -= (float)h;
-          qf[b][g][p][i] = h;
-        }
-      }
+    sees[b] = of_row(all, row);
+    const int up = load_queries<D, kParts, TQ>(a, first + row, head, in, lg, qf[b]);
+    f[b] = fmaxf(ldexpf(a.scale, -up), 0x1p-126f);  // (not 0: -inf times it is -inf)
   }
 
   f32x4 o[kBlocks][kDims];
@@ -645,23 +595,23 @@ __global__ __launch_bounds__(256, 2) void wide_kernel(Args a, Pool pool) {
 #pragma unroll
         for (int e = 0; e < 4; e++) top = fmaxf(top, s[b][k][e]);
       top = max_of_head(top);
-      float shift = top == -INFINITY ? 0.f : fmaf(top, f[b], -15.f);
-      // (past kLargest the max's own rounding would put weights out of f16's range: there it is taken from the
-      // scores instead, which leaves the largest exactly 0)
-      if (__builtin_amdgcn_ballot_w64(fabsf(shift) > kLargest) != 0) {
-        const float from = top == -INFINITY ? 0.f : top;  // (a column without a position yet)
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-#pragma unroll
-          for (int e = 0; e < 4; e++) s[b][k][e] -= from;
-        shift = -15.f;
-      }
-      if (__builtin_amdgcn_ballot_w64(top > m[b]) != 0) {
+      if (__builtin_amdgcn_ballot_w64((top - m[b]) * f[b] > kLag) != 0) {
         const float alpha = top > m[b] ? __builtin_amdgcn_exp2f((m[b] - top) * f[b]) : 1.f;
         l[b] *= alpha;
 #pragma unroll
         for (int i = 0; i < kDims; i++) o[b][i] *= alpha;
         m[b] = top;
+      }
+      float shift = m[b] == -INFINITY ? 0.f : fmaf(m[b], f[b], -kShift);
+      // (past kLargest the max's own rounding would put weights out of f16's range: there it is taken from the
+      // scores instead, which leaves the largest exactly 0)
+      if (__builtin_amdgcn_ballot_w64(fabsf(shift) > kLargest) != 0) {
+        const float from = m[b] == -INFINITY ? 0.f : m[b];  // (a column without a position yet)
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) s[b][k][e] -= from;
+        shift = -kShift;
       }
 #pragma unroll
       for (int k = 0; k < 4; k++)
@@ -747,54 +697,58 @@ __global__ __launch_bounds__(256, 2) void wide_kernel(Args a, Pool pool) {
   }
 }
 
-// A row's chunks joined: a workgroup per (row, head), its waves taking the chunks in turn.
+// The chunks of kTogether (row, head) joined by a workgroup, D / 4 threads each.
 template <int D, class TQ>
 __global__ __launch_bounds__(256) void join_kernel(Args a, uint32_t sequences) {
-  constexpr uint32_t kPer = D / 64;
-  const uint32_t head = blockIdx.x % a.heads, r = blockIdx.x / a.heads, tid = threadIdx.x;
-  const uint32_t lane = tid & 63u, wave = tid >> 6;
-  uint32_t seq, first, last;
-  if (!find_sequence(a.offsets, sequences, r, seq, first, last)) return;
-  const uint32_t reach = min(a.lengths[seq], a.capacity), chunk = chunk_of(a, reach);
-  if (!computed(a, first, last) || chunk >= reach) return;  // (one chunk: it wrote the result)
+  constexpr uint32_t kEach = D / 4, kTogether = kThreads / kEach;
+  const uint32_t i = blockIdx.x * kTogether + threadIdx.x / kEach, d = 4 * (threadIdx.x % kEach);
+  const uint32_t r = i / a.heads, head = i % a.heads;
+  if (r >= a.rows) return;
+  uint32_t lo = 0, hi = sequences;  // the sequence: the last that begins at r or before
+  while (hi - lo > 1) {
+    const uint32_t mid = (lo + hi) / 2;
+    if (a.offsets[mid] <= r) lo = mid;
+    else hi = mid;
+  }
+  const uint32_t first = a.offsets[lo], last = a.offsets[lo + 1];
+  if (r < first || r >= last || !computed(a, first, last)) return;
+  const uint32_t reach = min(a.lengths[lo], a.capacity), chunk = chunk_of(a, reach);
+  if (chunk >= reach) return;  // (one chunk: it wrote the result)
   const uint32_t count = (reach + chunk - 1) / chunk;
-  const size_t at_row = ((size_t)r * a.heads + head) * a.splits;
-  const float* ml = a.ml + 2 * at_row;
-  float top = -INFINITY;
-  for (uint32_t c = lane; c < count; c += 64) top = fmaxf(top, ml[2 * c]);
-  top = egd::team_allmax<64>(top);
-  float acc[kPer] = {}, sum = 0.f;
+  const size_t at_row = (size_t)i * a.splits;
+  const float2* ml = reinterpret_cast<const float2*>(a.ml) + at_row;
+  const float* o = a.o + at_row * D + d;
+  float top = -INFINITY, sum = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-  for (uint32_t c = wave; c < count; c += kWaves) {
-    const float w = ml[2 * c] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[2 * c] - top);
-    sum = fmaf(w, ml[2 * c + 1], sum);
-#pragma unroll
-    for (uint32_t j = 0; j < kPer; j++) acc[j] = fmaf(w, a.o[(at_row + c) * D + 64 * j + lane], acc[j]);
+  for (uint32_t c = 0; c < count; c++) {
+    const float2 s = ml[c];
+    const float4 v = *reinterpret_cast<const float4*>(o + (size_t)c * D);
+    const float to = fmaxf(top, s.x), from = to == -INFINITY ? 0.f : to;
+    const float x = __builtin_amdgcn_exp2f(top - from), y = __builtin_amdgcn_exp2f(s.x - from);
+    sum = fmaf(sum, x, s.y * y);
+    acc = make_float4(fmaf(acc.x, x, v.x * y), fmaf(acc.y, x, v.y * y), fmaf(acc.z, x, v.z * y), fmaf(acc.w, x, v.w * y));
+    top = to;
   }
-  __shared__ float part[kWaves][D], sums[kWaves];
-#pragma unroll
-  for (uint32_t j = 0; j < kPer; j++) part[wave][64 * j + lane] = acc[j];
-  if (lane == 0) sums[wave] = sum;
-  __syncthreads();
-  if (tid < D) {
-    const float total = (sums[0] + sums[1]) + (sums[2] + sums[3]);
-    const float v = (part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid]);
-    static_cast<TQ*>(a.out)[(size_t)r * a.out_stride + (size_t)head * D + tid] =
-        from_f32<TQ>(total == 0.f ? 0.f : v / total);
-  }
+  const float x = sum == 0.f ? 0.f : 1.f / sum;
+  struct alignas(4 * sizeof(TQ)) Four {
+    TQ v[4];
+  };
+  *reinterpret_cast<Four*>(static_cast<TQ*>(a.out) + (size_t)r * a.out_stride + (size_t)head * D + d) =
+      Four{{from_f32<TQ>(acc.x * x), from_f32<TQ>(acc.y * x), from_f32<TQ>(acc.z * x), from_f32<TQ>(acc.w * x)}};
 }
 
 template <int D, class TQ>
-void launch(eg_context* ctx, const Args& a, const Pool& p, uint32_t blocks_of_columns, uint64_t blocks) {
+void launch(eg_context* ctx, const Args& a, const Pool& p, uint32_t per_tile, uint64_t blocks) {
   constexpr int kParts = std::is_same<TQ, float>::value ? 2 : 1;
   const dim3 grid((uint32_t)blocks), threads(kThreads);
-  const auto kernel = blocks_of_columns == 1   ? tree_kernel<D, 1, kParts, TQ>
-                      : blocks_of_columns == 2 ? tree_kernel<D, 2, kParts, TQ>
-                      : blocks_of_columns == 4 ? wide_kernel<D, 1, kParts, TQ>
-                                               : wide_kernel<D, 2, kParts, TQ>;
+  const auto kernel = per_tile == 1   ? few_kernel<D, kParts, TQ>
+                      : per_tile == 4 ? wide_kernel<D, 1, kParts, TQ>
+                                      : wide_kernel<D, 2, kParts, TQ>;
   hipLaunchKernelGGL(kernel, grid, threads, 0, ctx->stream, a, p);
   if (a.splits > 1)
-    hipLaunchKernelGGL((join_kernel<D, TQ>), dim3(a.rows * a.heads), threads, 0, ctx->stream, a, p.sequences);
+    hipLaunchKernelGGL((join_kernel<D, TQ>), dim3((a.rows * a.heads * (D / 4) + kThreads - 1) / kThreads), threads, 0,
+                       ctx->stream, a, p.sequences);
 }
 
 }  // namespace
@@ -836,14 +790,23 @@ extern "C" int eg_attention_tree_kv4(eg_context* ctx, const void* q, const uint3
     return eg::fail(ctx, EG_ERR_INVALID, "%s: q and out must be 16-byte aligned", op);
   if (!some) return EG_OK;
   a.scale = (d.scale > 0.f ? d.scale : 1.0f / sqrtf((float)dims->head_dim)) * kLog2e;
-  const uint32_t columns = std::min(d.max_rows, d.rows) * a.group, per_tile = columns <= 16 ? 1 : columns <= 32 ? 2 : columns <= 64 ? 4 : 8;
-  a.tiles = (columns + 16 * per_tile - 1) / (16 * per_tile);
-  // Splits: workgroups for two a CU, of chunks of at least two steps a wave.
-  a.min_chunk = 256;
   a.capacity = dims->max_pages * dims->page_size;
-  const uint64_t tiles = (uint64_t)dims->sequences * dims->kv_heads * a.tiles;
+  // Blocks of 16 columns a workgroup: one where a kv head has up to 32 columns, or where tables reach up to 1024
+  // positions and all blocks are under way at once (1 of 517 with 5 rows, 14 / 2 heads of 64, f32: 8.5 us, shared
+  // tiles 10.7 to 14), else the four or eight of shared tiles (16 rows, 32 / 8 heads of 128, bf16: 32 of up to 4096 70.5
+  // us, in single blocks 95.7; 16 of up to 2048 31.7 for 32.1; with 8 rows 60.9 for 54.8 and 24.9 for 22.9).
+  const uint64_t columns = (uint64_t)std::min(d.max_rows, d.rows) * a.group;
+  const uint64_t heads_of_all = (uint64_t)dims->sequences * dims->kv_heads, ones = heads_of_all * ((columns + 15) / 16);
+  const bool few = columns <= 32 || (a.capacity <= 1024 && ones <= (uint64_t)ctx->cu_count);
+  const uint32_t per_tile = few ? 1 : columns <= 64 ? 4 : 8;
+  a.tiles = (uint32_t)((columns + 16 * per_tile - 1) / (16 * per_tile));
+  // Splits: a workgroup a CU, in chunks of at least 256; two a CU where that leaves chunks of 2048 (shared tiles of 8 x 64
+  // rows to 8192 117 us at one a CU, 92.6 at two; 4 x 32 rows to 4096 34.4 and 41; few columns, 32 x 4 rows to 8192 76.9 and
+  // 65.1, 16 x 8 rows to 2048 22.9 and 25.8). None of few columns up to 1024: the join is a launch.
+  a.min_chunk = few && a.capacity <= 1024 ? 1024 : 256;
+  const uint64_t tiles = heads_of_all * a.tiles, one = ctx->cu_count / tiles, two = 2ull * ctx->cu_count / tiles;
   const uint64_t most = ((uint64_t)a.capacity + a.min_chunk - 1) / a.min_chunk, per_split = (uint64_t)d.rows * d.heads * (dims->head_dim + 2) * 4;
-  uint64_t splits = std::max<uint64_t>(1, std::min<uint64_t>(2ull * ctx->cu_count / tiles, most));
+  uint64_t splits = std::max<uint64_t>(1, std::min<uint64_t>(two * 2048 <= a.capacity ? two : one, most));
   splits = std::max<uint64_t>(1, std::min<uint64_t>(splits, (eg::kPartialsBytes - 64) / per_split));
   a.splits = (uint32_t)splits;
   if (tiles * splits >= (1ull << 31) / kThreads || (uint64_t)d.rows * d.heads >= (1ull << 31) / kThreads)
