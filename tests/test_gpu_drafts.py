@@ -671,7 +671,7 @@ def test_refusals(device, up):  # noqa: F811
     fails("NULL argument", lambda: check(temperatures=b, accept=b))
     fails("not aligned to their type", lambda: check(K.Binding(b, 2), b, b, b, b, b))
     fails("over the workspace or the grid limit", lambda: check(rows=65536), _lib.EgRangeError)
-    fails("2097152 sequences", lambda: check(sequences=1 << 21), _lib.EgRangeError)
+    fails("65536 sequences, 1 rows", lambda: check(sequences=1 << 16), _lib.EgRangeError)
     check(None, None, None, None, None, None, sequences=0)
 
     ok = dict(max_rows=1, sequences=1, max_pages=1)
