@@ -1,17 +1,18 @@
 // Drafted tokens against the target's probabilities (eg_verify_drafts).
 //
-// Three quantities of a row of logits decide: its largest, Z = sum 2^((l - largest) log2(e) / temperature), and
-// the running sum that the next token is drawn by. All three come from partials per chunk of kChunk ids, made for
-// all rows at once by verify_stats: that pass reads the logits, and is what bounds the operator. Which rows the branch
-// goes through then takes single logits (verify_walk, a workgroup per sequence), and the draw reads one chunk
-// of one row again: the one in which the running sum passes the target. After a rejection by draft probabilities
-// the sums are of max(p - q, 0), so that row's chunks are summed once more: there a workgroup per chunk finds the
-// branch by itself, and sums its chunk (verify_draw then has the sums).
+// A row's largest logit and Z = sum 2^((l - largest) log2(e) / temperature) decide what is accepted. Both come from
+// partials per chunk of kChunk ids, made for all rows at once by verify_stats: that pass reads the logits, and is what
+// bounds the operator. Which rows the branch goes through then takes single logits. The next token's running sum goes
+// over the branch's last row only: a workgroup per few chunks finds the branch by itself and sums its chunks (verify_walk),
+// and the chunk in which the running sum passes the target is read once more (verify_draw; by the last workgroup to
+// arrive instead of a launch of its own, both took 18.5 us for 9.2 and 4.9, 16 sequences, and 19.5 for 14.4 and 5.7, 48).
 //
-// Sums and exponentials are f64: of 151,936 running sums some lie within f32's rounding of the drawn target in one
-// draw of a hundred, within these in none of 10^6. f64 vector instructions run at f32's rate, and an exponential is
-// 15 of them. (The largest is taken from a logit before the product with the scale: the difference is exact, where products
-// of large logits leave their rounding.)
+// What is decided is decided in f64: of 151,936 running sums some lie within f32's rounding of the drawn target in one draw
+// of a hundred, within these in none of 10^6. Exponentials in f64 are 15 f64 instructions, which over all rows take
+// longer than reading them (48 sequences of up to 8 rows: 56 us, with f32's 42): so Z is summed in f32 (kExact false),
+// which is off by less than kMargin of it, and a row for which that could decide otherwise is summed again in f64 where it comes up. Draft
+// probabilities are taken from p = e / Z itself, so their rows' Z are f64 from the start. (The largest is taken from a logit
+// before the product with the scale: the difference is exact, where products of large logits leave their rounding.)
 #include <algorithm>
 
 #include "eg_kv4.hpp"
@@ -25,15 +26,30 @@ constexpr uint32_t kWalkThreads = 512, kWalkEach = kChunk / kWalkThreads;
 constexpr uint32_t kMostVocab = 1u << 20;  // 256 chunks: a thread each
 constexpr uint32_t kNone = 0xFFFFFFFFu;
 
+// The error of a Z in f32, relative. Differences from the largest are rounded once, as is their product with the scale,
+// itself rounded: 3 x 2^-24 of exponents that matter down to -30 (2^-30 of 2^20 ids are 2^-10 of Z, and their own errors no
+// more than that times 1/8), so 6e-6 of an exponential, whose own error is 2^-23 and that of 16 added 2^-20.
+constexpr double kMargin = 0x1p-16;
+// Temperatures from which on scale and exponents fit f32; below, Z is f64.
+constexpr float kColdest = 1e-30f;
+
+// What a sequence's next token is drawn from: a row's p, or (of > 0) max(p - q, 0).
+struct Draw {
+  double scale, of;     // of: Z, 0 for p
+  uint64_t rejected;    // rows whose tokens p is without
+  uint32_t row, first;  // row: kNone where none is drawn; first: the sequence's
+  float reference;
+};
+
 struct VerifyArgs {
   const void* logits;
   const uint32_t *tokens, *offsets, *parents;
   const float *draft, *accept, *draws, *temperatures;
   uint32_t *path, *counts, *next;
-  struct Stats* stats;       // [row][chunk]
-  struct Residual* residual; // [sequence]
-  double* masses;            // [sequence][chunk] of the residual
-  uint32_t sequences, rows, max_rows, vocab, chunks;
+  struct Stats* stats;  // [row][chunk]
+  Draw* draw;           // [sequence]; NULL: all greedy
+  double* masses;       // [sequence][chunk] of what is drawn from
+  uint32_t sequences, rows, max_rows, vocab, chunks, together;  // together: chunks of a verify_walk's workgroup
   uint64_t stride, draft_stride;
 };
 
@@ -41,13 +57,6 @@ struct Stats {
   double sum;  // of 2^((l - reference(top)) scale)
   float top;
   uint32_t id;  // the lowest of `top` (0 where that is -inf)
-};
-
-// A sequence whose next token is drawn from max(p - q, 0) of a row.
-struct Residual {
-  double scale, total;  // total: Z
-  uint32_t row;         // kNone: no such draw
-  float reference;
 };
 
 // What a row's exponents are taken from: its largest, and 0 for a row of -inf alone (its sum is then 0).
@@ -147,7 +156,7 @@ __device__ __forceinline__ double block_before(double v, double& total) {
 }
 
 // A workgroup per (chunk, row): its largest logit and its sum.
-template <class T>
+template <bool kExact, class T>
 __global__ __launch_bounds__(256) void verify_stats(VerifyArgs a) {
   constexpr uint32_t kWide = 16 / sizeof(T);
   const uint32_t row = blockIdx.y, chunk = blockIdx.x, tid = threadIdx.x;
@@ -193,9 +202,16 @@ __global__ __launch_bounds__(256) void verify_stats(VerifyArgs a) {
     const double scale = scale_of(temperature), from = reference(top);
     bool bad = false;
 #pragma unroll
-    for (uint32_t j = 0; j < kEach; j++) {
-      sum += exp2_of(((double)v[j] - from) * scale);
-      bad |= broken(v[j]);
+    for (uint32_t j = 0; j < kEach; j++) bad |= broken(v[j]);
+    if (kExact || temperature < kColdest) {
+#pragma unroll
+      for (uint32_t j = 0; j < kEach; j++) sum += exp2_of(((double)v[j] - from) * scale);
+    } else {
+      const float s = (float)scale, f = reference(top);
+      float part[4] = {};
+#pragma unroll
+      for (uint32_t j = 0; j < kEach; j++) part[j % 4] += __builtin_amdgcn_exp2f((v[j] - f) * s);
+      sum = (double)((part[0] + part[1]) + (part[2] + part[3]));
     }
     sum = block_sum<4>(bad ? (double)NAN : sum);
   }
@@ -264,32 +280,53 @@ __device__ __forceinline__ uint32_t find_in_chunk(uint32_t chunk, double target,
   return first_or_last(hit, last);
 }
 
-// max(p - q, 0) of ids i .. of a sequence's last accepted row.
-template <class T, int N>
-__device__ __forceinline__ void left_over(const VerifyArgs& a, const Residual& r, uint32_t i, double (&e)[N]) {
-  const T* x = static_cast<const T*>(a.logits) + (uint64_t)r.row * a.stride;
-  const float* q = a.draft + (uint64_t)r.row * a.draft_stride;
-  const double from = r.reference, to = 1.0 / r.total;
-  float l[N], d[N];
-  load_ids<N>(x, i, a.vocab, -INFINITY, l);
-  load_ids<N>(q, i, a.vocab, 0.f, d);
+// What is drawn from, of ids i .. with logits l and draft probabilities q: p's exponentials without the rejected
+// rows' tokens, or max(p - q, 0).
+template <int N>
+__device__ __forceinline__ void drawn_from(const Draw& r, const uint32_t* tokens, uint32_t i, const float (&l)[N],
+                                           const float (&q)[N], double (&e)[N]) {
 #pragma unroll
-  for (int j = 0; j < N; j++) e[j] = fmax(exp2_of(((double)l[j] - from) * r.scale) * to - (double)d[j], 0.0);
+  for (int j = 0; j < N; j++) e[j] = exp2_of(((double)l[j] - (double)r.reference) * r.scale);
+  if (r.of > 0.0) {
+    const double to = 1.0 / r.of;
+#pragma unroll
+    for (int j = 0; j < N; j++) e[j] = fmax(e[j] * to - (double)q[j], 0.0);
+  } else {
+    for (uint64_t m = r.rejected; m != 0; m &= m - 1) {
+      const uint32_t gone = tokens[__builtin_ctzll(m)] - i;
+#pragma unroll
+      for (uint32_t j = 0; j < N; j++)
+        if (j == gone) e[j] = 0.0;
+    }
+  }
 }
 
-// A workgroup per sequence: its rows' sums from their chunks', the branch, and the next token. With draft
-// probabilities (kDraft) one per (chunk, sequence): the first of them writes what that finds, and where the draw is from
-// max(p - q, 0), each sums its chunk of that, for the launch after this one. A chain of dependent reads bounds it: offsets;
-// rows and sums; single logits; the chunk.
-template <bool kDraft, class T>
+// A row's Z in f64, by the whole workgroup.
+template <class T>
+__device__ __forceinline__ double exact_sum(const VerifyArgs& a, const T* row, float top, double scale) {
+  const double from = reference(top);
+  double sum = 0.0;
+  for (uint32_t i = threadIdx.x * kWalkEach; i < a.vocab; i += kChunk) {
+    float l[kWalkEach];
+    load_ids<kWalkEach>(row, i, a.vocab, -INFINITY, l);
+#pragma unroll
+    for (uint32_t j = 0; j < kWalkEach; j++) sum += exp2_of(((double)l[j] - from) * scale);
+  }
+  return block_sum<kWalkThreads / 64>(sum);
+}
+
+// A workgroup per (`together` chunks, sequence): the sequence's rows' sums from their chunks', the branch, and where a
+// token is drawn the sums of its chunks of what it is drawn from, for verify_draw. The first of a sequence writes what it finds. A chain of dependent reads bounds it: offsets; rows and sums; single logits; the chunks.
+// kBatch chunks of it at a time (1 or 4): all of their ids are under way before any is waited for.
+template <bool kDraft, uint32_t kBatch, class T>
 __global__ __launch_bounds__(kWalkThreads) void verify_walk(VerifyArgs a) {
   __shared__ float top_of[kMostRows], accept_of[kMostRows], q_of[kMostRows];
   __shared__ double sum_of[kMostRows], value_of[kMostRows];  // value_of: of a row's token where it was drafted
   __shared__ uint32_t id_of[kMostRows], token_of[kMostRows], path_of[kMostRows];
-  __shared__ uint32_t count_of, row_of;
+  __shared__ uint32_t count_of, row_of, unsure_of;
   __shared__ uint64_t rejected_of;  // rows, of the last row's children
   const uint32_t seq = blockIdx.y, tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
-  const bool writes = !kDraft || blockIdx.x == 0;
+  const bool writes = blockIdx.x == 0;
   const uint32_t first = a.offsets[seq], end = a.offsets[seq + 1], n = end - first;
   if (n == 0 || n > a.max_rows || first > end || end > a.rows) {
     if (!writes) return;
@@ -297,12 +334,12 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk(VerifyArgs a) {
     if (tid == 0) {
       a.counts[seq] = 0;
       a.next[seq] = kNone;
-      if (kDraft) a.residual[seq].row = kNone;
+      if (a.draw) a.draw[seq].row = kNone;
     }
     return;
   }
   const float temperature = temperature_of(a, seq);
-  const bool greedy = !(temperature > 0.f);
+  const bool greedy = !(temperature > 0.f), rough = !kDraft && temperature >= kColdest;
   const double scale = greedy ? 0.0 : scale_of(temperature);
   const T* logits = static_cast<const T*>(a.logits) + (uint64_t)first * a.stride;
   const Stats* stats = a.stats + (uint64_t)first * a.chunks;
@@ -362,116 +399,154 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk(VerifyArgs a) {
     }
   }
   __syncthreads();
-  if (wave == 0) {  // (the whole wave takes the same steps)
+  uint32_t at = 0, count = 1;
+  uint64_t rejected = 0, exact = rough ? 0 : ~0ull;  // exact: rows whose sum is
+  if (wave == 0) {
     token_of[lane] = token;
     accept_of[lane] = accept;
     q_of[lane] = q;
     value_of[lane] = parent == kNone ? 0.0 : exp2_of(((double)logit - (double)reference(top_of[parent])) * scale);
     if (lane == 0) path_of[0] = 0;
-    uint32_t at = 0, count = 1;
-    uint64_t rejected = 0;
-    for (;;) {
-      uint64_t children = __ballot(parent == at);
-      uint32_t to = kNone;
-      double left = sum_of[at];
-      rejected = 0;
-      while (children != 0) {
-        const uint32_t r = (uint32_t)__builtin_ctzll(children), x = token_of[r];
-        children &= children - 1;
-        bool ok;
-        if (greedy) {
-          ok = x == id_of[at];
-        } else if (kDraft) {
-          ok = (double)accept_of[r] * (double)q_of[r] * left < value_of[r];
-        } else {
-          const bool again = (__ballot(token == x) & rejected) != 0;
-          ok = !again && (double)accept_of[r] * left < value_of[r];
-          if (!ok && !again) left -= value_of[r];
-        }
-        if (ok) {
-          to = r;
-          break;
-        }
-        rejected |= 1ull << r;
-      }
-      if (to == kNone) break;
-      at = to;
-      if (lane == 0) path_of[count] = at;
-      count++;
-    }
-    if (lane == 0) {
-      count_of = count;
-      row_of = at;
-      rejected_of = rejected;
-    }
   }
-  __syncthreads();
-  const uint32_t count = count_of, at = row_of;
-  const uint64_t rejected = rejected_of;
+  for (;;) {
+    if (wave == 0) {  // (the whole wave takes the same steps)
+      uint32_t unsure = kNone;
+      for (;;) {
+        uint64_t children = __ballot(parent == at);
+        uint32_t to = kNone;
+        const double sum = sum_of[at];
+        double left = sum;
+        rejected = 0;
+        while (children != 0) {
+          const uint32_t r = (uint32_t)__builtin_ctzll(children), x = token_of[r];
+          children &= children - 1;
+          bool ok;
+          if (greedy) {
+            ok = x == id_of[at];
+          } else if (kDraft) {
+            ok = (double)accept_of[r] * (double)q_of[r] * left < value_of[r];
+          } else {
+            const bool again = (__ballot(token == x) & rejected) != 0;
+            const double than = (double)accept_of[r] * left;
+            if (!again && !(exact >> at & 1u) && fabs(than - value_of[r]) < (double)accept_of[r] * sum * kMargin) {
+              unsure = at;
+              break;
+            }
+            ok = !again && than < value_of[r];
+            if (!ok && !again) left -= value_of[r];
+          }
+          if (ok) {
+            to = r;
+            break;
+          }
+          rejected |= 1ull << r;
+        }
+        if (unsure != kNone || to == kNone) break;
+        at = to;
+        if (lane == 0) path_of[count] = at;
+        count++;
+      }
+      if (lane == 0) {
+        count_of = count;
+        row_of = at;
+        rejected_of = rejected;
+        unsure_of = unsure;
+      }
+    }
+    __syncthreads();
+    const uint32_t again = unsure_of;
+    if (again == kNone) break;
+    const double sum = exact_sum(a, logits + again * a.stride, top_of[again], scale);
+    if (tid == 0) sum_of[again] = sum;
+    exact |= 1ull << again;
+    __syncthreads();
+  }
+  count = count_of;
+  at = row_of;
   const double total = sum_of[at];
-  const bool draws = !greedy && total > 0.0 && total < (double)INFINITY, from_rest = kDraft && draws && rejected != 0;
+  const bool draws = !greedy && total > 0.0 && total < (double)INFINITY;
+  const Draw from{scale, kDraft && rejected_of != 0 ? total : 0.0, kDraft ? 0 : rejected_of, draws ? first + at : kNone, first,
+                  reference(top_of[at])};
   if (writes) {
     if (tid < a.max_rows) a.path[(uint64_t)seq * a.max_rows + tid] = tid < count ? path_of[tid] : kNone;
     if (tid == 0) {
       a.counts[seq] = count;
       a.next[seq] = id_of[at];  // (unless one is drawn)
-      if (kDraft) a.residual[seq] = Residual{scale, total, from_rest ? first + at : kNone, reference(top_of[at])};
+      if (a.draw) a.draw[seq] = from;
     }
   }
-  if (from_rest) {
-    const Residual r{scale, total, first + at, reference(top_of[at])};
-    double e[kWalkEach], sum = 0.0;
-    left_over<T>(a, r, blockIdx.x * kChunk + tid * kWalkEach, e);
+  if (!draws) return;
+  constexpr uint32_t kWaves = kWalkThreads / 64;
+  __shared__ double part[kBatch][kWaves];
+  const uint32_t last = min(a.chunks, (blockIdx.x + 1) * a.together);
+  const T* row = logits + at * a.stride;
+  const float* draft = a.draft + (uint64_t)(first + at) * a.draft_stride;
+  double* masses = a.masses + (uint64_t)seq * a.chunks;
+  for (uint32_t c0 = blockIdx.x * a.together; c0 < last; c0 += kBatch) {
+    float l[kBatch][kWalkEach], q[kBatch][kWalkEach] = {};
+    if (c0 + kBatch <= last && (c0 + kBatch) * kChunk <= a.vocab) {
 #pragma unroll
-    for (uint32_t j = 0; j < kWalkEach; j++) sum += e[j];
-    sum = block_sum<kWalkThreads / 64>(sum);
-    if (tid == 0) a.masses[(uint64_t)seq * a.chunks + blockIdx.x] = sum;
-    return;
-  }
-  if (!writes || !draws) return;
-  double mass = 0.0;
-  if (tid < a.chunks) {
-    mass = rescaled(stats[(uint64_t)at * a.chunks + tid], top_of[at], scale);
-    uint64_t seen = 0;  // (of a token that several rejected rows hold the first one counts)
-    for (uint64_t m = rejected; m != 0; m &= m - 1) {
-      const uint32_t r = (uint32_t)__builtin_ctzll(m);
-      bool again = false;
-      for (uint64_t o = seen; o != 0; o &= o - 1) again |= token_of[__builtin_ctzll(o)] == token_of[r];
-      seen |= 1ull << r;
-      if (!again && token_of[r] / kChunk == tid) mass -= value_of[r];
+      for (uint32_t b = 0; b < kBatch; b++) {
+        const uint32_t i = (c0 + b) * kChunk + tid * kWalkEach;
+        const Several<T, kWalkEach> x = *reinterpret_cast<const Several<T, kWalkEach>*>(row + i);
+#pragma unroll
+        for (uint32_t j = 0; j < kWalkEach; j++) l[b][j] = to_f32(x.v[j]);
+        if (kDraft) {
+          const Several<float, kWalkEach> y = *reinterpret_cast<const Several<float, kWalkEach>*>(draft + i);
+#pragma unroll
+          for (uint32_t j = 0; j < kWalkEach; j++) q[b][j] = y.v[j];
+        }
+      }
+    } else {
+#pragma unroll
+      for (uint32_t b = 0; b < kBatch; b++) {
+        const uint32_t i = (c0 + b) * kChunk + tid * kWalkEach, ids = c0 + b < last ? a.vocab : 0;
+        load_ids<kWalkEach>(row, i, ids, -INFINITY, l[b]);
+        if (kDraft) load_ids<kWalkEach>(draft, i, ids, 0.f, q[b]);
+      }
     }
-    mass = fmax(mass, 0.0);
-  }
-  uint32_t chunk;
-  double target;
-  if (!find_chunk(mass, a.draws[seq], chunk, target)) return;
-  const T* x = logits + at * a.stride;
-  const double from = reference(top_of[at]);
-  const uint32_t id = find_in_chunk(chunk, target, [&](uint32_t i, double (&e)[kWalkEach]) {
-    float l[kWalkEach];
-    load_ids<kWalkEach>(x, i, a.vocab, -INFINITY, l);
+    double sum[kBatch];
 #pragma unroll
-    for (uint32_t j = 0; j < kWalkEach; j++) e[j] = exp2_of(((double)l[j] - from) * scale);
-    for (uint64_t m = rejected; m != 0; m &= m - 1) {
-      const uint32_t gone = token_of[__builtin_ctzll(m)] - i;
+    for (uint32_t b = 0; b < kBatch; b++) {
+      double e[kWalkEach];
+      drawn_from(from, token_of, (c0 + b) * kChunk + tid * kWalkEach, l[b], q[b], e);
+      sum[b] = 0.0;
 #pragma unroll
-      for (uint32_t j = 0; j < kWalkEach; j++)
-        if (j == gone) e[j] = 0.0;
+      for (uint32_t j = 0; j < kWalkEach; j++) sum[b] += e[j];
     }
-  });
-  if (tid == 0) a.next[seq] = id;
+#pragma unroll
+    for (uint32_t b = 0; b < kBatch; b++) sum[b] = wave_sum(sum[b]);
+    __syncthreads();
+#pragma unroll
+    for (uint32_t b = 0; b < kBatch; b++)
+      if (lane == b) part[b][wave] = sum[b];
+    __syncthreads();
+    if (tid < kBatch && c0 + tid < last) {
+      double all = part[tid][0];
+#pragma unroll
+      for (uint32_t w = 1; w < kWaves; w++) all += part[tid][w];
+      masses[c0 + tid] = all;
+    }
+  }
 }
 
+// A workgroup per sequence: the chunk, and the id in it.
 template <class T>
 __global__ __launch_bounds__(kWalkThreads) void verify_draw(VerifyArgs a) {
   const uint32_t seq = blockIdx.x, tid = threadIdx.x;
-  const Residual r = a.residual[seq];
+  const Draw r = a.draw[seq];
   if (r.row == kNone) return;
   const double mass = tid < a.chunks ? a.masses[(uint64_t)seq * a.chunks + tid] : 0.0;
   uint32_t chunk;
   double target;
-  if (!find_chunk(mass, a.draws[seq], chunk, target)) return;  // (p and q leave nothing)
-  const uint32_t id = find_in_chunk(chunk, target, [&](uint32_t i, double (&e)[kWalkEach]) { left_over<T>(a, r, i, e); });
+  if (!find_chunk(mass, a.draws[seq], chunk, target)) return;  // (nothing is left to draw from)
+  const T* row = static_cast<const T*>(a.logits) + (uint64_t)r.row * a.stride;
+  const uint32_t id = find_in_chunk(chunk, target, [&](uint32_t i, double (&e)[kWalkEach]) {
+    float l[kWalkEach], q[kWalkEach] = {};
+    load_ids<kWalkEach>(row, i, a.vocab, -INFINITY, l);
+    if (r.of > 0.0) load_ids<kWalkEach>(a.draft + (uint64_t)r.row * a.draft_stride, i, a.vocab, 0.f, q);
+    drawn_from(r, a.tokens + r.first, i, l, q, e);
+  });
   if (tid == 0) a.next[seq] = id;
 }
 
@@ -505,10 +580,10 @@ extern "C" int eg_verify_drafts(eg_context* ctx, const void* logits, const uint3
     return eg::fail(ctx, EG_ERR_INVALID, "%s: logits are not aligned to their type", op);
   a.chunks = (d.vocab + kChunk - 1) / kChunk;
   const uint64_t stats = (uint64_t)d.rows * a.chunks * sizeof(Stats);
-  const uint64_t residual = draft ? (uint64_t)d.sequences * (sizeof(Residual) + a.chunks * sizeof(double)) : 0;
-  if (stats + residual > eg::kPartialsBytes || d.rows > 65535 || d.sequences > 65535)
-    return eg::fail(ctx, EG_ERR_RANGE, "%s: %u sequences, %u rows of %u ids over the workspace or the grid limit", op, d.sequences, d.rows,
-                    d.vocab);
+  const uint64_t draw = temperatures ? (uint64_t)d.sequences * (sizeof(Draw) + a.chunks * sizeof(double)) : 0;
+  if (stats + draw > eg::kPartialsBytes || d.rows > 65535 || d.sequences > 65535)
+    return eg::fail(ctx, EG_ERR_RANGE, "%s: %u sequences, %u rows of %u ids over the workspace or the grid limit", op, d.sequences,
+                    d.rows, d.vocab);
   a.logits = logits;
   a.tokens = tokens;
   a.offsets = offsets;
@@ -522,8 +597,11 @@ extern "C" int eg_verify_drafts(eg_context* ctx, const void* logits, const uint3
   a.next = next;
   uint8_t* at = eg::partials(ctx);
   a.stats = reinterpret_cast<Stats*>(at);
-  a.residual = reinterpret_cast<Residual*>(at + stats);
-  a.masses = reinterpret_cast<double*>(at + stats + (uint64_t)d.sequences * sizeof(Residual));
+  a.draw = temperatures ? reinterpret_cast<Draw*>(at + stats) : nullptr;
+  a.masses = reinterpret_cast<double*>(at + stats + (uint64_t)d.sequences * sizeof(Draw));
+  // A chunk a workgroup where all are then under way at once, else four and more.
+  const uint64_t all_chunks = (uint64_t)a.chunks * d.sequences, room = 4ull * ctx->cu_count;
+  a.together = all_chunks <= room ? 1 : 4 * (uint32_t)((all_chunks + 4 * room - 1) / (4 * room));
   a.sequences = d.sequences;
   a.rows = d.rows;
   a.max_rows = d.max_rows;
@@ -531,15 +609,16 @@ extern "C" int eg_verify_drafts(eg_context* ctx, const void* logits, const uint3
   const OnDevice on(ctx);
   with_type(d.type, [&](auto t) {
     using T = decltype(t);
-    const dim3 threads(kThreads);
-    if (d.rows != 0) hipLaunchKernelGGL(verify_stats<T>, dim3(a.chunks, d.rows), threads, 0, ctx->stream, a);
-    const dim3 walk(kWalkThreads);
-    if (draft && temperatures) {
-      hipLaunchKernelGGL((verify_walk<true, T>), dim3(a.chunks, d.sequences), walk, 0, ctx->stream, a);
-      hipLaunchKernelGGL(verify_draw<T>, dim3(d.sequences), walk, 0, ctx->stream, a);
-    } else {
-      hipLaunchKernelGGL((verify_walk<false, T>), dim3(1, d.sequences), walk, 0, ctx->stream, a);
+    const bool drafted = draft && temperatures;
+    const dim3 threads(kThreads), walk(kWalkThreads), grid(temperatures ? (a.chunks + a.together - 1) / a.together : 1, d.sequences);
+    if (d.rows != 0) {
+      if (drafted) hipLaunchKernelGGL((verify_stats<true, T>), dim3(a.chunks, d.rows), threads, 0, ctx->stream, a);
+      else hipLaunchKernelGGL((verify_stats<false, T>), dim3(a.chunks, d.rows), threads, 0, ctx->stream, a);
     }
+    const auto kernel = drafted ? (a.together == 1 ? verify_walk<true, 1, T> : verify_walk<true, 4, T>)
+                                : (a.together == 1 ? verify_walk<false, 1, T> : verify_walk<false, 4, T>);
+    hipLaunchKernelGGL(kernel, grid, walk, 0, ctx->stream, a);
+    if (temperatures) hipLaunchKernelGGL(verify_draw<T>, dim3(d.sequences), walk, 0, ctx->stream, a);
   });
   return eg::check_launch(ctx, op);
 }

@@ -503,6 +503,35 @@ def test_verify_temperatures(device, up):  # noqa: F811
     x, tokens, parents, _ = verify_case(rng, [8] * 6, 3000, False, False)
     check_verify(device, up, x, tokens, [8] * 6, parents, None, rng.random(48), rng.random(6),
                  [1e-6, 1e-38, 1e30, -1.0, float("nan"), 2.5])
+    check_verify(device, up, x, tokens, [8] * 6, parents, None, rng.random(48), rng.random(6), [9e-31, 1.1e-30, 1e-20, 1e38, 0.0, 0.01])
+
+
+def test_verify_numbers_next_to_a_border(device, up):  # noqa: F811
+    """Numbers that are p(x), and what p(x) is of what is left, to f32's rounding: just under, at and just over them. What a
+    sum in f32 would say of them is a coin's toss; 64 bits decide by the numbers' own roundings, of 2^-25 and more."""
+    rng = np.random.default_rng(9)
+    vocab, n = 30001, 4
+    x = (rng.standard_normal((n, vocab)) * 2).astype(np.float32)
+    x[:, :50] += 6
+    tokens, parents = np.array([0, 7, 33, 21]), np.array([9, 0, 0, 0], np.uint32)
+    for t in (1.0, 0.73):
+        t32 = np.float64(np.float32(t))
+        e = np.exp((x[0].astype(np.float64) - x[0].max()) / t32)
+        p = e / e.sum()
+        one = np.float32(1) - np.float32(2.0 ** -24)
+        for r, border in ((1, p[7]), (2, p[33] / (1 - p[7])), (3, p[21] / (1 - p[7] - p[33]))):
+            u = np.float32(border)
+            for number in (np.nextafter(u, np.float32(0)), u, np.nextafter(u, np.float32(1))):
+                accept = np.where(np.arange(n) < r, one, np.float32(0.5))
+                accept[r] = number
+                check_verify(device, up, x, tokens, [n], parents, None, accept, [0.4], [t])
+    # a chain: every row's number next to its border, so that several rows of a sequence are summed again
+    tokens = np.array([0, 3, 8, 40])
+    e = np.exp(x.astype(np.float64) - x.max(-1, keepdims=True))
+    p = (e / e.sum(-1, keepdims=True))[np.arange(3), tokens[1:]]
+    for down in (0, 1):
+        accept = np.concatenate([[0], np.nextafter(np.float32(p), np.float32(1 - down))])
+        check_verify(device, up, np.tile(x, (3, 1)), np.tile(tokens, 3), [4, 4, 4], None, None, np.tile(accept, 3), [0.1, 0.5, 0.9], [1.0] * 3)
 
 
 def test_verify_equal_logits_go_to_the_lowest_id(device, up):  # noqa: F811
