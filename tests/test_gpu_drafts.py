@@ -5,7 +5,10 @@ the same, over at most as many positions.
 
 A table's entry is one f32 rounding, 2^-24 of it, of amplitude (cos, sin) of an angle in 64 bits; a frequency is a few
 64-bit operations (of 2^-53 each, a power one last place), so angles of both sides are within 16 x 2^-53 of themselves,
-and the functions' own errors within 2^-50.
+and the functions' own errors within 2^-51 on each side. Seven of eight positions are made from the one before by a product
+of complex numbers of length 1: four products and sums of 2^-53 each, and the step's own 2^-51 in both of its parts, so up to
+2^-53 (2 sqrt 2) + 2^-51 sqrt 2 < 2^-50 more with each, 7 x 2^-50 in all. A step's angle is off by 16 x 2^-53 of itself, seven
+of them by less than 112 x 2^-53 of a step of at most 1: 2^-46 in all, which is 2^-22 of a table entry's f32 rounding.
 """
 
 import ctypes
@@ -41,7 +44,7 @@ def test_table(device, up, scaling, positions, first, rotary):  # noqa: F811
     got = got[: positions * rotary].reshape(positions, rotary // 2, 2)
     angle = (first + np.arange(positions, dtype=np.float64))[:, None] * frequencies(rotary, scaling=scaling, **how)
     want = 1.25 * np.stack([np.cos(angle), np.sin(angle)], -1)
-    bound = 2.0 ** -24 * np.abs(want) + 1.25 * (np.abs(angle) * 16 * 2.0 ** -53 + 2.0 ** -50)[..., None] * (1 + 2.0 ** -20)
+    bound = 2.0 ** -24 * np.abs(want) + 1.25 * (np.abs(angle) * 16 * 2.0 ** -53 + 2.0 ** -46)[..., None] * (1 + 2.0 ** -20)
     assert np.all(np.abs(got - want) <= bound)
 
 
