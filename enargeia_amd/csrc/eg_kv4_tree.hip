@@ -38,16 +38,12 @@ __device__ __forceinline__ bool computed(const Args& a, uint32_t first, uint32_t
   return first <= last && last <= a.rows && last - first <= a.max_rows;
 }
 
-// What a row of a sequence sees of its rows, itself among them: lane i of a wave gets row i's bits. Each turn
+// What a row of a sequence sees of its rows, itself among them: lane i of a wave, with row i's parent, gets row i's bits. Each turn
 // adds what the row at the end of the chain so far has, and moves that end to its own: 6 turns reach 64.
-__device__ __forceinline__ uint64_t ancestors(const uint32_t* parents, uint32_t first, uint32_t n) {
+__device__ __forceinline__ uint64_t ancestors(bool tree, uint32_t parent) {
   const uint32_t lane = threadIdx.x & 63u;
-  if (!parents) return ~0ull >> (63u - lane);
-  uint32_t end = lane;
-  if (lane < n) {
-    const uint32_t p = parents[first + lane];
-    if (p < lane) end = p;
-  }
+  if (!tree) return ~0ull >> (63u - lane);
+  uint32_t end = parent < lane ? parent : lane;
   uint32_t lo = lane < 32 ? 1u << lane : 0u, hi = lane < 32 ? 0u : 1u << (lane - 32);
 #pragma unroll
   for (int i = 0; i < 6; i++) {
@@ -64,25 +60,30 @@ __device__ __forceinline__ uint64_t of_row(uint64_t all, uint32_t row) {
          (uint32_t)__shfl((int)(uint32_t)all, (int)row, 64);
 }
 
-// A column's query as the first product's B operand: lane group g has dims 32 grp + 8 g + kOrder[slot], times the
-// power of two that puts the largest of the column's into [2^14, 2^15), whose exponent is returned.
-template <int D, int kParts, class TQ>
-__device__ __forceinline__ int load_queries(const Args& a, uint32_t row, uint32_t head, bool in, uint32_t lg,
-                                            half8 (&qf)[D / 32][kParts]) {
-  struct alignas(16) Eight {
-    TQ v[8];
-  };
+// A column's query as it comes from memory: lane group g has dims 32 grp + 8 g .. +8.
+template <class TQ>
+struct alignas(16) Eight {
+  TQ v[8];
+};
+template <int D, class TQ>
+__device__ __forceinline__ void load_query(const Args& a, uint32_t row, uint32_t head, uint32_t lg, Eight<TQ> (&raw)[D / 32]) {
   const TQ* src = static_cast<const TQ*>(a.q) + (size_t)row * a.q_stride + (size_t)head * D;
+#pragma unroll
+  for (int g = 0; g < D / 32; g++) raw[g] = *reinterpret_cast<const Eight<TQ>*>(src + 32 * g + 8 * lg);
+}
+
+// And as the first product's B operand: slots in kOrder's order, times the power of two that puts the largest of the
+// column's into [2^14, 2^15), whose exponent is returned.
+template <int D, int kParts, class TQ>
+__device__ __forceinline__ int make_query(const Eight<TQ> (&raw)[D / 32], bool in, half8 (&qf)[D / 32][kParts]) {
   float x[D / 32][8], top = 0.f;
 #pragma unroll
-  for (int g = 0; g < D / 32; g++) {
-    const Eight e = *reinterpret_cast<const Eight*>(src + 32 * g + 8 * lg);
+  for (int g = 0; g < D / 32; g++)
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-      x[g][i] = in ? to_f32(e.v[kOrder[i]]) : 0.f;
+      x[g][i] = in ? to_f32(raw[g].v[kOrder[i]]) : 0.f;
       top = fmaxf(top, fabsf(x[g][i]));
     }
-  }
   top = max_of_head(top);
   const int up = max(-100, min(110, top > 0.f ? 14 - ((int)(__float_as_uint(top) >> 23) - 127) : 0));
 #pragma unroll
@@ -122,9 +123,8 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Args a, Pool pool) {
   const uint32_t kv = id % pool.kv_heads, seq = id / pool.kv_heads;
 
   const uint32_t first = a.offsets[seq], last = a.offsets[seq + 1], n = last - first, length = a.lengths[seq];
-  if (!computed(a, first, last) || tile * kColumns >= n * a.group) return;
   const uint32_t reach = min(length, a.capacity), chunk = chunk_of(a, reach), begin = split * chunk;
-  if (split != 0 && begin >= reach) return;
+  if (!computed(a, first, last) | (tile * kColumns >= n * a.group) | ((split != 0) & (begin >= reach))) return;  // (read at once)
   const bool fits = n <= length;  // (else the rows give zeros)
   const uint32_t base = fits ? length - n : 0, end = fits ? min(reach, begin + chunk) : 0;
   const Magic bits_over = magic();
@@ -189,14 +189,19 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Args a, Pool pool) {
     load(t, (uint32_t)__builtin_amdgcn_readlane((int)ids, (int)i),
          (begin + (wave + kWaves * (i0 + i)) * kTile) & (page_size - 1u));
   };
+  // Reads that wait for nothing but offsets and lengths first, then the first tile's; the rest goes on beside those.
   uint32_t ids = pages_of(0);
+  const bool tail = end > base;
+  const uint32_t parent = tail && a.parents && lane < n ? a.parents[first + lane] : 0xFFFFFFFFu;
+  Eight<TQ> raw[kGroups];
+  load_query<D, TQ>(a, first + row, head, lg, raw);
+  Tile tiles[2];
+  if (mine != 0) fetch(tiles[0], ids, 0, 0);
+  const uint64_t sees = tail ? of_row(ancestors(a.parents != nullptr, parent), row) : 0;
 
-  const uint64_t sees = end > base ? of_row(ancestors(a.parents, first, n), row) : 0;
-
-  // The queries, B operand: lane group g has dims 32 grp + 8 g + kOrder[slot] of column lr.
   half8 qf[kGroups][kParts];
   f32x4 start[kGroups];  // -8 sum q per group: what makes codes of code - 8
-  const int up = load_queries<D, kParts, TQ>(a, first + row, head, in, lg, qf);
+  const int up = make_query<D, kParts, TQ>(raw, in, qf);
   const float f = fmaxf(ldexpf(a.scale, kSigned ? -up : 24 - up), 0x1p-126f);  // (not 0: -inf times it is -inf)
 #pragma unroll
   for (int g = 0; g < kGroups; g++) {
@@ -322,10 +327,11 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Args a, Pool pool) {
   // (The page ids are read outside the loop over their 64 steps: a wait for them inside would be a wait
   // for the tiles under way.)
   for (uint32_t i0 = 0; i0 < mine; i0 += 64) {
-    if (i0) ids = pages_of(i0);
+    if (i0) {
+      ids = pages_of(i0);
+      fetch(tiles[0], ids, i0, 0);
+    }
     const uint32_t count = min(64u, mine - i0);
-    Tile tiles[2];
-    fetch(tiles[0], ids, i0, 0);
     for (uint32_t i = 0; i < count; i += 2) {
       if (i + 1 < count) fetch(tiles[1], ids, i0, i + 1);
       compute(tiles[0], i0 + i);
@@ -417,9 +423,8 @@ __global__ __launch_bounds__(256, 2) void wide_kernel(Args a, Pool pool) {
   const uint32_t kv = id % pool.kv_heads, seq = id / pool.kv_heads;
 
   const uint32_t first = a.offsets[seq], last = a.offsets[seq + 1], n = last - first, length = a.lengths[seq];
-  if (!computed(a, first, last) || tile * kColumns >= n * a.group) return;
   const uint32_t reach = min(length, a.capacity), chunk = chunk_of(a, reach), begin = split * chunk;
-  if (split != 0 && begin >= reach) return;
+  if (!computed(a, first, last) | (tile * kColumns >= n * a.group) | ((split != 0) & (begin >= reach))) return;  // (read at once)
   const bool fits = n <= length;  // (else the rows give zeros)
   const uint32_t base = fits ? length - n : 0, end = fits ? min(reach, begin + chunk) : 0;
   const Magic bits_over = magic();
@@ -516,15 +521,23 @@ __global__ __launch_bounds__(256, 2) void wide_kernel(Args a, Pool pool) {
   float f[kBlocks];
   uint64_t sees[kBlocks];
   Stage stage;
-  if (steps != 0) load(stage, page_at(0, half_step), 0);
-  const uint64_t all = end > base ? ancestors(a.parents, first, n) : 0;
+  // (reads that wait for nothing but offsets and lengths first, then the first step's; the rest goes on beside those)
+  const bool tail_of = end > base;
+  const uint32_t parent = tail_of && a.parents && lane < n ? a.parents[first + lane] : 0xFFFFFFFFu;
+  Eight<TQ> raw[kBlocks][kGroups];
 #pragma unroll
   for (int b = 0; b < kBlocks; b++) {
-    const uint32_t c = c0 + 16 * b + lr;
-    const bool in = c < n * a.group;
-    const uint32_t row = in ? c / a.group : 0, head = kv * a.group + (in ? c % a.group : 0);
-    sees[b] = of_row(all, row);
-    const int up = load_queries<D, kParts, TQ>(a, first + row, head, in, lg, qf[b]);
+    const uint32_t c = min(c0 + 16 * b + lr, n * a.group - 1);
+    load_query<D, TQ>(a, first + c / a.group, kv * a.group + c % a.group, lg, raw[b]);
+  }
+  if (steps != 0) load(stage, page_at(0, half_step), 0);
+  const uint64_t all = tail_of ? ancestors(a.parents != nullptr, parent) : 0;
+#pragma unroll
+  for (int b = 0; b < kBlocks; b++) {
+    const uint32_t c = min(c0 + 16 * b + lr, n * a.group - 1);
+    const bool in = c0 + 16 * b + lr < n * a.group;
+    sees[b] = of_row(all, c / a.group);
+    const int up = make_query<D, kParts, TQ>(raw[b], in, qf[b]);
     f[b] = fmaxf(ldexpf(a.scale, -up), 0x1p-126f);  // (not 0: -inf times it is -inf)
   }
 
