@@ -764,6 +764,46 @@ void launch(eg_context* ctx, const Args& a, const Pool& p, uint32_t per_tile, ui
                        ctx->stream, a, p.sequences);
 }
 
+// Blocks of 16 columns a workgroup (1: few_kernel, 4 and 8: wide_kernel) and chunks of a sequence's positions: what
+// the times below, which these kernels were measured with, add up to least by. Lengths are on the device, so it goes by what
+// the tables reach less a page, whose last ones are seldom full. A step (128 positions of few_kernel, 64 of wide_kernel) of a workgroup alone on its CU, and of one of
+// two, in us at head_dim 128: 1.0 and 0.77 (32 x 4 rows to 8192, 32 / 8 heads, bf16: 76.9 us whole, 65.1 halved); 1.15 and
+// 1.15 (32 x 16 rows to 4096: 70.5 halved, 75.5 in four); 1.6 and 1.25 (8 x 64 rows to 8192: 117 halved, 92.6 in four).
+// 0.6 of that at 64, 1.4 times for f32 rows. A launch, its chain of reads and the waves' meeting take 6 us, a join
+// 4.5 and its partials a us for 4 MB written and read.
+struct Plan {
+  uint32_t per_tile, tiles, splits, min_chunk;
+};
+Plan plan_of(uint32_t cus, uint64_t pairs, uint64_t columns, uint32_t reach, uint64_t outputs, uint32_t head_dim, bool f32) {
+  struct Kind {
+    uint32_t per_tile, step;
+    double alone, shared;
+  };
+  constexpr Kind kKinds[] = {{1, 128, 1.0, 0.77}, {4, 64, 1.15, 1.15}, {8, 64, 1.6, 1.25}};
+  const uint64_t per_split = outputs * (head_dim + 2) * 4, room = (eg::kPartialsBytes - 64) / per_split;
+  const double unit = (head_dim == 64 ? 0.6 : 1.0) * (f32 ? 1.4 : 1.0);
+  Plan best{1, (uint32_t)((columns + 15) / 16), 1, 256};
+  double least = -1.0;
+  for (const Kind& kind : kKinds) {
+    const uint64_t tiles = (columns + 16 * kind.per_tile - 1) / (16 * kind.per_tile), all = pairs * tiles;
+    const uint64_t most = std::min<uint64_t>({std::max<uint64_t>(1, (reach + 255) / 256), std::max<uint64_t>(1, 4ull * cus / all),
+                                              std::max<uint64_t>(1, room)});
+    for (uint64_t s = 1; s <= most; s++) {
+      const uint64_t even = (reach + s - 1) / s, chunk = s == 1 ? reach : std::max<uint64_t>(256, (even + 63) & ~63ull);
+      const uint64_t chunks = s == 1 ? 1 : (reach + chunk - 1) / chunk, steps = (chunk + kind.step - 1) / kind.step;
+      const uint64_t each = (all * chunks + cus - 1) / cus;  // workgroups of the busiest CU
+      double us = 6.0 + steps * unit * (each == 1 ? kind.alone : each * kind.shared);
+      if (chunks > 1) us += 4.5 + chunks * per_split * 2 / 4e6;
+      if (least < 0.0 || us < least) {
+        least = us;
+        best = Plan{kind.per_tile, (uint32_t)tiles, (uint32_t)s, 256};
+      }
+    }
+  }
+  if (best.splits == 1) best.min_chunk = 0x7FFFFFC0u;  // (whole, however long)
+  return best;
+}
+
 }  // namespace
 
 extern "C" int eg_attention_tree_kv4(eg_context* ctx, const void* q, const uint32_t* offsets, const uint32_t* parents,
@@ -804,24 +844,12 @@ extern "C" int eg_attention_tree_kv4(eg_context* ctx, const void* q, const uint3
   if (!some) return EG_OK;
   a.scale = (d.scale > 0.f ? d.scale : 1.0f / sqrtf((float)dims->head_dim)) * kLog2e;
   a.capacity = dims->max_pages * dims->page_size;
-  // Blocks of 16 columns a workgroup: one where a kv head has up to 32 columns, or where tables reach up to 1024
-  // positions and all blocks are under way at once (1 of 517 with 5 rows, 14 / 2 heads of 64, f32: 8.5 us, shared
-  // tiles 10.7 to 14), else the four or eight of shared tiles (16 rows, 32 / 8 heads of 128, bf16: 32 of up to 4096 70.5
-  // us, in single blocks 95.7; 16 of up to 2048 31.7 for 32.1; with 8 rows 60.9 for 54.8 and 24.9 for 22.9).
-  const uint64_t columns = (uint64_t)std::min(d.max_rows, d.rows) * a.group;
-  const uint64_t heads_of_all = (uint64_t)dims->sequences * dims->kv_heads, ones = heads_of_all * ((columns + 15) / 16);
-  const bool few = columns <= 32 || (a.capacity <= 1024 && ones <= (uint64_t)ctx->cu_count);
-  const uint32_t per_tile = few ? 1 : columns <= 64 ? 4 : 8;
-  a.tiles = (uint32_t)((columns + 16 * per_tile - 1) / (16 * per_tile));
-  // Splits: a workgroup a CU, in chunks of at least 256; two a CU where that leaves chunks of 2048 (shared tiles of 8 x 64
-  // rows to 8192 117 us at one a CU, 92.6 at two; 4 x 32 rows to 4096 34.4 and 41; few columns, 32 x 4 rows to 8192 76.9 and
-  // 65.1, 16 x 8 rows to 2048 22.9 and 25.8). None of few columns up to 1024: the join is a launch.
-  a.min_chunk = few && a.capacity <= 1024 ? 1024 : 256;
-  const uint64_t tiles = heads_of_all * a.tiles, one = ctx->cu_count / tiles, two = 2ull * ctx->cu_count / tiles;
-  const uint64_t most = ((uint64_t)a.capacity + a.min_chunk - 1) / a.min_chunk, per_split = (uint64_t)d.rows * d.heads * (dims->head_dim + 2) * 4;
-  uint64_t splits = std::max<uint64_t>(1, std::min<uint64_t>(two * 2048 <= a.capacity ? two : one, most));
-  splits = std::max<uint64_t>(1, std::min<uint64_t>(splits, (eg::kPartialsBytes - 64) / per_split));
-  a.splits = (uint32_t)splits;
+  const Plan plan = plan_of(ctx->cu_count, (uint64_t)dims->sequences * dims->kv_heads, (uint64_t)std::min(d.max_rows, d.rows) * a.group,
+                            a.capacity - std::min(a.capacity, dims->page_size), (uint64_t)d.rows * d.heads, dims->head_dim, d.type == EG_ELEMENT_F32);
+  const uint64_t tiles = (uint64_t)dims->sequences * dims->kv_heads * plan.tiles, splits = plan.splits;
+  a.tiles = plan.tiles;
+  a.splits = plan.splits;
+  a.min_chunk = plan.min_chunk;
   if (tiles * splits >= (1ull << 31) / kThreads || (uint64_t)d.rows * d.heads >= (1ull << 31) / kThreads)
     return eg::fail(ctx, EG_ERR_RANGE, "%s: %u rows of %u heads in %u sequences over the grid limit", op, d.rows, d.heads,
                     dims->sequences);
@@ -831,8 +859,8 @@ extern "C" int eg_attention_tree_kv4(eg_context* ctx, const void* q, const uint3
   const OnDevice on(ctx);
   with_type(d.type, [&](auto t) {
     using TQ = decltype(t);
-    if (dims->head_dim == 64) launch<64, TQ>(ctx, a, p, per_tile, tiles * splits);
-    else launch<128, TQ>(ctx, a, p, per_tile, tiles * splits);
+    if (dims->head_dim == 64) launch<64, TQ>(ctx, a, p, plan.per_tile, tiles * splits);
+    else launch<128, TQ>(ctx, a, p, plan.per_tile, tiles * splits);
   });
   return eg::check_launch(ctx, op);
 }
