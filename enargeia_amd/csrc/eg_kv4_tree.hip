@@ -401,14 +401,18 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Args a, Pool pool) {
 // 16 bytes; positions in the order of the first product's rows (row 16 k + 4 a + e of 32: position 8 a + kOrder[4 k + e]),
 // dims 4 q + j (2 q + j at head_dim 64) at 32 j + q, which is how a thread's words of neighbouring dims are
 // stored without bank conflicts.
-template <int D, int kBlocks, int kParts, class TQ>
+//
+// kHalves 2, for up to 64 columns: two waves share 32 columns, each with half of a step's positions, and meet at the end. (Four
+// waves of 16 columns each read all of a step from LDS: 64 KB more a step, which is what bound them.)
+template <int D, int kBlocks, int kHalves, int kParts, class TQ>
 __global__ __launch_bounds__(256, 2) void wide_kernel(Args a, Pool pool) {
   constexpr int kGroups = D / 32, kDims = D / 16, kWords = D / 32;  // kWords: of K and of V, a thread and step
   // The max is taken up only where it has grown by kLag (in powers of two): with 16-bit rows, whose weights are scaled by
   // that much less, a column's sums are then rescaled about once (8 of up to 8192, 64 rows, 32 / 8 heads of 128, bf16: 92.6
   // us, rescaled at every new max 98).
   constexpr float kLag = kParts == 2 ? 0.f : 3.f, kShift = 15.f - kLag;
-  constexpr uint32_t kStep = 64, kColumns = 64 * kBlocks, kPad = kStep + 1;
+  constexpr uint32_t kStep = 64, kColumns = 64 * kBlocks / kHalves, kPad = kStep + 1;
+  constexpr int kKeys = 4 / kHalves;  // blocks of 16 positions of a step and wave
   __shared__ half8 k_of[2][D / 8][kPad], v_of[2][8][D];
   __shared__ __attribute__((aligned(8))) uint8_t bad_of[2][kGroups][8];  // of a tail step's V: positions (8 a byte) whose scale is no number
   const uint32_t tid = threadIdx.x, lane = tid & 63u;
@@ -428,7 +432,9 @@ __global__ __launch_bounds__(256, 2) void wide_kernel(Args a, Pool pool) {
   const bool fits = n <= length;  // (else the rows give zeros)
   const uint32_t base = fits ? length - n : 0, end = fits ? min(reach, begin + chunk) : 0;
   const Magic bits_over = magic();
-  const uint32_t c0 = tile * kColumns + 16 * kBlocks * wave;  // the wave's first column
+  const uint32_t share = kHalves == 2 ? wave >> 1 : 0;               // the wave's half of a step
+  const uint32_t group_of = kHalves == 2 ? wave & 1u : wave;         // its columns
+  const uint32_t c0 = tile * kColumns + 16 * kBlocks * group_of;     // the first of them
   const bool active = c0 < n * a.group;
 
   const uint32_t page_size = 1u << pool.page_shift;
@@ -553,16 +559,16 @@ __global__ __launch_bounds__(256, 2) void wide_kernel(Args a, Pool pool) {
 
   const auto compute = [&](uint32_t step) {
     const uint32_t buffer = step & 1u, j0 = begin + step * kStep;
-    f32x4 s[kBlocks][4];
+    f32x4 s[kBlocks][kKeys];
 #pragma unroll
     for (int b = 0; b < kBlocks; b++)
 #pragma unroll
-      for (int k = 0; k < 4; k++) s[b][k] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int k = 0; k < kKeys; k++) s[b][k] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int g = 0; g < kGroups; g++)
 #pragma unroll
-      for (int k = 0; k < 4; k++) {
-        const half8 kc = k_of[buffer][4 * g + lg][16 * k + lr];
+      for (int k = 0; k < kKeys; k++) {
+        const half8 kc = k_of[buffer][4 * g + lg][32 * share + 16 * k + lr];
 #pragma unroll
         for (int b = 0; b < kBlocks; b++)
 #pragma unroll
@@ -580,9 +586,10 @@ __global__ __launch_bounds__(256, 2) void wide_kernel(Args a, Pool pool) {
         uint64_t visible = j0 >= base ? sees[b] >> (j0 - base) : ~0ull;
         if (j0 < base && tail) visible = sees[b] << (base - j0) | ((1ull << (base - j0)) - 1u);
         visible &= real;
-        const uint64_t mine = visible >> (8 * lg);
+        if (kHalves == 2) visible &= 0xFFFFFFFFull << (32 * share);  // (the other half's are the other wave's)
+        const uint64_t mine = visible >> (32 * share + 8 * lg);
 #pragma unroll
-        for (int k = 0; k < 4; k++)
+        for (int k = 0; k < kKeys; k++)
 #pragma unroll
           for (int e = 0; e < 4; e++)
             if (!(mine >> (32 * (k >> 1) + kOrder[4 * (k & 1) + e]) & 1u)) s[b][k][e] = -INFINITY;
@@ -599,12 +606,12 @@ __global__ __launch_bounds__(256, 2) void wide_kernel(Args a, Pool pool) {
         }
       }
     }
-    half8 pb[kBlocks][2][kParts];
+    half8 pb[kBlocks][kKeys / 2][kParts];
 #pragma unroll
     for (int b = 0; b < kBlocks; b++) {
       float top = m[b];
 #pragma unroll
-      for (int k = 0; k < 4; k++)
+      for (int k = 0; k < kKeys; k++)
 #pragma unroll
         for (int e = 0; e < 4; e++) top = fmaxf(top, s[b][k][e]);
       top = max_of_head(top);
@@ -621,13 +628,13 @@ __global__ __launch_bounds__(256, 2) void wide_kernel(Args a, Pool pool) {
       if (__builtin_amdgcn_ballot_w64(fabsf(shift) > kLargest) != 0) {
         const float from = m[b] == -INFINITY ? 0.f : m[b];  // (a column without a position yet)
 #pragma unroll
-        for (int k = 0; k < 4; k++)
+        for (int k = 0; k < kKeys; k++)
 #pragma unroll
           for (int e = 0; e < 4; e++) s[b][k][e] -= from;
         shift = -kShift;
       }
 #pragma unroll
-      for (int k = 0; k < 4; k++)
+      for (int k = 0; k < kKeys; k++)
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           float p = __builtin_amdgcn_exp2f(fmaf(s[b][k][e], f[b], -shift));
@@ -641,10 +648,10 @@ __global__ __launch_bounds__(256, 2) void wide_kernel(Args a, Pool pool) {
         }
     }
 #pragma unroll
-    for (int h = 0; h < 2; h++)
+    for (int h = 0; h < kKeys / 2; h++)
 #pragma unroll
       for (int i = 0; i < kDims; i++) {
-        const half8 va = v_of[buffer][4 * h + lg][16 * i + lr];
+        const half8 va = v_of[buffer][4 * (share + h) + lg][16 * i + lr];
 #pragma unroll
         for (int b = 0; b < kBlocks; b++)
 #pragma unroll
@@ -670,14 +677,41 @@ __global__ __launch_bounds__(256, 2) void wide_kernel(Args a, Pool pool) {
     __syncthreads();
   }
 
+#pragma unroll
+  for (int b = 0; b < kBlocks; b++) {
+    l[b] += __shfl_xor(l[b], 16, 64);
+    l[b] += __shfl_xor(l[b], 32, 64);
+  }
+  if constexpr (kHalves == 2) {  // the other half's wave has the same columns and dims in the same lanes
+    f32x4* const sums = reinterpret_cast<f32x4*>(v_of) + group_of * (kBlocks * kDims * 64) + lane;
+    float2* const stats = reinterpret_cast<float2*>(k_of) + group_of * (kBlocks * 64) + lane;
+    if (share == 1) {
+#pragma unroll
+      for (int b = 0; b < kBlocks; b++) {
+        stats[64 * b] = make_float2(m[b], l[b]);
+#pragma unroll
+        for (int i = 0; i < kDims; i++) sums[64 * (kDims * b + i)] = o[b][i];
+      }
+    }
+    __syncthreads();
+    if (share == 1) return;
+#pragma unroll
+    for (int b = 0; b < kBlocks; b++) {
+      const float2 other = stats[64 * b];
+      const float top = fmaxf(m[b], other.x), from = top == -INFINITY ? 0.f : top;
+      const float x = __builtin_amdgcn_exp2f((m[b] - from) * f[b]), y = __builtin_amdgcn_exp2f((other.x - from) * f[b]);
+      l[b] = l[b] * x + other.y * y;
+#pragma unroll
+      for (int i = 0; i < kDims; i++) o[b][i] = o[b][i] * x + sums[64 * (kDims * b + i)] * y;
+      m[b] = top;
+    }
+  }
   if (!active) return;
   const bool whole = chunk >= reach;  // no other chunk: the result itself
 #pragma unroll
   for (int b = 0; b < kBlocks; b++) {
     const uint32_t c = c0 + 16 * b + lr;
-    float sum = l[b];
-    sum += __shfl_xor(sum, 16, 64);
-    sum += __shfl_xor(sum, 32, 64);
+    const float sum = l[b];
     if (c >= n * a.group) continue;
     const uint32_t r = first + c / a.group, hd = kv * a.group + c % a.group;
     const size_t at_row = ((size_t)r * a.heads + hd) * a.splits + split;
@@ -756,8 +790,8 @@ void launch(eg_context* ctx, const Args& a, const Pool& p, uint32_t per_tile, ui
   constexpr int kParts = std::is_same<TQ, float>::value ? 2 : 1;
   const dim3 grid((uint32_t)blocks), threads(kThreads);
   const auto kernel = per_tile == 1   ? few_kernel<D, kParts, TQ>
-                      : per_tile == 4 ? wide_kernel<D, 1, kParts, TQ>
-                                      : wide_kernel<D, 2, kParts, TQ>;
+                      : per_tile == 4 ? wide_kernel<D, 2, 2, kParts, TQ>
+                                      : wide_kernel<D, 2, 1, kParts, TQ>;
   hipLaunchKernelGGL(kernel, grid, threads, 0, ctx->stream, a, p);
   if (a.splits > 1)
     hipLaunchKernelGGL((join_kernel<D, TQ>), dim3((a.rows * a.heads * (D / 4) + kThreads - 1) / kThreads), threads, 0,
@@ -765,23 +799,24 @@ void launch(eg_context* ctx, const Args& a, const Pool& p, uint32_t per_tile, ui
 }
 
 // Blocks of 16 columns a workgroup (1: few_kernel, 4 and 8: wide_kernel) and chunks of a sequence's positions: what
-// the times below, which these kernels were measured with, add up to least by. Lengths are on the device, so it goes by what
-// the tables reach less a page, whose last ones are seldom full. A step (128 positions of few_kernel, 64 of wide_kernel) of a workgroup alone on its CU, and of one of
-// two, in us at head_dim 128: 1.0 and 0.77 (32 x 4 rows to 8192, 32 / 8 heads, bf16: 76.9 us whole, 65.1 halved); 1.15 and
-// 1.15 (32 x 16 rows to 4096: 70.5 halved, 75.5 in four); 1.6 and 1.25 (8 x 64 rows to 8192: 117 halved, 92.6 in four).
-// 0.6 of that at 64, 1.4 times for f32 rows. A launch, its chain of reads and the waves' meeting take 6 us, a join
-// 4.5 and its partials a us for 4 MB written and read.
+// the times below add up to least by. Lengths are on the device, so it goes by what the tables reach less a page, whose
+// last ones are seldom full. The times of a step (128 positions of few_kernel, 64 of wide_kernel) of a workgroup alone on
+// its CU and of one of several, in us, were measured with each kernel at 4096 positions: 32 sequences of 16 rows, 32 / 8
+// heads of 128, bf16, took 100 us in single blocks, 85 in fours and 76 with positions halved, 107 and 85 in eights; 64 of 16
+// / 4 heads of 64 54, 62 and 49, 81 and 63. A launch, its chain of reads and the waves' meeting take 6 us, a join 4.5 and its
+// partials a us for 4 MB written and read.
 struct Plan {
   uint32_t per_tile, tiles, splits, min_chunk;
 };
 Plan plan_of(uint32_t cus, uint64_t pairs, uint64_t columns, uint32_t reach, uint64_t outputs, uint32_t head_dim, bool f32) {
   struct Kind {
     uint32_t per_tile, step;
-    double alone, shared;
+    double alone[2][2], shared[2][2];  // [head_dim 128][f32]
   };
-  constexpr Kind kKinds[] = {{1, 128, 1.0, 0.77}, {4, 64, 1.15, 1.15}, {8, 64, 1.6, 1.25}};
+  constexpr Kind kKinds[] = {{1, 128, {{0.55, 0.75}, {1.0, 1.25}}, {{0.38, 0.52}, {0.74, 0.93}}},
+                             {4, 64, {{0.87, 1.16}, {1.22, 1.70}}, {{0.54, 0.78}, {0.88, 1.22}}},
+                             {8, 64, {{1.17, 1.84}, {1.59, 2.46}}, {{0.75, 1.23}, {1.03, 1.74}}}};
   const uint64_t per_split = outputs * (head_dim + 2) * 4, room = (eg::kPartialsBytes - 64) / per_split;
-  const double unit = (head_dim == 64 ? 0.6 : 1.0) * (f32 ? 1.4 : 1.0);
   Plan best{1, (uint32_t)((columns + 15) / 16), 1, 256};
   double least = -1.0;
   for (const Kind& kind : kKinds) {
@@ -792,7 +827,7 @@ Plan plan_of(uint32_t cus, uint64_t pairs, uint64_t columns, uint32_t reach, uin
       const uint64_t even = (reach + s - 1) / s, chunk = s == 1 ? reach : std::max<uint64_t>(256, (even + 63) & ~63ull);
       const uint64_t chunks = s == 1 ? 1 : (reach + chunk - 1) / chunk, steps = (chunk + kind.step - 1) / kind.step;
       const uint64_t each = (all * chunks + cus - 1) / cus;  // workgroups of the busiest CU
-      double us = 6.0 + steps * unit * (each == 1 ? kind.alone : each * kind.shared);
+      double us = 6.0 + steps * (each == 1 ? kind.alone[head_dim == 128][f32] : each * kind.shared[head_dim == 128][f32]);
       if (chunks > 1) us += 4.5 + chunks * per_split * 2 / 4e6;
       if (least < 0.0 || us < least) {
         least = us;
