@@ -1,7 +1,9 @@
 """The operators of a speculative step against their definitions in float64 (drafts_reference.py): tables within
 their roundings, rotations and kept rows bit for bit, accepted branches and tokens exactly, the tree attention within
 the decode attention's bounds (test_gpu_kv4.py), which count its roundings: the products, weights and sums are
-the same, over at most as many positions.
+the same, over at most as many positions. (Where columns share tiles 16-bit rows' weights are scaled by 2^12, not 2^15, and a
+row's scores by its largest one and not by the group's scale: the first is 2^-37 of the largest weight for 2^-40, which the
+2^-11 of every weight covers wherever the large weights' values are not 0; the second is one rounding less.)
 
 A table's entry is one f32 rounding, 2^-24 of it, of amplitude (cos, sin) of an angle in 64 bits; a frequency is a few
 64-bit operations (of 2^-53 each, a power one last place), so angles of both sides are within 16 x 2^-53 of themselves,
@@ -244,6 +246,35 @@ def test_tree_many_sequences(device, up):  # noqa: F811
     check_tree(device, up, rng, ns, [n + int(x) for n, x in zip(ns, rng.integers(0, 60, 150))], 4, 2, 64, 32, "f16", max_rows=64)
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("heads,d,page,n,length", [(4, 64, 64, 4, 9000), (2, 128, 32, 5, 8600), (8, 64, 32, 6, 2500), (16, 128, 64, 3, 4300),
+                                                   (16, 64, 64, 7, 4300), (16, 128, 256, 8, 2300)])
+def test_tree_chunks_of_more_steps_than_a_wave_holds_page_ids(device, up, heads, d, page, n, length, kind):  # noqa: F811
+    """More sequences than CUs, so that none is split, over the same pages: every kernel past the page ids that a wave reads at
+    once. Some of the sequences are checked."""
+    rng = np.random.default_rng(length + d)
+    pages, seqs = -(-length // page), 300
+    P, k, v = random_pages(rng, pages, 1, d, page)
+    order = rng.permutation(pages).astype(np.uint32)
+    kk, vv = (x[order].reshape(-1, 1, d) for x in (k, v))
+    lengths = rng.integers(length - 600, length + 1, seqs).astype(np.uint32)
+    lengths[:2] = length, n
+    parents = np.concatenate([random_tree(rng, n) for _ in range(seqs)])
+    raw, val = as_type(rng.standard_normal((seqs * n, heads * d)).astype(np.float32), kind)
+    out = up(raw.nbytes)
+    cache = kv4.Kv4Cache(device, 1, d, pages, page, pool=up(P.pool))
+    cache.attend_tree(up(raw), up(offsets_of([n] * seqs)), up(lengths), up(np.tile(order, (seqs, 1))), out, parents=up(parents),
+                      heads=heads, rows=seqs * n, max_rows=n, sequences=seqs, max_pages=pages, type=kind)
+    got = from_type(device.read(out, raw.nbytes), kind).reshape(seqs, n, heads, d)
+    for s in (0, 1, 2, 299):
+        m = int(lengths[s])
+        q = val.reshape(seqs, n, heads, d)[s]
+        want, seen = tree_attend(q, kk[:m], vv[:m], d ** -0.5, parents[s * n:(s + 1) * n], np.ones(m, bool))
+        for j in range(n):
+            bound = decode_bound(q[j], kk[:m], vv[:m], d ** -0.5, seen[j], want[j], kind)
+            assert np.all(np.abs(got[s, j] - want[j]) <= bound), (s, j, float(np.max(np.abs(got[s, j] - want[j]) / bound)))
+
+
 def test_tree_parents_that_are_none(device, up):  # noqa: F811
     """Parents that are not before their row: such rows are roots, and see no other row."""
     rng = np.random.default_rng(5)
@@ -461,6 +492,18 @@ def test_verify_draws_over_every_id(device, up):  # noqa: F811
     u[-1] = np.nextafter(np.float32(1), np.float32(0))
     want = check_verify(device, up, x, np.zeros(s, int), [1] * s, None, None, np.zeros(s), u, np.ones(s))
     assert want[2][0] == 0 and want[2][-1] >= vocab - 2 and len(set(want[2])) == s
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("how", ["chain", "tree", "draft"])
+def test_verify_many_sequences(device, up, how, kind):  # noqa: F811
+    """More chunks than are drawn from one a workgroup: four at a time, the last ones partial."""
+    rng = np.random.default_rng(len(how))
+    for vocab, s in ((20011, 260), (36864, 130)):
+        ns = [int(n) for n in rng.integers(0, 3, s)]
+        x, tokens, parents, draft = verify_case(rng, ns, vocab, how != "tree", how == "draft")
+        t = np.where(rng.random(s) < 0.9, rng.uniform(0.5, 1.5, s), 0.0)
+        check_verify(device, up, x, tokens, ns, parents, draft, rng.random(sum(ns)), rng.random(s), t, kind, 1, 2)
 
 
 def test_verify_many_children_and_tokens_again(device, up):  # noqa: F811
