@@ -15,7 +15,7 @@ namespace {
 
 using namespace eg_kv4;
 
-constexpr uint32_t kThreads = 256, kWaves = 4, kMostRows = 64;
+constexpr uint32_t kThreads = 256, kMostRows = 64;
 
 struct Args {
   const void* q;
@@ -101,12 +101,14 @@ __device__ __forceinline__ int make_query(const Eight<TQ> (&raw)[D / 32], bool i
   return up;
 }
 
-// Few columns: 16 a workgroup, whose waves take a chunk's tiles of 32 positions in turn and meet in LDS. D: head_dim. kParts:
+// Few columns: 16 a workgroup, whose waves take a chunk's tiles of 32 positions in turn and meet in LDS. D: head_dim. kWaves: 4, or
+// 8 where a CU has one workgroup, so that one wave's work is beside another's waits (16 sequences of 16 rows at up to 2048, 14 / 2
+// heads of 64: f32 15.3 us for 17.5, bf16 13.4 for 16.0; 1 of 5 rows at 517 8.8 for 8.1). kParts:
 // f16 parts of a query and of a weight (2 for f32 rows). (With two blocks of columns a wave, 32 / 8 heads of 128 in
 // bf16: 16 sequences of up to 2048 with 8 rows 35.1 us for 22.9, 32 of up to 4096 62.3 for 54.8: half as many workgroups,
 // and no registers left for the next tile's words.)
-template <int D, int kParts, class TQ>
-__global__ __launch_bounds__(256, 2) void few_kernel(Args a, Pool pool) {
+template <int D, int kWaves, int kParts, class TQ>
+__global__ __launch_bounds__(64 * kWaves, 2) void few_kernel(Args a, Pool pool) {
   constexpr int kGroups = D / 32, kDims = D / 16;  // dim groups of K; blocks of 16 dims of O^T
   constexpr bool kSigned = kParts == 2;
   constexpr uint32_t kTile = 32, kColumns = 16;
@@ -361,15 +363,15 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Args a, Pool pool) {
           make_float4(o[i][e], o[i + 1][e], o[i + 2][e], o[i + 3][e]);
   __syncthreads();
   const uint32_t columns = min(16u, n * a.group - c0);
-  for (uint32_t i = tid; i < columns * (D / 4); i += kThreads) {
+  for (uint32_t i = tid; i < columns * (D / 4); i += 64 * kWaves) {
     const uint32_t h = i / (D / 4), d = 4 * (i % (D / 4));
     float top = -INFINITY;
 #pragma unroll
-    for (uint32_t w = 0; w < kWaves; w++) top = fmaxf(top, top_of[w][h]);
+    for (int w = 0; w < kWaves; w++) top = fmaxf(top, top_of[w][h]);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float sum = 0.f;
 #pragma unroll
-    for (uint32_t w = 0; w < kWaves; w++) {
+    for (int w = 0; w < kWaves; w++) {
       const float c = top_of[w][h] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top_of[w][h] - top);
       const float4 v = *reinterpret_cast<const float4*>(&part_of[w][h][d]);
       sum = fmaf(c, sum_of[w][h], sum);
@@ -785,14 +787,18 @@ __global__ __launch_bounds__(256) void join_kernel(Args a, uint32_t sequences) {
       Four{{from_f32<TQ>(acc.x * x), from_f32<TQ>(acc.y * x), from_f32<TQ>(acc.z * x), from_f32<TQ>(acc.w * x)}};
 }
 
+struct Plan {
+  uint32_t per_tile, waves, tiles, splits, min_chunk;
+};
+
 template <int D, class TQ>
-void launch(eg_context* ctx, const Args& a, const Pool& p, uint32_t per_tile, uint64_t blocks) {
+void launch(eg_context* ctx, const Args& a, const Pool& p, const Plan& plan, uint64_t blocks) {
   constexpr int kParts = std::is_same<TQ, float>::value ? 2 : 1;
   const dim3 grid((uint32_t)blocks), threads(kThreads);
-  const auto kernel = per_tile == 1   ? few_kernel<D, kParts, TQ>
-                      : per_tile == 4 ? wide_kernel<D, 2, 2, kParts, TQ>
-                                      : wide_kernel<D, 2, 1, kParts, TQ>;
-  hipLaunchKernelGGL(kernel, grid, threads, 0, ctx->stream, a, p);
+  const auto kernel = plan.per_tile == 1   ? (plan.waves == 4 ? few_kernel<D, 4, kParts, TQ> : few_kernel<D, 8, kParts, TQ>)
+                      : plan.per_tile == 4 ? wide_kernel<D, 2, 2, kParts, TQ>
+                                           : wide_kernel<D, 2, 1, kParts, TQ>;
+  hipLaunchKernelGGL(kernel, grid, dim3(64 * plan.waves), 0, ctx->stream, a, p);
   if (a.splits > 1)
     hipLaunchKernelGGL((join_kernel<D, TQ>), dim3((a.rows * a.heads * (D / 4) + kThreads - 1) / kThreads), threads, 0,
                        ctx->stream, a, p.sequences);
@@ -805,19 +811,17 @@ void launch(eg_context* ctx, const Args& a, const Pool& p, uint32_t per_tile, ui
 // heads of 128, bf16, took 100 us in single blocks, 85 in fours and 76 with positions halved, 107 and 85 in eights; 64 of 16
 // / 4 heads of 64 54, 62 and 49, 81 and 63. A launch, its chain of reads and the waves' meeting take 6 us, a join 4.5 and its
 // partials a us for 4 MB written and read.
-struct Plan {
-  uint32_t per_tile, tiles, splits, min_chunk;
-};
 Plan plan_of(uint32_t cus, uint64_t pairs, uint64_t columns, uint32_t reach, uint64_t outputs, uint32_t head_dim, bool f32) {
   struct Kind {
-    uint32_t per_tile, step;
+    uint32_t per_tile, waves, step;
     double alone[2][2], shared[2][2];  // [head_dim 128][f32]
   };
-  constexpr Kind kKinds[] = {{1, 128, {{0.55, 0.75}, {1.0, 1.25}}, {{0.38, 0.52}, {0.74, 0.93}}},
-                             {4, 64, {{0.87, 1.16}, {1.22, 1.70}}, {{0.54, 0.78}, {0.88, 1.22}}},
-                             {8, 64, {{1.17, 1.84}, {1.59, 2.46}}, {{0.75, 1.23}, {1.03, 1.74}}}};
+  constexpr Kind kKinds[] = {{1, 4, 128, {{0.55, 0.75}, {1.0, 1.25}}, {{0.38, 0.52}, {0.74, 0.93}}},
+                             {1, 8, 256, {{0.76, 1.04}, {1.48, 1.86}}, {{0.76, 1.04}, {1.48, 1.86}}},
+                             {4, 4, 64, {{0.87, 1.16}, {1.22, 1.70}}, {{0.54, 0.78}, {0.88, 1.22}}},
+                             {8, 4, 64, {{1.17, 1.84}, {1.59, 2.46}}, {{0.75, 1.23}, {1.03, 1.74}}}};
   const uint64_t per_split = outputs * (head_dim + 2) * 4, room = (eg::kPartialsBytes - 64) / per_split;
-  Plan best{1, (uint32_t)((columns + 15) / 16), 1, 256};
+  Plan best{1, 4, (uint32_t)((columns + 15) / 16), 1, 256};
   double least = -1.0;
   for (const Kind& kind : kKinds) {
     const uint64_t tiles = (columns + 16 * kind.per_tile - 1) / (16 * kind.per_tile), all = pairs * tiles;
@@ -827,11 +831,11 @@ Plan plan_of(uint32_t cus, uint64_t pairs, uint64_t columns, uint32_t reach, uin
       const uint64_t even = (reach + s - 1) / s, chunk = s == 1 ? reach : std::max<uint64_t>(256, (even + 63) & ~63ull);
       const uint64_t chunks = s == 1 ? 1 : (reach + chunk - 1) / chunk, steps = (chunk + kind.step - 1) / kind.step;
       const uint64_t each = (all * chunks + cus - 1) / cus;  // workgroups of the busiest CU
-      double us = 6.0 + steps * (each == 1 ? kind.alone[head_dim == 128][f32] : each * kind.shared[head_dim == 128][f32]);
+      double us = (kind.waves == 8 ? 6.6 : 6.0) + steps * (each == 1 ? kind.alone[head_dim == 128][f32] : each * kind.shared[head_dim == 128][f32]);
       if (chunks > 1) us += 4.5 + chunks * per_split * 2 / 4e6;
       if (least < 0.0 || us < least) {
         least = us;
-        best = Plan{kind.per_tile, (uint32_t)tiles, (uint32_t)s, 256};
+        best = Plan{kind.per_tile, kind.waves, (uint32_t)tiles, (uint32_t)s, 256};
       }
     }
   }
@@ -894,8 +898,8 @@ extern "C" int eg_attention_tree_kv4(eg_context* ctx, const void* q, const uint3
   const OnDevice on(ctx);
   with_type(d.type, [&](auto t) {
     using TQ = decltype(t);
-    if (dims->head_dim == 64) launch<64, TQ>(ctx, a, p, plan.per_tile, tiles * splits);
-    else launch<128, TQ>(ctx, a, p, plan.per_tile, tiles * splits);
+    if (dims->head_dim == 64) launch<64, TQ>(ctx, a, p, plan, tiles * splits);
+    else launch<128, TQ>(ctx, a, p, plan, tiles * splits);
   });
   return eg::check_launch(ctx, op);
 }

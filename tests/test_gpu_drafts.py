@@ -254,13 +254,14 @@ def test_tree_many_sequences(device, up):  # noqa: F811
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
-@pytest.mark.parametrize("heads,d,page,n,length", [(4, 64, 64, 4, 9000), (2, 128, 32, 5, 8600), (8, 64, 32, 6, 2500), (16, 128, 64, 3, 4300),
-                                                   (16, 64, 64, 7, 4300), (16, 128, 256, 8, 2300)])
-def test_tree_chunks_of_more_steps_than_a_wave_holds_page_ids(device, up, heads, d, page, n, length, kind):  # noqa: F811
-    """More sequences than CUs, so that none is split, over the same pages: every kernel past the page ids that a wave reads at
+@pytest.mark.parametrize("heads,d,page,n,length,seqs", [(4, 64, 64, 4, 9000, 300), (2, 128, 32, 5, 8600, 300), (8, 64, 32, 6, 2500, 300),
+                                                        (16, 128, 64, 3, 4300, 300), (16, 64, 64, 7, 4300, 300),
+                                                        (16, 128, 256, 8, 2300, 300), (4, 64, 64, 4, 17500, 256)])
+def test_tree_chunks_of_more_steps_than_a_wave_holds_page_ids(device, up, heads, d, page, n, length, seqs, kind):  # noqa: F811
+    """As many sequences as CUs or more, so that none is split, over the same pages: every kernel past the page ids that a wave reads at
     once. Some of the sequences are checked."""
     rng = np.random.default_rng(length + d)
-    pages, seqs = -(-length // page), 300
+    pages = -(-length // page)
     P, k, v = random_pages(rng, pages, 1, d, page)
     order = rng.permutation(pages).astype(np.uint32)
     kk, vv = (x[order].reshape(-1, 1, d) for x in (k, v))
@@ -273,7 +274,7 @@ def test_tree_chunks_of_more_steps_than_a_wave_holds_page_ids(device, up, heads,
     cache.attend_tree(up(raw), up(offsets_of([n] * seqs)), up(lengths), up(np.tile(order, (seqs, 1))), out, parents=up(parents),
                       heads=heads, rows=seqs * n, max_rows=n, sequences=seqs, max_pages=pages, type=kind)
     got = from_type(device.read(out, raw.nbytes), kind).reshape(seqs, n, heads, d)
-    for s in (0, 1, 2, 299):
+    for s in (0, 1, 2, seqs - 1):
         m = int(lengths[s])
         q = val.reshape(seqs, n, heads, d)[s]
         want, seen = tree_attend(q, kk[:m], vv[:m], d ** -0.5, parents[s * n:(s + 1) * n], np.ones(m, bool))
