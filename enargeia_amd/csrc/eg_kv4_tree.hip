@@ -406,20 +406,25 @@ __global__ __launch_bounds__(64 * kWaves, 2) void few_kernel(Args a, Pool pool) 
 //
 // kHalves 2, for up to 64 columns: two waves share 32 columns, each with half of a step's positions, and meet at the end. (Four
 // waves of 16 columns each read all of a step from LDS: 64 KB more a step, which is what bound them.)
-template <int D, int kBlocks, int kHalves, int kParts, class TQ>
-__global__ __launch_bounds__(256, 2) void wide_kernel(Args a, Pool pool) {
-  constexpr int kGroups = D / 32, kDims = D / 16, kWords = D / 32;  // kWords: of K and of V, a thread and step
+//
+// kWaves 8, for more than 128 columns: a word is unpacked once for 256, two steps between barriers (8 sequences of 64 rows at up
+// to 8192, 32 / 8 heads of 128, bf16: 81 us for 87). Eight waves that share positions, for up to 128 and up to 64 columns,
+// were as fast as four with the sequences in twice as many chunks.
+template <int D, int kWaves, int kHalves, int kParts, class TQ>
+__global__ __launch_bounds__(64 * kWaves, 2) void wide_kernel(Args a, Pool pool) {
+  constexpr int kBlocks = 2, kGroups = D / 32, kDims = D / 16, kWords = D / 32;  // kWords: of K and of V, a thread and step
+  constexpr uint32_t kSub = kWaves / 4;  // steps between barriers
   // The max is taken up only where it has grown by kLag (in powers of two): with 16-bit rows, whose weights are scaled by
-  // that much less, a column's sums are then rescaled about once (8 of up to 8192, 64 rows, 32 / 8 heads of 128, bf16: 92.6
+  // that much less, a column's sums are then rescaled about once (8 of up to 8192, 64 rows, 32 / 8 heads of 128, bf16, in eights: 92.6
   // us, rescaled at every new max 98).
   constexpr float kLag = kParts == 2 ? 0.f : 3.f, kShift = 15.f - kLag;
-  constexpr uint32_t kStep = 64, kColumns = 64 * kBlocks / kHalves, kPad = kStep + 1;
+  constexpr uint32_t kStep = 64, kColumns = 16 * kBlocks * kWaves / kHalves, kPad = kStep + 1;
   constexpr int kKeys = 4 / kHalves;  // blocks of 16 positions of a step and wave
-  __shared__ half8 k_of[2][D / 8][kPad], v_of[2][8][D];
-  __shared__ __attribute__((aligned(8))) uint8_t bad_of[2][kGroups][8];  // of a tail step's V: positions (8 a byte) whose scale is no number
+  __shared__ half8 k_of[2 * kSub][D / 8][kPad], v_of[2 * kSub][8][D];
+  __shared__ __attribute__((aligned(8))) uint8_t bad_of[2 * kSub][kGroups][8];  // of a tail step's V: positions (8 a byte) whose scale is no number
   const uint32_t tid = threadIdx.x, lane = tid & 63u;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint32_t lr = lane & 15u, lg = lane >> 4, half_step = wave >> 1;  // the 32 positions that this wave unpacks
+  const uint32_t lr = lane & 15u, lg = lane >> 4, sub = kSub == 1 ? 0 : wave >> 2, half_step = kSub == 1 ? wave >> 1 : (wave >> 1) & 1u;  // the 32 positions that this wave unpacks
 
   uint32_t id = blockIdx.x;
   const uint32_t split = id % a.splits;
@@ -434,9 +439,8 @@ __global__ __launch_bounds__(256, 2) void wide_kernel(Args a, Pool pool) {
   const bool fits = n <= length;  // (else the rows give zeros)
   const uint32_t base = fits ? length - n : 0, end = fits ? min(reach, begin + chunk) : 0;
   const Magic bits_over = magic();
-  const uint32_t share = kHalves == 2 ? wave >> 1 : 0;               // the wave's half of a step
-  const uint32_t group_of = kHalves == 2 ? wave & 1u : wave;         // its columns
-  const uint32_t c0 = tile * kColumns + 16 * kBlocks * group_of;     // the first of them
+  const uint32_t half = kHalves == 1 ? 0 : wave >> 1, of_half = kHalves == 1 ? wave : wave & 1u;  // the wave's half of a step
+  const uint32_t c0 = tile * kColumns + 16 * kBlocks * of_half;                   // the first of its columns
   const bool active = c0 < n * a.group;
 
   const uint32_t page_size = 1u << pool.page_shift;
@@ -491,7 +495,7 @@ __global__ __launch_bounds__(256, 2) void wide_kernel(Args a, Pool pool) {
     t.vs = egd::load_b128(r, vs_off, slot * 2);
   };
   const auto put = [&](Stage& t, uint32_t s) {
-    const uint32_t buffer = s & 1u;
+    const uint32_t buffer = s & (2 * kSub - 1);
     const uint32_t two = t.ks * 0x00010001u;  // (each group's by its quad of lanes)
     const uint32_t scale[4] = {(uint32_t)__builtin_amdgcn_update_dpp(0, (int)two, 0x00, 0xF, 0xF, true),
                                (uint32_t)__builtin_amdgcn_update_dpp(0, (int)two, 0x55, 0xF, 0xF, true),
@@ -538,7 +542,7 @@ __global__ __launch_bounds__(256, 2) void wide_kernel(Args a, Pool pool) {
     const uint32_t c = min(c0 + 16 * b + lr, n * a.group - 1);
     load_query<D, TQ>(a, first + c / a.group, kv * a.group + c % a.group, lg, raw[b]);
   }
-  if (steps != 0) load(stage, page_at(0, half_step), 0);
+  if (sub < steps) load(stage, page_at(sub, half_step), sub);
   const uint64_t all = tail_of ? ancestors(a.parents != nullptr, parent) : 0;
 #pragma unroll
   for (int b = 0; b < kBlocks; b++) {
@@ -560,7 +564,7 @@ __global__ __launch_bounds__(256, 2) void wide_kernel(Args a, Pool pool) {
   }
 
   const auto compute = [&](uint32_t step) {
-    const uint32_t buffer = step & 1u, j0 = begin + step * kStep;
+    const uint32_t buffer = step & (2 * kSub - 1), j0 = begin + step * kStep;
     f32x4 s[kBlocks][kKeys];
 #pragma unroll
     for (int b = 0; b < kBlocks; b++)
@@ -570,7 +574,7 @@ __global__ __launch_bounds__(256, 2) void wide_kernel(Args a, Pool pool) {
     for (int g = 0; g < kGroups; g++)
 #pragma unroll
       for (int k = 0; k < kKeys; k++) {
-        const half8 kc = k_of[buffer][4 * g + lg][32 * share + 16 * k + lr];
+        const half8 kc = k_of[buffer][4 * g + lg][32 * half + 16 * k + lr];
 #pragma unroll
         for (int b = 0; b < kBlocks; b++)
 #pragma unroll
@@ -588,8 +592,8 @@ __global__ __launch_bounds__(256, 2) void wide_kernel(Args a, Pool pool) {
         uint64_t visible = j0 >= base ? sees[b] >> (j0 - base) : ~0ull;
         if (j0 < base && tail) visible = sees[b] << (base - j0) | ((1ull << (base - j0)) - 1u);
         visible &= real;
-        if (kHalves == 2) visible &= 0xFFFFFFFFull << (32 * share);  // (the other half's are the other wave's)
-        const uint64_t mine = visible >> (32 * share + 8 * lg);
+        if (kHalves == 2) visible &= 0xFFFFFFFFull << (32 * half);  // (the other half's are the other wave's)
+        const uint64_t mine = visible >> (32 * half + 8 * lg);
 #pragma unroll
         for (int k = 0; k < kKeys; k++)
 #pragma unroll
@@ -653,7 +657,7 @@ __global__ __launch_bounds__(256, 2) void wide_kernel(Args a, Pool pool) {
     for (int h = 0; h < kKeys / 2; h++)
 #pragma unroll
       for (int i = 0; i < kDims; i++) {
-        const half8 va = v_of[buffer][4 * (share + h) + lg][16 * i + lr];
+        const half8 va = v_of[buffer][4 * (half + h) + lg][16 * i + lr];
 #pragma unroll
         for (int b = 0; b < kBlocks; b++)
 #pragma unroll
@@ -662,18 +666,19 @@ __global__ __launch_bounds__(256, 2) void wide_kernel(Args a, Pool pool) {
       }
   };
 
-  if (steps != 0) put(stage, 0);
-  if (steps > 1) load(stage, page_at(1, half_step), 1);
+  if (sub < steps) put(stage, sub);
+  if (kSub + sub < steps) load(stage, page_at(kSub + sub, half_step), kSub + sub);
   __syncthreads();
-  for (uint32_t s = 0; s < steps; s++) {
-    if (active) compute(s);
-    if (s + 1 < steps) put(stage, s + 1);
-    if ((s & 31u) == 31u) ids = later;  // (the next step's)
-    if ((s & 31u) == 29u) later = pages_of(s + 3);
-    if (s + 2 < steps) {
-      const uint32_t next = s + 2;
-      const uint32_t page = (next & 31u) == 0 && (s & 31u) == 30u ? (uint32_t)__builtin_amdgcn_readlane((int)later, (int)half_step)
-                                                                : page_at(next, half_step);
+  for (uint32_t s = 0; s < steps; s += kSub) {
+    if (active) compute(s);  // (both in a loop take 24 registers more)
+    if (kSub == 2 && active && s + 1 < steps) compute(s + 1);
+    if (s + kSub + sub < steps) put(stage, s + kSub + sub);
+    if ((s & 31u) == 32u - kSub) ids = later;  // (the next steps')
+    if ((s & 31u) == 32u - 3 * kSub) later = pages_of(s + 3 * kSub);
+    const uint32_t next = s + 2 * kSub + sub;
+    if (next < steps) {
+      const uint32_t page = (next & 31u) == sub && (s & 31u) == 32u - 2 * kSub ? (uint32_t)__builtin_amdgcn_readlane((int)later, (int)(2 * sub + half_step))
+                                                       : page_at(next, half_step);
       load(stage, page, next);
     }
     __syncthreads();
@@ -685,9 +690,9 @@ __global__ __launch_bounds__(256, 2) void wide_kernel(Args a, Pool pool) {
     l[b] += __shfl_xor(l[b], 32, 64);
   }
   if constexpr (kHalves == 2) {  // the other half's wave has the same columns and dims in the same lanes
-    f32x4* const sums = reinterpret_cast<f32x4*>(v_of) + group_of * (kBlocks * kDims * 64) + lane;
-    float2* const stats = reinterpret_cast<float2*>(k_of) + group_of * (kBlocks * 64) + lane;
-    if (share == 1) {
+    f32x4* const sums = reinterpret_cast<f32x4*>(v_of) + of_half * (kBlocks * kDims * 64) + lane;
+    float2* const stats = reinterpret_cast<float2*>(k_of) + of_half * (kBlocks * 64) + lane;
+    if (half == 1) {
 #pragma unroll
       for (int b = 0; b < kBlocks; b++) {
         stats[64 * b] = make_float2(m[b], l[b]);
@@ -696,7 +701,7 @@ __global__ __launch_bounds__(256, 2) void wide_kernel(Args a, Pool pool) {
       }
     }
     __syncthreads();
-    if (share == 1) return;
+    if (half == 1) return;
 #pragma unroll
     for (int b = 0; b < kBlocks; b++) {
       const float2 other = stats[64 * b];
@@ -788,7 +793,7 @@ __global__ __launch_bounds__(256) void join_kernel(Args a, uint32_t sequences) {
 }
 
 struct Plan {
-  uint32_t per_tile, waves, tiles, splits, min_chunk;
+  uint32_t per_tile, waves, tiles, splits, min_chunk;  // per_tile: blocks of 16 columns a workgroup
 };
 
 template <int D, class TQ>
@@ -796,21 +801,23 @@ void launch(eg_context* ctx, const Args& a, const Pool& p, const Plan& plan, uin
   constexpr int kParts = std::is_same<TQ, float>::value ? 2 : 1;
   const dim3 grid((uint32_t)blocks), threads(kThreads);
   const auto kernel = plan.per_tile == 1   ? (plan.waves == 4 ? few_kernel<D, 4, kParts, TQ> : few_kernel<D, 8, kParts, TQ>)
-                      : plan.per_tile == 4 ? wide_kernel<D, 2, 2, kParts, TQ>
-                                           : wide_kernel<D, 2, 1, kParts, TQ>;
+                      : plan.per_tile == 4 ? wide_kernel<D, 4, 2, kParts, TQ>
+                      : plan.per_tile == 8 ? wide_kernel<D, 4, 1, kParts, TQ>
+                                           : wide_kernel<D, 8, 1, kParts, TQ>;
   hipLaunchKernelGGL(kernel, grid, dim3(64 * plan.waves), 0, ctx->stream, a, p);
   if (a.splits > 1)
     hipLaunchKernelGGL((join_kernel<D, TQ>), dim3((a.rows * a.heads * (D / 4) + kThreads - 1) / kThreads), threads, 0,
                        ctx->stream, a, p.sequences);
 }
 
-// Blocks of 16 columns a workgroup (1: few_kernel, 4 and 8: wide_kernel) and chunks of a sequence's positions: what
-// the times below add up to least by. Lengths are on the device, so it goes by what the tables reach less a page, whose
-// last ones are seldom full. The times of a step (128 positions of few_kernel, 64 of wide_kernel) of a workgroup alone on
-// its CU and of one of several, in us, were measured with each kernel at 4096 positions: 32 sequences of 16 rows, 32 / 8
+// The kernel and the chunks of a sequence's positions: what the times below add up to least by. Lengths are on the device, so
+// it goes by what the tables reach less a page, whose last ones are seldom full. The times of a step of a workgroup alone on its
+// CU and of one of several, in us, were measured with each kernel: at up to 4096 positions 32 sequences of 16 rows, 32 / 8
 // heads of 128, bf16, took 100 us in single blocks, 85 in fours and 76 with positions halved, 107 and 85 in eights; 64 of 16
-// / 4 heads of 64 54, 62 and 49, 81 and 63. A launch, its chain of reads and the waves' meeting take 6 us, a join 4.5 and its
-// partials a us for 4 MB written and read.
+// / 4 heads of 64 54, 62 and 49, 81 and 63. Sixteens (256 columns) are set by what they gain on eights over sizes of the whole
+// range, whose sequences differ in length, which a workgroup alone on its CU has to wait for: of 32 rows of 64 / 8 heads they
+// take 149 us for 173 (128, bf16), 243 for 269 (f32), 100 for 116 and 168 for 176 (64). A launch, its chain of reads and the
+// waves' meeting take 6 us, a join 4.5 and its partials a us for 4 MB written and read.
 Plan plan_of(uint32_t cus, uint64_t pairs, uint64_t columns, uint32_t reach, uint64_t outputs, uint32_t head_dim, bool f32) {
   struct Kind {
     uint32_t per_tile, waves, step;
@@ -819,19 +826,27 @@ Plan plan_of(uint32_t cus, uint64_t pairs, uint64_t columns, uint32_t reach, uin
   constexpr Kind kKinds[] = {{1, 4, 128, {{0.55, 0.75}, {1.0, 1.25}}, {{0.38, 0.52}, {0.74, 0.93}}},
                              {1, 8, 256, {{0.76, 1.04}, {1.48, 1.86}}, {{0.76, 1.04}, {1.48, 1.86}}},
                              {4, 4, 64, {{0.87, 1.16}, {1.22, 1.70}}, {{0.54, 0.78}, {0.88, 1.22}}},
-                             {8, 4, 64, {{1.17, 1.84}, {1.59, 2.46}}, {{0.75, 1.23}, {1.03, 1.74}}}};
+                             {8, 4, 64, {{1.17, 1.84}, {1.59, 2.46}}, {{0.75, 1.23}, {1.03, 1.74}}},
+                             {16, 8, 64, {{1.45, 2.40}, {2.00, 3.45}}, {{1.45, 2.40}, {2.00, 3.45}}}};
   const uint64_t per_split = outputs * (head_dim + 2) * 4, room = (eg::kPartialsBytes - 64) / per_split;
-  Plan best{1, 4, (uint32_t)((columns + 15) / 16), 1, 256};
+  Plan best{};
   double least = -1.0;
   for (const Kind& kind : kKinds) {
-    const uint64_t tiles = (columns + 16 * kind.per_tile - 1) / (16 * kind.per_tile), all = pairs * tiles;
+    const uint64_t width = 16 * kind.per_tile, tiles = (columns + width - 1) / width, all = pairs * tiles;
+    const double alone = kind.alone[head_dim == 128][f32], shared = kind.shared[head_dim == 128][f32];
+    if (kind.per_tile != 1 && 2 * columns < width) continue;
     const uint64_t most = std::min<uint64_t>({std::max<uint64_t>(1, (reach + 255) / 256), std::max<uint64_t>(1, 4ull * cus / all),
                                               std::max<uint64_t>(1, room)});
-    for (uint64_t s = 1; s <= most; s++) {
+    // (each number of chunks up to 8; of more, those that give a CU 1 to 4 workgroups. All of them, where tables are long, are
+    // microseconds of the host's time.)
+    for (uint64_t i = 1, last = 0; i <= 12; i++) {
+      const uint64_t s = std::min(most, i <= 8 ? i : (i - 8) * cus / all);
+      if (s <= last) continue;
+      last = s;
       const uint64_t even = (reach + s - 1) / s, chunk = s == 1 ? reach : std::max<uint64_t>(256, (even + 63) & ~63ull);
       const uint64_t chunks = s == 1 ? 1 : (reach + chunk - 1) / chunk, steps = (chunk + kind.step - 1) / kind.step;
       const uint64_t each = (all * chunks + cus - 1) / cus;  // workgroups of the busiest CU
-      double us = (kind.waves == 8 ? 6.6 : 6.0) + steps * (each == 1 ? kind.alone[head_dim == 128][f32] : each * kind.shared[head_dim == 128][f32]);
+      double us = (kind.waves == 8 ? 6.6 : 6.0) + steps * (each == 1 ? alone : each * shared);
       if (chunks > 1) us += 4.5 + chunks * per_split * 2 / 4e6;
       if (least < 0.0 || us < least) {
         least = us;

@@ -256,7 +256,8 @@ def test_tree_many_sequences(device, up):  # noqa: F811
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
 @pytest.mark.parametrize("heads,d,page,n,length,seqs", [(4, 64, 64, 4, 9000, 300), (2, 128, 32, 5, 8600, 300), (8, 64, 32, 6, 2500, 300),
                                                         (16, 128, 64, 3, 4300, 300), (16, 64, 64, 7, 4300, 300),
-                                                        (16, 128, 256, 8, 2300, 300), (4, 64, 64, 4, 17500, 256)])
+                                                        (16, 128, 256, 8, 2300, 300), (4, 64, 64, 4, 17500, 256), (16, 64, 64, 16, 2500, 256),
+                                                        (16, 128, 32, 16, 4300, 256)])
 def test_tree_chunks_of_more_steps_than_a_wave_holds_page_ids(device, up, heads, d, page, n, length, seqs, kind):  # noqa: F811
     """As many sequences as CUs or more, so that none is split, over the same pages: every kernel past the page ids that a wave reads at
     once. Some of the sequences are checked."""
@@ -284,15 +285,16 @@ def test_tree_chunks_of_more_steps_than_a_wave_holds_page_ids(device, up, heads,
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("d,page,n,extra", [(64, 32, 8, 12), (64, 64, 16, 4), (64, 128, 40, 2), (128, 32, 8, 12), (128, 256, 16, 1),
-                                            (128, 64, 40, 5), (128, 32, 16, 90)])
-def test_tree_many_columns_and_sequences(device, up, d, page, n, extra, kind):  # noqa: F811
-    """Enough columns and sequences that they share tiles (64 and 128 a workgroup), at every place in a step; tables that reach
+@pytest.mark.parametrize("d,page,n,extra,seqs", [(64, 32, 8, 12, 36), (64, 64, 16, 4, 36), (64, 128, 40, 2, 36), (128, 32, 8, 12, 36),
+                                                 (128, 256, 16, 1, 36), (128, 64, 40, 5, 36), (128, 32, 16, 90, 36),
+                                                 (64, 64, 32, 8, 32), (128, 32, 32, 24, 32)])
+def test_tree_many_columns_and_sequences(device, up, d, page, n, extra, seqs, kind):  # noqa: F811
+    """Enough columns and sequences that they share tiles (64, 128 and 256 a workgroup), at every place in a step; tables that reach
     far past the lengths; pages that are none under the rows and before them. 16-bit rows' weights are scaled by 2^12 at least, of
     which half a step of f16's smallest numbers, 2^-25, is 2^-37."""
     floor = 0.0 if kind == "f32" else 2.0 ** -37
     rng = np.random.default_rng(d + n + extra)
-    ns = [n if i % 5 == 0 else int(rng.integers(0, n + 1)) for i in range(36)]
+    ns = [n if i % 5 == 0 else int(rng.integers(0, n + 1)) for i in range(seqs)]
     places = [0, 1, 15, 31, 32, 33, 63, 64, 65, 95, 96, 97, 127, 128, 130]
     lengths = [max(1, k + places[i % len(places)]) for i, k in enumerate(ns)]
     lengths[0] = 330
@@ -302,12 +304,13 @@ def test_tree_many_columns_and_sequences(device, up, d, page, n, extra, kind):  
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
-@pytest.mark.parametrize("d,n,length", [(64, 8, 500), (64, 16, 40), (64, 40, 200), (128, 8, 450), (128, 16, 47), (128, 40, 300)])
-def test_tree_not_finite_rows_where_columns_share_tiles(device, up, d, n, length, kind):  # noqa: F811
-    """As test_tree_not_finite_rows_stay_with_who_sees_them, in one of 36 sequences over one table: the others, whose rows lie
+@pytest.mark.parametrize("d,n,length,seqs", [(64, 8, 500, 36), (64, 16, 40, 36), (64, 40, 200, 36), (128, 8, 450, 36), (128, 16, 47, 36),
+                                             (128, 40, 300, 36), (64, 32, 480, 32), (128, 32, 700, 32)])
+def test_tree_not_finite_rows_where_columns_share_tiles(device, up, d, n, length, seqs, kind):  # noqa: F811
+    """As test_tree_not_finite_rows_stay_with_who_sees_them, in one of many sequences over one table: the others, whose rows lie
     in other pages, keep their bits."""
     rng = np.random.default_rng(n + d)
-    heads, kv, page, seqs = 64, 8, 32, 36
+    heads, kv, page = 64, 8, 32
     parents = random_tree(rng, n, 5)
     each = -(-length // page)
     whole = (length - n) // page  # the pages of no sequence's rows are shared
