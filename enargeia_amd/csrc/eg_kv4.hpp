@@ -33,6 +33,12 @@ struct Pool {
   }
 };
 
+// Whether `n` words (32 bits) from a on and `m` from b on have one in common.
+inline bool share_words(const void* a, uint64_t n, const void* b, uint64_t m) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a && b && x < y + 4 * m && y < x + 4 * n;
+}
+
 inline uint32_t log2_of(uint32_t v) { return 31u - (uint32_t)__builtin_clz(v); }
 
 inline Pool pool_of(const eg_kv4_dims& d, const void* pool, const uint32_t* table) {

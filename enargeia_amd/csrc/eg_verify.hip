@@ -584,6 +584,15 @@ extern "C" int eg_verify_drafts(eg_context* ctx, const void* logits, const uint3
   if (stats + draw > eg::kPartialsBytes || d.rows > 65535 || d.sequences > 65535)
     return eg::fail(ctx, EG_ERR_RANGE, "%s: %u sequences, %u rows of %u ids over the workspace or the grid limit", op, d.sequences,
                     d.rows, d.vocab);
+  const uint64_t n = d.sequences;  // (a sequence's workgroups read its inputs at any time)
+  const struct {
+    const void* at;
+    uint64_t words;
+  } outputs[] = {{path, n * d.max_rows}, {counts, n}, {next, n}},
+    inputs[] = {{tokens, d.rows}, {offsets, n + 1}, {parents, d.rows}, {accept, d.rows}, {draws, n}, {temperatures, n}};
+  for (const auto& x : outputs)
+    for (const auto& y : inputs)
+      if (share_words(x.at, x.words, y.at, y.words)) return eg::fail(ctx, EG_ERR_INVALID, "%s: an output lies in an input", op);
   a.logits = logits;
   a.tokens = tokens;
   a.offsets = offsets;

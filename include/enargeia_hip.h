@@ -712,11 +712,11 @@ EG_API int eg_attention_tree_kv4(eg_context* ctx, const void* q, const uint32_t*
  * temperature that is not above 0, and without temperatures, a row is accepted if it holds its parent's largest
  * logit (the lowest id of them; 0 where none is above -inf), which else is the next token. Above 0, ids whose
  * logit is -inf have p = 0, and a row with a NaN or +inf among its logits, or without one above -inf, accepts
- * nothing, its next token as at 0. Probabilities and sums are 64 bits. Temperatures are finite.
+ * nothing, its next token as at 0. What is decided is what sums in 64 bits decide. Temperatures are finite.
  * path [sequences][max_rows]: the accepted rows, counted from the sequence's first, then 0xFFFFFFFF; counts
  * [sequences]: how many, the root among them; next [sequences]. A sequence of no rows, or of more than max_rows, has
  * a count of 0 and 0xFFFFFFFF for the rest. logits are [rows][vocab] of `type`, draft f32 [rows][vocab]. accept
- * (per row) and draws (per sequence), in [0, 1), may be NULL without temperatures. */
+ * (per row) and draws (per sequence), in [0, 1), may be NULL without temperatures. No output lies in an input. */
 typedef struct eg_verify_dims {
   uint32_t sequences, rows, max_rows; /* max_rows to 64                                           */
   uint32_t vocab;                     /* 1 to 2^20                                                */
@@ -734,7 +734,7 @@ EG_API int eg_verify_drafts(eg_context* ctx, const void* logits, const uint32_t*
  * written. Positions from there on keep what they held, or what lay there before. The pool is that of layer 0, and a page
  * holds `layers` layers. Entries of path that are not below n, and rows that come from or go to no page, are not
  * moved; a count past n is n. A sequence of fewer positions than rows, or of more than max_rows rows, stays as it is.
- * The pages that rows go to are one sequence's alone. */
+ * The pages that rows go to are one sequence's alone; new_lengths are apart from the inputs. */
 EG_API int eg_kv4_keep_rows(eg_context* ctx, const uint32_t* path, const uint32_t* counts, const uint32_t* offsets,
                             const uint32_t* lengths, const uint32_t* table, void* pool, uint32_t* new_lengths,
                             const eg_kv4_dims* dims, uint32_t layers, uint32_t max_rows);

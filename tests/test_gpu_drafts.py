@@ -843,6 +843,36 @@ def test_refusals(device, up):  # noqa: F811
     device.sync()
 
 
+def test_outputs_that_lie_in_an_input_are_refused(device, up):  # noqa: F811
+    """A sequence's workgroups read its inputs while its first one writes."""
+    words = lambda n: up(np.zeros(n, np.uint32))  # noqa: E731
+    cache = kv4.Kv4Cache(device, 1, 64, 2, 32)
+    path, counts, offsets, lengths, table, new = words(12), words(3), words(4), words(3), words(3), words(3)
+    keep_rows = lambda to: cache.keep(path, counts, offsets, lengths, table, to, max_rows=4, sequences=3, max_pages=1)  # noqa: E731
+    for to in (lengths, counts, offsets, K.Binding(offsets, 12), path, K.Binding(path, 44), K.Binding(lengths, 8)):
+        with pytest.raises(_lib.EgError, match="new_lengths lie in an input"):
+            keep_rows(to)
+    keep_rows(new)
+    logits, ins = up(np.zeros((6, 8), np.float32)), dict(tokens=words(6), offsets=words(4), parents=words(6), accept=words(6), draws=words(3),
+                                                        temperatures=words(3))
+    outs = dict(path=words(12), counts=words(3), next=words(3))
+
+    def check(**c):
+        a = {**ins, **outs, **c}
+        drafts.verify(device, logits, a["tokens"], a["offsets"], a["path"], a["counts"], a["next"], sequences=3, rows=6, max_rows=4, vocab=8,
+                      parents=a["parents"], accept=a["accept"], draws=a["draws"], temperatures=a["temperatures"])
+
+    for name in outs:
+        for b in ins.values():
+            with pytest.raises(_lib.EgError, match="an output lies in an input"):
+                check(**{name: b})
+    with pytest.raises(_lib.EgError, match="an output lies in an input"):
+        check(next=K.Binding(ins["tokens"], 20))
+    check()
+    device.sync()
+    cache.release()
+
+
 # ---- together, captured, on other streams -------------------------------------------------------------
 
 
