@@ -103,8 +103,8 @@ __device__ __forceinline__ int make_query(const Eight<TQ> (&raw)[D / 32], bool i
 
 // Few columns: 16 a workgroup, whose waves take a chunk's tiles of 32 positions in turn and meet in LDS. D: head_dim. kWaves: 4, or
 // 8 where a CU has one workgroup, so that one wave's work is beside another's waits (16 sequences of 16 rows at up to 2048, 14 / 2
-// heads of 64: f32 15.3 us for 17.5, bf16 13.4 for 16.0; 1 of 5 rows at 517 8.8 for 8.1). kParts:
-// f16 parts of a query and of a weight (2 for f32 rows). (With two blocks of columns a wave, 32 / 8 heads of 128 in
+// heads of 64: f32 15.3 us for 17.5, bf16 13.4 for 16.0; 1 of 5 rows at 517 7.3 for 7.4). kParts: f16 parts of a query and of a
+// weight (2 for f32 rows). (With two blocks of columns a wave, 32 / 8 heads of 128 in
 // bf16: 16 sequences of up to 2048 with 8 rows 35.1 us for 22.9, 32 of up to 4096 62.3 for 54.8: half as many workgroups,
 // and no registers left for the next tile's words.)
 template <int D, int kWaves, int kParts, class TQ>
@@ -415,16 +415,19 @@ __global__ __launch_bounds__(64 * kWaves, 2) void wide_kernel(Args a, Pool pool)
   constexpr int kBlocks = 2, kGroups = D / 32, kDims = D / 16, kWords = D / 32;  // kWords: of K and of V, a thread and step
   constexpr uint32_t kSub = kWaves / 4;  // steps between barriers
   // The max is taken up only where it has grown by kLag (in powers of two): with 16-bit rows, whose weights are scaled by
-  // that much less, a column's sums are then rescaled about once (8 of up to 8192, 64 rows, 32 / 8 heads of 128, bf16, in eights: 92.6
-  // us, rescaled at every new max 98).
+  // that much less, a column's sums are then rescaled about once (8 of up to 8192, 64 rows, 32 / 8 heads of 128, bf16, in eights:
+  // 92.6 us, rescaled at every new max 98).
   constexpr float kLag = kParts == 2 ? 0.f : 3.f, kShift = 15.f - kLag;
   constexpr uint32_t kStep = 64, kColumns = 16 * kBlocks * kWaves / kHalves, kPad = kStep + 1;
   constexpr int kKeys = 4 / kHalves;  // blocks of 16 positions of a step and wave
   __shared__ half8 k_of[2 * kSub][D / 8][kPad], v_of[2 * kSub][8][D];
-  __shared__ __attribute__((aligned(8))) uint8_t bad_of[2 * kSub][kGroups][8];  // of a tail step's V: positions (8 a byte) whose scale is no number
+  // of a tail step's V: positions (8 a byte) whose scale is no number
+  __shared__ __attribute__((aligned(8))) uint8_t bad_of[2 * kSub][kGroups][8];
   const uint32_t tid = threadIdx.x, lane = tid & 63u;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint32_t lr = lane & 15u, lg = lane >> 4, sub = kSub == 1 ? 0 : wave >> 2, half_step = kSub == 1 ? wave >> 1 : (wave >> 1) & 1u;  // the 32 positions that this wave unpacks
+  const uint32_t lr = lane & 15u, lg = lane >> 4;
+  // the step and the 32 positions of it that this wave unpacks
+  const uint32_t sub = kSub == 1 ? 0 : wave >> 2, half_step = kSub == 1 ? wave >> 1 : (wave >> 1) & 1u;
 
   uint32_t id = blockIdx.x;
   const uint32_t split = id % a.splits;
@@ -677,8 +680,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void wide_kernel(Args a, Pool pool)
     if ((s & 31u) == 32u - 3 * kSub) later = pages_of(s + 3 * kSub);
     const uint32_t next = s + 2 * kSub + sub;
     if (next < steps) {
-      const uint32_t page = (next & 31u) == sub && (s & 31u) == 32u - 2 * kSub ? (uint32_t)__builtin_amdgcn_readlane((int)later, (int)(2 * sub + half_step))
-                                                       : page_at(next, half_step);
+      const uint32_t page = (next & 31u) == sub && (s & 31u) == 32u - 2 * kSub
+                                ? (uint32_t)__builtin_amdgcn_readlane((int)later, (int)(2 * sub + half_step))
+                                : page_at(next, half_step);
       load(stage, page, next);
     }
     __syncthreads();
@@ -723,7 +727,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void wide_kernel(Args a, Pool pool)
     const uint32_t r = first + c / a.group, hd = kv * a.group + c % a.group;
     const size_t at_row = ((size_t)r * a.heads + hd) * a.splits + split;
     const float x = whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f;
-    if (!whole && lg == 0) *reinterpret_cast<float2*>(a.ml + 2 * at_row) = make_float2(m[b] == -INFINITY ? -INFINITY : m[b] * f[b], sum);
+    const float top = m[b] == -INFINITY ? -INFINITY : m[b] * f[b];
+    if (!whole && lg == 0) *reinterpret_cast<float2*>(a.ml + 2 * at_row) = make_float2(top, sum);
 #pragma unroll
     for (int i = 0; i < 2; i++)
 #pragma unroll
@@ -898,9 +903,10 @@ extern "C" int eg_attention_tree_kv4(eg_context* ctx, const void* q, const uint3
   if (!some) return EG_OK;
   a.scale = (d.scale > 0.f ? d.scale : 1.0f / sqrtf((float)dims->head_dim)) * kLog2e;
   a.capacity = dims->max_pages * dims->page_size;
-  const Plan plan = plan_of(ctx->cu_count, (uint64_t)dims->sequences * dims->kv_heads, (uint64_t)std::min(d.max_rows, d.rows) * a.group,
-                            a.capacity - std::min(a.capacity, dims->page_size), (uint64_t)d.rows * d.heads, dims->head_dim, d.type == EG_ELEMENT_F32);
-  const uint64_t tiles = (uint64_t)dims->sequences * dims->kv_heads * plan.tiles, splits = plan.splits;
+  const uint64_t pairs = (uint64_t)dims->sequences * dims->kv_heads, columns = (uint64_t)std::min(d.max_rows, d.rows) * a.group;
+  const Plan plan = plan_of(ctx->cu_count, pairs, columns, a.capacity - std::min(a.capacity, dims->page_size),
+                            (uint64_t)d.rows * d.heads, dims->head_dim, d.type == EG_ELEMENT_F32);
+  const uint64_t tiles = pairs * plan.tiles, splits = plan.splits;
   a.tiles = plan.tiles;
   a.splits = plan.splits;
   a.min_chunk = plan.min_chunk;

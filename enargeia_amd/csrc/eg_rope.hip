@@ -46,8 +46,8 @@ __device__ __forceinline__ double2 turned(double turns) {
 // from the one before, turned by one position (4 f64 instructions for 32, off by up to 2^-51 more with each). 131,072
 // positions of 64 pairs 12.7 us, with a series each 19.3; stores alone 12.
 constexpr uint32_t kRows = 8;
-__global__ __launch_bounds__(256) void table_kernel(float4* table, Frequencies fs, uint32_t first, uint32_t positions, uint32_t halves,
-                                                    uint32_t count, double amplitude) {
+__global__ __launch_bounds__(256) void table_kernel(float4* table, Frequencies fs, uint32_t first, uint32_t positions,
+                                                    uint32_t halves, uint32_t count, double amplitude) {
   const uint32_t i = blockIdx.x * kThreads + threadIdx.x;
   if (i >= count) return;
   const uint32_t rows = i / halves, j = i - rows * halves;
@@ -59,7 +59,8 @@ __global__ __launch_bounds__(256) void table_kernel(float4* table, Frequencies f
 #pragma unroll
   for (uint32_t k = 0; k < kRows; k++) {
     const uint32_t row = kRows * rows + k;
-    if (row < positions) table[(uint64_t)row * halves + j] = make_float4((float)at[0].x, (float)at[0].y, (float)at[1].x, (float)at[1].y);
+    if (row < positions)
+      table[(uint64_t)row * halves + j] = make_float4((float)at[0].x, (float)at[0].y, (float)at[1].x, (float)at[1].y);
 #pragma unroll
     for (int e = 0; e < 2; e++)
       at[e] = make_double2(fma(at[e].x, step[e].x, -at[e].y * step[e].y), fma(at[e].y, step[e].x, at[e].x * step[e].y));
@@ -84,7 +85,9 @@ struct alignas(sizeof(T) * 4) Four {
   T v[4];
 };
 
-// A workgroup per row; a unit is 8 elements of a head: 4 pairs, or 8 elements past the rotary part.
+// A workgroup per row, so that the position and its table row are found once; a unit is 8 elements of a head: 4 pairs,
+// or 8 elements past the rotary part. Memory bounds it: 32,768 rows of 40 heads of 128, half rotated, bf16, in 120 us, 5.6 TB/s
+// read and written; 16 rows of 16 heads of 64 in 2.8 us, a chain of offsets, position, table.
 template <bool kInterleaved, class TI, class TO>
 __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
 #pragma clang fp contract(off)
@@ -199,7 +202,8 @@ int eg_rope_table(eg_context* ctx, float* table, const eg_rope_table_dims* dims)
   }
   const OnDevice on(ctx);
   hipLaunchKernelGGL(table_kernel, dim3((uint32_t)blocks), dim3(kThreads), 0, ctx->stream,
-                     reinterpret_cast<float4*>(table), fs, d.first, d.positions, pairs / 2, (uint32_t)count, d.amplitude == 0.0 ? 1.0 : d.amplitude);
+                     reinterpret_cast<float4*>(table), fs, d.first, d.positions, pairs / 2, (uint32_t)count,
+                     d.amplitude == 0.0 ? 1.0 : d.amplitude);
   return eg::check_launch(ctx, op);
 }
 

@@ -9,10 +9,10 @@
 //
 // What is decided is decided in f64: of 151,936 running sums some lie within f32's rounding of the drawn target in one draw
 // of a hundred, within these in none of 10^6. Exponentials in f64 are 15 f64 instructions, which over all rows take
-// longer than reading them (48 sequences of up to 8 rows: 56 us, with f32's 42): so Z is summed in f32 (kExact false),
-// which is off by less than kMargin of it, and a row for which that could decide otherwise is summed again in f64 where it comes up. Draft
-// probabilities are taken from p = e / Z itself, so their rows' Z are f64 from the start. (The largest is taken from a logit
-// before the product with the scale: the difference is exact, where products of large logits leave their rounding.)
+// longer than reading them (48 sequences of up to 8 rows: 47 us, in f32 30.5): so Z is summed in f32 (kExact false),
+// which is off by less than kMargin of it, and a row for which that could decide otherwise is summed again in f64 where it comes
+// up. Draft probabilities are taken from p = e / Z itself, so their rows' Z are f64 from the start. (The largest is taken from a
+// logit before the product with the scale: the difference is exact, where products of large logits leave their rounding.)
 #include <algorithm>
 
 #include "eg_kv4.hpp"
@@ -316,7 +316,8 @@ __device__ __forceinline__ double exact_sum(const VerifyArgs& a, const T* row, f
 }
 
 // A workgroup per (`together` chunks, sequence): the sequence's rows' sums from their chunks', the branch, and where a
-// token is drawn the sums of its chunks of what it is drawn from, for verify_draw. The first of a sequence writes what it finds. A chain of dependent reads bounds it: offsets; rows and sums; single logits; the chunks.
+// token is drawn the sums of its chunks of what it is drawn from, for verify_draw. The first of a sequence writes what it finds.
+// A chain of dependent reads bounds it: offsets; rows and sums; single logits; the chunks.
 // kBatch chunks of it at a time (1 or 4): all of their ids are under way before any is waited for.
 template <bool kDraft, uint32_t kBatch, class T>
 __global__ __launch_bounds__(kWalkThreads) void verify_walk(VerifyArgs a) {
@@ -619,7 +620,8 @@ extern "C" int eg_verify_drafts(eg_context* ctx, const void* logits, const uint3
   with_type(d.type, [&](auto t) {
     using T = decltype(t);
     const bool drafted = draft && temperatures;
-    const dim3 threads(kThreads), walk(kWalkThreads), grid(temperatures ? (a.chunks + a.together - 1) / a.together : 1, d.sequences);
+    const dim3 threads(kThreads), walk(kWalkThreads);
+    const dim3 grid(temperatures ? (a.chunks + a.together - 1) / a.together : 1, d.sequences);
     if (d.rows != 0) {
       if (drafted) hipLaunchKernelGGL((verify_stats<true, T>), dim3(a.chunks, d.rows), threads, 0, ctx->stream, a);
       else hipLaunchKernelGGL((verify_stats<false, T>), dim3(a.chunks, d.rows), threads, 0, ctx->stream, a);
