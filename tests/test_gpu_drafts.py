@@ -118,6 +118,24 @@ def test_rope_positions_past_the_table_and_many_sequences(device, up):  # noqa: 
     check_rope(device, up, rng, [4000, 1], [0, 3], None, 14, 2, 64, 64, "half", "f16", "f16", before=1)
 
 
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_rope_of_q_and_k_in_one_buffer_in_place(device, up, layout):  # noqa: F811
+    """Rows of q, k and v side by side, as one projection makes them: q and k rotated where they lie, v as it was."""
+    rng = np.random.default_rng(12)
+    rows, heads, kv, d = 37, 5, 2, 64
+    x = rng.standard_normal((rows, (heads + 2 * kv) * d)).astype(np.float32)
+    p = rng.integers(0, 90, rows).astype(np.uint32)
+    angle = np.arange(90)[:, None] * 1e4 ** (-np.arange(0, d, 2) / d)
+    cs = np.stack([np.cos(angle), np.sin(angle)], -1).astype(np.float32)
+    b = up(x)
+    q, k, wide = K.Binding(b, 0), K.Binding(b, heads * d * 4), x.shape[1]
+    drafts.rope(device, up(cs), rows=rows, head_dim=d, table_positions=90, q=q, q_out=q, heads=heads, k=k, k_out=k, kv_heads=kv, positions=up(p),
+                layout=layout, q_stride=wide, k_stride=wide, q_out_stride=wide, k_out_stride=wide)
+    want = x.copy()
+    want[:, : (heads + kv) * d] = rotate(x[:, : (heads + kv) * d].reshape(rows, -1, d), cs[p], d, layout).reshape(rows, -1)
+    np.testing.assert_array_equal(device.read_array(b, np.float32, x.size).reshape(x.shape), want)
+
+
 def test_rope_without_sequences_and_without_starts(device, up):  # noqa: F811
     rng = np.random.default_rng(8)
     x, p = rng.standard_normal((6, 2, 64)).astype(np.float32), np.array([4, 0, 9, 2, 2, 10], np.uint32)
@@ -350,6 +368,14 @@ def test_tree_not_finite_rows_where_columns_share_tiles(device, up, d, n, length
         np.testing.assert_array_equal(got[~bad], clean[~bad])
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("heads,kv,d,n,length", [(128, 1, 64, 64, 150), (96, 1, 128, 37, 600), (1, 1, 128, 1, 1), (33, 33, 64, 2, 70)])
+def test_tree_of_the_most_and_fewest_columns(device, up, heads, kv, d, n, length, kind):  # noqa: F811
+    """8,192 columns of a kv head, and one; 16-bit rows' weights as in test_tree_many_columns_and_sequences."""
+    rng = np.random.default_rng(heads)
+    check_tree(device, up, rng, [n, max(1, n // 3)], [length, length], heads, kv, d, 32, kind, floor=0.0 if kind == "f32" else 2.0 ** -37)
+
+
 def test_tree_parents_that_are_none(device, up):  # noqa: F811
     """Parents that are not before their row: such rows are roots, and see no other row."""
     rng = np.random.default_rng(5)
@@ -556,6 +582,18 @@ def test_verify_the_whole_vocabulary(device, up):  # noqa: F811
         x, tokens, parents, q = verify_case(rng, ns, 151936, chain, draft, peak=14.0)
         for _ in range(3):
             check_verify(device, up, x, tokens, ns, parents, q, rng.random(6), rng.random(2), [0.9, 1.1])
+
+
+@pytest.mark.parametrize("how", ["chain", "tree", "draft"])
+@pytest.mark.parametrize("vocab,kind", [(1 << 20, "f32"), ((1 << 20) - 4097, "bf16")])
+def test_verify_the_largest_vocabularies(device, up, vocab, kind, how):  # noqa: F811
+    """256 and 255 chunks: a row's sums in four reads of a wave, a chunk a thread in the draw; the ends of what can be drawn."""
+    rng = np.random.default_rng(vocab + len(how))
+    ns = [3, 1]
+    x, tokens, parents, q = verify_case(rng, ns, vocab, how != "tree", how == "draft", peak=14.0)
+    one = np.nextafter(np.float32(1), np.float32(0))
+    for draws in ([0.0, one], rng.random(2)):
+        check_verify(device, up, x, tokens, ns, parents, q, rng.random(4), draws, [0.9, 1.3], kind)
 
 
 def test_verify_draws_over_every_id(device, up):  # noqa: F811
