@@ -2,6 +2,7 @@
 // their own. Both move bytes: their floor is what they read and write once at the memory's rate.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "eg_kv4.hpp"
 
@@ -76,18 +77,16 @@ struct RopeArgs {
   uint32_t q_stride, k_stride, q_out_stride, k_out_stride, table_positions, sequences;
 };
 
-template <class T>
-struct alignas(16) Eight {
-  T v[8];
-};
-template <class T>
-struct alignas(sizeof(T) * 4) Four {
-  T v[4];
+template <class T, int N>
+struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Several {
+  T v[N];
 };
 
 // A workgroup per row, so that the position and its table row are found once; a unit is 8 elements of a head: 4 pairs,
-// or 8 elements past the rotary part. Memory bounds it: 32,768 rows of 40 heads of 128, half rotated, bf16, in 120 us, 5.6 TB/s
-// read and written; 16 rows of 16 heads of 64 in 2.8 us, a chain of offsets, position, table.
+// or 8 elements past the rotary part. Memory bounds it: 32,768 rows of 40 heads of 128, half rotated, bf16, in 116 us, 5.8 TB/s
+// read and written; 16 rows of 16 heads of 64 in 2.8 us, a chain of offsets, position, table. Neighbours as pairs, f32 out: 4
+// elements, so that a wave's 16-byte stores follow each other, and two units under way (16,384 rows of 40 heads of 128, f16 to f32,
+// in 97 us for 107). Halves apart: the units that rotate first, so that a wave does one thing (half rotated, bf16, 59 us for 69).
 template <bool kInterleaved, class TI, class TO>
 __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
 #pragma clang fp contract(off)
@@ -101,47 +100,90 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
   }
   if (position >= a.table_positions) return;
   const float2* cs = a.table + position * (a.rotary_dim / 2);
-  const uint32_t per_head = a.head_dim / 8, turned = a.rotary_dim / 8;
-  const uint32_t units = (a.heads + a.kv_heads) * per_head;
-  for (uint32_t i = threadIdx.x; i < units; i += kThreads) {
-    uint32_t head = i / per_head;
-    const uint32_t u = i % per_head;
+  constexpr uint32_t kUnit = kInterleaved && sizeof(TO) == 4 ? 4 : 8;
+  const uint32_t per_head = a.head_dim / kUnit, turned = a.rotary_dim / kUnit;
+  const uint32_t units = (a.heads + a.kv_heads) * per_head, half = a.rotary_dim / 2;
+  const uint32_t split = (a.heads + a.kv_heads) * turned;  // halves apart: units before it rotate, so that waves do one or the other
+  struct Unit {
+    const TI* src;
+    TO* dst;
+    uint32_t u;
+    Several<TI, kUnit> x;
+    Several<TI, 4> y, z;
+  };
+  // (apart: a unit whose pairs lie half the rotary part from each other)
+  const auto load = [&](auto apart, uint32_t i, Unit& t) {
+    uint32_t head;
+    if constexpr (!decltype(apart)::value) {
+      const uint32_t first = kInterleaved ? 0 : turned, each = per_head - first, j = kInterleaved ? i : i - split;
+      head = j / each;
+      t.u = first + j % each;
+    } else {
+      head = i / turned;
+      t.u = i % turned;
+    }
     const bool is_q = head < a.heads;
     if (!is_q) head -= a.heads;
-    const TI* src = static_cast<const TI*>(is_q ? a.q : a.k) + (size_t)r * (is_q ? a.q_stride : a.k_stride) +
-                    (size_t)head * a.head_dim;
-    TO* dst = static_cast<TO*>(is_q ? a.q_out : a.k_out) + (size_t)r * (is_q ? a.q_out_stride : a.k_out_stride) +
-              (size_t)head * a.head_dim;
-    if (kInterleaved || u >= turned) {
-      const Eight<TI> x = *reinterpret_cast<const Eight<TI>*>(src + 8 * u);
-      Eight<TO> y;
-      if (u < turned) {
+    t.src = static_cast<const TI*>(is_q ? a.q : a.k) + (size_t)r * (is_q ? a.q_stride : a.k_stride) + (size_t)head * a.head_dim;
+    t.dst = static_cast<TO*>(is_q ? a.q_out : a.k_out) + (size_t)r * (is_q ? a.q_out_stride : a.k_out_stride) +
+            (size_t)head * a.head_dim;
+    if constexpr (decltype(apart)::value) {
+      t.y = *reinterpret_cast<const Several<TI, 4>*>(t.src + 4 * t.u);
+      t.z = *reinterpret_cast<const Several<TI, 4>*>(t.src + half + 4 * t.u);
+    } else {
+      t.x = *reinterpret_cast<const Several<TI, kUnit>*>(t.src + kUnit * t.u);
+    }
+  };
+  const auto store = [&](auto apart, const Unit& t) {
+    if constexpr (decltype(apart)::value) {
+      Several<TO, 4> y, w;
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const float2 t = cs[4 * u + e];
-          const float p = to_f32(x.v[2 * e]), w = to_f32(x.v[2 * e + 1]);
-          y.v[2 * e] = from_f32<TO>(p * t.x - w * t.y);
-          y.v[2 * e + 1] = from_f32<TO>(w * t.x + p * t.y);
+      for (int e = 0; e < 4; e++) {
+        const float2 c = cs[4 * t.u + e];
+        const float p = to_f32(t.y.v[e]), o = to_f32(t.z.v[e]);
+        y.v[e] = from_f32<TO>(p * c.x - o * c.y);
+        w.v[e] = from_f32<TO>(o * c.x + p * c.y);
+      }
+      *reinterpret_cast<Several<TO, 4>*>(t.dst + 4 * t.u) = y;
+      *reinterpret_cast<Several<TO, 4>*>(t.dst + half + 4 * t.u) = w;
+    } else {
+      Several<TO, kUnit> y;
+      if (kInterleaved && t.u < turned) {
+#pragma unroll
+        for (uint32_t e = 0; e < kUnit / 2; e++) {
+          const float2 c = cs[kUnit / 2 * t.u + e];
+          const float p = to_f32(t.x.v[2 * e]), w = to_f32(t.x.v[2 * e + 1]);
+          y.v[2 * e] = from_f32<TO>(p * c.x - w * c.y);
+          y.v[2 * e + 1] = from_f32<TO>(w * c.x + p * c.y);
         }
       } else {
 #pragma unroll
-        for (int e = 0; e < 8; e++) y.v[e] = from_f32<TO>(to_f32(x.v[e]));
+        for (uint32_t e = 0; e < kUnit; e++) y.v[e] = from_f32<TO>(to_f32(t.x.v[e]));
       }
-      *reinterpret_cast<Eight<TO>*>(dst + 8 * u) = y;
-    } else {
-      const uint32_t half = a.rotary_dim / 2;
-      const Four<TI> x = *reinterpret_cast<const Four<TI>*>(src + 4 * u);
-      const Four<TI> z = *reinterpret_cast<const Four<TI>*>(src + half + 4 * u);
-      Four<TO> y, w;
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const float2 t = cs[4 * u + e];
-        const float p = to_f32(x.v[e]), o = to_f32(z.v[e]);
-        y.v[e] = from_f32<TO>(p * t.x - o * t.y);
-        w.v[e] = from_f32<TO>(o * t.x + p * t.y);
+      *reinterpret_cast<Several<TO, kUnit>*>(t.dst + kUnit * t.u) = y;
+    }
+  };
+  constexpr std::true_type apart{};
+  constexpr std::false_type whole{};
+  if constexpr (kInterleaved) {  // two units under way together (a load does not pass a store by itself: an output may be its input)
+    for (uint32_t i = threadIdx.x; i < units; i += 2 * kThreads) {
+      Unit one, two;
+      load(whole, i, one);
+      const bool more = i + kThreads < units;
+      if (more) load(whole, i + kThreads, two);
+      store(whole, one);
+      if (more) store(whole, two);
+    }
+  } else {  // (which have two loads each)
+    for (uint32_t i = threadIdx.x; i < units; i += kThreads) {
+      Unit one;
+      if (i < split) {
+        load(apart, i, one);
+        store(apart, one);
+      } else {
+        load(whole, i, one);
+        store(whole, one);
       }
-      *reinterpret_cast<Four<TO>*>(dst + 4 * u) = y;
-      *reinterpret_cast<Four<TO>*>(dst + half + 4 * u) = w;
     }
   }
 }
