@@ -155,6 +155,26 @@ __device__ __forceinline__ double block_before(double v, double& total) {
   return lane == 0 ? before : before + o;
 }
 
+// Whether a sequence of packed rows first .. end is computed.
+__device__ __forceinline__ bool computed(const VerifyArgs& a, uint32_t first, uint32_t end) {
+  return first < end && end <= a.rows && end - first <= a.max_rows;
+}
+
+// The lowest sequence that is computed and holds `row`: by its own two offsets, as verify_walk has it, whatever the other
+// sequences' are. (The walk reads the sums of every row of such a sequence: each is made in this call.) A wave looks at 64.
+__device__ __forceinline__ bool find_computed(const VerifyArgs& a, uint32_t row, uint32_t& seq) {
+  for (uint32_t i0 = 0; i0 < a.sequences; i0 += 64) {
+    const uint32_t i = i0 + (threadIdx.x & 63u), s = min(i, a.sequences - 1);
+    const uint32_t first = a.offsets[s], end = a.offsets[s + 1];
+    const uint64_t holds = __ballot(i < a.sequences && computed(a, first, end) && first <= row && row < end);
+    if (holds != 0) {
+      seq = i0 + (uint32_t)__builtin_ctzll(holds);
+      return true;
+    }
+  }
+  return false;
+}
+
 // A workgroup per (chunk, row): its largest logit and its sum.
 template <bool kExact, class T>
 __global__ __launch_bounds__(256) void verify_stats(VerifyArgs a) {
@@ -170,8 +190,8 @@ __global__ __launch_bounds__(256) void verify_stats(VerifyArgs a) {
 #pragma unroll
     for (uint32_t e = 0; e < kWide; e++) v[j * kWide + e] = w[e];
   }
-  uint32_t seq, first, end;
-  if (!find_sequence(a.offsets, a.sequences, row, seq, first, end)) return;
+  uint32_t seq;
+  if (!find_computed(a, row, seq)) return;
   const float temperature = temperature_of(a, seq);
   float top = -INFINITY;
   uint32_t id = 0;
@@ -329,7 +349,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk(VerifyArgs a) {
   const uint32_t seq = blockIdx.y, tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
   const bool writes = blockIdx.x == 0;
   const uint32_t first = a.offsets[seq], end = a.offsets[seq + 1], n = end - first;
-  if (n == 0 || n > a.max_rows || first > end || end > a.rows) {
+  if (!computed(a, first, end)) {
     if (!writes) return;
     if (tid < a.max_rows) a.path[(uint64_t)seq * a.max_rows + tid] = kNone;
     if (tid == 0) {

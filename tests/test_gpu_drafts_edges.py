@@ -1,0 +1,56 @@
+"""The operators of a speculative step at the ends of their ranges. The definitions (drafts_reference.py) are test_gpu_drafts.py's."""
+
+import numpy as np
+import pytest
+
+from drafts_reference import NO_ROW, verify
+from enargeia_amd import drafts
+from test_gpu_drafts import random_tree, verify_case
+from test_gpu_kv4 import up  # noqa: F401 (a fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- verification -------------------------------------------------------------------------------------
+
+
+def run_verify(device, up, logits, tokens, off, parents, accept, draws, temperatures, max_rows):  # noqa: F811
+    s, (rows, vocab) = len(off) - 1, logits.shape
+    path, counts, token = up(np.full((s, max_rows), 5, np.uint32)), up(np.full(s, 5, np.uint32)), up(np.full(s, 5, np.uint32))
+    f32 = lambda a: None if a is None else up(np.asarray(a, np.float32))  # noqa: E731
+    drafts.verify(device, up(logits), up(np.asarray(tokens, np.uint32)), up(np.array(off, np.uint32)), path, counts, token,
+                  parents=up(parents), accept=f32(accept), draws=f32(draws), temperatures=f32(temperatures), sequences=s, rows=rows,
+                  max_rows=max_rows, vocab=vocab)
+    return (device.read_array(path, np.uint32, s * max_rows).reshape(s, max_rows), device.read_array(counts, np.uint32, s),
+            device.read_array(token, np.uint32, s))
+
+
+@pytest.mark.parametrize("hot", [False, True])
+@pytest.mark.parametrize("off", [[9, 5, 5, 16], [0xFFFFFFFF, 5, 16, 16], [0, 5, 17, 17], [8, 12, 0, 6], [12, 16, 4, 12, 0, 4]])
+def test_verify_of_offsets_that_do_not_ascend(device, up, off, hot):  # noqa: F811
+    """What a sequence that is computed is given comes from this call's logits, wherever the others lie."""
+    for seed in range(4):
+        rng = np.random.default_rng(10 * seed + hot)
+        rows, vocab, s = 16, 9000, len(off) - 1
+        before, tokens, _, _ = verify_case(rng, [rows], vocab, False, False)
+        logits, tokens, _, _ = verify_case(rng, [rows], vocab, False, False)
+        parents = np.full(rows, NO_ROW, np.uint32)
+        want = np.full((s, rows), NO_ROW, np.uint32), np.zeros(s, np.uint32), np.full(s, NO_ROW, np.uint32)
+        accept, draws = rng.random(rows), rng.random(s)
+        heat = rng.uniform(0.5, 1.5, s) if hot else None
+        f32 = np.float32
+        for i in range(s):
+            a, b = off[i], off[i + 1]
+            if not 0 < b - a <= rows or b > rows:
+                continue
+            parents[a:b] = random_tree(rng, b - a, 2)
+            for r in range(a + 1, b):  # drafts that are often accepted
+                if rng.random() < 0.7:
+                    tokens[r] = logits[a + int(parents[r])].argmax()
+            got, want[2][i] = verify(logits[a:b], tokens[a:b], parents[a:b], None, f32(accept[a:b]), f32(draws[i]),
+                                     f32(heat[i]) if hot else 0.0)
+            want[1][i] = len(got)
+            want[0][i, : len(got)] = got
+        run_verify(device, up, before, tokens, [0, rows], parents, accept, draws[:1], heat[:1] if hot else None, rows)
+        for x, y, name in zip(run_verify(device, up, logits, tokens, off, parents, accept, draws, heat, rows), want, ("path", "counts", "next")):
+            np.testing.assert_array_equal(x, y, err_msg=name)
