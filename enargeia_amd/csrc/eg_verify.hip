@@ -30,8 +30,10 @@ constexpr uint32_t kNone = 0xFFFFFFFFu;
 // itself rounded: 3 x 2^-24 of exponents that matter down to -30 (2^-30 of 2^20 ids are 2^-10 of Z, and their own errors no
 // more than that times 1/8), so 6e-6 of an exponential, whose own error is 2^-23 and that of 16 added 2^-20.
 constexpr double kMargin = 0x1p-16;
-// Temperatures from which on scale and exponents fit f32; below, Z is f64.
-constexpr float kColdest = 1e-30f;
+// Temperatures between which scales and exponents fit f32; beyond, Z is f64. (A difference of two logits that passes f32's
+// largest is -inf there, its exponential 0: up to 2^120 that is an exponent under -2^8. A scale is a normal number to 2^126.)
+constexpr float kColdest = 1e-30f, kHottest = 0x1p120f;
+__device__ __forceinline__ bool fits_f32(float temperature) { return temperature >= kColdest && temperature <= kHottest; }
 
 // What a sequence's next token is drawn from: a row's p, or (of > 0) max(p - q, 0).
 struct Draw {
@@ -223,7 +225,7 @@ __global__ __launch_bounds__(256) void verify_stats(VerifyArgs a) {
     bool bad = false;
 #pragma unroll
     for (uint32_t j = 0; j < kEach; j++) bad |= broken(v[j]);
-    if (kExact || temperature < kColdest) {
+    if (kExact || !fits_f32(temperature)) {
 #pragma unroll
       for (uint32_t j = 0; j < kEach; j++) sum += exp2_of(((double)v[j] - from) * scale);
     } else {
@@ -360,7 +362,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk(VerifyArgs a) {
     return;
   }
   const float temperature = temperature_of(a, seq);
-  const bool greedy = !(temperature > 0.f), rough = !kDraft && temperature >= kColdest;
+  const bool greedy = !(temperature > 0.f), rough = !kDraft && fits_f32(temperature);
   const double scale = greedy ? 0.0 : scale_of(temperature);
   const T* logits = static_cast<const T*>(a.logits) + (uint64_t)first * a.stride;
   const Stats* stats = a.stats + (uint64_t)first * a.chunks;

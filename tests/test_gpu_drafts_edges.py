@@ -5,7 +5,7 @@ import pytest
 
 from drafts_reference import NO_ROW, verify
 from enargeia_amd import drafts
-from test_gpu_drafts import random_tree, verify_case
+from test_gpu_drafts import check_verify, random_tree, verify_case
 from test_gpu_kv4 import up  # noqa: F401 (a fixture)
 
 pytestmark = pytest.mark.gpu
@@ -54,3 +54,22 @@ def test_verify_of_offsets_that_do_not_ascend(device, up, off, hot):  # noqa: F8
         run_verify(device, up, before, tokens, [0, rows], parents, accept, draws[:1], heat[:1] if hot else None, rows)
         for x, y, name in zip(run_verify(device, up, logits, tokens, off, parents, accept, draws, heat, rows), want, ("path", "counts", "next")):
             np.testing.assert_array_equal(x, y, err_msg=name)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("temperature", [2.0 ** 120, 2.0 ** 121, 1e37, 1e38, 3.4e38])
+def test_verify_temperatures_next_to_the_largest(device, up, temperature, kind):  # noqa: F811
+    """Logits of both signs next to f32's largest: their differences pass it, and at such a temperature still count."""
+    vocab, rows = 5000, 4
+    for top, rest in ((3.38e38, -3.38e38), (3.38e38, -np.inf), (3.38e38, 0.0)):
+        x = np.full((rows, vocab), rest, np.float32)
+        x[:, 3:9] = (np.linspace(0.9, 1.0, 6) * top).astype(np.float32)
+        x[:, 4100:4105] = -top
+        x[:, 20] = 1.0
+        for accept in (0.004, 0.02, 0.1, 0.3, 0.6):
+            for draw in (0.05, 0.95):
+                check_verify(device, up, x, [0, 8, 7, 4102], [rows], None, None, np.full(rows, accept), [draw], [temperature], kind)
+                check_verify(device, up, x, [0, 8, 20, 4102], [rows], np.array([9, 0, 0, 0], np.uint32), None, np.full(rows, accept), [draw],
+                             [temperature], kind)
+        q = np.full((rows, vocab), 1.0 / vocab, np.float32)
+        check_verify(device, up, x, [0, 8, 7, 4102], [rows], None, q, np.full(rows, 0.9), [0.4], [temperature], kind)
