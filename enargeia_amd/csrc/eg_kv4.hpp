@@ -33,10 +33,29 @@ struct Pool {
   }
 };
 
-// Whether `n` words (32 bits) from a on and `m` from b on have one in common.
-inline bool share_words(const void* a, uint64_t n, const void* b, uint64_t m) {
-  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-  return a && b && x < y + 4 * m && y < x + 4 * n;
+// Memory as a call names it: `rows` of `width` bytes, `step` bytes apart (at least `width`).
+struct Extent {
+  const void* at;
+  uint64_t rows, step, width;
+};
+inline Extent words(const void* at, uint64_t n) { return Extent{at, 1, 4 * n, 4 * n}; }  // of 32 bits
+
+// Whether two have a byte in common. (Rows may lie between the other's: q and k of one projection.)
+inline bool overlap(const Extent& a, const Extent& b) {
+  if (!a.at || !b.at || a.rows * a.width == 0 || b.rows * b.width == 0) return false;
+  const uint64_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
+  if (x >= y + (b.rows - 1) * b.step + b.width || y >= x + (a.rows - 1) * a.step + a.width) return false;
+  // A row of e bytes at p, and the first row of those from z on that ends behind p.
+  const auto meets = [](uint64_t p, uint64_t e, uint64_t z, const Extent& o) {
+    const uint64_t i = p < z + o.width ? 0 : (p - z - o.width) / o.step + 1;
+    return i < o.rows && z + i * o.step < p + e;
+  };
+  if (a.step == b.step) return meets(x, a.width, y, b) || meets(y, b.width, x, a);  // (rows meet as the one's first and one of the other's)
+  const bool fewer = a.rows <= b.rows;
+  const Extent &few = fewer ? a : b, &many = fewer ? b : a;
+  for (uint64_t i = 0; i < few.rows; i++)
+    if (meets((fewer ? x : y) + i * few.step, few.width, fewer ? y : x, many)) return true;
+  return false;
 }
 
 inline uint32_t log2_of(uint32_t v) { return 31u - (uint32_t)__builtin_clz(v); }

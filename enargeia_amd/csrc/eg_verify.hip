@@ -608,14 +608,17 @@ extern "C" int eg_verify_drafts(eg_context* ctx, const void* logits, const uint3
     return eg::fail(ctx, EG_ERR_RANGE, "%s: %u sequences, %u rows of %u ids over the workspace or the grid limit", op, d.sequences,
                     d.rows, d.vocab);
   const uint64_t n = d.sequences;  // (a sequence's workgroups read its inputs at any time)
-  const struct {
-    const void* at;
-    uint64_t words;
-  } outputs[] = {{path, n * d.max_rows}, {counts, n}, {next, n}},
-    inputs[] = {{tokens, d.rows}, {offsets, n + 1}, {parents, d.rows}, {accept, d.rows}, {draws, n}, {temperatures, n}};
-  for (const auto& x : outputs)
-    for (const auto& y : inputs)
-      if (share_words(x.at, x.words, y.at, y.words)) return eg::fail(ctx, EG_ERR_INVALID, "%s: an output lies in an input", op);
+  const uint64_t size = d.type == EG_ELEMENT_F32 ? 4 : 2;
+  const Extent outputs[] = {words(path, n * d.max_rows), words(counts, n), words(next, n)};
+  const Extent inputs[] = {words(tokens, d.rows), words(offsets, n + 1), words(parents, d.rows), words(accept, d.rows),
+                           words(draws, n), words(temperatures, n), {logits, d.rows, size * a.stride, size * d.vocab},
+                           {draft, d.rows, 4 * a.draft_stride, 4ull * d.vocab}};
+  for (const Extent& out : outputs) {
+    for (const Extent& in : inputs)
+      if (overlap(out, in)) return eg::fail(ctx, EG_ERR_INVALID, "%s: an output lies in an input", op);
+    for (const Extent& other : outputs)
+      if (&out != &other && overlap(out, other)) return eg::fail(ctx, EG_ERR_INVALID, "%s: an output lies in another", op);
+  }
   a.logits = logits;
   a.tokens = tokens;
   a.offsets = offsets;

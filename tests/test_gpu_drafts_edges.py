@@ -4,9 +4,10 @@ import numpy as np
 import pytest
 
 from drafts_reference import NO_ROW, verify
-from enargeia_amd import drafts
+from enargeia_amd import _lib, drafts
+from enargeia_amd import kernels as K
 from test_gpu_drafts import check_verify, random_tree, verify_case
-from test_gpu_kv4 import up  # noqa: F401 (a fixture)
+from test_gpu_kv4 import kv4_size, up  # noqa: F401 (a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -73,3 +74,38 @@ def test_verify_temperatures_next_to_the_largest(device, up, temperature, kind):
                              [temperature], kind)
         q = np.full((rows, vocab), 1.0 / vocab, np.float32)
         check_verify(device, up, x, [0, 8, 7, 4102], [rows], None, q, np.full(rows, 0.9), [0.4], [temperature], kind)
+
+
+# ---- outputs that overlap -----------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_verify_outputs_in_the_logits_the_draft_or_each_other_are_refused(device, up, kind):  # noqa: F811
+    """To the first and last word of them; what lies between their rows, or next to them, is no part of them."""
+    rows, vocab, stride, size = 4, 10, 16, kv4_size(kind)
+    logits, draft = up(np.zeros((rows, stride * size), np.uint8)), up(np.zeros((rows, stride), np.float32))
+    words = lambda n: up(np.zeros(n, np.uint32))  # noqa: E731
+    tokens, offsets, numbers, b = words(rows), up(np.array([0, 2, 4], np.uint32)), up(np.zeros(rows, np.float32)), words(64)
+
+    def check(path=0, counts=64, token=128):
+        a = [x if not isinstance(x, int) else K.Binding(b, x) for x in (path, counts, token)]
+        drafts.verify(device, logits, tokens, offsets, *a, draft=draft, accept=numbers, draws=numbers, temperatures=numbers,
+                      sequences=2, rows=rows, max_rows=3, vocab=vocab, type=kind, logits_stride=stride, draft_stride=stride)
+
+    row, end = stride * size, vocab * size
+    for at in (0, row + end - 4, 3 * row + end - 4):
+        for name in ("path", "counts", "token"):
+            with pytest.raises(_lib.EgError, match="an output lies in an input"):
+                check(**{name: K.Binding(logits, at)})
+    for at in (0, stride * 4 + 36, 3 * stride * 4 + 36):
+        for name in ("path", "counts", "token"):
+            with pytest.raises(_lib.EgError, match="an output lies in an input"):
+                check(**{name: K.Binding(draft, at)})
+    check(token=K.Binding(draft, 40), counts=K.Binding(logits, row + end))
+    check(path=K.Binding(draft, 40))  # (24 bytes: the whole of what lies between two rows)
+    for at in (dict(counts=0), dict(counts=20), dict(token=64), dict(token=68), dict(token=60), dict(path=44, counts=64), dict(path=108, token=128)):
+        with pytest.raises(_lib.EgError, match="an output lies in another"):
+            check(**at)
+    check(path=0, counts=24, token=32)
+    check(path=16, counts=0, token=8)
+    device.sync()
