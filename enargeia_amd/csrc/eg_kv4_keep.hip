@@ -145,9 +145,13 @@ extern "C" int eg_kv4_keep_rows(eg_context* ctx, const uint32_t* path, const uin
     return eg::fail(ctx, EG_ERR_INVALID, "%s: NULL argument", op);
   if (dims->sequences == 0) return EG_OK;
   const uint64_t n = dims->sequences;  // (a sequence's workgroups read its length at any time)
-  const Extent made = words(new_lengths, n);
-  for (const Extent& in : {words(lengths, n), words(counts, n), words(offsets, n + 1), words(path, n * max_rows)})
+  const Extent made = words(new_lengths, n), held{pool, dims->pages, dims->page_stride, layers * layer_bytes};
+  for (const Extent& in : {words(lengths, n), words(counts, n), words(offsets, n + 1), words(path, n * max_rows),
+                           words(table, n * dims->max_pages)}) {
     if (overlap(made, in)) return eg::fail(ctx, EG_ERR_INVALID, "%s: new_lengths lie in an input", op);
+    if (overlap(held, in)) return eg::fail(ctx, EG_ERR_INVALID, "%s: an input lies in the pool", op);
+  }
+  if (overlap(made, held)) return eg::fail(ctx, EG_ERR_INVALID, "%s: new_lengths lie in the pool", op);
   // A pair a wave, more where that would be more waves than the device holds at once.
   const uint64_t pairs = (uint64_t)layers * dims->kv_heads, room = (uint64_t)ctx->cu_count * 32;
   const uint64_t each = std::max<uint64_t>(1, pairs * dims->sequences / room), waves = (pairs + each - 1) / each;

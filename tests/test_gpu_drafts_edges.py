@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 from drafts_reference import NO_ROW, verify
-from enargeia_amd import _lib, drafts
+from enargeia_amd import _lib, drafts, kv4
 from enargeia_amd import kernels as K
 from test_gpu_drafts import check_verify, random_tree, verify_case
 from test_gpu_kv4 import kv4_size, up  # noqa: F401 (a fixture)
@@ -108,4 +108,32 @@ def test_verify_outputs_in_the_logits_the_draft_or_each_other_are_refused(device
             check(**at)
     check(path=0, counts=24, token=32)
     check(path=16, counts=0, token=8)
+    device.sync()
+
+
+def test_keep_of_lengths_in_the_table_or_the_pool_is_refused(device, up):  # noqa: F811
+    """A new length written over a page id would send another workgroup's rows to a wrong page."""
+    words = lambda n: up(np.zeros(n, np.uint32))  # noqa: E731
+    kv, d, page, pages, layers, seqs = 1, 64, 32, 3, 2, 3
+    size = kv4.page_bytes(kv, d, page) * layers
+    pool, table = up(np.zeros(pages * (size + 64), np.uint8)), up(np.zeros((seqs, 2), np.uint32))
+    cache = kv4.Kv4Cache(device, kv, d, pages, page, layers=layers, pool=pool)
+    cache.dims.page_stride = size + 64  # (64 bytes of no page behind each)
+    ok = dict(path=words(12), counts=words(seqs), offsets=words(seqs + 1), lengths=words(seqs), table=table, new=words(seqs))
+
+    def kept(**c):
+        a = {**ok, **c}
+        cache.keep(a["path"], a["counts"], a["offsets"], a["lengths"], a["table"], a["new"], max_rows=4, sequences=seqs, max_pages=2)
+
+    for at in (0, 20):
+        with pytest.raises(_lib.EgError, match="new_lengths lie in an input"):
+            kept(new=K.Binding(table, at))
+    for at in (0, size - 4, size + 64, 3 * (size + 64) - 68):
+        with pytest.raises(_lib.EgError, match="new_lengths lie in the pool"):
+            kept(new=K.Binding(pool, at))
+        for name in ("path", "counts", "offsets", "lengths", "table"):
+            with pytest.raises(_lib.EgError, match="an input lies in the pool"):
+                kept(**{name: K.Binding(pool, at)})
+    kept(new=K.Binding(pool, size), lengths=K.Binding(pool, 2 * size + 64))  # (between pages)
+    kept()
     device.sync()
