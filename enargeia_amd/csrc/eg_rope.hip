@@ -292,6 +292,20 @@ int eg_rope(eg_context* ctx, const void* q, const void* k, const float* table, c
   if (!some || (d.heads == 0 && d.kv_heads == 0)) return EG_OK;
   if (d.rows >= (1u << 31) / kThreads)
     return eg::fail(ctx, EG_ERR_RANGE, "%s: %u rows over the grid limit", op, d.rows);
+  // An output is its input, row by row, or apart from all that other workgroups read and write.
+  const auto rows_of = [&](const void* at, uint32_t stride, uint32_t row, int type) {
+    const uint64_t size = type == EG_ELEMENT_F32 ? 4 : 2;
+    return Extent{at, d.rows, size * stride, size * row};
+  };
+  const Extent outputs[] = {rows_of(q_out, a.q_out_stride, width, d.out_type), rows_of(k_out, a.k_out_stride, kv_width, d.out_type)};
+  const Extent inputs[] = {rows_of(q, a.q_stride, width, d.in_type), rows_of(k, a.k_stride, kv_width, d.in_type),
+                           words(table, (uint64_t)d.table_positions * rotary), words(positions, d.rows),
+                           words(offsets, (uint64_t)d.sequences + 1), words(starts, d.sequences)};
+  for (int o = 0; o < 2; o++)
+    for (int i = 0; i < 6; i++)
+      if (!(i == o && outputs[o].at == inputs[i].at) && overlap(outputs[o], inputs[i]))
+        return eg::fail(ctx, EG_ERR_INVALID, "%s: an output lies in an input (it may be its own, row by row)", op);
+  if (overlap(outputs[0], outputs[1])) return eg::fail(ctx, EG_ERR_INVALID, "%s: q_out and k_out overlap", op);
   const OnDevice on(ctx);
   with_type(d.in_type, [&](auto ti) {
     with_type(d.out_type, [&](auto to) {

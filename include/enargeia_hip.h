@@ -671,7 +671,7 @@ EG_API int eg_rope_table(eg_context* ctx, float* table, const eg_rope_table_dims
  * head are rotated, in pairs (i, i + rotary_dim / 2) or (2 i, 2 i + 1), the others pass as they are. Rows outside
  * the sequences, and of a position that the table does not reach, are skipped: nothing is written. q, q_out and
  * heads go together, as do k, k_out and kv_heads; either may be absent. An output may be its input, of the same type
- * and stride. Rows are 16-byte aligned. */
+ * and stride; else outputs overlap neither inputs nor each other. Rows are 16-byte aligned. */
 typedef enum eg_rope_layout { EG_ROPE_HALF = 0, EG_ROPE_INTERLEAVED = 1 } eg_rope_layout;
 typedef struct eg_rope_dims {
   uint32_t rows, heads, kv_heads;
@@ -716,7 +716,8 @@ EG_API int eg_attention_tree_kv4(eg_context* ctx, const void* q, const uint32_t*
  * path [sequences][max_rows]: the accepted rows, counted from the sequence's first, then 0xFFFFFFFF; counts
  * [sequences]: how many, the root among them; next [sequences]. A sequence of no rows, or of more than max_rows, has
  * a count of 0 and 0xFFFFFFFF for the rest. logits are [rows][vocab] of `type`, draft f32 [rows][vocab]. accept
- * (per row) and draws (per sequence), in [0, 1), may be NULL without temperatures. No output lies in an input. */
+ * (per row) and draws (per sequence), in [0, 1), may be NULL without temperatures. Outputs overlap neither inputs nor each
+ * other. */
 typedef struct eg_verify_dims {
   uint32_t sequences, rows, max_rows; /* max_rows to 64                                           */
   uint32_t vocab;                     /* 1 to 2^20                                                */
@@ -734,7 +735,7 @@ EG_API int eg_verify_drafts(eg_context* ctx, const void* logits, const uint32_t*
  * written. Positions from there on keep what they held, or what lay there before. The pool is that of layer 0, and a page
  * holds `layers` layers. Entries of path that are not below n, and rows that come from or go to no page, are not
  * moved; a count past n is n. A sequence of fewer positions than rows, or of more than max_rows rows, stays as it is.
- * The pages that rows go to are one sequence's alone; new_lengths are apart from the inputs. */
+ * The pages that rows go to are one sequence's alone; new_lengths and the pool are apart from the inputs and from each other. */
 EG_API int eg_kv4_keep_rows(eg_context* ctx, const uint32_t* path, const uint32_t* counts, const uint32_t* offsets,
                             const uint32_t* lengths, const uint32_t* table, void* pool, uint32_t* new_lengths,
                             const eg_kv4_dims* dims, uint32_t layers, uint32_t max_rows);

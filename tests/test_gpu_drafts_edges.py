@@ -137,3 +137,39 @@ def test_keep_of_lengths_in_the_table_or_the_pool_is_refused(device, up):  # noq
     kept(new=K.Binding(pool, size), lengths=K.Binding(pool, 2 * size + 64))  # (between pages)
     kept()
     device.sync()
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_rope_outputs_that_overlap_are_refused(device, up, layout):  # noqa: F811
+    """An output that is its input, or lies between the rows of others, is taken; any other overlap is a race of workgroups."""
+    rows, heads, kv, d = 5, 3, 2, 64
+    wide = (heads + 2 * kv) * d  # q, k and v side by side
+    b, far = up(np.zeros((rows + 3, wide), np.float32)), up(np.zeros((rows + 3, wide), np.float32))
+    table, words = up(np.zeros((8, d), np.float32)), up(np.zeros(64, np.uint32))
+    at = lambda row, head=0, of=b: K.Binding(of, (row * wide + head * d) * 4)  # noqa: E731
+    ok = dict(rows=rows, head_dim=d, table_positions=8, q=at(0), heads=heads, k=at(0, heads), kv_heads=kv, positions=K.Binding(words, 0),
+              offsets=K.Binding(words, 32), starts=K.Binding(words, 48), sequences=2, layout=layout, q_stride=wide, k_stride=wide,
+              q_out_stride=wide, k_out_stride=wide)
+
+    def turn(q_out, k_out, **c):
+        drafts.rope(device, table, **{**ok, "q_out": q_out, "k_out": k_out, **c})
+
+    turn(at(0), at(0, heads))  # in place
+    turn(at(0, 0, far), at(0, heads, far))
+    turn(at(0), at(0, heads + kv))  # k's rows over v's
+    for q_out, k_out in ((at(1), at(0, heads)), (at(0, 1), at(0, 5)), (at(0, heads + kv), at(0, heads)), (at(0, 0, far), at(0, heads - 1)),
+                         (at(0, 0, far), at(0, heads + 1)), (at(0, 0, far), at(2, heads)), (at(0, heads), at(0, 0, far)),
+                         (at(0, 0, far), at(0)), (table, at(0, 0, far))):
+        with pytest.raises(_lib.EgError, match="an output lies in an input"):
+            turn(q_out, k_out)
+    for offset, where in ((0, "positions"), (16, "positions"), (32, "offsets"), (48, "starts")):
+        assert where in ok
+        with pytest.raises(_lib.EgError, match="an output lies in an input"):
+            turn(at(0, 0, far), K.Binding(words, offset))
+    for k_out in (at(0, 2, far), at(0, 0, far), at(rows - 1, 1, far), at(1, 0, far)):
+        with pytest.raises(_lib.EgError, match="q_out and k_out overlap"):
+            turn(at(0, 0, far), k_out)
+    with pytest.raises(_lib.EgError, match="an output lies in an input"):  # rows of another step
+        turn(at(1), at(0, heads, far), q_out_stride=heads * d)
+    turn(at(rows), at(0, heads, far), q_out_stride=heads * d)  # behind the rows of q and k
+    device.sync()
