@@ -913,6 +913,15 @@ extern "C" int eg_attention_tree_kv4(eg_context* ctx, const void* q, const uint3
   if (tiles * splits >= (1ull << 31) / kThreads || (uint64_t)d.rows * d.heads >= (1ull << 31) / kThreads)
     return eg::fail(ctx, EG_ERR_RANGE, "%s: %u rows of %u heads in %u sequences over the grid limit", op, d.rows, d.heads,
                     dims->sequences);
+  // A workgroup writes the columns that it alone uses, after their queries are read: the result may take q's place, row by row. What the
+  // others read of all else it would overwrite.
+  const uint64_t size = d.type == EG_ELEMENT_F32 ? 4 : 2, n = dims->sequences;
+  const Extent result{out, d.rows, size * a.out_stride, size * width}, queries{q, d.rows, size * a.q_stride, size * width};
+  bool apart = (q == out && a.q_stride == a.out_stride) || !overlap(result, queries);
+  for (const Extent& in : {words(offsets, n + 1), words(parents, d.rows), words(lengths, n), words(table, n * dims->max_pages),
+                           Extent{pool, dims->pages, dims->page_stride, eg_kv4::page_bytes(*dims)}})
+    apart = apart && !overlap(result, in);
+  if (!apart) return eg::fail(ctx, EG_ERR_INVALID, "%s: out lies in an input (it may be q, row by row)", op);
   a.ml = reinterpret_cast<float*>(eg::partials(ctx));
   a.o = a.ml + (((size_t)d.rows * d.heads * splits * 2 + 3) & ~(size_t)3);
   const Pool p = eg_kv4::pool_of(*dims, pool, table);

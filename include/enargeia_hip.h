@@ -688,7 +688,8 @@ EG_API int eg_rope(eg_context* ctx, const void* q, const void* k, const float* t
  * It sees the positions before lengths[s] - n, its ancestors and itself (not what is behind the table or on no
  * page): softmax and values as eg_attention_decode_kv4, which is the case of one row. A row that sees nothing
  * gives zeros; so do the rows of a sequence with fewer positions than rows. Rows outside the sequences, and those
- * of a sequence of more than max_rows rows, are not written. q and out are [rows][heads][head_dim] of `type`. */
+ * of a sequence of more than max_rows rows, are not written. q and out are [rows][heads][head_dim] of `type`.out may be
+ * q, of the same stride. */
 typedef struct eg_attention_tree_dims {
   uint32_t rows, max_rows;       /* rows of q and out; the most of a sequence, to 64              */
   uint32_t heads;

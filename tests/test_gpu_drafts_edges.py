@@ -6,8 +6,9 @@ import pytest
 from drafts_reference import NO_ROW, verify
 from enargeia_amd import _lib, drafts, kv4
 from enargeia_amd import kernels as K
+from kv4_reference import as_type, random_pages
 from test_gpu_drafts import check_verify, random_tree, verify_case
-from test_gpu_kv4 import kv4_size, up  # noqa: F401 (a fixture)
+from test_gpu_kv4 import kv4_size, offsets_of, up  # noqa: F401 (a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -173,3 +174,46 @@ def test_rope_outputs_that_overlap_are_refused(device, up, layout):  # noqa: F81
         turn(at(1), at(0, heads, far), q_out_stride=heads * d)
     turn(at(rows), at(0, heads, far), q_out_stride=heads * d)  # behind the rows of q and k
     device.sync()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("heads,kv,ns,lengths", [(4, 1, [5, 3], [40, 31]), (4, 1, [9], [3000]), (64, 8, [16] * 36, [90] * 36), (64, 8, [32] * 32, [140] * 32),
+                                                 (64, 8, [8] * 36, [70] * 36)])
+def test_tree_in_place(device, up, heads, kv, ns, lengths, kind):  # noqa: F811
+    """The result in q's place, gaps between rows among it: the bits that it has elsewhere."""
+    rng = np.random.default_rng(heads + len(ns))
+    d, page, pad, seqs, rows = 64, 32, 16, len(ns), sum(ns)
+    pages = -(-max(lengths) // page)
+    P, _, _ = random_pages(rng, pages, kv, d, page)
+    table = np.tile(rng.permutation(pages).astype(np.uint32), (seqs, 1))
+    raw, _ = as_type(rng.standard_normal((rows, heads * d + pad)).astype(np.float32), kind)
+    cache = kv4.Kv4Cache(device, kv, d, pages, page, pool=up(P.pool))
+    q, own = up(raw), up(raw)
+    ins = [up(x) for x in (offsets_of(ns), np.array(lengths, np.uint32), table)]
+    for out in (own, q):
+        cache.attend_tree(q, *ins, out, parents=up(np.concatenate([random_tree(np.random.default_rng(n), n) for n in ns])), heads=heads, rows=rows,
+                          max_rows=max(ns), sequences=seqs, max_pages=pages, type=kind, q_stride=heads * d + pad, out_stride=heads * d + pad)
+    a, b = (device.read_array(x, np.uint8, raw.nbytes) for x in (own, q))
+    np.testing.assert_array_equal(a, b)
+
+
+def test_tree_results_that_lie_in_an_input_are_refused(device, up):  # noqa: F811
+    kv, d, page, pages, heads, rows = 1, 64, 32, 3, 2, 6
+    size = kv4.page_bytes(kv, d, page)
+    cache = kv4.Kv4Cache(device, kv, d, pages, page, pool=up(pages * size))
+    b, words = up(np.zeros((2 * rows + 1, heads * d), np.float32)), up(np.zeros(64, np.uint32))
+    row = 4 * heads * d
+    ins = [K.Binding(words, 64 * i) for i in range(4)]  # offsets, lengths, table, parents
+
+    def attend(out, **c):
+        cache.attend_tree(b, *ins[:3], out, parents=ins[3], **{**dict(heads=heads, rows=rows, max_rows=6, sequences=2, max_pages=2), **c})
+
+    for out in (K.Binding(b, row), K.Binding(b, 16), K.Binding(b, 5 * row), *ins, cache.pool, K.Binding(cache.pool, pages * size - 16)):
+        with pytest.raises(_lib.EgError, match="out lies in an input"):
+            attend(out)
+    with pytest.raises(_lib.EgError, match="out lies in an input"):  # of another step
+        attend(b, out_stride=heads * d + 8)
+    attend(b)
+    attend(K.Binding(b, 6 * row))
+    device.sync()
+    cache.release()
