@@ -1,14 +1,16 @@
-"""The operators of a speculative step at the ends of their ranges. The definitions (drafts_reference.py) are test_gpu_drafts.py's."""
+"""The operators of a speculative step at the ends of their ranges: sizes past a workgroup's first turn of each loop, offsets that
+do not ascend, temperatures next to f32's largest, scores past 2^20, memory behind the outputs, and outputs that overlap. The definitions
+(drafts_reference.py) and their bounds are test_gpu_drafts.py's."""
 
 import numpy as np
 import pytest
 
-from drafts_reference import NO_ROW, verify
+from drafts_reference import NO_ROW, keep, tree_attend, verify, verify_all
 from enargeia_amd import _lib, drafts, kv4
 from enargeia_amd import kernels as K
-from kv4_reference import as_type, random_pages
-from test_gpu_drafts import check_verify, random_tree, verify_case
-from test_gpu_kv4 import kv4_size, offsets_of, up  # noqa: F401 (a fixture)
+from kv4_reference import Pages, as_type, from_type, random_pages
+from test_gpu_drafts import check_rope, check_verify, random_tree, verify_case
+from test_gpu_kv4 import decode_bound, kv4_size, offsets_of, tables, up  # noqa: F401 (a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -75,6 +77,146 @@ def test_verify_temperatures_next_to_the_largest(device, up, temperature, kind):
                              [temperature], kind)
         q = np.full((rows, vocab), 1.0 / vocab, np.float32)
         check_verify(device, up, x, [0, 8, 7, 4102], [rows], None, q, np.full(rows, 0.9), [0.4], [temperature], kind)
+
+
+@pytest.mark.parametrize("how", ["chain", "tree", "draft"])
+@pytest.mark.parametrize("chunks,seqs", [(7, 620), (11, 760)])
+def test_verify_of_more_chunks_than_a_workgroup_takes_at_once(device, up, chunks, seqs, how):  # noqa: F811
+    """More than 16 and 32 chunks a CU: a workgroup draws from 8 and 12, four at a time, the last of them partial."""
+    rng = np.random.default_rng(chunks + len(how))
+    vocab = 4096 * chunks - 700
+    ns = [1 + (i % 7 == 3) for i in range(seqs)]
+    x, tokens, parents, draft = verify_case(rng, ns, vocab, how != "tree", how == "draft")
+    t = np.where(rng.random(seqs) < 0.95, rng.uniform(0.5, 1.5, seqs), 0.0)
+    check_verify(device, up, x, tokens, ns, parents, draft, rng.random(sum(ns)), rng.random(seqs), t)
+
+
+@pytest.mark.parametrize("hot", [False, True])
+def test_verify_writes_its_outputs_alone(device, up, hot):  # noqa: F811
+    """Words behind path, counts and next stay, whether sequences are computed or not."""
+    rng = np.random.default_rng(43)
+    ns, width = [5, 0, 9, 2, 1], 5
+    x, tokens, parents, _ = verify_case(rng, ns, 5000, False, False)
+    s, rows, off = len(ns), sum(ns), offsets_of(ns)
+    sizes = (s * width, s, s)
+    outs = [up(np.full(n + 80, 0xA5A5A5A5, np.uint32)) for n in sizes]
+    accept, draws, heat = (rng.random(n).astype(np.float32) for n in (rows, s, s))
+    heat = heat + np.float32(0.5) if hot else None
+    drafts.verify(device, up(x), up(np.asarray(tokens, np.uint32)), up(off), *outs, parents=up(parents), accept=up(accept), draws=up(draws),
+                  temperatures=up(heat) if hot else None, sequences=s, rows=rows, max_rows=width, vocab=5000)
+    want = verify_all(x, tokens, off, parents, None, accept, draws, heat, width)
+    for b, n, w in zip(outs, sizes, want):
+        got = device.read_array(b, np.uint32, n + 80)
+        np.testing.assert_array_equal(got[:n].reshape(w.shape), w)
+        assert np.all(got[n:] == 0xA5A5A5A5)
+
+
+# ---- rotary positions and kept rows -------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("heads,kv,rotary", [(32, 8, 128), (32, 8, 64), (40, 8, 128), (40, 8, 64), (40, 8, 40)])
+def test_rope_of_rows_longer_than_a_workgroups_turn(device, up, layout, heads, kv, rotary):  # noqa: F811
+    rng = np.random.default_rng(heads + rotary)
+    for kinds in (("f32", "f32"), ("f16", "f32"), ("bf16", "bf16"), ("f32", "f16")):
+        check_rope(device, up, rng, [3, 0, 6], [7, 9, 30], None, heads, kv, 128, rotary, layout, *kinds, before=1, after=2)
+        if kinds[0] == kinds[1]:
+            check_rope(device, up, rng, [5], [11], None, heads, kv, 128, rotary, layout, *kinds, in_place=True, pad=8)
+
+
+@pytest.mark.parametrize("kv,d,layers,seqs", [(5, 64, 33, 110), (4, 128, 64, 100)])
+def test_keep_of_several_heads_a_wave(device, up, kv, d, layers, seqs):  # noqa: F811
+    """More (layer, kv head, sequence) than waves the device holds: two and three of a wave's, which do not divide them."""
+    rng = np.random.default_rng(kv)
+    page, most = 32, 4
+    ns = [int(n) for n in rng.integers(1, most + 1, seqs)]
+    lengths = [n + int(x) for n, x in zip(ns, rng.integers(0, 40, seqs))]
+    width = max(-(-n // page) for n in lengths)
+    pages = sum(-(-n // page) for n in lengths)
+    table = tables(rng, lengths, page, pages, width)
+    P = [Pages(pages, kv, d, page) for _ in range(layers)]
+    for p in P:
+        p.pool[:] = rng.integers(0, 256, p.pool.shape, dtype=np.uint8)
+    pool = up(np.concatenate([p.pool for p in P], 1))
+    path, counts = np.full((seqs, most), NO_ROW, np.uint32), np.zeros(seqs, np.uint32)
+    for i, n in enumerate(ns):
+        chosen = np.flatnonzero(rng.random(n) < 0.6)
+        path[i, : len(chosen)], counts[i] = chosen, len(chosen)
+    cache = kv4.Kv4Cache(device, kv, d, pages, page, layers=layers, pool=pool)
+    new = up(4 * seqs)
+    cache.keep(up(path), up(counts), up(offsets_of(ns)), up(np.array(lengths, np.uint32)), up(table), new, max_rows=most, sequences=seqs,
+               max_pages=width)
+    for p in P:
+        want = keep(p, table, path, counts, ns, lengths, page)
+    np.testing.assert_array_equal(device.read_array(new, np.uint32, seqs), want)
+    np.testing.assert_array_equal(device.read_array(pool, np.uint8, pages * layers * P[0].bytes).reshape(pages, -1),
+                                  np.concatenate([p.pool for p in P], 1))
+
+
+# ---- the tree attention -------------------------------------------------------------------------------
+
+
+def far_scores(rng, pages, kv, d, page):
+    """A pool whose keys are 4 in dim 0, a whole number from -7 to 7 in dim 32 and 0 elsewhere; keys and values."""
+    P, _, v = random_pages(rng, pages, kv, d, page)
+    k = np.zeros((pages, page, kv, d))
+    k[..., 0], k[..., 32] = 4, rng.integers(-7, 8, (pages, page, kv))
+    for p in range(pages):
+        for h in range(kv):
+            kw, _, ks, _ = P._streams(p, h)
+            ks[:] = 1
+            kw[:] = 0x88888888
+            kw[:, 0, 0] = 0x8888888C
+            kw[:, 0, 1] = 0x88888880 + (k[p, :, h, 32] + 8).astype(np.uint32)
+    return P, k, v
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("heads,kv,ns,most", [(4, 1, [5, 1], 32), (4, 2, [16, 9], 300), (64, 8, [8] * 36, 200), (64, 8, [16] * 36, 200),
+                                              (64, 8, [40] * 36, 130), (64, 8, [32] * 32, 200)])
+def test_tree_of_scores_past_2_to_20(device, up, heads, kv, ns, most, d, kind):  # noqa: F811
+    """Scores of +-2^20 and half numbers up to 3.5 beside them, in heads between ordinary ones: what the largest part adds to all of a
+    head's is the same, so the outputs are those of queries without it. Every product and sum of a score is exact (23 bits at most), and
+    so is a score less the largest one; what is left is the ordinary bound of the rest. Where a head's positions meet by the waves'
+    maxima in f32 (few columns, more than a wave's 32 positions) each of the two maxima, of 1.5 x 2^20 in powers of two, is rounded by up
+    to 2^-4, so shares of the weights are off by factors from 2^(-1/8) to 2^(1/8), and an output by up to 2^(1/4) - 1 of the largest value. Weights of 16-bit rows are scaled by 2^12 at least, of which half a step of
+    f16's smallest numbers is 2^-37."""
+    rng = np.random.default_rng(len(ns) * most + d)
+    page, seqs, group = 32, len(ns), heads // kv
+    lengths = [max(n, most - 7 * (i % 9)) for i, n in enumerate(ns)]
+    width = -(-max(lengths) // page) + 12
+    pages = max(-(-n // page) for n in lengths)
+    P, kk, vv = far_scores(rng, pages, kv, d, page)
+    order = rng.permutation(pages).astype(np.uint32)
+    table = np.full((seqs, width), 0xFFFFFFFF, np.uint32)
+    table[:, :pages] = order
+    kk, vv = (x[order].reshape(-1, kv, d) for x in (kk, vv))
+    parents = np.concatenate([random_tree(rng, n) for n in ns])
+    q = np.zeros((sum(ns), heads, d), np.float32)
+    q[..., 32] = 2.0 ** -4
+    far = np.arange(sum(ns))[:, None] + np.arange(heads) * 3
+    q[..., 0] = np.array([0.0, 2.0 ** 15, -2.0 ** 15], np.float32)[far % 3]
+    raw, val = as_type(q, kind)
+    np.testing.assert_array_equal(val, q)
+    out = up(raw.nbytes)
+    cache = kv4.Kv4Cache(device, kv, d, pages, page, pool=up(P.pool))
+    cache.attend_tree(up(raw), up(offsets_of(ns)), up(np.array(lengths, np.uint32)), up(table), out, parents=up(parents), heads=heads,
+                      rows=sum(ns), max_rows=max(ns), sequences=seqs, max_pages=width, type=kind, scale=8.0)
+    got = from_type(device.read(out, raw.nbytes), kind).reshape(q.shape)
+    meet = 2.0 ** 0.25 - 1 if max(ns) * group <= 64 and most > 32 else 0.0
+    off = offsets_of(ns)
+    near = val.copy()
+    near[..., 0] = 0.0
+    for s in range(0, seqs, 5):
+        r = slice(int(off[s]), int(off[s + 1]))
+        k, v = kk[: lengths[s]], vv[: lengths[s]]
+        want, seen = tree_attend(val[r], k, v, 8.0, parents[r], np.ones(lengths[s], bool))
+        for j in range(ns[s]):
+            bound = decode_bound(near[r][j], k, v, 8.0, seen[j], want[j], kind)
+            bound = bound + (seen[j].sum() * 2.0 ** -37 + meet) * np.abs(v).max() + (2.0 ** -25 if kind == "f16" else 0.0)
+            off_by = np.abs(got[r][j] - want[j])
+            assert np.all(off_by <= bound), (s, j, float(np.nanmax(off_by / bound)))
 
 
 # ---- outputs that overlap -----------------------------------------------------------------------------
