@@ -816,7 +816,8 @@ void launch(eg_context* ctx, const Args& a, const Pool& p, const Plan& plan, uin
 }
 
 // The kernel and the chunks of a sequence's positions: what the times below add up to least by. Lengths are on the device, so
-// it goes by what the tables reach less a page, whose last ones are seldom full. The times of a step of a workgroup alone on its
+// it goes by what the tables reach less a page, whose last ones are seldom full, and by a page at least (of no positions all kinds cost
+// the same: 32 and 64 sequences of 32 rows in a page of 256 each, 32 / 8 heads of 128, bf16, took 30.8 and 57.0 us for 14.6 and 21.5). The times of a step of a workgroup alone on its
 // CU and of one of several, in us, were measured with each kernel: at up to 4096 positions 32 sequences of 16 rows, 32 / 8
 // heads of 128, bf16, took 100 us in single blocks, 85 in fours and 76 with positions halved, 107 and 85 in eights; 64 of 16
 // / 4 heads of 64 54, 62 and 49, 81 and 63. Sixteens (256 columns) are set by what they gain on eights over sizes of the whole
@@ -904,8 +905,9 @@ extern "C" int eg_attention_tree_kv4(eg_context* ctx, const void* q, const uint3
   a.scale = (d.scale > 0.f ? d.scale : 1.0f / sqrtf((float)dims->head_dim)) * kLog2e;
   a.capacity = dims->max_pages * dims->page_size;
   const uint64_t pairs = (uint64_t)dims->sequences * dims->kv_heads, columns = (uint64_t)std::min(d.max_rows, d.rows) * a.group;
-  const Plan plan = plan_of(ctx->cu_count, pairs, columns, a.capacity - std::min(a.capacity, dims->page_size),
-                            (uint64_t)d.rows * d.heads, dims->head_dim, d.type == EG_ELEMENT_F32);
+  const uint32_t page = std::min(a.capacity, dims->page_size), reach = std::max(page, a.capacity - page);
+  const Plan plan = plan_of(ctx->cu_count, pairs, columns, reach, (uint64_t)d.rows * d.heads, dims->head_dim,
+                            d.type == EG_ELEMENT_F32);
   const uint64_t tiles = pairs * plan.tiles, splits = plan.splits;
   a.tiles = plan.tiles;
   a.splits = plan.splits;

@@ -9,7 +9,7 @@ from drafts_reference import NO_ROW, keep, tree_attend, verify, verify_all
 from enargeia_amd import _lib, drafts, kv4
 from enargeia_amd import kernels as K
 from kv4_reference import Pages, as_type, from_type, random_pages
-from test_gpu_drafts import check_rope, check_verify, random_tree, verify_case
+from test_gpu_drafts import check_rope, check_tree, check_verify, random_tree, verify_case
 from test_gpu_kv4 import decode_bound, kv4_size, offsets_of, tables, up  # noqa: F401 (a fixture)
 
 pytestmark = pytest.mark.gpu
@@ -217,6 +217,19 @@ def test_tree_of_scores_past_2_to_20(device, up, heads, kv, ns, most, d, kind): 
             bound = bound + (seen[j].sum() * 2.0 ** -37 + meet) * np.abs(v).max() + (2.0 ** -25 if kind == "f16" else 0.0)
             off_by = np.abs(got[r][j] - want[j])
             assert np.all(off_by <= bound), (s, j, float(np.nanmax(off_by / bound)))
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,kv,d,page,n,length,seqs", [(32, 8, 128, 256, 32, 256, 32), (32, 8, 128, 256, 13, 200, 33), (64, 8, 64, 256, 32, 255, 32),
+                                                           (64, 8, 64, 32, 16, 32, 36), (64, 8, 64, 32, 32, 64, 32), (14, 2, 64, 128, 16, 128, 16),
+                                                           (8, 8, 128, 256, 1, 512, 40), (4, 1, 64, 32, 3, 3, 1)])
+def test_tree_of_tables_as_wide_as_the_sequences(device, up, heads, kv, d, page, n, length, seqs, kind):  # noqa: F811
+    """Tables of one page and of two, with no entry to spare. 16-bit rows' weights are scaled by 2^12 at least, of which half a step
+    of f16's smallest numbers, 2^-25, is 2^-37."""
+    rng = np.random.default_rng(page + n)
+    ns = [n if i % 3 == 0 else int(rng.integers(1, n + 1)) for i in range(seqs)]
+    lengths = [length if i % 3 == 0 else int(rng.integers(max(k, length // 3), length + 1)) for i, k in enumerate(ns)]
+    check_tree(device, up, rng, ns, lengths, heads, kv, d, page, kind, extra=-1, floor=0.0 if kind == "f32" else 2.0 ** -37, step=4)
 
 
 # ---- outputs that overlap -----------------------------------------------------------------------------
