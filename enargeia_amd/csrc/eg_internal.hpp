@@ -722,7 +722,8 @@ __device__ __forceinline__ void drain() {
 
 // (a, b) rotated by (cos, sin) in double, each product rounded on its own - no fused multiply-add,
 // as a host evaluates a * cos - b * sin and b * cos + a * sin - then rounded to f32. Every RoPE
-// here goes through it, so a row rotated in any kernel is the same to the bit.
+// that makes its own angles (decode, prefill) goes through it, so a row rotated in any of those kernels
+// is the same to the bit; eg_kv4_append and eg_rope multiply in f32 by the table that they are given.
 __device__ __forceinline__ float2 rotate(double a, double b, double2 cs) {
 #pragma clang fp contract(off)
   return make_float2((float)(a * cs.x - b * cs.y), (float)(b * cs.x + a * cs.y));

@@ -344,7 +344,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void few_kernel(Args a, Pool pool) 
     }
   }
 
-  // The waves meet in LDS.
+  // The waves meet in LDS. (A lane's rows there are D floats apart, so the 16 columns' stores meet in the same banks: 1,536 cycles a
+  // workgroup, 60% of the kernel's LDS cycles with 16 sequences of 16 rows.)
   __shared__ float top_of[kWaves][16], sum_of[kWaves][16];
   __shared__ __attribute__((aligned(16))) float part_of[kWaves][16][D];
   const bool whole = chunk >= reach;  // no other chunk: the result itself
@@ -401,8 +402,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void few_kernel(Args a, Pool pool) 
 //
 // K lies as [8 dims][position], V as [8 positions][dim], so that a product's 16 rows are 16 consecutive operands of
 // 16 bytes; positions in the order of the first product's rows (row 16 k + 4 a + e of 32: position 8 a + kOrder[4 k + e]),
-// dims 4 q + j (2 q + j at head_dim 64) at 32 j + q, which is how a thread's words of neighbouring dims are
-// stored without bank conflicts.
+// dims 4 q + j (2 q + j at head_dim 64) at 32 j + q, so that V's stores follow each other. K's do
+// not: of eight lanes that store together two positions share two slots of four, and conflicts are 4.4 of the 13.2 million LDS
+// cycles of 8 sequences of 64 rows at up to 8192.
 //
 // kHalves 2, for up to 64 columns: two waves share 32 columns, each with half of a step's positions, and meet at the end. (Four
 // waves of 16 columns each read all of a step from LDS: 64 KB more a step, which is what bound them.)
@@ -816,14 +818,15 @@ void launch(eg_context* ctx, const Args& a, const Pool& p, const Plan& plan, uin
 }
 
 // The kernel and the chunks of a sequence's positions: what the times below add up to least by. Lengths are on the device, so
-// it goes by what the tables reach less a page, whose last ones are seldom full, and by a page at least (of no positions all kinds cost
-// the same: 32 and 64 sequences of 32 rows in a page of 256 each, 32 / 8 heads of 128, bf16, took 30.8 and 57.0 us for 14.6 and 21.5). The times of a step of a workgroup alone on its
-// CU and of one of several, in us, were measured with each kernel: at up to 4096 positions 32 sequences of 16 rows, 32 / 8
-// heads of 128, bf16, took 100 us in single blocks, 85 in fours and 76 with positions halved, 107 and 85 in eights; 64 of 16
-// / 4 heads of 64 54, 62 and 49, 81 and 63. Sixteens (256 columns) are set by what they gain on eights over sizes of the whole
-// range, whose sequences differ in length, which a workgroup alone on its CU has to wait for: of 32 rows of 64 / 8 heads they
-// take 149 us for 173 (128, bf16), 243 for 269 (f32), 100 for 116 and 168 for 176 (64). A launch, its chain of reads and the
-// waves' meeting take 6 us, a join 4.5 and its partials a us for 4 MB written and read.
+// it goes by what the tables reach less a page, whose last ones are seldom full, and by a page at least (of no positions all kinds
+// cost the same: 32 and 64 sequences of 32 rows in a page of 256 each, 32 / 8 heads of 128, bf16, took 30.8 and 57.0 us for 14.5
+// and 21.5). The times of a step of a workgroup alone on its CU and of one of several, in us: measured with each kernel of four
+// waves - at up to 4096 positions 32 sequences of 16 rows, 32 / 8 heads of 128, bf16, took 100 us in single blocks, 85 in fours
+// and 76 with positions halved, 107 and 85 in eights; 64 of 16 / 4 heads of 64 54, 62 and 49, 81 and 63. Of eight waves, fitted:
+// single blocks by two shared steps of four waves; sixteens (256 columns), alone or not, by what they gain on eights over sizes of
+// the whole range, whose sequences differ in length, which a workgroup alone on its CU has to wait for - of 32 rows of 64 / 8
+// heads they take 149 us for 173 (128, bf16), 243 for 269 (f32), 100 for 116 and 168 for 176 (64). A launch, its chain of reads
+// and the waves' meeting take 6 us, a join 4.5 and its partials a us for 4 MB written and read.
 Plan plan_of(uint32_t cus, uint64_t pairs, uint64_t columns, uint32_t reach, uint64_t outputs, uint32_t head_dim, bool f32) {
   struct Kind {
     uint32_t per_tile, waves, step;

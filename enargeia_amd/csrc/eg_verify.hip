@@ -5,7 +5,8 @@
 // bounds the operator. Which rows the branch goes through then takes single logits. The next token's running sum goes
 // over the branch's last row only: a workgroup per few chunks finds the branch by itself and sums its chunks (verify_walk),
 // and the chunk in which the running sum passes the target is read once more (verify_draw; by the last workgroup to
-// arrive instead of a launch of its own, both took 18.5 us for 9.2 and 4.9, 16 sequences, and 19.5 for 14.4 and 5.7, 48).
+// arrive instead of a launch of its own, both took 18.5 us for 9.2 and 4.9 with 16 sequences, and 19.5 for 14.4 and 5.7 with 48: one
+// form for both, the one that never loses much).
 //
 // What is decided is decided in f64: of 151,936 running sums some lie within f32's rounding of the drawn target in one draw
 // of a hundred, within these in none of 10^6. Exponentials in f64 are 15 f64 instructions, which over all rows take

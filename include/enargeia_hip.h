@@ -716,11 +716,12 @@ EG_API int eg_attention_tree_kv4(eg_context* ctx, const void* q, const uint32_t*
  * nothing, its next token as at 0. What is decided is what sums in 64 bits decide. Temperatures are finite.
  * path [sequences][max_rows]: the accepted rows, counted from the sequence's first, then 0xFFFFFFFF; counts
  * [sequences]: how many, the root among them; next [sequences]. A sequence of no rows, or of more than max_rows, has
- * a count of 0 and 0xFFFFFFFF for the rest. logits are [rows][vocab] of `type`, draft f32 [rows][vocab]. accept
+ * a count of 0 and 0xFFFFFFFF for the rest, as has one that ends past `rows`. logits are [rows][vocab] of `type`, draft f32 [rows][vocab]. accept
  * (per row) and draws (per sequence), in [0, 1), may be NULL without temperatures. Outputs overlap neither inputs nor each
  * other. */
 typedef struct eg_verify_dims {
-  uint32_t sequences, rows, max_rows; /* max_rows to 64                                           */
+  uint32_t sequences, rows, max_rows; /* to 65535, 65535 and 64; with chunks = vocab / 4096 rounded up: rows * chunks * 16 bytes,
+                                         and with temperatures sequences * (chunks * 8 + 40), within 64 MiB less 8 KiB */
   uint32_t vocab;                     /* 1 to 2^20                                                */
   uint32_t logits_stride, draft_stride; /* elements from row to row; 0: vocab                     */
   int type;                             /* eg_element of the logits                               */

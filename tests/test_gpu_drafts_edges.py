@@ -111,6 +111,15 @@ def test_verify_writes_its_outputs_alone(device, up, hot):  # noqa: F811
         assert np.all(got[n:] == 0xA5A5A5A5)
 
 
+def test_verify_rows_that_the_workspace_does_not_hold_are_refused(device, up):  # noqa: F811
+    b = up(64)
+    check = lambda **c: drafts.verify(device, *[b] * 6, **{**dict(sequences=1, rows=16383, max_rows=1, vocab=1 << 20), **c})  # noqa: E731
+    for c in (dict(), dict(vocab=(1 << 20) - 4095), dict(rows=16382, accept=b, draws=b, temperatures=b), dict(sequences=65536, vocab=8),
+              dict(rows=65536, vocab=8)):
+        with pytest.raises(_lib.EgRangeError, match="over the workspace or the grid limit"):
+            check(**c)
+
+
 # ---- rotary positions and kept rows -------------------------------------------------------------------
 
 
