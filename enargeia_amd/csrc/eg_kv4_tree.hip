@@ -9,7 +9,7 @@
 // columns bind by what a wave waits for and unpacks, many by issue (products and vector instructions hardly overlap).
 //
 // Maxima, sums and results are f32. A weight enters the second product as f16: f32 rows' in two parts, 22 bits; 16-bit rows' in one, 11
-// bits, while the sum that divides has all of them. Results of 16-bit rows are then off, relative to their norm, by 2.6e-4 to 2.9e-4 in
+// bits, while the sum that divides has all of them. Results of 16-bit rows are then off, relative to their norm, by 2.5e-4 to 2.9e-4 in
 // f16, whose own rounding is 2.1e-4, and by 1.67e-3 in bf16 for 1.66e-3; two parts take 126 us where one takes 80 (8 sequences of 64 rows
 // at up to 8192, 32 / 8 heads of 128, f32 and bf16).
 #include <algorithm>
